@@ -17,7 +17,9 @@ import sys
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "libhive_gpu.so")
-SOURCES = [os.path.join(PKG, "csrc", n) for n in ("hive_engine.hip", "hive_mcts.hip", "hive_fnn.hip", "hive_probe.hip")]
+SOURCES = [os.path.join(PKG, "csrc", n) for n in (
+    "hive_engine.hip", "hive_mcts.hip", "hive_fnn.hip", "hive_probe.hip", "hive_norm.hip", "hive_loss.hip",
+    "hive_adamw.hip")]
 ARCH = os.environ.get("HIVE_GPU_ARCH", "gfx950")
 
 FLAGS = [

@@ -19,6 +19,8 @@ import threading
 
 import torch
 
+from . import training_ops
+
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libhive_gpu.so")
 
@@ -136,6 +138,8 @@ _SIGS_I64 = {  # entry points returning a size (int64_t)
     "hg_mcts_expand_backprop_dense_workspace": [_c_i64, _c_i64],
     "hg_legal_features_actions_ordered_workspace": [_c_i64],
 }
+_SIGS.update(training_ops.SIGS)
+_SIGS_I64.update(training_ops.SIGS_I64)
 
 
 class HgTree(ctypes.Structure):
@@ -1035,6 +1039,10 @@ def _mcts_methods():
 for _name, _fn in _mcts_methods().items():
     setattr(HiveGpuExtension, _name, _fn)
 
+
+# the training operators (layer norm, loss, AdamW): training_ops.py
+for _fn in training_ops.METHODS:
+    setattr(HiveGpuExtension, _fn.__name__, _fn)
 
 _extension = None
 

@@ -1,0 +1,334 @@
+"""The training operators' entry points, bound onto HiveGpuExtension:
+
+    ext.layer_norm_forward / layer_norm_backward   layer norm (of x or sigmoid(x)) and its gradients
+    ext.policy_value_loss                          the loss of a batch of positions and its gradient
+    ext.prepare_adamw(params).step(grads, ...)     one AdamW step of many tensors, moments in 32 or 8 bits
+
+They work in float32 inside, on float32, float16 or bfloat16 tensors, on
+torch.cuda.current_stream() without synchronising it, and raise ValueError
+for what they do not serve before anything is launched.  training.py builds
+autograd functions, an optimizer and a training step of HiveFNN on them.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import numpy as np
+import torch
+
+_c_void_p = ctypes.c_void_p
+_c_i64 = ctypes.c_int64
+_c_int = ctypes.c_int
+_c_float = ctypes.c_float
+_c_double = ctypes.c_double
+
+TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # HG_F32, HG_F16, HG_BF16
+ADAMW_BLOCK = 256  # HG_ADAMW_BLOCK: elements under one scale of 8-bit moments
+
+SIGS = {
+    "hg_layer_norm_forward": [_c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_void_p, _c_void_p, _c_int, _c_float,
+                              _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
+    "hg_layer_norm_backward": [_c_void_p, _c_i64, _c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_void_p, _c_void_p,
+                               _c_void_p, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
+    "hg_policy_value_loss": [_c_void_p, _c_int, _c_i64, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_i64, _c_void_p,
+                             _c_void_p, _c_void_p, _c_i64, _c_float, _c_float, _c_void_p, _c_void_p, _c_void_p,
+                             _c_void_p, _c_void_p],
+    "hg_adamw_step": [_c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_i64, _c_double, _c_double, _c_double, _c_double,
+                      _c_double, _c_void_p, ctypes.c_uint32, _c_void_p],
+}
+SIGS_I64 = {
+    "hg_layer_norm_backward_workspace": [_c_i64, _c_i64],
+    "hg_policy_value_loss_workspace": [_c_i64],
+}
+
+
+class HgAdamwTensor(ctypes.Structure):
+    """C layout of `hg_adamw_tensor` (include/hive_gpu.h)."""
+
+    _fields_ = [(name, ctypes.c_void_p) for name in (
+        "param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")] + [
+        ("count", ctypes.c_int64), ("place", ctypes.c_int64)]
+
+
+def _stream() -> int:
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _check(err: int, what: str) -> None:
+    if err != 0:
+        raise RuntimeError(f"{what}: HIP error {err}")
+
+
+def _float_tensor(t, name: str) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+        raise ValueError(f"{name} must be a GPU tensor")
+    if t.dtype not in TYPES:
+        raise ValueError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is {torch.cuda.current_device()}")
+    return t
+
+
+def _vector(t, name: str, n: int, dtype: torch.dtype) -> torch.Tensor:
+    """A contiguous GPU tensor of n elements, [n] or [n, 1]."""
+    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+        raise ValueError(f"{name} must be a GPU tensor")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) not in ((n,), (n, 1)):
+        raise ValueError(f"{name} must have shape ({n},) or ({n}, 1), got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is {torch.cuda.current_device()}")
+    return t
+
+
+def _rows(t: torch.Tensor, name: str):
+    """(rows, cols, row stride) of a tensor whose last dimension is contiguous
+    and whose other dimensions are evenly spaced rows."""
+    if t.dim() == 0:
+        raise ValueError(f"{name} must have at least one dimension")
+    cols = int(t.shape[-1])
+    if t.is_contiguous():
+        return (t.numel() // cols if cols else math.prod(t.shape[:-1])), cols, cols
+    if cols > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}'s last dimension must be contiguous")
+    if t.dim() == 2:
+        return int(t.shape[0]), cols, int(t.stride(0))
+    try:
+        v = t.view(-1, cols)
+    except RuntimeError:
+        raise ValueError(f"{name}'s rows must be evenly spaced") from None
+    return int(v.shape[0]), cols, int(v.stride(0))
+
+
+def _activation(activation) -> int:
+    if activation not in (None, "sigmoid"):
+        raise ValueError(f"activation must be None or 'sigmoid', got {activation!r}")
+    return 1 if activation else 0
+
+
+def _norm_params(weight, bias, cols: int):
+    """(weight pointer, bias pointer, type): one type for both."""
+    ptr, kind = [None, None], None
+    for i, (t, name) in enumerate(((weight, "weight"), (bias, "bias"))):
+        if t is None:
+            continue
+        _float_tensor(t, name)
+        _vector(t, name, cols, t.dtype)
+        if kind is not None and t.dtype != kind:
+            raise ValueError(f"weight and bias must have one type, got {kind} and {t.dtype}")
+        kind = t.dtype
+        ptr[i] = t.data_ptr()
+    return ptr[0], ptr[1], TYPES[kind or torch.float32]
+
+
+def layer_norm_forward(self, x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, activation=None):
+    """(y, mean, rstd): layer norm over the last dimension of x, or of
+    sigmoid(x) with activation="sigmoid" (HiveFNN's encoder,
+    fnn_network.py:175-187).  x [..., cols] float32 / float16 / bfloat16, its
+    rows contiguous and evenly spaced (a slice of a wider tensor's columns
+    is); weight, bias [cols] of one type, or None; y has x's shape and type
+    and is contiguous, mean and rstd = 1 / sqrt(var + eps) are float32
+    [...]."""
+    _float_tensor(x, "x")
+    rows, cols, stride = _rows(x, "x")
+    if cols == 0:
+        raise ValueError("x must have at least one column")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    sigmoid = _activation(activation)
+    w, b, kind = _norm_params(weight, bias, cols)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    _check(self._lib.hg_layer_norm_forward(x.data_ptr(), TYPES[x.dtype], rows, cols, stride, w, b, kind, eps, sigmoid,
+                                           y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _stream()),
+           "layer_norm_forward")
+    return y, mean, rstd
+
+
+def layer_norm_backward(self, dy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor, weight=None,
+                        bias=None, activation=None, need_dx: bool = True):
+    """(dx, dweight, dbias): the gradients of layer_norm_forward from dy, the
+    gradient of y, with the forward pass's x, mean, rstd, weight and
+    activation.  dweight and dbias (of the parameters' type; None for a
+    parameter that is None) are sums over all rows, the same bits on every
+    call; dx (x's shape and type, contiguous; None with need_dx=False)."""
+    _float_tensor(x, "x")
+    _float_tensor(dy, "dy")
+    if dy.shape != x.shape or dy.dtype != x.dtype:
+        raise ValueError(f"dy must be {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
+    rows, cols, stride = _rows(x, "x")
+    if cols == 0:
+        raise ValueError("x must have at least one column")
+    dy_stride = _rows(dy, "dy")[2]
+    sigmoid = _activation(activation)
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if not isinstance(t, torch.Tensor) or t.device != x.device or t.dtype != torch.float32 or \
+                t.numel() != rows or not t.is_contiguous():
+            raise ValueError(f"{name} must be the forward pass's: {rows} float32 values on {x.device}")
+    w, _, kind = _norm_params(weight, bias, cols)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_dx else None
+    dw = torch.empty((cols,), dtype=weight.dtype, device=x.device) if weight is not None else None
+    db = torch.empty((cols,), dtype=bias.dtype, device=x.device) if bias is not None else None
+    ws = None
+    if dw is not None or db is not None:
+        ws = torch.empty((int(self._lib.hg_layer_norm_backward_workspace(rows, cols)),), dtype=torch.uint8,
+                         device=x.device)
+    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+    _check(self._lib.hg_layer_norm_backward(dy.data_ptr(), dy_stride, x.data_ptr(), TYPES[x.dtype], rows, cols, stride,
+                                            mean.data_ptr(), rstd.data_ptr(), w, kind, sigmoid, ptr(dx), ptr(dw),
+                                            ptr(db), ptr(ws), _stream()), "layer_norm_backward")
+    return dx, dw, db
+
+
+def policy_value_loss(self, logits: torch.Tensor, values: torch.Tensor, num_actions: torch.Tensor,
+                      policy_targets: torch.Tensor, policy_weights: torch.Tensor, value_targets: torch.Tensor,
+                      value_weights: torch.Tensor, value_coef: float = 1.0, loss_scale: float = 1.0):
+    """(losses, dlogits, dvalues): the training loss of B positions and its
+    gradient in one call.
+
+    logits [N]: each position's logits over its legal moves, the positions
+    one after the other (build_forward_batch's rows); num_actions [B] int64
+    (clamped to [0, width], as there); policy_targets [B, width] (the slots
+    past num_actions are not read); policy_weights, value_targets,
+    value_weights float32 [B] or [B, 1], the weights not negative; values
+    [B] or [B, 1] of the logits' type.
+    losses is float32 [total, policy, value], total = policy + value_coef
+    value: the weighted means of the cross-entropy and of the squared error.
+    dlogits and dvalues are loss_scale times the gradients of the total.
+    Positions of weight 0, without moves, or with no logit above -inf add
+    nothing and have gradients of zero."""
+    _float_tensor(logits, "logits")
+    if logits.dim() != 1 or not logits.is_contiguous():
+        raise ValueError(f"logits must be one contiguous row, got {tuple(logits.shape)}")
+    _float_tensor(policy_targets, "policy_targets")
+    if policy_targets.dim() != 2 or not policy_targets.is_contiguous():
+        raise ValueError("policy_targets must be contiguous [B, width]")
+    B, width = policy_targets.shape
+    N = logits.shape[0]
+    if B == 0 and N > 0:
+        raise ValueError(f"{N} logits of no position")
+    _vector(values, "values", B, logits.dtype)
+    _vector(num_actions, "num_actions", B, torch.int64)
+    for t, name in ((policy_weights, "policy_weights"), (value_targets, "value_targets"),
+                    (value_weights, "value_weights")):
+        _vector(t, name, B, torch.float32)
+    dev = logits.device
+    losses = torch.empty((3,), dtype=torch.float32, device=dev)
+    dlogits = torch.empty((N,), dtype=logits.dtype, device=dev)
+    dvalues = torch.empty(values.shape, dtype=values.dtype, device=dev)
+    ws = torch.empty((int(self._lib.hg_policy_value_loss_workspace(B)),), dtype=torch.uint8, device=dev)
+    _check(self._lib.hg_policy_value_loss(
+        logits.data_ptr(), TYPES[logits.dtype], N, values.data_ptr(), num_actions.data_ptr(),
+        policy_targets.data_ptr(), TYPES[policy_targets.dtype], width, policy_weights.data_ptr(),
+        value_targets.data_ptr(), value_weights.data_ptr(), B, float(value_coef), float(loss_scale),
+        losses.data_ptr(), dlogits.data_ptr(), dvalues.data_ptr(), ws.data_ptr(), _stream()), "policy_value_loss")
+    return losses, dlogits, dvalues
+
+
+class AdamWPlan:
+    """hg_adamw_step over a fixed list of tensors, checked and laid out once.
+
+    The moments of all tensors are flat arrays, each tensor's at a multiple
+    of 256 elements (`places`): exp_avg and exp_avg_sq in float32, or with
+    state_bits=8 as float8_e4m3fn codes with exp_avg_scale and
+    exp_avg_sq_scale, a float32 per 256 elements; a code stands for code *
+    scale, in exp_avg_sq for the square root of the moment.  The plan enters
+    the parameters by address: updates in place are seen, a parameter whose
+    memory is replaced needs a new plan."""
+
+    def __init__(self, lib, params, state_bits: int = 32, state=None):
+        params = list(params)
+        if not params:
+            raise ValueError("prepare_adamw needs at least one parameter")
+        if state_bits not in (32, 8):
+            raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
+        for i, p in enumerate(params):
+            _float_tensor(p, f"params[{i}]")
+            if p.dtype != params[0].dtype:
+                raise ValueError(f"params[{i}] is {p.dtype}, params[0] {params[0].dtype}: one plan serves one type")
+            if not p.is_contiguous():
+                raise ValueError(f"params[{i}] must be contiguous")
+        self._lib, self.params, self.state_bits = lib, params, state_bits
+        self._ptrs = [p.data_ptr() for p in params]
+        self.places, total = [], 0
+        for p in params:
+            self.places.append(total)
+            total += -(-p.numel() // ADAMW_BLOCK) * ADAMW_BLOCK
+        self.total = total
+        dev = params[0].device
+        kind = torch.float32 if state_bits == 32 else torch.float8_e4m3fn
+        want = {"exp_avg": (total, kind), "exp_avg_sq": (total, kind)}
+        if state_bits == 8:
+            want["exp_avg_scale"] = want["exp_avg_sq_scale"] = (total // ADAMW_BLOCK, torch.float32)
+        if state is None:
+            state = {k: torch.zeros((n,), dtype=t, device=dev) for k, (n, t) in want.items()}
+        if set(state) != set(want):
+            raise ValueError(f"the state must hold {sorted(want)}, got {sorted(state)}")
+        for k, (n, t) in want.items():
+            v = state[k]
+            if not isinstance(v, torch.Tensor) or v.device != dev or v.dtype != t or tuple(v.shape) != (n,) or \
+                    not v.is_contiguous():
+                raise ValueError(f"{k} must be a contiguous {t} tensor of {n} values on {dev}")
+        self.state = {k: state[k] for k in want}
+        self._table = np.zeros((len(params),), dtype=np.dtype(HgAdamwTensor))
+        at = np.array(self.places, dtype=np.uint64)
+        size = np.uint64(4 if state_bits == 32 else 1)
+        self._table["param"] = self._ptrs
+        for k in ("exp_avg", "exp_avg_sq"):
+            self._table[k] = np.uint64(self.state[k].data_ptr()) + size * at
+            if state_bits == 8:
+                self._table[k + "_scale"] = np.uint64(self.state[k + "_scale"].data_ptr()) + \
+                    np.uint64(4) * (at // np.uint64(ADAMW_BLOCK))
+        self._table["count"] = [p.numel() for p in params]
+        self._table["place"] = self.places
+        self._shapes = [p.shape for p in params]
+
+    def step(self, grads, step: int, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+             weight_decay: float = 0.01, grad_scale: torch.Tensor | None = None, seed: int = 0) -> None:
+        """Step number `step` (the first is 1) of every parameter from `grads`
+        (one type, contiguous, the parameters' shapes), in place.  grad_scale:
+        a float32 tensor of one value that multiplies the gradients (1 / the
+        loss scale, a clipping factor).  seed: of the 8-bit moments' rounding;
+        give each step another one."""
+        grads = list(grads)
+        if len(grads) != len(self.params):
+            raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
+        kind, dev = grads[0].dtype, self.params[0].device
+        if kind not in TYPES:
+            raise ValueError(f"gradients must be float32, float16 or bfloat16, got {kind}")
+        if dev.index != torch.cuda.current_device():
+            raise ValueError(f"the parameters are on {dev}, the current device is {torch.cuda.current_device()}")
+        for i, (g, shape) in enumerate(zip(grads, self._shapes)):
+            if g.dtype != kind or g.shape != shape or g.device != dev or not g.is_contiguous():
+                raise ValueError(f"grads[{i}] must be a contiguous {kind} tensor {tuple(shape)} on {dev}, got "
+                                 f"{g.dtype} {tuple(g.shape)} on {g.device}")
+        if step < 1:
+            raise ValueError(f"steps count from 1, got {step}")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and eps >= 0.0):
+            raise ValueError(f"betas must be in [0, 1) and eps not negative, got {betas} and {eps}")
+        if [p.data_ptr() for p in self.params] != self._ptrs:
+            raise ValueError("a parameter's memory was replaced: make a new plan")
+        scale = None
+        if grad_scale is not None:
+            if grad_scale.numel() != 1 or grad_scale.dtype != torch.float32 or grad_scale.device != dev:
+                raise ValueError(f"grad_scale must be one float32 value on {dev}")
+            scale = grad_scale.data_ptr()
+        self._table["grad"] = [g.data_ptr() for g in grads]
+        _check(self._lib.hg_adamw_step(
+            self._table.ctypes.data, len(grads), TYPES[self.params[0].dtype], TYPES[kind], self.state_bits, int(step),
+            lr, betas[0], betas[1], eps, weight_decay, scale, int(seed) & 0xFFFFFFFF, _stream()), "adamw_step")
+
+
+def prepare_adamw(self, params, state_bits: int = 32, state=None) -> AdamWPlan:
+    """An AdamWPlan of contiguous parameters of one type.  `state`: the
+    `state` of an earlier plan over tensors of the same sizes (a checkpoint),
+    taken as it is, not copied; None: moments of zero."""
+    return AdamWPlan(self._lib, params, state_bits, state)
+
+
+METHODS = (layer_norm_forward, layer_norm_backward, policy_value_loss, prepare_adamw)

@@ -501,6 +501,82 @@ int hg_mcts_wave_root_slots(const hg_tree* tree, const uint8_t* root_states, con
                             float non_root_sigma, float q_penalty, const hg_fnn_net* net,
                             const hg_wave_buffers* buffers, void* stream);
 
+/* ---- training operators ----
+ * What turns a sampled batch into a step of the weights, next to the products
+ * of the network's layers.  The reference trains with torch's operators
+ * (hive_fnn/fnn_trainer.py, fnn_network.py:175-253); these have no entry
+ * points there.  Element types of tensors: */
+#define HG_F32 0
+#define HG_F16 1
+#define HG_BF16 2
+
+/* Layer norm over the cols values of each row of a = x, or of a = sigmoid(x):
+ * y = (a - mean) rstd weight + bias with rstd = 1 / sqrt(var + eps), var the
+ * biased variance.  Row r of x begins at x + r * x_stride elements; y[rows][cols]
+ * has x's type, weight / bias (NULL = 1 / 0) w_type, mean[rows] and rstd[rows]
+ * are float. */
+int hg_layer_norm_forward(const void* x, int x_type, int64_t rows, int64_t cols, int64_t x_stride,
+                          const void* weight, const void* bias, int w_type, float eps, int sigmoid, void* y,
+                          float* mean, float* rstd, void* stream);
+
+/* Its gradients from dy, that of y: dx[rows][cols] in x's type, dweight[cols]
+ * and dbias[cols] in w_type (each NULL = not wanted; the last two are sums over
+ * all rows in one order whatever runs beside them, zeros for no rows).  mean,
+ * rstd: the forward pass's.  workspace: hg_layer_norm_backward_workspace bytes,
+ * 16-byte aligned, needed for dweight / dbias only. */
+int64_t hg_layer_norm_backward_workspace(int64_t rows, int64_t cols);
+int hg_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int x_type, int64_t rows, int64_t cols,
+                           int64_t x_stride, const float* mean, const float* rstd, const void* weight, int w_type,
+                           int sigmoid, void* dx, void* dweight, void* dbias, void* workspace, void* stream);
+
+/* The training loss of B positions and its gradient.  Position b has n[b] =
+ * num_actions[b] clamped to [0, width] legal moves; its logits are n[b] of the
+ * N values of logits, the positions one after the other (the rows of
+ * hg_successor_rows), its policy target the first n[b] values of row b of
+ * targets[B][width] (target_type).  values[B] are the value head's results, of
+ * the logits' type.
+ *   losses[0] = losses[1] + value_coef * losses[2]
+ *   losses[1] = sum w_b CE_b / sum w, CE_b the cross-entropy of the softmax of
+ *               b's logits against its target, w = policy_weights
+ *   losses[2] = sum u_b (values_b - value_targets_b)^2 / sum u, u = value_weights
+ *   dlogits[N], dvalues[B] = loss_scale times the gradient of losses[0], of the
+ *               logits' type
+ * Positions of weight 0, without moves, or whose logits are all -inf add
+ * nothing and have gradients of 0; a sum of weights of 0 counts as 1.  Logits
+ * past the positions' own have gradients of 0, moves past N are left out.
+ * workspace: hg_policy_value_loss_workspace(B) bytes, 16-byte aligned. */
+int64_t hg_policy_value_loss_workspace(int64_t B);
+int hg_policy_value_loss(const void* logits, int type, int64_t N, const void* values, const int64_t* num_actions,
+                         const void* targets, int target_type, int64_t width, const float* policy_weights,
+                         const float* value_targets, const float* value_weights, int64_t B, float value_coef,
+                         float loss_scale, float* losses, void* dlogits, void* dvalues, void* workspace,
+                         void* stream);
+
+/* One AdamW step (step >= 1) of `count` tensors, in place:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps)
+ * with g = grad * grad_scale[0] (NULL = 1; device memory).  `tensors` is a host
+ * array, read before the call returns.  state_bits 32: exp_avg and exp_avg_sq
+ * are float[count] (the scales NULL).  state_bits 8: they are float8 e4m3 codes
+ * in whole blocks of HG_ADAMW_BLOCK elements, 4-byte aligned, each block with a
+ * float scale: exp_avg = code * scale, exp_avg_sq = (code * scale)^2; new values
+ * are rounded to a neighbouring code at random, by bits that depend on `seed`
+ * and `place` + the element's index alone (place: a multiple of the block). */
+#define HG_ADAMW_BLOCK 256
+typedef struct hg_adamw_tensor {
+    void* param;
+    const void* grad;
+    void* exp_avg;
+    void* exp_avg_sq;
+    float* exp_avg_scale;
+    float* exp_avg_sq_scale;
+    int64_t count;  /* elements */
+    int64_t place;  /* of its first element among all states of the step */
+} hg_adamw_tensor;
+int hg_adamw_step(const hg_adamw_tensor* tensors, int64_t count, int param_type, int grad_type, int state_bits,
+                  int64_t step, double lr, double beta1, double beta2, double eps, double weight_decay,
+                  const float* grad_scale, uint32_t seed, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
