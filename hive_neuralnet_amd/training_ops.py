@@ -51,8 +51,8 @@ class HgAdamwTensor(ctypes.Structure):
         ("count", ctypes.c_int64), ("place", ctypes.c_int64)]
 
 
-def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+# the current stream's handle without a Stream object around it (2.8 us of a call's 10)
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _check(err: int, what: str) -> None:
@@ -60,69 +60,82 @@ def _check(err: int, what: str) -> None:
         raise RuntimeError(f"{what}: HIP error {err}")
 
 
-def _float_tensor(t, name: str) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+def _place(t, name: str) -> int:
+    """The device of a GPU tensor on the current device."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{name} must be a GPU tensor")
+    dev = t.get_device()
+    if dev != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is {torch.cuda.current_device()}")
+    return dev
+
+
+def _float_tensor(t, name: str) -> int:
+    dev = _place(t, name)
     if t.dtype not in TYPES:
         raise ValueError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name} is on {t.device}, the current device is {torch.cuda.current_device()}")
-    return t
+    return dev
 
 
-def _vector(t, name: str, n: int, dtype: torch.dtype) -> torch.Tensor:
-    """A contiguous GPU tensor of n elements, [n] or [n, 1]."""
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
-        raise ValueError(f"{name} must be a GPU tensor")
+def _vector(t, name: str, n: int, dtype: torch.dtype, dev: int) -> int:
+    """The address of a contiguous tensor of n elements, [n] or [n, 1], on `dev`."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != dev:
+        raise ValueError(f"{name} must be a GPU tensor on device {dev}")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) not in ((n,), (n, 1)):
-        raise ValueError(f"{name} must have shape ({n},) or ({n}, 1), got {tuple(t.shape)}")
+    shape = t.shape
+    if shape[0] != n if len(shape) == 1 else shape != (n, 1):
+        raise ValueError(f"{name} must have shape ({n},) or ({n}, 1), got {tuple(shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name} is on {t.device}, the current device is {torch.cuda.current_device()}")
-    return t
+    return t.data_ptr()
 
 
 def _rows(t: torch.Tensor, name: str):
     """(rows, cols, row stride) of a tensor whose last dimension is contiguous
     and whose other dimensions are evenly spaced rows."""
-    if t.dim() == 0:
+    shape = t.shape
+    if len(shape) == 0:
         raise ValueError(f"{name} must have at least one dimension")
-    cols = int(t.shape[-1])
+    cols = shape[-1]
+    if cols == 0:
+        raise ValueError(f"{name} must have at least one column")
     if t.is_contiguous():
-        return (t.numel() // cols if cols else math.prod(t.shape[:-1])), cols, cols
+        return t.numel() // cols, cols, cols
     if cols > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name}'s last dimension must be contiguous")
-    if t.dim() == 2:
-        return int(t.shape[0]), cols, int(t.stride(0))
+    if len(shape) == 2:
+        return shape[0], cols, t.stride(0)
     try:
         v = t.view(-1, cols)
     except RuntimeError:
         raise ValueError(f"{name}'s rows must be evenly spaced") from None
-    return int(v.shape[0]), cols, int(v.stride(0))
+    return v.shape[0], cols, v.stride(0)
 
 
 def _activation(activation) -> int:
-    if activation not in (None, "sigmoid"):
+    if activation is None:
+        return 0
+    if activation != "sigmoid":
         raise ValueError(f"activation must be None or 'sigmoid', got {activation!r}")
-    return 1 if activation else 0
+    return 1
 
 
-def _norm_params(weight, bias, cols: int):
+def _norm_params(weight, bias, cols: int, dev: int):
     """(weight pointer, bias pointer, type): one type for both."""
-    ptr, kind = [None, None], None
-    for i, (t, name) in enumerate(((weight, "weight"), (bias, "bias"))):
-        if t is None:
-            continue
-        _float_tensor(t, name)
-        _vector(t, name, cols, t.dtype)
-        if kind is not None and t.dtype != kind:
-            raise ValueError(f"weight and bias must have one type, got {kind} and {t.dtype}")
-        kind = t.dtype
-        ptr[i] = t.data_ptr()
-    return ptr[0], ptr[1], TYPES[kind or torch.float32]
+    w = b = None
+    kind = torch.float32
+    if weight is not None:
+        kind = weight.dtype
+        w = _vector(weight, "weight", cols, kind, dev)
+    if bias is not None:
+        if weight is not None and bias.dtype != kind:
+            raise ValueError(f"weight and bias must have one type, got {kind} and {bias.dtype}")
+        kind = bias.dtype
+        b = _vector(bias, "bias", cols, kind, dev)
+    if kind not in TYPES:
+        raise ValueError(f"weight and bias must be float32, float16 or bfloat16, got {kind}")
+    return w, b, TYPES[kind]
 
 
 def layer_norm_forward(self, x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, activation=None):
@@ -133,19 +146,16 @@ def layer_norm_forward(self, x: torch.Tensor, weight=None, bias=None, eps: float
     is); weight, bias [cols] of one type, or None; y has x's shape and type
     and is contiguous, mean and rstd = 1 / sqrt(var + eps) are float32
     [...]."""
-    _float_tensor(x, "x")
+    dev = _float_tensor(x, "x")
     rows, cols, stride = _rows(x, "x")
-    if cols == 0:
-        raise ValueError("x must have at least one column")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
     sigmoid = _activation(activation)
-    w, b, kind = _norm_params(weight, bias, cols)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    w, b, kind = _norm_params(weight, bias, cols, dev)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    mean, rstd = x.new_empty((2, *x.shape[:-1]), dtype=torch.float32).unbind(0)
     _check(self._lib.hg_layer_norm_forward(x.data_ptr(), TYPES[x.dtype], rows, cols, stride, w, b, kind, eps, sigmoid,
-                                           y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _stream()),
+                                           y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _raw_stream(dev)),
            "layer_norm_forward")
     return y, mean, rstd
 
@@ -157,31 +167,32 @@ def layer_norm_backward(self, dy: torch.Tensor, x: torch.Tensor, mean: torch.Ten
     activation.  dweight and dbias (of the parameters' type; None for a
     parameter that is None) are sums over all rows, the same bits on every
     call; dx (x's shape and type, contiguous; None with need_dx=False)."""
-    _float_tensor(x, "x")
-    _float_tensor(dy, "dy")
+    dev = _float_tensor(x, "x")
+    _place(dy, "dy")
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise ValueError(f"dy must be {tuple(x.shape)} {x.dtype}, got {tuple(dy.shape)} {dy.dtype}")
     rows, cols, stride = _rows(x, "x")
-    if cols == 0:
-        raise ValueError("x must have at least one column")
     dy_stride = _rows(dy, "dy")[2]
     sigmoid = _activation(activation)
     for t, name in ((mean, "mean"), (rstd, "rstd")):
-        if not isinstance(t, torch.Tensor) or t.device != x.device or t.dtype != torch.float32 or \
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != dev or t.dtype != torch.float32 or \
                 t.numel() != rows or not t.is_contiguous():
             raise ValueError(f"{name} must be the forward pass's: {rows} float32 values on {x.device}")
-    w, _, kind = _norm_params(weight, bias, cols)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_dx else None
-    dw = torch.empty((cols,), dtype=weight.dtype, device=x.device) if weight is not None else None
-    db = torch.empty((cols,), dtype=bias.dtype, device=x.device) if bias is not None else None
-    ws = None
+    w, b, kind = _norm_params(weight, bias, cols, dev)
+    dx = dw = db = ws = None
+    if need_dx:
+        dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    if w is not None:
+        dw = torch.empty_like(weight, memory_format=torch.contiguous_format)
+    if b is not None:
+        db = torch.empty_like(bias, memory_format=torch.contiguous_format)
     if dw is not None or db is not None:
-        ws = torch.empty((int(self._lib.hg_layer_norm_backward_workspace(rows, cols)),), dtype=torch.uint8,
-                         device=x.device)
-    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-    _check(self._lib.hg_layer_norm_backward(dy.data_ptr(), dy_stride, x.data_ptr(), TYPES[x.dtype], rows, cols, stride,
-                                            mean.data_ptr(), rstd.data_ptr(), w, kind, sigmoid, ptr(dx), ptr(dw),
-                                            ptr(db), ptr(ws), _stream()), "layer_norm_backward")
+        ws = x.new_empty((self._lib.hg_layer_norm_backward_workspace(rows, cols),), dtype=torch.uint8)
+    _check(self._lib.hg_layer_norm_backward(
+        dy.data_ptr(), dy_stride, x.data_ptr(), TYPES[x.dtype], rows, cols, stride, mean.data_ptr(), rstd.data_ptr(), w,
+        kind, sigmoid, None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
+        None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(), _raw_stream(dev)),
+        "layer_norm_backward")
     return dx, dw, db
 
 
@@ -202,7 +213,7 @@ def policy_value_loss(self, logits: torch.Tensor, values: torch.Tensor, num_acti
     dlogits and dvalues are loss_scale times the gradients of the total.
     Positions of weight 0, without moves, or with no logit above -inf add
     nothing and have gradients of zero."""
-    _float_tensor(logits, "logits")
+    dev = _float_tensor(logits, "logits")
     if logits.dim() != 1 or not logits.is_contiguous():
         raise ValueError(f"logits must be one contiguous row, got {tuple(logits.shape)}")
     _float_tensor(policy_targets, "policy_targets")
@@ -212,21 +223,19 @@ def policy_value_loss(self, logits: torch.Tensor, values: torch.Tensor, num_acti
     N = logits.shape[0]
     if B == 0 and N > 0:
         raise ValueError(f"{N} logits of no position")
-    _vector(values, "values", B, logits.dtype)
-    _vector(num_actions, "num_actions", B, torch.int64)
-    for t, name in ((policy_weights, "policy_weights"), (value_targets, "value_targets"),
-                    (value_weights, "value_weights")):
-        _vector(t, name, B, torch.float32)
-    dev = logits.device
-    losses = torch.empty((3,), dtype=torch.float32, device=dev)
-    dlogits = torch.empty((N,), dtype=logits.dtype, device=dev)
-    dvalues = torch.empty(values.shape, dtype=values.dtype, device=dev)
-    ws = torch.empty((int(self._lib.hg_policy_value_loss_workspace(B)),), dtype=torch.uint8, device=dev)
+    v = _vector(values, "values", B, logits.dtype, dev)
+    n = _vector(num_actions, "num_actions", B, torch.int64, dev)
+    pw = _vector(policy_weights, "policy_weights", B, torch.float32, dev)
+    vt = _vector(value_targets, "value_targets", B, torch.float32, dev)
+    vw = _vector(value_weights, "value_weights", B, torch.float32, dev)
+    losses = logits.new_empty((3,), dtype=torch.float32)
+    dlogits = torch.empty_like(logits)
+    dvalues = torch.empty_like(values)
+    ws = logits.new_empty((self._lib.hg_policy_value_loss_workspace(B),), dtype=torch.uint8)
     _check(self._lib.hg_policy_value_loss(
-        logits.data_ptr(), TYPES[logits.dtype], N, values.data_ptr(), num_actions.data_ptr(),
-        policy_targets.data_ptr(), TYPES[policy_targets.dtype], width, policy_weights.data_ptr(),
-        value_targets.data_ptr(), value_weights.data_ptr(), B, float(value_coef), float(loss_scale),
-        losses.data_ptr(), dlogits.data_ptr(), dvalues.data_ptr(), ws.data_ptr(), _stream()), "policy_value_loss")
+        logits.data_ptr(), TYPES[logits.dtype], N, v, n, policy_targets.data_ptr(), TYPES[policy_targets.dtype], width,
+        pw, vt, vw, B, value_coef, loss_scale, losses.data_ptr(), dlogits.data_ptr(), dvalues.data_ptr(),
+        ws.data_ptr(), _raw_stream(dev)), "policy_value_loss")
     return losses, dlogits, dvalues
 
 
@@ -287,6 +296,10 @@ class AdamWPlan:
         self._table["count"] = [p.numel() for p in params]
         self._table["place"] = self.places
         self._shapes = [p.shape for p in params]
+        self._grad = self._table["grad"]
+        self._table_ptr = self._table.ctypes.data
+        self._type = TYPES[params[0].dtype]
+        self._device = params[0].get_device()
 
     def step(self, grads, step: int, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
              weight_decay: float = 0.01, grad_scale: torch.Tensor | None = None, seed: int = 0) -> None:
@@ -295,17 +308,16 @@ class AdamWPlan:
         a float32 tensor of one value that multiplies the gradients (1 / the
         loss scale, a clipping factor).  seed: of the 8-bit moments' rounding;
         give each step another one."""
-        grads = list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
-        kind, dev = grads[0].dtype, self.params[0].device
+        kind, dev = grads[0].dtype, self._device
         if kind not in TYPES:
             raise ValueError(f"gradients must be float32, float16 or bfloat16, got {kind}")
-        if dev.index != torch.cuda.current_device():
-            raise ValueError(f"the parameters are on {dev}, the current device is {torch.cuda.current_device()}")
-        for i, (g, shape) in enumerate(zip(grads, self._shapes)):
-            if g.dtype != kind or g.shape != shape or g.device != dev or not g.is_contiguous():
-                raise ValueError(f"grads[{i}] must be a contiguous {kind} tensor {tuple(shape)} on {dev}, got "
+        if dev != torch.cuda.current_device():
+            raise ValueError(f"the parameters are on device {dev}, the current one is {torch.cuda.current_device()}")
+        for g, shape in zip(grads, self._shapes):
+            if g.dtype != kind or g.shape != shape or g.get_device() != dev or not g.is_contiguous():
+                raise ValueError(f"a gradient must be a contiguous {kind} tensor {tuple(shape)} on device {dev}, got "
                                  f"{g.dtype} {tuple(g.shape)} on {g.device}")
         if step < 1:
             raise ValueError(f"steps count from 1, got {step}")
@@ -315,13 +327,13 @@ class AdamWPlan:
             raise ValueError("a parameter's memory was replaced: make a new plan")
         scale = None
         if grad_scale is not None:
-            if grad_scale.numel() != 1 or grad_scale.dtype != torch.float32 or grad_scale.device != dev:
-                raise ValueError(f"grad_scale must be one float32 value on {dev}")
+            if grad_scale.numel() != 1 or grad_scale.dtype != torch.float32 or grad_scale.get_device() != dev:
+                raise ValueError(f"grad_scale must be one float32 value on device {dev}")
             scale = grad_scale.data_ptr()
-        self._table["grad"] = [g.data_ptr() for g in grads]
+        self._grad[:] = [g.data_ptr() for g in grads]
         _check(self._lib.hg_adamw_step(
-            self._table.ctypes.data, len(grads), TYPES[self.params[0].dtype], TYPES[kind], self.state_bits, int(step),
-            lr, betas[0], betas[1], eps, weight_decay, scale, int(seed) & 0xFFFFFFFF, _stream()), "adamw_step")
+            self._table_ptr, len(grads), self._type, TYPES[kind], self.state_bits, step, lr, betas[0], betas[1], eps,
+            weight_decay, scale, seed & 0xFFFFFFFF, _raw_stream(dev)), "adamw_step")
 
 
 def prepare_adamw(self, params, state_bits: int = 32, state=None) -> AdamWPlan:
