@@ -3,7 +3,7 @@
 // Position b has n[b] = clamp(num_actions[b], 0, width) legal moves; its
 // logits x are n[b] values of one flat array, the positions one after the
 // other, its searched policy pi the first n[b] values of row b of
-// targets[B][width] (what lies beyond is not read).
+// targets[B][width] (what lies beyond is not used).
 //   lse_b = log sum exp x,  CE_b = sum pi (lse_b - x) over pi != 0
 //   policy = sum w_b CE_b / sum w,      value = sum u_b (v_b - z_b)^2 / sum u
 //   total = policy + c value
@@ -12,138 +12,497 @@
 // A position of weight zero, without moves, or whose logits are all -inf adds
 // nothing and has a gradient of zeros; weights that sum to zero give a loss
 // of zero.  A logit of -inf has p = 0; where pi says otherwise the loss is inf.
+//
+// Where a position's logits begin is a sum over the positions before it.
+// Every block adds up what it needs itself: the counts before its first
+// position and all the weights, up to kInline positions read in full, past
+// them the sums of ranges of kRange positions that a first launch leaves.
+//
+// Lists of up to 256 moves (16 lanes a position) and up to 1,024 (a wave) are
+// read once and held in registers.  Longer ones are cut into slices, a block
+// each, so that few positions fill the card too: one launch leaves each
+// slice's largest logit and sums, the next joins a position's slices and
+// writes the gradient from a second read.
+//
+// Measured (MI355X): 16 positions 6 us, one launch; 2,048 of 60 moves on
+// average 10 us, of which the second launch, the sum of the blocks' shares,
+// takes 3; 65,521 of 85 in bf16 28 us, 18 of them in k_loss_held (latency: a
+// position's place, then its list; the sums before it 9 more in two launches,
+// where every block looking back itself took 46 in all); 192 x 85,834 bf16
+// logits 51 us: 22 for the slices, 4.5 TB/s, and 23 for the gradient.
 #include "hive_train.hpp"
 
 namespace {
 
 using namespace ht;
 
-constexpr int kWaves = 4;
-constexpr int kPlanThreads = 1024;
+constexpr int64_t kInline = 4096, kRange = 1024;
+constexpr int kThreads = 256;
+constexpr int kHeld = 16;  // logits of a position a lane holds
+
+struct Range {  // of kRange positions
+    int64_t moves;
+    float policy, value;
+};
+struct Slice {  // of a long list: its largest logit, sum exp(x - top), sum pi, sum pi (x - top)
+    float top, total, mass, cross;
+};
+
+struct Batch {
+    const void *logits, *values, *targets;
+    const int64_t* num_actions;
+    const float *pw, *vt, *vw;
+    int64_t N, width, B;
+    float value_coef, loss_scale;
+    const Range* ranges;  // nullptr: up to kInline positions
+    int64_t* begin;       // [B] where a position's logits begin, and the weights' sums (1 where they are 0);
+    float* sums;          // nullptr in k_loss_held: every block looks back itself
+    float2* row_loss;     // [blocks or B]: shares of the policy loss and of the value loss
+    float* losses;
+    void *dlogits, *dvalues;
+};
 
 __device__ __forceinline__ int64_t clamp_count(int64_t n, int64_t width) {
     return n < 0 ? 0 : (n > width ? width : n);
 }
-
-// the sum over a block of kPlanThreads, in every thread
-template <typename V> __device__ __forceinline__ V block_sum(V v, V* lds) {
-    __syncthreads();
-    lds[threadIdx.x] = v;
-    __syncthreads();
-    for (int o = kPlanThreads / 2; o > 0; o >>= 1) {
-        if ((int)threadIdx.x < o) lds[threadIdx.x] += lds[threadIdx.x + o];
-        __syncthreads();
-    }
-    return lds[0];
+template <typename V> __device__ __forceinline__ V wave_sum(V v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
 }
 
-// one block: offsets[b] = n[0] + ... + n[b - 1] (offsets[B] the sum of all),
-// sums = {sum of policy weights, sum of value weights}
-__global__ void __launch_bounds__(kPlanThreads)
-k_loss_plan(const int64_t* __restrict__ num_actions, int64_t B, int64_t width, const float* __restrict__ pw,
-            const float* __restrict__ vw, int64_t* __restrict__ offsets, float* __restrict__ sums) {
-    __shared__ int64_t scan[kPlanThreads];
-    __shared__ float part[kPlanThreads];
-    const int t = threadIdx.x;
-    const int64_t per = (B + kPlanThreads - 1) / kPlanThreads, lo = min(B, t * per), hi = min(B, lo + per);
-    int64_t n = 0;
-    float sp = 0.0f, sv = 0.0f;
-    for (int64_t b = lo; b < hi; b++) {
-        n += clamp_count(num_actions[b], width);
-        sp += pw[b];
-        sv += vw[b];
-    }
-    scan[t] = n;
-    __syncthreads();
-    for (int o = 1; o < kPlanThreads; o <<= 1) {
-        const int64_t before = t >= o ? scan[t - o] : 0;
-        __syncthreads();
-        scan[t] += before;
-        __syncthreads();
-    }
-    int64_t at = scan[t] - n;
-    for (int64_t b = lo; b < hi; b++) {
-        offsets[b] = at;
-        at += clamp_count(num_actions[b], width);
-    }
-    if (t == kPlanThreads - 1) offsets[B] = scan[t];
-    sp = block_sum(sp, part);
-    sv = block_sum(sv, part);
-    if (t == 0) {
-        sums[0] = sp;
-        sums[1] = sv;
-    }
-}
-
-// one wave a position; row_loss[b] = {its share of the policy loss, of the value loss}
-template <typename T, typename P>
-__global__ void __launch_bounds__(64 * kWaves)
-k_loss_rows(const T* __restrict__ logits, int64_t N, const T* __restrict__ values, const int64_t* __restrict__ offsets,
-            const float* __restrict__ sums, const P* __restrict__ targets, int64_t width,
-            const float* __restrict__ pw, const float* __restrict__ vt, const float* __restrict__ vw, int64_t B,
-            float value_coef, float loss_scale, float2* __restrict__ row_loss, T* __restrict__ dlogits,
-            T* __restrict__ dvalues) {
-    const int lane = threadIdx.x & 63;
-    const int64_t b = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6);
-    if (b >= B) return;
-    const int64_t lo = min(N, offsets[b]), n = min(N, offsets[b + 1]) - lo;
-    const T* x = logits + lo;
-    const P* pi = targets + b * width;
-    const float W = sums[0], U = sums[1];
-    const float w = pw[b], share = W > 0.0f ? w / W : w;
-    float top = -INFINITY;
-    for (int64_t i = lane; i < n; i += 64) top = max_nan(top, to_f32(x[i]));
-    top = group_max<64>(top);
-    const bool used = w != 0.0f && top != -INFINITY;
-    float total = 0.0f, mass = 0.0f, cross = 0.0f;
-    if (used)
-        for (int64_t i = lane; i < n; i += 64) {
-            const float z = to_f32(x[i]) - top, q = to_f32(pi[i]);
-            total += expf(z);
-            mass += q;
-            if (q != 0.0f) cross += q * z;
+// What a block needs of the positions before its first one and of all.
+struct Before {
+    int64_t moves;       // of the positions before `first`
+    float policy, value; // sums of all weights, 1 where they are 0
+};
+template <int threads> __device__ __forceinline__ Before look_back(const Batch& a, int64_t first) {
+    __shared__ int64_t lds_moves[threads / 64];
+    __shared__ float lds_policy[threads / 64], lds_value[threads / 64];
+    int64_t moves = 0, from = 0;
+    float policy = 0.0f, value = 0.0f;
+    if (a.ranges) {
+        const int64_t all = (a.B + kRange - 1) / kRange, mine = first / kRange;
+        from = mine * kRange;
+        for (int64_t i = threadIdx.x; i < all; i += threads) {
+            const Range r = a.ranges[i];
+            moves += i < mine ? r.moves : 0;
+            policy += r.policy;
+            value += r.value;
         }
-    total = group_sum<64>(total);
+    } else {
+        for (int64_t i = threadIdx.x; i < a.B; i += threads) {
+            policy += a.pw[i];
+            value += a.vw[i];
+        }
+    }
+    for (int64_t i = from + threadIdx.x; i < first; i += threads) moves += clamp_count(a.num_actions[i], a.width);
+    moves = wave_sum(moves);
+    policy = group_sum<64>(policy);
+    value = group_sum<64>(value);
+    if ((threadIdx.x & 63) == 0) {
+        lds_moves[threadIdx.x >> 6] = moves;
+        lds_policy[threadIdx.x >> 6] = policy;
+        lds_value[threadIdx.x >> 6] = value;
+    }
+    __syncthreads();
+    Before r = {0, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < threads / 64; i++) {
+        r.moves += lds_moves[i];
+        r.policy += lds_policy[i];
+        r.value += lds_value[i];
+    }
+    if (!(r.policy > 0.0f)) r.policy = 1.0f;
+    if (!(r.value > 0.0f)) r.value = 1.0f;
+    return r;
+}
+
+// a block a range of kRange positions
+__global__ void __launch_bounds__(kThreads)
+k_loss_ranges(const int64_t* __restrict__ num_actions, int64_t B, int64_t width, const float* __restrict__ pw,
+              const float* __restrict__ vw, Range* __restrict__ ranges) {
+    __shared__ int64_t lds_moves[kThreads / 64];
+    __shared__ float lds[2][kThreads / 64];
+    int64_t moves = 0;
+    float policy = 0.0f, value = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kRange / kThreads; k++) {
+        const int64_t i = (int64_t)blockIdx.x * kRange + k * kThreads + threadIdx.x;
+        if (i < B) {
+            moves += clamp_count(num_actions[i], width);
+            policy += pw[i];
+            value += vw[i];
+        }
+    }
+    moves = wave_sum(moves);
+    policy = group_sum<64>(policy);
+    value = group_sum<64>(value);
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+        lds_moves[wave] = moves;
+        lds[0][wave] = policy;
+        lds[1][wave] = value;
+    }
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    Range r = {0, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; i++) {
+        r.moves += lds_moves[i];
+        r.policy += lds[0][i];
+        r.value += lds[1][i];
+    }
+    ranges[blockIdx.x] = r;
+}
+
+// begin and sums, a range of kRange positions a block
+__global__ void __launch_bounds__(kRange) k_loss_begins(Batch a) {
+    __shared__ int64_t lds[kRange / 64];
+    const int64_t first = (int64_t)blockIdx.x * kRange, b = first + threadIdx.x;
+    const Before before = look_back<kRange>(a, first);
+    const int lane = threadIdx.x & 63;
+    const int64_t n = b < a.B ? clamp_count(a.num_actions[b], a.width) : 0;
+    int64_t upto = n;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t v = __shfl_up(upto, o, 64);
+        upto += lane >= o ? v : 0;
+    }
+    if (lane == 63) lds[threadIdx.x >> 6] = upto;
+    __syncthreads();
+    for (int i = 0; i < (int)(threadIdx.x >> 6); i++) upto += lds[i];
+    if (b < a.B) a.begin[b] = before.moves + upto - n;
+    if (b == 0) {
+        a.sums[0] = before.policy;
+        a.sums[1] = before.value;
+    }
+}
+
+// elements at .. at + n - 1 of an array of `all`; what lies past its end is not read (its values: anything)
+template <typename T, int n>
+__device__ __forceinline__ void load_flat(const T* p, int64_t at, int64_t all, float v[n]) {
+    typedef T vec __attribute__((ext_vector_type(n), aligned(sizeof(T))));
+    if (at + n <= all) {
+        const vec q = *(const vec*)(p + at);
+#pragma unroll
+        for (int i = 0; i < n; i++) v[i] = to_f32<T>(q[i]);
+    } else {
+        skipped();
+#pragma unroll
+        for (int i = 0; i < n; i++) v[i] = at + i < all ? to_f32<T>(p[at + i]) : 0.0f;
+    }
+}
+
+// what a position holds besides its list, read before the list is waited for
+struct Scalars {
+    float w, u, off;  // policy weight, value weight, value less its target
+};
+template <typename T> __device__ __forceinline__ Scalars scalars_of(const Batch& a, int64_t b) {
+    return Scalars{a.pw[b], a.vw[b], to_f32(((const T*)a.values)[b]) - a.vt[b]};
+}
+// the value loss of position b, and its gradient
+template <typename T>
+__device__ __forceinline__ float value_loss(const Batch& a, int64_t b, const Scalars& s, float weights) {
+    const float u = s.u / weights;
+    const bool used = u != 0.0f;
+    ((T*)a.dvalues)[b] = from_f32<T>(used ? 2.0f * a.value_coef * u * s.off * a.loss_scale : 0.0f);
+    return used ? u * s.off * s.off : 0.0f;
+}
+__device__ __forceinline__ void store_losses(const Batch& a, float policy, float value) {
+    a.losses[0] = policy + a.value_coef * value;
+    a.losses[1] = policy;
+    a.losses[2] = value;
+}
+// s + p z, s where p is 0 whatever z is
+__device__ __forceinline__ float plus(float s, float p, float z) { return p != 0.0f ? fmaf(p, z, s) : s; }
+__device__ __forceinline__ float exp_(float z) { return __builtin_amdgcn_exp2f(z * 1.44269504f); }
+
+// gradients of zero for the logits that no position has
+template <typename T> __device__ __forceinline__ void clear_rest(const Batch& a, int64_t from, int tid, int threads) {
+    for (int64_t i = from + tid; i < a.N; i += threads) ((T*)a.dlogits)[i] = from_f32<T>(0.0f);
+}
+
+// kLanes lanes a position, its list held in registers
+template <typename T, typename P, int kLanes>
+__global__ void __launch_bounds__(kThreads) k_loss_held(Batch a) {
+    constexpr int n = Vector<T>::n, vecs = kHeld / n, rows = kThreads / kLanes;
+    const int lane = threadIdx.x % kLanes, mine = threadIdx.x / kLanes;
+    const int64_t first = (int64_t)blockIdx.x * rows, b = first + mine;
+    int64_t lo;
+    int count = 0;
+    float policy_sum, value_sum, policy = 0.0f, value = 0.0f;
+    Scalars own = {};
+    if (b < a.B) own = scalars_of<T>(a, b);
+    if (a.begin) {
+        policy_sum = a.sums[0];
+        value_sum = a.sums[1];
+        if (b < a.B) {
+            lo = a.begin[b];
+            count = (int)clamp_count(a.num_actions[b], a.width);
+        }
+    } else {
+        const Before before = look_back<kThreads>(a, first);
+        policy_sum = before.policy;
+        value_sum = before.value;
+        lo = before.moves;
+#pragma unroll
+        for (int i = 0; i < rows; i++) {  // every lane group adds the counts before its own
+            const int c = first + i < a.B ? (int)clamp_count(a.num_actions[first + i], a.width) : 0;
+            lo += i < mine ? c : 0;
+            count = i == mine ? c : count;
+        }
+    }
+    if (b < a.B) {
+        const int64_t left = a.N - lo;
+        count = left <= 0 ? 0 : (left < count ? (int)left : count);
+        // a position of weight 0 is taken as one without moves, but for its gradient's zeros
+        const float share = own.w / policy_sum;
+        const int live = own.w != 0.0f ? count : 0;
+        float x[vecs][n], pi[vecs][n];
+#pragma unroll
+        for (int k = 0; k < vecs; k++) {
+            const int c = (lane + k * kLanes) * n;
+            if (c < live) {
+                load_flat<T, n>((const T*)a.logits, lo + c, a.N, x[k]);
+                load_flat<P, n>((const P*)a.targets, b * a.width + c, a.B * a.width, pi[k]);
+            }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < vecs; k++)
+#pragma unroll
+            for (int i = 0; i < n; i++) {
+                const bool in = (lane + k * kLanes) * n + i < live;
+                x[k][i] = in ? x[k][i] : -INFINITY;
+                pi[k][i] = in ? pi[k][i] : 0.0f;
+                top = fmaxf(top, x[k][i]);  // passes a NaN by: it comes through the sums
+            }
+        top = group_join<kLanes>(top, [](float p, float q) { return fmaxf(p, q); });
+        const float shift = top == -INFINITY ? 0.0f : top;
+        float total = 0.0f, mass = 0.0f, cross = 0.0f;
+#pragma unroll
+        for (int k = 0; k < vecs; k++)
+#pragma unroll
+            for (int i = 0; i < n; i++) {
+                const float z = x[k][i] - shift;
+                mass += pi[k][i];
+                cross = plus(cross, pi[k][i], z);
+                x[k][i] = exp_(z);
+                total += x[k][i];
+            }
+        total = group_sum<kLanes>(total);
+        mass = group_sum<kLanes>(mass);
+        cross = group_sum<kLanes>(cross);
+        const bool used = total != 0.0f;  // some logit above -inf, or a NaN
+        const float scale = used ? share * a.loss_scale : 0.0f, p_scale = used ? mass / total * scale : 0.0f;
+#pragma unroll
+        for (int k = 0; k < vecs; k++) {
+            const int c = (lane + k * kLanes) * n;
+            if (c >= count) break;
+#pragma unroll
+            for (int i = 0; i < n; i++) x[k][i] = fmaf(x[k][i], p_scale, -(pi[k][i] * scale));
+            if (!used) {  // whatever the target holds
+                skipped();
+#pragma unroll
+                for (int i = 0; i < n; i++) x[k][i] = 0.0f;
+            }
+            store_some((T*)a.dlogits + lo + c, count - c, x[k]);
+        }
+        if (b == a.B - 1) clear_rest<T>(a, lo + count, lane, kLanes);
+        if (lane == 0) {
+            policy = used ? (logf(total) * mass - cross) * share : 0.0f;
+            value = value_loss<T>(a, b, own, value_sum);
+        }
+    }
+    __shared__ float lds[2][kThreads / 64];
+    policy = group_sum<64>(policy);
+    value = group_sum<64>(value);
+    if ((threadIdx.x & 63) == 0) {
+        lds[0][threadIdx.x >> 6] = policy;
+        lds[1][threadIdx.x >> 6] = value;
+    }
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    policy = value = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; i++) {
+        policy += lds[0][i];
+        value += lds[1][i];
+    }
+    if (gridDim.x == 1) store_losses(a, policy, value);
+    else a.row_loss[blockIdx.x] = make_float2(policy, value);
+}
+
+// ---- long lists: block (slice, position) -------------------------------------
+
+// the slice of a position: elements [from, to) of its `count` from logit lo on
+struct Cut {
+    int64_t lo, count, from, to;
+};
+__device__ __forceinline__ Cut cut_of(const Batch& a, int64_t b, int64_t slice) {
+    Cut c;
+    c.lo = min(a.N, a.begin[b]);
+    c.count = min(clamp_count(a.num_actions[b], a.width), a.N - c.lo);
+    c.from = min(c.count, (int64_t)blockIdx.x * slice);
+    c.to = min(c.count, c.from + slice);
+    return c;
+}
+
+// {top, total, mass, cross} of two parts of one list as of one
+__device__ __forceinline__ Slice join(const Slice& p, const Slice& q) {
+    Slice r;
+    r.top = fmaxf(p.top, q.top);
+    const float top = r.top == -INFINITY ? 0.0f : r.top, dp = p.top - top, dq = q.top - top;
+    r.total = p.total * exp_(dp) + q.total * exp_(dq);
+    r.mass = p.mass + q.mass;
+    r.cross = plus(p.cross, p.mass, dp) + plus(q.cross, q.mass, dq);
+    return r;
+}
+
+template <typename T, typename P>
+__global__ void __launch_bounds__(kThreads)
+k_loss_slices(Batch a, int64_t first, int64_t slice, Slice* __restrict__ slices) {
+    constexpr int n = Vector<T>::n;
+    const int64_t b = first + blockIdx.y;
+    const Cut cut = cut_of(a, b, slice);
+    const int64_t at = cut.lo, row = b * a.width, all = a.B * a.width;
+    // one pass: each thread's largest logit so far, its sums brought to a new one as it comes
+    float top = -INFINITY, total = 0.0f, mass = 0.0f, cross = 0.0f;
+    for (int64_t c = cut.from + threadIdx.x * n; c < cut.to; c += kThreads * n) {
+        float x[n], pi[n];
+        load_flat<T, n>((const T*)a.logits, at + c, a.N, x);
+        load_flat<P, n>((const P*)a.targets, row + c, all, pi);
+        float most = top;
+#pragma unroll
+        for (int i = 0; i < n; i++) {
+            if (c + i >= cut.to) {
+                x[i] = -INFINITY;
+                pi[i] = 0.0f;
+            }
+            most = fmaxf(most, x[i]);  // passes a NaN by: it comes through the sums
+        }
+        if (most != top) {
+            total *= exp_(top - most);  // 0 * 0 where this is the first logit above -inf
+            cross = plus(cross, mass, top - most);
+            top = most;
+        }
+        const float shift = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int i = 0; i < n; i++) {
+            const float z = x[i] - shift;
+            total += exp_(z);
+            mass += pi[i];
+            cross = plus(cross, pi[i], z);
+        }
+    }
+    // the block's largest, the sums brought to it and added
+    __shared__ float lds[4][kThreads / 64];
+    const int wave = threadIdx.x >> 6;
+    float most = group_join<64>(top, [](float p, float q) { return fmaxf(p, q); });
+    if ((threadIdx.x & 63) == 0) lds[0][wave] = most;
+    __syncthreads();
+    most = lds[0][0];
+#pragma unroll
+    for (int i = 1; i < kThreads / 64; i++) most = fmaxf(most, lds[0][i]);
+    const float down = most == -INFINITY ? 0.0f : top - most;
+    cross = plus(cross, mass, down);
+    total = group_sum<64>(total * exp_(down));
     mass = group_sum<64>(mass);
     cross = group_sum<64>(cross);
-    const float scale = share * loss_scale, k = mass / total;
-    for (int64_t i = lane; i < n; i += 64) {
-        const float g = used ? (expf(to_f32(x[i]) - top) * k - to_f32(pi[i])) * scale : 0.0f;
-        dlogits[lo + i] = from_f32<T>(g);
+    if ((threadIdx.x & 63) == 0) {
+        lds[1][wave] = total;
+        lds[2][wave] = mass;
+        lds[3][wave] = cross;
     }
-    if (b == B - 1)  // logits that no position has
-        for (int64_t i = lo + n + lane; i < N; i += 64) dlogits[i] = from_f32<T>(0.0f);
-    if (lane == 0) {
-        const float u = U > 0.0f ? vw[b] / U : vw[b], off = to_f32(values[b]) - vt[b];
-        row_loss[b] = make_float2(used ? (logf(total) * mass - cross) * share : 0.0f, u != 0.0f ? u * off * off : 0.0f);
-        dvalues[b] = from_f32<T>(u != 0.0f ? 2.0f * value_coef * u * off * loss_scale : 0.0f);
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    Slice s = {most, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; i++) {
+        s.total += lds[1][i];
+        s.mass += lds[2][i];
+        s.cross += lds[3][i];
     }
+    slices[b * gridDim.x + blockIdx.x] = s;
 }
 
-__global__ void __launch_bounds__(kPlanThreads)
-k_loss_join(const float2* __restrict__ row_loss, int64_t B, float value_coef, float* __restrict__ losses) {
-    __shared__ float part[kPlanThreads];
-    float p = 0.0f, v = 0.0f;
-    for (int64_t b = threadIdx.x; b < B; b += kPlanThreads) {
-        p += row_loss[b].x;
-        v += row_loss[b].y;
+template <typename T, typename P>
+__global__ void __launch_bounds__(kThreads)
+k_loss_gradient(Batch a, int64_t first, int64_t slice, const Slice* __restrict__ slices) {
+    constexpr int n = Vector<T>::n;
+    const int64_t b = first + blockIdx.y;
+    const Cut cut = cut_of(a, b, slice);
+    Slice s = slices[b * gridDim.x];
+    for (int i = 1; i < (int)gridDim.x; i++) s = join(s, slices[b * gridDim.x + i]);
+    const Scalars own = scalars_of<T>(a, b);
+    const float share = own.w / a.sums[0];
+    const bool used = own.w != 0.0f && s.total != 0.0f;
+    const float shift = s.top == -INFINITY ? 0.0f : s.top;
+    const float scale = used ? share * a.loss_scale : 0.0f, p_scale = used ? s.mass / s.total * scale : 0.0f;
+    const int64_t at = cut.lo, row = b * a.width, all = a.B * a.width;
+    for (int64_t c = cut.from + threadIdx.x * n; c < cut.to; c += kThreads * n) {
+        float x[n], pi[n];
+        load_flat<T, n>((const T*)a.logits, at + c, a.N, x);
+        load_flat<P, n>((const P*)a.targets, row + c, all, pi);
+#pragma unroll
+        for (int i = 0; i < n; i++) x[i] = used ? fmaf(exp_(x[i] - shift), p_scale, -(pi[i] * scale)) : 0.0f;
+        store_some((T*)a.dlogits + at + c, (int)min((int64_t)n, cut.to - c), x);
     }
-    p = block_sum(p, part);
-    v = block_sum(v, part);
-    if (threadIdx.x == 0) {
-        losses[0] = p + value_coef * v;
-        losses[1] = p;
-        losses[2] = v;
-    }
+    if (b == a.B - 1 && blockIdx.x == 0) clear_rest<T>(a, cut.lo + cut.count, threadIdx.x, kThreads);
+    if (threadIdx.x == 0 && blockIdx.x == 0)
+        a.row_loss[b] = make_float2(used ? (logf(s.total) * s.mass - s.cross) * share : 0.0f,
+                                    value_loss<T>(a, b, own, a.sums[1]));
 }
+
+__global__ void __launch_bounds__(1024) k_loss_join(Batch a, int64_t parts) {
+    __shared__ float lds[2][16];
+    float p = 0.0f, v = 0.0f;
+    for (int64_t i = threadIdx.x; i < parts; i += 1024) {
+        const float2 r = a.row_loss[i];
+        p += r.x;
+        v += r.y;
+    }
+    p = group_sum<64>(p);
+    v = group_sum<64>(v);
+    if ((threadIdx.x & 63) == 0) {
+        lds[0][threadIdx.x >> 6] = p;
+        lds[1][threadIdx.x >> 6] = v;
+    }
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    p = v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        p += lds[0][i];
+        v += lds[1][i];
+    }
+    store_losses(a, p, v);
+}
+
+constexpr int64_t kShort = 16 * kHeld, kMiddle = 64 * kHeld;  // widths whose lists 16 lanes, a wave hold
+constexpr int64_t kSlice = 4096;                                 // moves of a slice
+constexpr int64_t kMaxBatch = (int64_t)1 << 31;
+constexpr int64_t kGridRows = 32768;  // positions of a launch over slices: a grid has 65,535 rows at most
+
+inline int64_t ranges_of(int64_t B) { return B <= kInline ? 0 : (B + kRange - 1) / kRange; }
+// Slices of a list: of 4,096 moves, or 256 of them.  They depend on the width
+// alone, so that a position's gradient is the same in every batch.
+inline int64_t slices_of(int64_t width) {
+    const int64_t n = (width + kSlice - 1) / kSlice;
+    return n < 256 ? n : 256;
+}
+// float2 per block or position, then the slices
+inline int64_t losses_of(int64_t B) { return (B + 1) / 2 * 2; }
 
 }  // namespace
 
 extern "C" {
 
-int64_t hg_policy_value_loss_workspace(int64_t B) {
+int64_t hg_policy_value_loss_workspace(int64_t B, int64_t width) {
     if (B <= 0) return 16;
-    return 16 + (B + 1) * (int64_t)sizeof(int64_t) + B * (int64_t)sizeof(float2);
+    const int64_t slices = width > kMiddle ? B * slices_of(width) : 0;
+    return ranges_of(B) * (int64_t)sizeof(Range) + losses_of(B) * (int64_t)sizeof(float2) +
+           slices * (int64_t)sizeof(Slice) + B * (int64_t)sizeof(int64_t) + 2 * (int64_t)sizeof(float);
 }
 
 int hg_policy_value_loss(const void* logits, int type, int64_t N, const void* values, const int64_t* num_actions,
@@ -151,7 +510,8 @@ int hg_policy_value_loss(const void* logits, int type, int64_t N, const void* va
                          const float* value_targets, const float* value_weights, int64_t B, float value_coef,
                          float loss_scale, float* losses, void* dlogits, void* dvalues, void* workspace,
                          void* stream) {
-    if (N < 0 || B < 0 || width < 0 || !is_type(type) || !is_type(target_type) || B > (int64_t)1 << 31)
+    if (N < 0 || B < 0 || width < 0 || !is_type(type) || !is_type(target_type) || B > kMaxBatch ||
+        width > (int64_t)1 << 31)
         return (int)hipErrorInvalidValue;
     if (!losses || !workspace || ((uintptr_t)workspace & 15)) return (int)hipErrorInvalidValue;
     if (B > 0 && (!values || !num_actions || !policy_weights || !value_targets || !value_weights || !dvalues))
@@ -159,26 +519,62 @@ int hg_policy_value_loss(const void* logits, int type, int64_t N, const void* va
     if (N > 0 && (!logits || !dlogits || (B > 0 && width > 0 && !targets))) return (int)hipErrorInvalidValue;
     if (B == 0 && N > 0) return (int)hipErrorInvalidValue;
     hipStream_t st = (hipStream_t)stream;
-    float* sums = (float*)workspace;
-    int64_t* offsets = (int64_t*)((uint8_t*)workspace + 16);
-    float2* row_loss = (float2*)(offsets + B + 1);
-    hipLaunchKernelGGL(k_loss_plan, dim3(1), dim3(kPlanThreads), 0, st, num_actions, B, width, policy_weights,
-                       value_weights, offsets, sums);
-    if (B > 0) {
-        const int e = with_type(type, [&](auto tx) {
+    Range* ranges = (Range*)workspace;
+    Batch a;
+    a.logits = logits;
+    a.values = values;
+    a.targets = targets;
+    a.num_actions = num_actions;
+    a.pw = policy_weights;
+    a.vt = value_targets;
+    a.vw = value_weights;
+    a.N = N;
+    a.width = width;
+    a.B = B;
+    a.value_coef = value_coef;
+    a.loss_scale = loss_scale;
+    a.ranges = ranges_of(B) ? ranges : nullptr;
+    a.row_loss = (float2*)(ranges + ranges_of(B));
+    a.losses = losses;
+    a.dlogits = dlogits;
+    a.dvalues = dvalues;
+    Slice* slices = (Slice*)(a.row_loss + losses_of(B));
+    a.begin = (int64_t*)(slices + (width > kMiddle ? B * slices_of(width) : 0));
+    a.sums = (float*)(a.begin + B);
+    if (a.ranges) {
+        hipLaunchKernelGGL(k_loss_ranges, dim3((unsigned)ranges_of(B)), dim3(kThreads), 0, st, num_actions, B, width,
+                           policy_weights, value_weights, ranges);
+    }
+    if (B > 0 && (a.ranges || width > kMiddle))
+        hipLaunchKernelGGL(k_loss_begins, dim3((unsigned)((B + kRange - 1) / kRange)), dim3(kRange), 0, st, a);
+    else
+        a.begin = nullptr;
+    int64_t parts = 0;
+    if (B > 0)
+        with_type(type, [&](auto tx) {
             using T = decltype(tx);
             return with_type(target_type, [&](auto tp) {
                 using P = decltype(tp);
-                hipLaunchKernelGGL((k_loss_rows<T, P>), dim3((unsigned)((B + kWaves - 1) / kWaves)), dim3(64 * kWaves),
-                                   0, st, (const T*)logits, N, (const T*)values, offsets, sums, (const P*)targets,
-                                   width, policy_weights, value_targets, value_weights, B, value_coef, loss_scale,
-                                   row_loss, (T*)dlogits, (T*)dvalues);
-                return (int)hipGetLastError();
+                if (width <= kMiddle) {
+                    const int rows = width <= kShort ? kThreads / 16 : kThreads / 64;
+                    parts = (B + rows - 1) / rows;
+                    auto f = width <= kShort ? k_loss_held<T, P, 16> : k_loss_held<T, P, 64>;
+                    hipLaunchKernelGGL(f, dim3((unsigned)parts), dim3(kThreads), 0, st, a);
+                } else {
+                    const int64_t cuts = slices_of(width);
+                    const int64_t slice = ((width + cuts - 1) / cuts + 7) / 8 * 8;
+                    parts = B;
+                    for (int64_t b = 0; b < B; b += kGridRows) {
+                        const dim3 grid((unsigned)cuts, (unsigned)(B - b < kGridRows ? B - b : kGridRows));
+                        hipLaunchKernelGGL((k_loss_slices<T, P>), grid, dim3(kThreads), 0, st, a, b, slice, slices);
+                        hipLaunchKernelGGL((k_loss_gradient<T, P>), grid, dim3(kThreads), 0, st, a, b, slice, slices);
+                    }
+                }
+                return 0;
             });
         });
-        if (e) return e;
-    }
-    hipLaunchKernelGGL(k_loss_join, dim3(1), dim3(kPlanThreads), 0, st, row_loss, B, value_coef, losses);
+    if (parts != 1 || width > kMiddle)
+        hipLaunchKernelGGL(k_loss_join, dim3(1), dim3(1024), 0, st, a, parts);
     return (int)hipGetLastError();
 }
 

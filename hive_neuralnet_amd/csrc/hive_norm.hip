@@ -335,9 +335,9 @@ k_norm_backward(const typename Sh::T* __restrict__ dy, int64_t dy_stride, const 
                     sb[k][i] = q;
                 }
         }
-        if ((int)threadIdx.x < Sh::kLanes)
+        if ((int)threadIdx.x < Sh::kLanes) {
 #pragma unroll
-            for (int i = 0; i < n; i += 4)
+            for (int i = 0; i < n; i += 4) {
                 if (gridDim.x > 1) {
                     store_some(part + 2 * (int64_t)blockIdx.x * cols + c + i, cols - c - i, sw[k] + i);
                     store_some(part + (2 * (int64_t)blockIdx.x + 1) * cols + c + i, cols - c - i, sb[k] + i);
@@ -347,6 +347,8 @@ k_norm_backward(const typename Sh::T* __restrict__ dy, int64_t dy_stride, const 
                         if (db) store_param(db, w_type, c + j, sb[k][j]);
                     }
                 }
+            }
+        }
     }
 }
 

@@ -39,7 +39,7 @@ SIGS = {
 }
 SIGS_I64 = {
     "hg_layer_norm_backward_workspace": [_c_i64, _c_i64],
-    "hg_policy_value_loss_workspace": [_c_i64],
+    "hg_policy_value_loss_workspace": [_c_i64, _c_i64],
 }
 
 
@@ -231,7 +231,7 @@ def policy_value_loss(self, logits: torch.Tensor, values: torch.Tensor, num_acti
     losses = logits.new_empty((3,), dtype=torch.float32)
     dlogits = torch.empty_like(logits)
     dvalues = torch.empty_like(values)
-    ws = logits.new_empty((self._lib.hg_policy_value_loss_workspace(B),), dtype=torch.uint8)
+    ws = logits.new_empty((self._lib.hg_policy_value_loss_workspace(B, width),), dtype=torch.uint8)
     _check(self._lib.hg_policy_value_loss(
         logits.data_ptr(), TYPES[logits.dtype], N, v, n, policy_targets.data_ptr(), TYPES[policy_targets.dtype], width,
         pw, vt, vw, B, value_coef, loss_scale, losses.data_ptr(), dlogits.data_ptr(), dvalues.data_ptr(),

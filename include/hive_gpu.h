@@ -544,8 +544,8 @@ int hg_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int
  * Positions of weight 0, without moves, or whose logits are all -inf add
  * nothing and have gradients of 0; a sum of weights of 0 counts as 1.  Logits
  * past the positions' own have gradients of 0, moves past N are left out.
- * workspace: hg_policy_value_loss_workspace(B) bytes, 16-byte aligned. */
-int64_t hg_policy_value_loss_workspace(int64_t B);
+ * workspace: hg_policy_value_loss_workspace(B, width) bytes, 16-byte aligned. */
+int64_t hg_policy_value_loss_workspace(int64_t B, int64_t width);
 int hg_policy_value_loss(const void* logits, int type, int64_t N, const void* values, const int64_t* num_actions,
                          const void* targets, int target_type, int64_t width, const float* policy_weights,
                          const float* value_targets, const float* value_weights, int64_t B, float value_coef,

@@ -75,8 +75,8 @@ def test_loss_refusals():
                 dict(values=None), dict(losses=None), dict(dv=None), dict(ws=None), dict(ws=p + 8), dict(B=0),
                 dict(B=1 << 40)):
         assert loss(**bad) == INVALID, bad
-    assert lib.hg_policy_value_loss_workspace(0) > 0
-    assert lib.hg_policy_value_loss_workspace(100) >= 100 * 16
+    assert lib.hg_policy_value_loss_workspace(0, 256) > 0
+    assert lib.hg_policy_value_loss_workspace(100, 256) >= 100 * 8
 
 
 @needs_library
