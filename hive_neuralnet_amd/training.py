@@ -1,0 +1,220 @@
+"""Training HiveFNN on the device operators.
+
+The step that the reference's trainer takes with torch's operators
+(hive_fnn/fnn_trainer.py:531-600 over fnn_network.py:175-253): a sampled
+FNNTrainingBatch -> features of the roots and of every legal successor
+(build_forward_batch) -> the network, its layer norms with the sigmoid in
+front of them in one kernel -> the policy and value loss over the ragged
+legal lists, with its gradient -> one AdamW launch for all weights.
+
+    optimizer = AdamW(net.parameters(), lr=1e-3)           # moments in 32 bits; state_bits=8 in 8
+    losses = train_batch(net, optimizer, buffer.sample_batch(2048))   # [total, policy, value], on the device
+
+    python -m hive_neuralnet_amd.training --steps 50 --batch 2048     # the same on synthetic targets
+
+layer_norm and policy_value_loss are autograd functions over the entry points
+of training_ops.py; AdamW is a torch.optim.Optimizer.
+"""
+from __future__ import annotations
+
+import torch
+import torch.nn.functional as F
+
+from . import hive_gpu
+from .fnn import HiveFNN
+from .replay import FNNTrainingBatch, build_forward_batch
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, activation):
+        y, mean, rstd = hive_gpu.load_extension().layer_norm_forward(x, weight, bias, eps, activation)
+        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, mean, rstd = ctx.saved_tensors
+        dx, dw, db = hive_gpu.load_extension().layer_norm_backward(
+            dy.contiguous(), x, mean, rstd, weight, bias, ctx.activation, need_dx=ctx.needs_input_grad[0])
+        return dx, dw, db, None, None
+
+
+def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, activation=None) -> torch.Tensor:
+    """Layer norm over the last dimension of x (activation="sigmoid": of
+    sigmoid(x)), differentiable once in x, weight and bias."""
+    return _LayerNorm.apply(x, weight, bias, eps, activation)
+
+
+class _PolicyValueLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, values, num_actions, targets, pw, vt, vw, value_coef, loss_scale):
+        losses, dlogits, dvalues = hive_gpu.load_extension().policy_value_loss(
+            logits, values, num_actions, targets, pw, vt, vw, value_coef, loss_scale)
+        ctx.save_for_backward(dlogits, dvalues)
+        total, policy, value = losses.unbind(0)
+        ctx.mark_non_differentiable(policy, value)
+        return total.clone(), policy, value
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, _policy, _value):
+        dlogits, dvalues = ctx.saved_tensors
+        return (dlogits * grad).to(dlogits.dtype), (dvalues * grad).to(dvalues.dtype), *([None] * 7)
+
+
+def policy_value_loss(logits, values, num_actions, policy_targets, policy_weights, value_targets, value_weights,
+                      value_coef: float = 1.0, loss_scale: float = 1.0):
+    """(total, policy, value) of HiveGpuExtension.policy_value_loss; total is
+    differentiable in logits and values (its gradients times loss_scale)."""
+    return _PolicyValueLoss.apply(logits, values, num_actions, policy_targets, policy_weights, value_targets,
+                                  value_weights, value_coef, loss_scale)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW with decoupled weight decay, all parameters of a group and type
+    in one launch, the moments in 32 bits or, with state_bits=8, in 8
+    (AdamWPlan).  A parameter without a gradient is left as it is; the step's
+    number counts the optimizer's steps.  `seed` seeds the rounding of 8-bit
+    moments; each step takes the next one."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
+                 state_bits: int = 32, seed: int = 0):
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        self._ext = hive_gpu.load_extension()
+        self.state_bits, self.seed, self.steps = state_bits, int(seed), 0
+        self._plans: list = []  # (group, plan)
+        self._make_plans(None)
+
+    def _make_plans(self, states) -> None:
+        plans = []
+        for group in self.param_groups:
+            by_type: dict = {}
+            for p in group["params"]:
+                by_type.setdefault(p.dtype, []).append(p)
+            for members in by_type.values():
+                state = None
+                if states is not None:
+                    if len(plans) >= len(states):
+                        raise ValueError("the saved state has fewer parameter lists than the optimizer")
+                    state = {k: v.to(members[0].device, copy=True) for k, v in states[len(plans)].items()}
+                plans.append((group, self._ext.prepare_adamw(members, self.state_bits, state)))
+        if states is not None and len(states) != len(plans):
+            raise ValueError(f"the saved state has {len(states)} parameter lists, the optimizer {len(plans)}")
+        self._plans = plans
+
+    def add_param_group(self, param_group) -> None:
+        if getattr(self, "_plans", None):
+            raise ValueError("AdamW's parameters are fixed when it is made")
+        super().add_param_group(param_group)
+
+    @torch.no_grad()
+    def step(self, closure=None, grad_scale: torch.Tensor | None = None):
+        """One step from the parameters' gradients, times grad_scale[0] (a
+        float32 tensor on the device) where given."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        self.steps += 1
+        for group, plan in self._plans:
+            grads = [None if p.grad is None else p.grad.contiguous() for p in plan.params]
+            plan.step(grads, self.steps, lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                      weight_decay=group["weight_decay"], grad_scale=grad_scale, seed=self.seed + self.steps)
+        return loss
+
+    def state_dict(self):
+        """The moments as they are held, the step's number, the groups' settings."""
+        groups = [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups]
+        return {"state_bits": self.state_bits, "seed": self.seed, "steps": self.steps,
+                "states": [dict(plan.state) for _, plan in self._plans], "param_groups": groups}
+
+    def load_state_dict(self, state_dict) -> None:
+        if state_dict["state_bits"] != self.state_bits:
+            raise ValueError(f"the saved moments are in {state_dict['state_bits']} bits, these in {self.state_bits}")
+        if len(state_dict["param_groups"]) != len(self.param_groups):
+            raise ValueError(f"{len(state_dict['param_groups'])} saved groups, {len(self.param_groups)} here")
+        self._make_plans(state_dict["states"])
+        for group, saved in zip(self.param_groups, state_dict["param_groups"]):
+            group.update(saved)
+        self.seed, self.steps = state_dict["seed"], state_dict["steps"]
+
+
+def encode(net: HiveFNN, features: torch.Tensor) -> torch.Tensor:
+    """HiveFNN.encode, the sigmoid and the layer norm in one kernel."""
+    h = layer_norm(F.linear(features, net.fc1.weight, net.fc1.bias), net.ln1.weight, net.ln1.bias, net.ln1.eps,
+                   "sigmoid")
+    return net.fc2(h)
+
+
+def forward(net: HiveFNN, root_features, successor_features, action_to_root):
+    """HiveFNN.forward on the training operators: (action_logits [N], root_values [B, 1])."""
+    root = encode(net, root_features)
+    values = net.value_head(root)
+    if action_to_root.shape[0] == 0:
+        return root_features.new_zeros((0,)), values
+    return net.score_actions(root[action_to_root], encode(net, successor_features)), values
+
+
+def train_batch(net: HiveFNN, optimizer, batch: FNNTrainingBatch, value_coef: float = 1.0) -> torch.Tensor:
+    """One training step on a sampled batch; returns [total, policy, value]
+    (float32, on the device: reading them waits for the step)."""
+    ext = hive_gpu.load_extension()
+    B = int(batch.num_actions.shape[0])
+    root, succ, action_to_root, num_actions = build_forward_batch(
+        ext, batch.state_bytes, B, batch.num_actions, batch.root_features, batch.legal_moves)
+    logits, values = forward(net, root, succ, action_to_root)
+    losses, dlogits, dvalues = ext.policy_value_loss(
+        logits.detach(), values.detach(), num_actions, batch.policy_targets, batch.policy_mask, batch.value_targets,
+        batch.value_mask * batch.value_weights, value_coef)
+    optimizer.zero_grad(set_to_none=True)
+    heads, grads = (values,), (dvalues,)
+    if logits.requires_grad:
+        heads, grads = (logits, values), (dlogits, dvalues)
+    torch.autograd.backward(heads, grads)
+    optimizer.step()
+    return losses
+
+
+def synthetic_batch(batch_size: int, expansion_mask: int = 0, max_ply: int = 120, seed: int = 0) -> FNNTrainingBatch:
+    """Seeded random-play positions with random searched policies and results."""
+    ext = hive_gpu.load_extension()
+    B = int(batch_size)
+    states, _ = hive_gpu.random_positions(B, expansion_mask, max_ply, seed)
+    legal, n, features = ext.generate_legal_moves_and_fnn_features_batch(states, B)
+    g = torch.Generator(device="cuda").manual_seed(int(seed))
+    live = torch.arange(legal.shape[1], device="cuda") < n.unsqueeze(1)
+    policy = torch.rand(live.shape, generator=g, device="cuda").pow(6) * live
+    ones = torch.ones((B, 1), device="cuda")
+    return FNNTrainingBatch(states, policy / policy.sum(1, keepdim=True).clamp(min=1e-30), n.to(torch.int64),
+                            torch.randint(-1, 2, (B, 1), generator=g, device="cuda").float(), ones, ones, ones,
+                            features, legal)
+
+
+def main() -> None:
+    import argparse
+    import time
+
+    from .fnn import FNNConfig
+    ap = argparse.ArgumentParser(description="train HiveFNN on synthetic targets")
+    ap.add_argument("--steps", type=int, default=50)
+    ap.add_argument("--batch", type=int, default=2048)
+    ap.add_argument("--lr", type=float, default=1e-2)
+    ap.add_argument("--state-bits", type=int, default=32, choices=(32, 8))
+    a = ap.parse_args()
+    torch.manual_seed(0)
+    net = HiveFNN(FNNConfig.large()).cuda()
+    optimizer = AdamW(net.parameters(), lr=a.lr, state_bits=a.state_bits)
+    batch = synthetic_batch(a.batch)
+    for i in range(a.steps):
+        t = time.perf_counter()
+        total, policy, value = train_batch(net, optimizer, batch).tolist()
+        if i % max(1, a.steps // 10) == 0 or i == a.steps - 1:
+            print(f"step {i:4d}  total {total:.4f}  policy {policy:.4f}  value {value:.4f}  "
+                  f"{(time.perf_counter() - t) * 1e3:.2f} ms", flush=True)
+
+
+if __name__ == "__main__":
+    main()

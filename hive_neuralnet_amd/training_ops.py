@@ -293,10 +293,10 @@ class AdamWPlan:
             if state_bits == 8:
                 self._table[k + "_scale"] = np.uint64(self.state[k + "_scale"].data_ptr()) + \
                     np.uint64(4) * (at // np.uint64(ADAMW_BLOCK))
-        self._table["count"] = [p.numel() for p in params]
+        self._counts = np.array([p.numel() for p in params], dtype=np.int64)
         self._table["place"] = self.places
         self._shapes = [p.shape for p in params]
-        self._grad = self._table["grad"]
+        self._grad, self._count = self._table["grad"], self._table["count"]
         self._table_ptr = self._table.ctypes.data
         self._type = TYPES[params[0].dtype]
         self._device = params[0].get_device()
@@ -304,19 +304,24 @@ class AdamWPlan:
     def step(self, grads, step: int, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
              weight_decay: float = 0.01, grad_scale: torch.Tensor | None = None, seed: int = 0) -> None:
         """Step number `step` (the first is 1) of every parameter from `grads`
-        (one type, contiguous, the parameters' shapes), in place.  grad_scale:
+        (one type, contiguous, the parameters' shapes; None leaves its parameter
+        and moments as they are), in place.  grad_scale:
         a float32 tensor of one value that multiplies the gradients (1 / the
         loss scale, a clipping factor).  seed: of the 8-bit moments' rounding;
         give each step another one."""
         if len(grads) != len(self.params):
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
-        kind, dev = grads[0].dtype, self._device
+        dev = self._device
+        kind = next((g.dtype for g in grads if g is not None), torch.float32)
         if kind not in TYPES:
             raise ValueError(f"gradients must be float32, float16 or bfloat16, got {kind}")
         if dev != torch.cuda.current_device():
             raise ValueError(f"the parameters are on device {dev}, the current one is {torch.cuda.current_device()}")
+        missing = False
         for g, shape in zip(grads, self._shapes):
-            if g.dtype != kind or g.shape != shape or g.get_device() != dev or not g.is_contiguous():
+            if g is None:
+                missing = True
+            elif g.dtype != kind or g.shape != shape or g.get_device() != dev or not g.is_contiguous():
                 raise ValueError(f"a gradient must be a contiguous {kind} tensor {tuple(shape)} on device {dev}, got "
                                  f"{g.dtype} {tuple(g.shape)} on {g.device}")
         if step < 1:
@@ -330,7 +335,12 @@ class AdamWPlan:
             if grad_scale.numel() != 1 or grad_scale.dtype != torch.float32 or grad_scale.get_device() != dev:
                 raise ValueError(f"grad_scale must be one float32 value on device {dev}")
             scale = grad_scale.data_ptr()
-        self._grad[:] = [g.data_ptr() for g in grads]
+        if missing:
+            self._grad[:] = [0 if g is None else g.data_ptr() for g in grads]
+            self._count[:] = [0 if g is None else n for g, n in zip(grads, self._counts)]
+        else:
+            self._grad[:] = [g.data_ptr() for g in grads]
+            self._count[:] = self._counts
         _check(self._lib.hg_adamw_step(
             self._table_ptr, len(grads), self._type, TYPES[kind], self.state_bits, step, lr, betas[0], betas[1], eps,
             weight_decay, scale, seed & 0xFFFFFFFF, _raw_stream(dev)), "adamw_step")

@@ -1,0 +1,270 @@
+"""The training step and its parts: autograd functions against torch's in 64
+bits, the optimizer against torch's, whole steps of HiveFNN, graph replays."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+def _randn(shape, seed):
+    return torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+
+
+def _near(got, want, rel, what):
+    """Within rel of the largest value: float32 sums of up to a few thousand terms are about 1e-6 of it off, and
+    chains of five layers under 20 times that."""
+    want = want.double()
+    assert float((got.double() - want).abs().max()) <= rel * float(want.abs().max()) + 1e-30, what
+
+
+def test_layer_norm_autograd():
+    from hive_neuralnet_amd.training import layer_norm
+    x, w, b, g = _randn((4, 33, 64), 1), _randn((64,), 2), _randn((64,), 3), _randn((4, 33, 64), 4)
+    for act in (None, "sigmoid"):
+        ins = [t.clone().requires_grad_() for t in (x, w, b)]
+        ref = [t.double().requires_grad_() for t in (x, w, b)]
+        y = layer_norm(*ins, activation=act)
+        a = torch.sigmoid(ref[0]) if act else ref[0]
+        z = F.layer_norm(a, (64,), ref[1], ref[2], 1e-5)
+        _near(y.detach(), z.detach(), 1e-6, act)
+        for p, q in zip(torch.autograd.grad(y, ins, g), torch.autograd.grad(z, ref, g.double())):
+            _near(p, q, 1e-5, act)
+    x = x.clone().requires_grad_()  # a broadcast gradient, no parameters, a frozen input
+    layer_norm(x).sum().backward()
+    assert float(x.grad.abs().max()) < 1e-4
+    w = w.clone().requires_grad_()
+    layer_norm(x.detach(), w, None).sum().backward()
+    assert w.grad.shape == (64,)
+
+
+def test_loss_autograd():
+    from hive_neuralnet_amd.training import policy_value_loss
+    n = torch.tensor([5, 0, 130, 1, 77], device="cuda")
+    B, N = 5, int(n.sum())
+    logits, values = _randn((N,), 1), torch.tanh(_randn((B, 1), 2))
+    targets = torch.rand((B, 256), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    live = torch.arange(256, device="cuda") < n.unsqueeze(1)
+    targets = targets * live / (targets * live).sum(1, keepdim=True).clamp(min=1e-9)
+    pw, vt, vw = torch.tensor([1.0, 1, 1, 0, 1], device="cuda"), _randn((B, 1), 4), torch.full((B, 1), 2.0, device="cuda")
+    ins = [t.clone().requires_grad_() for t in (logits, values)]
+    total, policy, value = policy_value_loss(*ins, n, targets, pw, vt, vw, 0.3)
+    assert not policy.requires_grad and not value.requires_grad
+    ref = [t.double().requires_grad_() for t in (logits, values)]
+    dense = torch.full((B, 256), -1e30, dtype=torch.float64, device="cuda")
+    dense[live] = ref[0]
+    ce = -(targets.double() * torch.log_softmax(dense, 1) * live).sum(1)
+    want = (pw * ce).sum() / pw.sum() + 0.3 * (ref[1] - vt.double()).square().mean()
+    _near(total.detach(), want.detach(), 1e-6, "total")
+    for p, q in zip(torch.autograd.grad(3.0 * total, ins), torch.autograd.grad(3.0 * want, ref)):
+        _near(p, q, 1e-5, "gradient")
+
+
+def _plain_step(net, batch, value_coef):
+    """The losses and gradients of a step, from a double copy of the network and torch's operators on the host."""
+    from hive_neuralnet_amd import hive_gpu
+    from hive_neuralnet_amd.fnn import HiveFNN
+    from hive_neuralnet_amd.replay import build_forward_batch
+    twin = HiveFNN(net.config)
+    twin.load_state_dict(net.state_dict())
+    twin = twin.double()
+    ext = hive_gpu.load_extension()
+    B = batch.num_actions.shape[0]
+    root, succ, a2r, n = build_forward_batch(ext, batch.state_bytes, B, batch.num_actions, batch.root_features,
+                                             batch.legal_moves)
+    host = lambda t: t.cpu().double() if t.is_floating_point() else t.cpu()  # noqa: E731
+    logits, values = twin(host(root), host(succ), host(a2r), host(n))
+    logits.retain_grad()
+    live = torch.arange(256) < host(n).unsqueeze(1)
+    dense = torch.full((B, 256), -1e30, dtype=torch.float64)
+    dense[live] = logits
+    ce = -(host(batch.policy_targets) * torch.log_softmax(dense, 1) * live).sum(1, keepdim=True)
+    pw, vw = host(batch.policy_mask), host(batch.value_mask * batch.value_weights)
+    policy = (pw * ce).sum() / pw.sum()
+    value = (vw * (values - host(batch.value_targets)).square()).sum() / vw.sum()
+    total = policy + value_coef * value
+    total.backward()
+    # a position's logit gradients add up to zero, so the action tower's biases get sums that cancel: what counts
+    # there is the size of the terms, |dlogit| and |dlogit w2 sigmoid'|
+    terms = {"action_fc2.bias": float(logits.grad.abs().sum())}
+    terms["action_fc1.bias"] = 0.25 * terms["action_fc2.bias"] * float(twin.action_fc2.weight.detach().abs().max())
+    return torch.stack([total, policy, value]).detach(), {k: p.grad for k, p in twin.named_parameters()}, terms
+
+
+@pytest.mark.parametrize("config,mask", [("large", 0), ("medium", 7), ("small", 0)])
+def test_train_batch_gradients_match_torch(config, mask):
+    from hive_neuralnet_amd.fnn import FNNConfig, HiveFNN
+    from hive_neuralnet_amd.training import synthetic_batch, train_batch
+    torch.manual_seed(3)
+    net = HiveFNN(getattr(FNNConfig, config)()).cuda()
+    batch = synthetic_batch(96, mask, 80, 5)
+    batch.policy_mask = (torch.arange(96, device="cuda") % 5 != 0).float().unsqueeze(1)
+    batch.value_weights = 1.0 + torch.arange(96, device="cuda").float().unsqueeze(1) % 3
+    want, grads, terms = _plain_step(net, batch, 0.6)
+
+    class Keep:  # the gradients as the optimizer would see them
+        def zero_grad(self, set_to_none):
+            net.zero_grad(set_to_none=True)
+
+        def step(self):
+            self.grads = {k: p.grad.clone() for k, p in net.named_parameters()}
+
+    keep = Keep()
+    losses = train_batch(net, keep, batch, 0.6)
+    _near(losses.cpu(), want, 1e-6, "losses")
+    for k, g in grads.items():
+        if k in terms:  # a term 8 u off, a sum of thousands in a tree 16 u
+            assert float((keep.grads[k].cpu().double() - g).abs().max()) <= 24 * U * terms[k], k
+        else:
+            _near(keep.grads[k].cpu(), g, 5e-5, k)
+
+
+def test_training_goes_as_torch_does():
+    """Fifty steps on one batch against the same network under torch's operators and torch.optim.AdamW in 64 bits
+    on the host: the losses stay together (float32 noise of 1e-6 a step, at most 50 of them, each passed on), and
+    moments in 8 bits give up less than a tenth of what the steps gain."""
+    from hive_neuralnet_amd import hive_gpu
+    from hive_neuralnet_amd.fnn import FNNConfig, HiveFNN
+    from hive_neuralnet_amd.replay import build_forward_batch
+    from hive_neuralnet_amd.training import AdamW, synthetic_batch, train_batch
+    batch = synthetic_batch(64, 0, 100, 9)
+
+    def ours(bits):
+        torch.manual_seed(1)
+        net = HiveFNN(FNNConfig.medium()).cuda()
+        optimizer = AdamW(net.parameters(), lr=1e-2, state_bits=bits)
+        return torch.stack([train_batch(net, optimizer, batch)[0] for _ in range(50)]).cpu().double()
+
+    torch.manual_seed(1)
+    twin = HiveFNN(FNNConfig.medium()).double()
+    optimizer = torch.optim.AdamW(twin.parameters(), lr=1e-2)
+    root, succ, a2r, n = [t.cpu() for t in build_forward_batch(
+        hive_gpu.load_extension(), batch.state_bytes, 64, batch.num_actions, batch.root_features, batch.legal_moves)]
+    live = torch.arange(256) < n.unsqueeze(1)
+    theirs = []
+    for _ in range(50):
+        logits, values = twin(root.double(), succ.double(), a2r, n)
+        dense = torch.full((64, 256), -1e30, dtype=torch.float64)
+        dense[live] = logits
+        ce = -(batch.policy_targets.cpu().double() * torch.log_softmax(dense, 1) * live).sum(1)
+        total = ce.mean() + (values - batch.value_targets.cpu().double()).square().mean()
+        theirs.append(float(total.detach()))
+        optimizer.zero_grad()
+        total.backward()
+        optimizer.step()
+    theirs = torch.tensor(theirs, dtype=torch.float64)
+    wide, narrow = ours(32), ours(8)
+    assert float((wide - theirs).abs().max()) < 50 * 50 * 1e-6 * float(theirs.max())
+    assert float(theirs[0] - narrow[-1]) > 0.9 * float(theirs[0] - theirs[-1]) > 0.0
+
+
+def test_optimizer_matches_torch():
+    """Ten steps of two groups against torch.optim.AdamW in 64 bits: each step moves a weight by at most lr, 16 u
+    of that and 4 u of the weight off."""
+    from hive_neuralnet_amd.training import AdamW
+    shapes = [(64, 122), (64,), (1,), (33, 5)]
+    a = [torch.nn.Parameter(_randn(s, i)) for i, s in enumerate(shapes)]
+    b = [torch.nn.Parameter(p.detach().double()) for p in a]
+    groups = lambda ps: [{"params": ps[:2], "weight_decay": 0.2}, {"params": ps[2:], "lr": 3e-3}]  # noqa: E731
+    ours = AdamW(groups(a), lr=1e-2, betas=(0.8, 0.95))
+    theirs = torch.optim.AdamW(groups(b), lr=1e-2, betas=(0.8, 0.95))
+    for k in range(10):
+        for i, (p, q) in enumerate(zip(a, b)):
+            p.grad = _randn(p.shape, 100 * k + i)
+            q.grad = p.grad.double()
+        ours.step()
+        theirs.step()
+    for p, q in zip(a, b):
+        bound = 10 * (16 * U * 1e-2 + 4 * U * float(q.detach().abs().max()))
+        assert float((p.detach().double() - q.detach()).abs().max()) < bound
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_optimizer_state_and_missing_gradients(bits):
+    from hive_neuralnet_amd.training import AdamW
+
+    def make():
+        ps = [torch.nn.Parameter(_randn(s, i)) for i, s in enumerate([(40, 9), (300,)])]
+        ps.append(torch.nn.Parameter(_randn((70,), 7).bfloat16()))
+        return ps, AdamW(ps, lr=1e-2, state_bits=bits, seed=5)
+
+    def steps(ps, opt, ks):
+        for k in ks:
+            for i, p in enumerate(ps):
+                p.grad = _randn(p.shape, 50 * k + i).to(p.dtype)
+            opt.step()
+
+    a, opt_a = make()
+    steps(a, opt_a, range(6))
+    b, opt_b = make()
+    steps(b, opt_b, range(3))
+    c, opt_c = make()
+    for p, q in zip(c, b):
+        p.data.copy_(q.data)
+    saved = {k: v for k, v in opt_b.state_dict().items()}
+    opt_c.load_state_dict(saved)
+    steps(c, opt_c, range(3, 6))
+    for p, q in zip(a, c):
+        assert torch.equal(p, q)
+    held = [t.clone() for t in opt_c._plans[0][1].state.values()]
+    before = [p.detach().clone() for p in c]
+    c[0].grad = None
+    c[1].grad, c[2].grad = torch.ones_like(c[1]), torch.ones_like(c[2])
+    opt_c.step()
+    assert torch.equal(c[0], before[0]) and not torch.equal(c[1], before[1]) and not torch.equal(c[2], before[2])
+    for t, u in zip(opt_c._plans[0][1].state.values(), held):
+        n = 512 if t.shape[0] >= 512 else 2  # the first parameter's two blocks
+        assert torch.equal(t[:n].view(torch.uint8), u[:n].view(torch.uint8))
+    with pytest.raises(ValueError, match="bits"):
+        make_other = AdamW(c, state_bits=40 - bits)
+        make_other.load_state_dict(saved)
+    with pytest.raises(ValueError, match="fixed"):
+        opt_c.add_param_group({"params": [torch.nn.Parameter(_randn((3,), 1))]})
+
+
+def test_graph_replays_match_eager():
+    """Layer norm both ways and the loss captured in a graph, replayed with other inputs and eager work between."""
+    from hive_neuralnet_amd import hive_gpu
+    ext = hive_gpu.load_extension()
+    w = _randn((64,), 1)
+    x, dy = _randn((5000, 64), 2), _randn((5000, 64), 3)
+    n = torch.randint(0, 60, (5000,), generator=torch.Generator(device="cuda").manual_seed(4), device="cuda")
+    N = int(n.sum())
+    logits, values, vt = _randn((N,), 5), _randn((5000,), 6), _randn((5000,), 7)
+    targets = torch.softmax(_randn((5000, 64), 8), 1)
+    ones = torch.ones((5000,), device="cuda")
+
+    def work():
+        y, mean, rstd = ext.layer_norm_forward(x, w, w, activation="sigmoid")
+        return (y, *ext.layer_norm_backward(dy, x, mean, rstd, w, w, "sigmoid"),
+                *ext.policy_value_loss(logits, values, n, targets, ones, vt, ones))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work()
+    for k in range(4):
+        for t, seed in ((x, 20), (dy, 30), (logits, 40), (values, 50)):
+            t.copy_(_randn(t.shape, seed + k))
+        torch.cuda.synchronize()
+        want = [t.clone() for t in work()]
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(out, want):
+            assert torch.equal(p, q), k
+
+
+def test_training_command(capsys, monkeypatch):
+    import sys
+
+    from hive_neuralnet_amd import training
+    monkeypatch.setattr(sys, "argv", ["training", "--steps", "3", "--batch", "32", "--state-bits", "8"])
+    training.main()
+    lines = capsys.readouterr().out.strip().splitlines()
+    assert len(lines) == 3 and "policy" in lines[0]
