@@ -19,12 +19,15 @@
 // beside it, and no atomics.
 //
 // Bound by memory.  Measured (MI355X, inputs not in cache): forward 16,384 x
-// 2,048 f32 45 us, 5.9 TB/s; 8,192 x 4,096 bf16 28 us, 4.9; 118,271 x 64 f32
-// with the sigmoid 14 us, 4.4.  Backward 90 us, 4.5 TB/s; 64 us, 3.2; 29 us,
-// 3.2, 4 to 6 of them the second launch.  Reading the next row ahead in the
-// backward pass took more registers than it hid time (52 -> 82 us for 32,768 x
-// 1,024 bf16), as did keeping h and dh between the two passes over a row
-// (52 -> 75): they are worked out again from the row's own 16 bits.
+// 2,048 f32 45 us, 5.9 TB/s; 8,192 x 4,096 bf16 26 us, 5.2; 118,271 x 64 f32
+// with the sigmoid 13 us, 4.6; 4,096 x 5,119 bf16, rows at odd addresses, 24
+// us, 3.5.  Backward 78 us, 5.2 TB/s; 40 us, 5.0; 23 us, 3.9; 40 us, 3.1; 4 to
+// 6 us of each are the second launch.  In the backward pass the next row is
+// read while this one is worked on (8,192 x 4,096: 61 us without) and h and dh
+// are worked out again for dx, from the row's own 16 bits, which leaves the
+// registers for it; loads wait for nothing, an end that cuts a vector is
+// settled where the vector is used (4,096 x 5,119: 65 us where each load was
+// settled before the next).
 #include "hive_train.hpp"
 
 namespace {
@@ -36,7 +39,7 @@ constexpr int kCus = 256;
 // The forward pass holds 16 values of a row a lane (its weights and biases
 // stay in registers besides; 32 values took 42 us against 28 for 8,192 x 4,096
 // bf16 at half the waves).  The backward pass holds 32 bytes of x and of dy,
-// under 128 registers with the columns' sums, so that 16 waves fit a CU.
+// those of the next row and the columns' sums.
 constexpr int kValues = 16, kBackwardVecs = 2;
 constexpr int64_t kMaxCols = 1024 * kValues;  // wider rows take kernels of their own
 
@@ -53,7 +56,7 @@ template <typename W, int n> __device__ __forceinline__ void load_param_of(const
         if (cols >= m) {
 #pragma unroll
             for (int k = 0; k < n; k += m) {
-                const typename Vector<W>::type q = load_vector((const W*)p, c + k, cols);
+                const typename Vector<W>::type q = settle<W>(load_vector((const W*)p, c + k, cols), c + k, cols);
 #pragma unroll
                 for (int i = 0; i < m; i++) v[k + i] = to_f32<W>(q[i]);
             }
@@ -93,6 +96,8 @@ template <typename T_, int kThreads_, int kLanes_, int kVecs_> struct Shape {
     static constexpr int kLanes = kLanes_, kVecs = kVecs_, kN = Vector<T>::n;
     static constexpr int kThreads = kThreads_, kGroups = kThreads / kLanes;
     static constexpr int kWaves = kLanes > 64 ? kLanes / 64 : 1;  // of a row
+    // whether the backward pass has the registers to read the next row ahead
+    static constexpr bool kAhead = kThreads <= 512 || kVecs * 4 <= (kN == 4 ? 8 : 4);
 };
 
 // v, its registers' contents unknown to the optimiser: what follows from it is worked out from it again
@@ -103,7 +108,7 @@ template <typename V> __device__ __forceinline__ V again(V v) {
     return __builtin_bit_cast(V, q);
 }
 
-// vector k of the lane's row
+// vector k of the lane's row: its load, and what is left to do when it is used
 template <typename Sh>
 __device__ __forceinline__ typename Vector<typename Sh::T>::type load_row(const typename Sh::T* row, int lane, int k,
                                                                           int cols) {
@@ -117,6 +122,12 @@ __device__ __forceinline__ typename Vector<typename Sh::T>::type load_row(const 
         }
     }
     return load_vector(row, (lane + k * Sh::kLanes) * Sh::kN, cols);
+}
+template <typename Sh, bool kZeros>
+__device__ __forceinline__ typename Vector<typename Sh::T>::type settle_row(typename Vector<typename Sh::T>::type q,
+                                                                            int lane, int k, int cols) {
+    if (Sh::kLanes == 1 && cols < Sh::kN) return q;
+    return settle<typename Sh::T, kZeros>(q, (lane + k * Sh::kLanes) * Sh::kN, cols);
 }
 
 // the sums of S values over the lanes of a row; `lds`: [2][S][waves of the block], the halves used in turn
@@ -171,6 +182,7 @@ k_norm_forward(const typename Sh::T* __restrict__ x, int64_t rows, int cols, int
         float s[1] = {0.0f};
 #pragma unroll
         for (int k = 0; k < Sh::kVecs; k++) {
+            raw[k] = settle_row<Sh, true>(raw[k], lane, k, cols);
             const int live = cols - (lane + k * Sh::kLanes) * n;
 #pragma unroll
             for (int i = 0; i < n; i++) a[k][i] = to_f32<typename Sh::T>(raw[k][i]);
@@ -222,7 +234,7 @@ k_norm_forward(const typename Sh::T* __restrict__ x, int64_t rows, int cols, int
 
 // part[block][2][cols]: the block's sums of dw and db; one block writes dw and db themselves
 template <typename Sh>
-__global__ void __launch_bounds__(Sh::kThreads, 4)
+__global__ void __launch_bounds__(Sh::kThreads, (Sh::kVecs == 1 ? 4 : 2))
 k_norm_backward(const typename Sh::T* __restrict__ dy, int64_t dy_stride, const typename Sh::T* __restrict__ x,
                 int64_t x_stride, int64_t rows, int cols, const float* __restrict__ mean,
                 const float* __restrict__ rstd, const void* __restrict__ w, int w_type, int sigmoid,
@@ -238,21 +250,39 @@ k_norm_backward(const typename Sh::T* __restrict__ dy, int64_t dy_stride, const 
     float wv[Sh::kVecs][n], sw[Sh::kVecs][n] = {}, sb[Sh::kVecs][n] = {};
 #pragma unroll
     for (int k = 0; k < Sh::kVecs; k++) load_param<n>(w, w_type, (lane + k * Sh::kLanes) * n, cols, 1.0f, wv[k]);
+    V next[Sh::kVecs], next_dy[Sh::kVecs];
+    float next_m, next_r;
+    auto fetch = [&](int64_t row) {
+        const bool there = row < rows;
+        const typename Sh::T *xr = x + (there ? row * x_stride : 0), *dyr = dy + (there ? row * dy_stride : 0);
+#pragma unroll
+        for (int k = 0; k < Sh::kVecs; k++) {
+            next[k] = load_row<Sh>(xr, lane, k, cols);
+            next_dy[k] = load_row<Sh>(dyr, lane, k, cols);
+        }
+        next_m = there ? mean[row] : 0.0f;
+        next_r = there ? rstd[row] : 0.0f;
+    };
+    if (Sh::kAhead) fetch((int64_t)blockIdx.x * Sh::kGroups + threadIdx.x / Sh::kLanes);
     for (int64_t base = (int64_t)blockIdx.x * Sh::kGroups; base < rows; base += step) {
         const int64_t row = base + threadIdx.x / Sh::kLanes;
         const bool there = row < rows;
-        const typename Sh::T *xr = x + (there ? row * x_stride : 0), *dyr = dy + (there ? row * dy_stride : 0);
+        if (!Sh::kAhead) fetch(row);
         V raw[Sh::kVecs], raw_dy[Sh::kVecs];
 #pragma unroll
         for (int k = 0; k < Sh::kVecs; k++) {
-            raw[k] = load_row<Sh>(xr, lane, k, cols);
-            raw_dy[k] = load_row<Sh>(dyr, lane, k, cols);
+            raw[k] = next[k];
+            raw_dy[k] = next_dy[k];
         }
-        const float m = there ? mean[row] : 0.0f, r = there ? rstd[row] : 0.0f;
+        const float m = next_m, r = next_r, mr = m * r;
+        if (Sh::kAhead && base + step < rows) fetch(row + step);
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < Sh::kVecs; k++) {
-            if (!there) raw_dy[k] = V{};
+            raw[k] = settle_row<Sh, false>(raw[k], lane, k, cols);
+            raw_dy[k] = settle_row<Sh, false>(raw_dy[k], lane, k, cols);
+            // past the row dy is 0: what h holds there adds nothing
+            if (!there || (lane + k * Sh::kLanes) * n >= cols) raw_dy[k] = V{};
             float a[n];
 #pragma unroll
             for (int i = 0; i < n; i++) a[i] = to_f32<typename Sh::T>(raw[k][i]);
@@ -262,8 +292,8 @@ k_norm_backward(const typename Sh::T* __restrict__ dy, int64_t dy_stride, const 
                 for (int i = 0; i < n; i++) a[i] = sigmoid_(a[i]);
             }
 #pragma unroll
-            for (int i = 0; i < n; i++) {  // past the row dy is 0: what h holds there adds nothing
-                const float h = (a[i] - m) * r;
+            for (int i = 0; i < n; i++) {
+                const float h = fmaf(a[i], r, -mr);
                 const float d = to_f32<typename Sh::T>(raw_dy[k][i]), dh = d * wv[k][i];
                 sw[k][i] = fmaf(d, h, sw[k][i]);
                 sb[k][i] += d;
@@ -273,7 +303,7 @@ k_norm_backward(const typename Sh::T* __restrict__ dy, int64_t dy_stride, const 
         }
         row_sums<Sh>(s, lds, turn);
         if (!there || !dx) continue;
-        const float r1 = -r * (s[0] * inv), r2 = r * r * (s[1] * inv);
+        const float r2 = r * r * (s[1] * inv), r1 = fmaf(m, r2, -r * (s[0] * inv));
 #pragma unroll
         for (int k = 0; k < Sh::kVecs; k++) {
             const int c = (lane + k * Sh::kLanes) * n, live = cols - c;
@@ -294,7 +324,7 @@ k_norm_backward(const typename Sh::T* __restrict__ dy, int64_t dy_stride, const 
             }
 #pragma unroll
             for (int i = 0; i < n; i++)  // r (dh - s1 - h s2)
-                da[i] = fmaf(to_f32<typename Sh::T>(q_dy[i]), r * wv[k][i], fmaf(m - a[i], r2, r1));
+                da[i] = fmaf(to_f32<typename Sh::T>(q_dy[i]), r * wv[k][i], fmaf(a[i], -r2, r1));
             if (sigmoid) {
                 skipped();
 #pragma unroll
@@ -501,11 +531,12 @@ template <typename Sh> int64_t forward_blocks(int64_t rows) {
     const int64_t need = (rows + Sh::kGroups - 1) / Sh::kGroups, most = (int64_t)kCus * 1024 / Sh::kThreads;
     return need < most ? need : most;
 }
-// 16 waves a CU, and two rows a lane group at least: a block ends with its
+// As many waves as the registers leave room for, 8 a CU where a lane holds two
+// vectors, else 16, and two rows a lane group at least: a block ends with its
 // sums' way through LDS and memory (2,048 x 64: 8.1 us at one row, 8.7 at two,
 // 10.7 at four; 300 x 4,096: 14.5, 12.0, 13.9)
 template <typename Sh> int64_t backward_blocks(int64_t rows) {
-    const int64_t need = (rows + 2 * Sh::kGroups - 1) / (2 * Sh::kGroups), most = (int64_t)kCus * 1024 / Sh::kThreads;
+    const int64_t need = (rows + 2 * Sh::kGroups - 1) / (2 * Sh::kGroups), most = (int64_t)kCus * (Sh::kVecs == 1 || Sh::kThreads > 512 ? 1024 : 512) / Sh::kThreads;
     return need < most ? need : most;
 }
 constexpr int64_t kWideParts = 64;  // row ranges of k_norm_dw_wide

@@ -32,19 +32,27 @@ template <typename T> struct Vector {
 // one, where the optimiser would work both sides out and choose.
 __device__ __forceinline__ void skipped() { asm volatile(""); }
 
-// Elements c .. c + n - 1 of a row of cols >= n elements, zeros past its end.
-// Every lane loads 16 bytes that lie in the row, so that loads follow each
-// other without branches: a vector that the row's end cuts loads the row's
-// last n elements and moves them down, in the steps of a shifter.
+// Elements c .. c + n - 1 of a row of cols >= n elements, in two steps, so that
+// the loads of several vectors follow each other: every lane loads 16 bytes
+// that lie in the row (a vector that the row's end cuts, the row's last n
+// elements), and what the end cut is moved down when it is used, in the steps
+// of a shifter, by the waves that hold such a vector.
 template <typename T>
 __device__ __forceinline__ typename Vector<T>::type load_vector(const T* row, int c, int cols) {
     constexpr int n = Vector<T>::n;
+    return *(const typename Vector<T>::type*)(row + min(c, cols - n));
+}
+// The second step: zeros past the row's end (kZeros false: a vector wholly
+// past it holds elements of the row instead).
+template <typename T, bool kZeros = true>
+__device__ __forceinline__ typename Vector<T>::type settle(typename Vector<T>::type v, int c, int cols) {
+    constexpr int n = Vector<T>::n;
     typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-    const int over = max(0, c - (cols - n));
-    u4 q = __builtin_bit_cast(u4, *(const typename Vector<T>::type*)(row + (c - over)));
-    if (cols % n != 0) {  // the same for every lane
+    const int over = c - (cols - n);
+    u4 q = __builtin_bit_cast(u4, v);
+    if (__any(over > 0 && over < n)) {
         skipped();
-        const int bytes = over * (int)sizeof(T);
+        const int bytes = over > 0 ? over * (int)sizeof(T) : 0;
         if constexpr (sizeof(T) == 2) {
             const bool b = bytes & 2;
 #pragma unroll
@@ -55,7 +63,7 @@ __device__ __forceinline__ typename Vector<T>::type load_vector(const T* row, in
 #pragma unroll
         for (int i = 0; i < 4; i++) q[i] = bytes & 8 ? (i < 2 ? q[i < 2 ? i + 2 : 3] : 0) : q[i];
     }
-    if (over >= n) q = u4{0, 0, 0, 0};
+    if (kZeros && over >= n) q = u4{0, 0, 0, 0};
     return __builtin_bit_cast(typename Vector<T>::type, q);
 }
 // the first `live` of n values to p, a cut vector in pieces of 4, 2 and 1
