@@ -26,10 +26,11 @@
 //
 // Measured (MI355X): 16 positions 6 us, one launch; 2,048 of 60 moves on
 // average 10 us, of which the second launch, the sum of the blocks' shares,
-// takes 3; 65,521 of 85 in bf16 28 us, 18 of them in k_loss_held (latency: a
-// position's place, then its list; the sums before it 9 more in two launches,
-// where every block looking back itself took 46 in all); 192 x 85,834 bf16
-// logits 51 us: 22 for the slices, 4.5 TB/s, and 23 for the gradient.
+// takes 3; 65,521 of 85 in bf16 28 us: the sums before them 9 in two launches
+// (46 us in all where every block looked back itself), the lists 17, of which
+// the VALU is busy 12 (450 instructions a wave; a third of the slots it works
+// on hold a move); 192 x 85,834 bf16 logits 51 us: 22 for the slices, 4.5
+// TB/s, and 23 for the gradient, which finds its second read in the cache.
 #include "hive_train.hpp"
 
 namespace {
@@ -56,7 +57,7 @@ struct Batch {
     float value_coef, loss_scale;
     const Range* ranges;  // nullptr: up to kInline positions
     int64_t* begin;       // [B] where a position's logits begin, and the weights' sums (1 where they are 0);
-    float* sums;          // nullptr in k_loss_held: every block looks back itself
+    float* sums;          // nullptr: every block looks back itself
     float2* row_loss;     // [blocks or B]: shares of the policy loss and of the value loss
     float* losses;
     void *dlogits, *dvalues;
@@ -225,7 +226,7 @@ template <typename T> __device__ __forceinline__ void clear_rest(const Batch& a,
 // kLanes lanes a position, its list held in registers
 template <typename T, typename P, int kLanes>
 __global__ void __launch_bounds__(kThreads) k_loss_held(Batch a) {
-    constexpr int n = Vector<T>::n, vecs = kHeld / n, rows = kThreads / kLanes;
+    constexpr int n = 4, vecs = kHeld / n, rows = kThreads / kLanes;
     const int lane = threadIdx.x % kLanes, mine = threadIdx.x / kLanes;
     const int64_t first = (int64_t)blockIdx.x * rows, b = first + mine;
     int64_t lo;
@@ -267,9 +268,14 @@ __global__ void __launch_bounds__(kThreads) k_loss_held(Batch a) {
                 load_flat<P, n>((const P*)a.targets, b * a.width + c, a.B * a.width, pi[k]);
             }
         }
+        // a step that no list of the wave reaches is passed by
+        bool reached[vecs];
+#pragma unroll
+        for (int k = 0; k < vecs; k++) reached[k] = __any(k * kLanes * n < live);
         float top = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < vecs; k++)
+        for (int k = 0; k < vecs; k++) {
+            if (!reached[k]) break;
 #pragma unroll
             for (int i = 0; i < n; i++) {
                 const bool in = (lane + k * kLanes) * n + i < live;
@@ -277,11 +283,13 @@ __global__ void __launch_bounds__(kThreads) k_loss_held(Batch a) {
                 pi[k][i] = in ? pi[k][i] : 0.0f;
                 top = fmaxf(top, x[k][i]);  // passes a NaN by: it comes through the sums
             }
+        }
         top = group_join<kLanes>(top, [](float p, float q) { return fmaxf(p, q); });
         const float shift = top == -INFINITY ? 0.0f : top;
         float total = 0.0f, mass = 0.0f, cross = 0.0f;
 #pragma unroll
-        for (int k = 0; k < vecs; k++)
+        for (int k = 0; k < vecs; k++) {
+            if (!reached[k]) break;
 #pragma unroll
             for (int i = 0; i < n; i++) {
                 const float z = x[k][i] - shift;
@@ -290,6 +298,7 @@ __global__ void __launch_bounds__(kThreads) k_loss_held(Batch a) {
                 x[k][i] = exp_(z);
                 total += x[k][i];
             }
+        }
         total = group_sum<kLanes>(total);
         mass = group_sum<kLanes>(mass);
         cross = group_sum<kLanes>(cross);
@@ -301,12 +310,12 @@ __global__ void __launch_bounds__(kThreads) k_loss_held(Batch a) {
             if (c >= count) break;
 #pragma unroll
             for (int i = 0; i < n; i++) x[k][i] = fmaf(x[k][i], p_scale, -(pi[k][i] * scale));
-            if (!used) {  // whatever the target holds
+            if (!used) {  // whatever the target holds, or nothing was read
                 skipped();
 #pragma unroll
                 for (int i = 0; i < n; i++) x[k][i] = 0.0f;
             }
-            store_some((T*)a.dlogits + lo + c, count - c, x[k]);
+            store_some<T, n>((T*)a.dlogits + lo + c, count - c, x[k]);
         }
         if (b == a.B - 1) clear_rest<T>(a, lo + count, lane, kLanes);
         if (lane == 0) {
@@ -335,13 +344,17 @@ __global__ void __launch_bounds__(kThreads) k_loss_held(Batch a) {
 
 // ---- long lists: block (slice, position) -------------------------------------
 
+// what k_loss_begins left, or the block's own
+__device__ __forceinline__ Before begin_of(const Batch& a, int64_t b) {
+    return a.begin ? Before{a.begin[b], a.sums[0], a.sums[1]} : look_back<kThreads>(a, b);
+}
 // the slice of a position: elements [from, to) of its `count` from logit lo on
 struct Cut {
     int64_t lo, count, from, to;
 };
-__device__ __forceinline__ Cut cut_of(const Batch& a, int64_t b, int64_t slice) {
+__device__ __forceinline__ Cut cut_of(const Batch& a, int64_t b, int64_t begin, int64_t slice) {
     Cut c;
-    c.lo = min(a.N, a.begin[b]);
+    c.lo = min(a.N, begin);
     c.count = min(clamp_count(a.num_actions[b], a.width), a.N - c.lo);
     c.from = min(c.count, (int64_t)blockIdx.x * slice);
     c.to = min(c.count, c.from + slice);
@@ -364,7 +377,8 @@ __global__ void __launch_bounds__(kThreads)
 k_loss_slices(Batch a, int64_t first, int64_t slice, Slice* __restrict__ slices) {
     constexpr int n = Vector<T>::n;
     const int64_t b = first + blockIdx.y;
-    const Cut cut = cut_of(a, b, slice);
+    const Before before = begin_of(a, b);
+    const Cut cut = cut_of(a, b, before.moves, slice);
     const int64_t at = cut.lo, row = b * a.width, all = a.B * a.width;
     // one pass: each thread's largest logit so far, its sums brought to a new one as it comes
     float top = -INFINITY, total = 0.0f, mass = 0.0f, cross = 0.0f;
@@ -431,11 +445,12 @@ __global__ void __launch_bounds__(kThreads)
 k_loss_gradient(Batch a, int64_t first, int64_t slice, const Slice* __restrict__ slices) {
     constexpr int n = Vector<T>::n;
     const int64_t b = first + blockIdx.y;
-    const Cut cut = cut_of(a, b, slice);
+    const Before before = begin_of(a, b);
+    const Cut cut = cut_of(a, b, before.moves, slice);
     Slice s = slices[b * gridDim.x];
     for (int i = 1; i < (int)gridDim.x; i++) s = join(s, slices[b * gridDim.x + i]);
     const Scalars own = scalars_of<T>(a, b);
-    const float share = own.w / a.sums[0];
+    const float share = own.w / before.policy;
     const bool used = own.w != 0.0f && s.total != 0.0f;
     const float shift = s.top == -INFINITY ? 0.0f : s.top;
     const float scale = used ? share * a.loss_scale : 0.0f, p_scale = used ? s.mass / s.total * scale : 0.0f;
@@ -451,7 +466,7 @@ k_loss_gradient(Batch a, int64_t first, int64_t slice, const Slice* __restrict__
     if (b == a.B - 1 && blockIdx.x == 0) clear_rest<T>(a, cut.lo + cut.count, threadIdx.x, kThreads);
     if (threadIdx.x == 0 && blockIdx.x == 0)
         a.row_loss[b] = make_float2(used ? (logf(s.total) * s.mass - s.cross) * share : 0.0f,
-                                    value_loss<T>(a, b, own, a.sums[1]));
+                                    value_loss<T>(a, b, own, before.value));
 }
 
 __global__ void __launch_bounds__(1024) k_loss_join(Batch a, int64_t parts) {
@@ -545,7 +560,8 @@ int hg_policy_value_loss(const void* logits, int type, int64_t N, const void* va
         hipLaunchKernelGGL(k_loss_ranges, dim3((unsigned)ranges_of(B)), dim3(kThreads), 0, st, num_actions, B, width,
                            policy_weights, value_weights, ranges);
     }
-    if (B > 0 && (a.ranges || width > kMiddle))
+    // past that a slice's look back would cost more than the launch
+    if (a.ranges || (width > kMiddle && B > kThreads))
         hipLaunchKernelGGL(k_loss_begins, dim3((unsigned)((B + kRange - 1) / kRange)), dim3(kRange), 0, st, a);
     else
         a.begin = nullptr;

@@ -66,14 +66,14 @@ __device__ __forceinline__ typename Vector<T>::type settle(typename Vector<T>::t
     if (kZeros && over >= n) q = u4{0, 0, 0, 0};
     return __builtin_bit_cast(typename Vector<T>::type, q);
 }
-// the first `live` of n values to p, a cut vector in pieces of 4, 2 and 1
-template <typename T> __device__ __forceinline__ void store_some(T* p, int live, const float v[Vector<T>::n]) {
-    constexpr int n = Vector<T>::n;
-    typename Vector<T>::type q;
+// the first `live` of n values (4 or 8) to p, a cut vector in pieces of 4, 2 and 1
+template <typename T, int n = Vector<T>::n> __device__ __forceinline__ void store_some(T* p, int live, const float v[n]) {
+    typedef T vec __attribute__((ext_vector_type(n), aligned(sizeof(T))));
+    vec q;
 #pragma unroll
     for (int i = 0; i < n; i++) q[i] = from_f32<T>(v[i]);
     if (live >= n) {
-        *(typename Vector<T>::type*)p = q;
+        *(vec*)p = q;
     } else if (live > 0) {
         typedef T two __attribute__((ext_vector_type(2), aligned(sizeof(T))));
         typedef T four __attribute__((ext_vector_type(4), aligned(sizeof(T))));
@@ -100,7 +100,7 @@ template <typename T> __device__ __forceinline__ void store_some(T* p, int live,
 // other half of the wave
 template <int kControl> __device__ __forceinline__ float dpp(float v) {
     const int i = __float_as_int(v);
-    return __int_as_float(__builtin_amdgcn_update_dpp(i, i, kControl, 0xF, 0xF, false));
+    return __int_as_float(__builtin_amdgcn_mov_dpp(i, kControl, 0xF, 0xF, true));  // every lane has a source
 }
 // f over the G lanes of a lane group (G a power of two); every lane of the
 // group gets the same bits, f being commutative

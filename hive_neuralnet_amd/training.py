@@ -123,6 +123,9 @@ class AdamW(torch.optim.Optimizer):
             grads = [None if p.grad is None else p.grad.contiguous() for p in plan.params]
             plan.step(grads, self.steps, lr=group["lr"], betas=group["betas"], eps=group["eps"],
                       weight_decay=group["weight_decay"], grad_scale=grad_scale, seed=self.seed + self.steps)
+            for p, g in zip(plan.params, grads):  # autograd sees that a weight it saved has changed
+                if g is not None:
+                    torch.autograd.graph.increment_version(p)
         return loss
 
     def state_dict(self):

@@ -224,6 +224,18 @@ def test_optimizer_state_and_missing_gradients(bits):
         opt_c.add_param_group({"params": [torch.nn.Parameter(_randn((3,), 1))]})
 
 
+def test_a_step_invalidates_what_autograd_saved():
+    from hive_neuralnet_amd.training import AdamW
+    w = torch.nn.Parameter(_randn((8, 8), 1))
+    optimizer = AdamW([w])
+    x = _randn((8, 8), 2).requires_grad_()
+    y = (x @ w).sum()
+    w.grad = torch.ones_like(w)
+    optimizer.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
 def test_graph_replays_match_eager():
     """Layer norm both ways and the loss captured in a graph, replayed with other inputs and eager work between."""
     from hive_neuralnet_amd import hive_gpu
