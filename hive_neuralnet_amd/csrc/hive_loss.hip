@@ -26,7 +26,8 @@
 //
 // Measured (MI355X): 16 positions 6 us, one launch; 2,048 of 60 moves on
 // average 10 us, of which the second launch, the sum of the blocks' shares,
-// takes 3; 65,521 of 85 in bf16 28 us: the sums before them 9 in two launches
+// takes 3 (the last block adding them: 17 in all, as every block's write-back
+// for it has to come first); 65,521 of 85 in bf16 28 us: the sums before them 9 in two launches
 // (46 us in all where every block looked back itself), the lists 17, of which
 // the VALU is busy 12 (450 instructions a wave; a third of the slots it works
 // on hold a move); 192 x 85,834 bf16 logits 51 us: 22 for the slices, 4.5
