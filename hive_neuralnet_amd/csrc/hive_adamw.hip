@@ -18,15 +18,17 @@
 // takes the smallest code at least: a code of zero would leave the next step's
 // m to be divided by nearly nothing.
 //
-// A lane takes four neighbouring elements, a wave a scale's 256, and each of a
-// block's waves four such rounds, whose loads are all under way before the
-// first is worked on.
+// A lane takes four neighbouring elements in 16-byte accesses, a wave a
+// scale's 256; the waves that a CU holds keep its loads under way (four rounds
+// a wave: 7 us against 2.8 for 20,546 elements, 196 against 174 for 64 M in 8
+// bits, the same for 64 M in 32).
 //
-// Bound by memory in 32 bits: 201 M float weights with bf16 gradients 994 us,
+// Bound by memory in 32 bits: 201 M float weights with bf16 gradients 985 us,
 // 5.3 TB/s of what has to move, the rate of a large copy (one element's loads
 // at a time: 1,655 us).  In 8 bits the VALU comes near it, 66 operations an
-// element: 144 M weights in bf16 311 us, 4.7 TB/s, where codes made by a
-// divide, a correctly rounded root and float arithmetic took 130 and 571 us.
+// element: 144 M float weights 405 us, 5.7 TB/s, in bf16 303 us, 4.8 TB/s, where
+// codes made by a divide, a correctly rounded root and float arithmetic took
+// 130 and 571 us.
 #include <cmath>
 #include <type_traits>
 
@@ -38,12 +40,14 @@ using namespace ht;
 
 constexpr int kBlock = 256;   // elements under one scale
 constexpr int kTensors = 48;  // tensors of a launch: their table is a kernel argument (4 KB at most)
-constexpr int kThreads = 256, kRounds = 4;
-constexpr int64_t kChunk = 4 * kThreads * kRounds;  // elements of a thread block
+constexpr int kThreads = 256;
+constexpr int64_t kChunk = 4 * kThreads;  // elements of a thread block
+
+constexpr int64_t kMaxChunks = ((int64_t)1 << 24) - 1;  // of a launch: a grid holds under 2^32 threads
 
 struct Table {
     hg_adamw_tensor t[kTensors];
-    int64_t first[kTensors + 1];  // each tensor's first chunk
+    int64_t first[kTensors];  // each tensor's first chunk
     int32_t n;
 };
 struct Step {
@@ -101,121 +105,100 @@ __device__ __forceinline__ float scale_of(float largest) {
     return s < 0x1p-110f ? 0x1p-110f : s;  // NaN stays
 }
 
-// what a lane has read of its four elements
-template <typename P, typename G> struct Read {
-    typename Four<P>::type p;
-    typename Four<G>::type g;
-    Four<float>::type m, v;  // 32 bits
-    uint32_t codes_m, codes_r;
-    float scale_m, scale_r;
-};
-
 template <typename P, typename G, int kBits, bool kFull>
 __device__ __forceinline__ void step_chunk(const hg_adamw_tensor& t, int64_t chunk, const Step& s) {
-    const int64_t base = chunk * kChunk + 4 * (int)threadIdx.x;
-    auto live_at = [&](int64_t at) { return kFull ? 4 : (int)max((int64_t)0, min((int64_t)4, t.count - at)); };
-    Read<P, G> in[kRounds];
+    const int64_t at = chunk * kChunk + 4 * (int)threadIdx.x;
+    const int live = kFull ? 4 : (int)max((int64_t)0, min((int64_t)4, t.count - at));
+    auto p = load_four<P, kFull>((const P*)t.param + at, live);
+    const auto g4 = load_four<G, kFull>((const G*)t.grad + at, live);
+    float m[4], v[4], r[4];
+    if constexpr (kBits == 32) {
+        const auto m4 = load_four<float, kFull>((const float*)t.exp_avg + at, live);
+        const auto v4 = load_four<float, kFull>((const float*)t.exp_avg_sq + at, live);
 #pragma unroll
-    for (int k = 0; k < kRounds; k++) {
-        const int64_t at = base + k * 4 * kThreads;
-        const int live = live_at(at);
-        in[k].p = load_four<P, kFull>((const P*)t.param + at, live);
-        in[k].g = load_four<G, kFull>((const G*)t.grad + at, live);
-        if constexpr (kBits == 32) {
-            in[k].m = load_four<float, kFull>((const float*)t.exp_avg + at, live);
-            in[k].v = load_four<float, kFull>((const float*)t.exp_avg_sq + at, live);
-        } else if (live > 0) {  // codes are held in whole blocks
-            in[k].codes_m = ((const uint32_t*)t.exp_avg)[at >> 2];
-            in[k].codes_r = ((const uint32_t*)t.exp_avg_sq)[at >> 2];
-            in[k].scale_m = t.exp_avg_scale[at / kBlock];
-            in[k].scale_r = t.exp_avg_sq_scale[at / kBlock];
+        for (int i = 0; i < 4; i++) {
+            m[i] = m4[i];
+            v[i] = v4[i];
+        }
+    } else {
+        int codes_m = 0, codes_r = 0;
+        float scale_m = 0.0f, scale_r = 0.0f;
+        if (live > 0) {  // codes are held in whole blocks
+            codes_m = ((const int*)t.exp_avg)[at >> 2];
+            codes_r = ((const int*)t.exp_avg_sq)[at >> 2];
+            scale_m = t.exp_avg_scale[at / kBlock];
+            scale_r = t.exp_avg_sq_scale[at / kBlock];
+        }
+        const auto m01 = __builtin_amdgcn_cvt_pk_f32_fp8(codes_m, false);
+        const auto m23 = __builtin_amdgcn_cvt_pk_f32_fp8(codes_m, true);
+        const auto r01 = __builtin_amdgcn_cvt_pk_f32_fp8(codes_r, false);
+        const auto r23 = __builtin_amdgcn_cvt_pk_f32_fp8(codes_r, true);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            m[i] = (i < 2 ? m01[i & 1] : m23[i & 1]) * scale_m;
+            const float q = (i < 2 ? r01[i & 1] : r23[i & 1]) * scale_r;
+            v[i] = q * q;
         }
     }
     const float gs = s.grad_scale ? *s.grad_scale : 1.0f;
 #pragma unroll
-    for (int k = 0; k < kRounds; k++) {
-        const int64_t at = base + k * 4 * kThreads;
-        const int live = live_at(at);
-        float m[4], v[4], r[4];
+    for (int i = 0; i < 4; i++) {
+        const float g = to_f32<G>(g4[i]) * gs;
+        m[i] = m[i] * s.beta1 + g * s.one_beta1;
+        v[i] = v[i] * s.beta2 + (g * g) * s.one_beta2;
+        float step;
         if constexpr (kBits == 32) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                m[i] = in[k].m[i];
-                v[i] = in[k].v[i];
-            }
+            step = m[i] / (sqrtf(v[i]) * s.inv_sqrt_c2 + s.eps);
         } else {
-            const auto m01 = __builtin_amdgcn_cvt_pk_f32_fp8((int)in[k].codes_m, false);
-            const auto m23 = __builtin_amdgcn_cvt_pk_f32_fp8((int)in[k].codes_m, true);
-            const auto r01 = __builtin_amdgcn_cvt_pk_f32_fp8((int)in[k].codes_r, false);
-            const auto r23 = __builtin_amdgcn_cvt_pk_f32_fp8((int)in[k].codes_r, true);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                m[i] = (i < 2 ? m01[i & 1] : m23[i & 1]) * in[k].scale_m;
-                const float q = (i < 2 ? r01[i & 1] : r23[i & 1]) * in[k].scale_r;
-                v[i] = q * q;
-            }
+            r[i] = root(v[i]);
+            step = m[i] * __builtin_amdgcn_rcpf(fmaf(r[i], s.inv_sqrt_c2, s.eps));
         }
-        typename Four<P>::type p;
+        p[i] = from_f32<P>(to_f32<P>(p[i]) * s.keep - s.rate * step);
+    }
+    store_four<P, kFull>((P*)t.param + at, live, p);
+    if constexpr (kBits == 32) {
+        store_four<float, kFull>((float*)t.exp_avg + at, live, Four<float>::type{m[0], m[1], m[2], m[3]});
+        store_four<float, kFull>((float*)t.exp_avg_sq + at, live, Four<float>::type{v[0], v[1], v[2], v[3]});
+    } else {
+        uint32_t most_m = 0, most_r = 0;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float g = to_f32<G>(in[k].g[i]) * gs;
-            m[i] = m[i] * s.beta1 + g * s.one_beta1;
-            v[i] = v[i] * s.beta2 + (g * g) * s.one_beta2;
-            float step;
-            if constexpr (kBits == 32) {
-                step = m[i] / (sqrtf(v[i]) * s.inv_sqrt_c2 + s.eps);
-            } else {
-                r[i] = root(v[i]);
-                step = m[i] * __builtin_amdgcn_rcpf(fmaf(r[i], s.inv_sqrt_c2, s.eps));
-            }
-            p[i] = from_f32<P>(to_f32<P>(in[k].p[i]) * s.keep - s.rate * step);
+            if (!kFull && i >= live) m[i] = r[i] = 0.0f;
+            most_m = max(most_m, size_bits(m[i]));
+            most_r = max(most_r, __float_as_uint(r[i]));
         }
-        store_four<P, kFull>((P*)t.param + at, live, p);
-        if constexpr (kBits == 32) {
-            store_four<float, kFull>((float*)t.exp_avg + at, live, Four<float>::type{m[0], m[1], m[2], m[3]});
-            store_four<float, kFull>((float*)t.exp_avg_sq + at, live, Four<float>::type{v[0], v[1], v[2], v[3]});
-        } else {
-            uint32_t most_m = 0, most_r = 0;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (!kFull && i >= live) m[i] = r[i] = 0.0f;
-                most_m = max(most_m, size_bits(m[i]));
-                most_r = max(most_r, __float_as_uint(r[i]));
-            }
-            const float scale_m = scale_of(wave_largest(most_m)), scale_r = scale_of(wave_largest(most_r));
-            const float inv_m = 1.0f / scale_m, inv_r = 1.0f / scale_r;
-            int codes_m = 0, codes_r = 0;
-            auto round = [&](auto place) {
-                constexpr int i = decltype(place)::value;
-                const uint32_t h = random_bits(t.place + at + i, s.seed);
-                const float a = __builtin_amdgcn_fmed3f(m[i] * inv_m, -448.0f, 448.0f);
-                const float b = __builtin_amdgcn_fmed3f(r[i] * inv_r, r[i] == 0.0f ? 0.0f : 0x1p-9f, 448.0f);
-                codes_m = __builtin_amdgcn_cvt_sr_fp8_f32(a, h << 16, codes_m, i);
-                codes_r = __builtin_amdgcn_cvt_sr_fp8_f32(b, h & 0xFFFF0000u, codes_r, i);
-            };
-            round(std::integral_constant<int, 0>{});
-            round(std::integral_constant<int, 1>{});
-            round(std::integral_constant<int, 2>{});
-            round(std::integral_constant<int, 3>{});
-            if (live > 0) {
-                ((uint32_t*)t.exp_avg)[at >> 2] = (uint32_t)codes_m;
-                ((uint32_t*)t.exp_avg_sq)[at >> 2] = (uint32_t)codes_r;
-                if ((threadIdx.x & 63) == 0) {
-                    t.exp_avg_scale[at / kBlock] = scale_m;
-                    t.exp_avg_sq_scale[at / kBlock] = scale_r;
-                }
+        const float scale_m = scale_of(wave_largest(most_m)), scale_r = scale_of(wave_largest(most_r));
+        const float inv_m = 1.0f / scale_m, inv_r = 1.0f / scale_r;
+        int codes_m = 0, codes_r = 0;
+        auto round = [&](auto place) {
+            constexpr int i = decltype(place)::value;
+            const uint32_t h = random_bits(t.place + at + i, s.seed);
+            const float a = __builtin_amdgcn_fmed3f(m[i] * inv_m, -448.0f, 448.0f);
+            const float b = __builtin_amdgcn_fmed3f(r[i] * inv_r, r[i] == 0.0f ? 0.0f : 0x1p-9f, 448.0f);
+            codes_m = __builtin_amdgcn_cvt_sr_fp8_f32(a, h << 16, codes_m, i);
+            codes_r = __builtin_amdgcn_cvt_sr_fp8_f32(b, h & 0xFFFF0000u, codes_r, i);
+        };
+        round(std::integral_constant<int, 0>{});
+        round(std::integral_constant<int, 1>{});
+        round(std::integral_constant<int, 2>{});
+        round(std::integral_constant<int, 3>{});
+        if (live > 0) {
+            ((int*)t.exp_avg)[at >> 2] = codes_m;
+            ((int*)t.exp_avg_sq)[at >> 2] = codes_r;
+            if ((threadIdx.x & 63) == 0) {
+                t.exp_avg_scale[at / kBlock] = scale_m;
+                t.exp_avg_sq_scale[at / kBlock] = scale_r;
             }
         }
     }
 }
 
 template <typename P, typename G, int kBits> __global__ void __launch_bounds__(kThreads) k_adamw(Table tab, Step s) {
-    int lo = 0, hi = tab.n;  // the tensor of this chunk: first[lo] <= blockIdx.x < first[lo + 1]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (tab.first[mid] <= (int64_t)blockIdx.x) lo = mid;
-        else hi = mid;
-    }
+    // the tensor of this chunk, the last whose first chunk is not past it: one load by as many lanes as there are
+    // tensors (the table is in host memory; a search would wait for it at every step)
+    const int lane = threadIdx.x & 63;
+    const uint64_t begun = __ballot(lane < tab.n && tab.first[lane < kTensors ? lane : 0] <= (int64_t)blockIdx.x);
+    const int lo = __popcll(begun) - 1;
     const hg_adamw_tensor& t = tab.t[lo];
     const int64_t chunk = (int64_t)blockIdx.x - tab.first[lo];
     if ((chunk + 1) * kChunk <= t.count) step_chunk<P, G, kBits, true>(t, chunk, s);
@@ -262,14 +245,13 @@ int hg_adamw_step(const hg_adamw_tensor* tensors, int64_t count, int param_type,
         for (; i < count && tab.n < kTensors; i++) {
             if (tensors[i].count == 0) continue;
             const int64_t c = (tensors[i].count + kChunk - 1) / kChunk;
-            if (chunks + c > (int64_t)1 << 23 && tab.n > 0) break;  // a grid holds under 2^32 threads
-            if (c > (int64_t)1 << 23) return (int)hipErrorInvalidValue;
+            if (c > kMaxChunks) return (int)hipErrorInvalidValue;
+            if (chunks + c > kMaxChunks) break;
             tab.t[tab.n] = tensors[i];
             tab.first[tab.n++] = chunks;
             chunks += c;
         }
         if (tab.n == 0) break;
-        tab.first[tab.n] = chunks;
         const int e = with_type(param_type, [&](auto tp) {
             using P = decltype(tp);
             return with_type(grad_type, [&](auto tg) {

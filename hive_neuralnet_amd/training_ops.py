@@ -60,14 +60,17 @@ def _check(err: int, what: str) -> None:
         raise RuntimeError(f"{what}: HIP error {err}")
 
 
+_current_device = torch._C._cuda_getDevice
+
+
 def _place(t, name: str) -> int:
     """The device of a GPU tensor on the current device."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise ValueError(f"{name} must be a GPU tensor")
-    dev = t.get_device()
-    if dev != torch.cuda.current_device():
-        raise ValueError(f"{name} is on {t.device}, the current device is {torch.cuda.current_device()}")
-    return dev
+    if isinstance(t, torch.Tensor) and t.is_cuda:
+        dev = t.get_device()
+        if dev == _current_device():
+            return dev
+        raise ValueError(f"{name} is on {t.device}, the current device is {_current_device()}")
+    raise ValueError(f"{name} must be a GPU tensor")
 
 
 def _float_tensor(t, name: str) -> int:
@@ -79,13 +82,12 @@ def _float_tensor(t, name: str) -> int:
 
 def _vector(t, name: str, n: int, dtype: torch.dtype, dev: int) -> int:
     """The address of a contiguous tensor of n elements, [n] or [n, 1], on `dev`."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.get_device() != dev:
+    if not isinstance(t, torch.Tensor) or t.get_device() != dev:
         raise ValueError(f"{name} must be a GPU tensor on device {dev}")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    shape = t.shape
-    if shape[0] != n if len(shape) == 1 else shape != (n, 1):
-        raise ValueError(f"{name} must have shape ({n},) or ({n}, 1), got {tuple(shape)}")
+    if t.shape != (n,) and t.shape != (n, 1):
+        raise ValueError(f"{name} must have shape ({n},) or ({n}, 1), got {tuple(t.shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return t.data_ptr()
@@ -315,8 +317,8 @@ class AdamWPlan:
         kind = next((g.dtype for g in grads if g is not None), torch.float32)
         if kind not in TYPES:
             raise ValueError(f"gradients must be float32, float16 or bfloat16, got {kind}")
-        if dev != torch.cuda.current_device():
-            raise ValueError(f"the parameters are on device {dev}, the current one is {torch.cuda.current_device()}")
+        if dev != _current_device():
+            raise ValueError(f"the parameters are on device {dev}, the current one is {_current_device()}")
         missing = False
         for g, shape in zip(grads, self._shapes):
             if g is None:
