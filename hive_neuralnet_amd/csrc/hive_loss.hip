@@ -362,15 +362,25 @@ __device__ __forceinline__ Cut cut_of(const Batch& a, int64_t b, int64_t begin, 
     return c;
 }
 
-// {top, total, mass, cross} of two parts of one list as of one
-__device__ __forceinline__ Slice join(const Slice& p, const Slice& q) {
-    Slice r;
-    r.top = fmaxf(p.top, q.top);
-    const float top = r.top == -INFINITY ? 0.0f : r.top, dp = p.top - top, dq = q.top - top;
-    r.total = p.total * exp_(dp) + q.total * exp_(dq);
-    r.mass = p.mass + q.mass;
-    r.cross = plus(p.cross, p.mass, dp) + plus(q.cross, q.mass, dq);
-    return r;
+// the n slices of a list as one, by a wave: a lane takes every 64th, all bring theirs to the largest logit
+__device__ __forceinline__ Slice join(const Slice* slices, int n) {
+    const int lane = threadIdx.x & 63;
+    float top = -INFINITY;
+    for (int i = lane; i < n; i += 64) top = fmaxf(top, slices[i].top);
+    top = group_join<64>(top, [](float p, float q) { return fmaxf(p, q); });
+    const float shift = top == -INFINITY ? 0.0f : top;
+    Slice s = {top, 0.0f, 0.0f, 0.0f};
+    for (int i = lane; i < n; i += 64) {
+        const Slice q = slices[i];
+        const float down = q.top - shift;
+        s.total = fmaf(q.total, exp_(down), s.total);
+        s.mass += q.mass;
+        s.cross += plus(q.cross, q.mass, down);
+    }
+    s.total = group_sum<64>(s.total);
+    s.mass = group_sum<64>(s.mass);
+    s.cross = group_sum<64>(s.cross);
+    return s;
 }
 
 template <typename T, typename P>
@@ -448,8 +458,7 @@ k_loss_gradient(Batch a, int64_t first, int64_t slice, const Slice* __restrict__
     const int64_t b = first + blockIdx.y;
     const Before before = begin_of(a, b);
     const Cut cut = cut_of(a, b, before.moves, slice);
-    Slice s = slices[b * gridDim.x];
-    for (int i = 1; i < (int)gridDim.x; i++) s = join(s, slices[b * gridDim.x + i]);
+    const Slice s = join(slices + b * gridDim.x, gridDim.x);
     const Scalars own = scalars_of<T>(a, b);
     const float share = own.w / before.policy;
     const bool used = own.w != 0.0f && s.total != 0.0f;

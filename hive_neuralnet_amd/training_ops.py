@@ -295,7 +295,9 @@ class AdamWPlan:
             if state_bits == 8:
                 self._table[k + "_scale"] = np.uint64(self.state[k + "_scale"].data_ptr()) + \
                     np.uint64(4) * (at // np.uint64(ADAMW_BLOCK))
-        self._counts = np.array([p.numel() for p in params], dtype=np.int64)
+        self._counts = [p.numel() for p in params]
+        self._table["count"] = self._counts
+        self._partial = False  # whether the last step left a parameter out
         self._table["place"] = self.places
         self._shapes = [p.shape for p in params]
         self._grad, self._count = self._table["grad"], self._table["count"]
@@ -305,12 +307,12 @@ class AdamWPlan:
 
     def step(self, grads, step: int, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
              weight_decay: float = 0.01, grad_scale: torch.Tensor | None = None, seed: int = 0) -> None:
-        """Step number `step` (the first is 1) of every parameter from `grads`
-        (one type, contiguous, the parameters' shapes; None leaves its parameter
-        and moments as they are), in place.  grad_scale:
-        a float32 tensor of one value that multiplies the gradients (1 / the
-        loss scale, a clipping factor).  seed: of the 8-bit moments' rounding;
-        give each step another one."""
+        """Step number `step` (the first is 1) of every parameter, in place, from
+        the list `grads` (one type, contiguous, the parameters' shapes; None
+        leaves its parameter and moments as they are).  grad_scale: a float32
+        tensor of one value that multiplies the gradients (1 / the loss scale, a
+        clipping factor).  seed: of the 8-bit moments' rounding; give each step
+        another one."""
         if len(grads) != len(self.params):
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
         dev = self._device
@@ -319,11 +321,13 @@ class AdamWPlan:
             raise ValueError(f"gradients must be float32, float16 or bfloat16, got {kind}")
         if dev != _current_device():
             raise ValueError(f"the parameters are on device {dev}, the current one is {_current_device()}")
-        missing = False
+        ptrs = []
         for g, shape in zip(grads, self._shapes):
             if g is None:
-                missing = True
-            elif g.dtype != kind or g.shape != shape or g.get_device() != dev or not g.is_contiguous():
+                ptrs.append(0)
+            elif g.dtype is kind and g.shape == shape and g.get_device() == dev and g.is_contiguous():
+                ptrs.append(g.data_ptr())
+            else:
                 raise ValueError(f"a gradient must be a contiguous {kind} tensor {tuple(shape)} on device {dev}, got "
                                  f"{g.dtype} {tuple(g.shape)} on {g.device}")
         if step < 1:
@@ -337,12 +341,11 @@ class AdamWPlan:
             if grad_scale.numel() != 1 or grad_scale.dtype != torch.float32 or grad_scale.get_device() != dev:
                 raise ValueError(f"grad_scale must be one float32 value on device {dev}")
             scale = grad_scale.data_ptr()
-        if missing:
-            self._grad[:] = [0 if g is None else g.data_ptr() for g in grads]
+        self._grad[:] = ptrs
+        missing = 0 in ptrs and any(g is None for g in grads)
+        if missing or self._partial:
             self._count[:] = [0 if g is None else n for g, n in zip(grads, self._counts)]
-        else:
-            self._grad[:] = [g.data_ptr() for g in grads]
-            self._count[:] = self._counts
+            self._partial = missing
         _check(self._lib.hg_adamw_step(
             self._table_ptr, len(grads), self._type, TYPES[kind], self.state_bits, step, lr, betas[0], betas[1], eps,
             weight_decay, scale, seed & 0xFFFFFFFF, _raw_stream(dev)), "adamw_step")
