@@ -23,10 +23,10 @@
 // a wave: 7 us against 2.8 for 20,546 elements, 196 against 174 for 64 M in 8
 // bits, the same for 64 M in 32).
 //
-// Bound by memory in 32 bits: 201 M float weights with bf16 gradients 985 us,
+// Bound by memory in 32 bits: 201 M float weights with bf16 gradients 980 us,
 // 5.3 TB/s of what has to move, the rate of a large copy (one element's loads
 // at a time: 1,655 us).  In 8 bits the VALU comes near it, 60 operations an
-// element: 144 M float weights 405 us, 5.7 TB/s, in bf16 290 us, 5.0 TB/s, where
+// element: 144 M float weights 405 us, 5.7 TB/s, in bf16 286 us, 5.1 TB/s, where
 // codes made by a divide, a correctly rounded root and float arithmetic took
 // 130 and 571 us.
 #include <cmath>
@@ -211,7 +211,7 @@ template <typename P, typename G, int kBits> __global__ void __launch_bounds__(k
 }
 
 bool bad_tensor(const hg_adamw_tensor& t, int bits) {
-    if (t.count < 0) return true;
+    if (t.count < 0 || t.count > kMaxChunks * kChunk) return true;
     if (t.count == 0) return false;
     if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq) return true;
     return bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale || t.place % kBlock != 0 ||
@@ -250,7 +250,6 @@ int hg_adamw_step(const hg_adamw_tensor* tensors, int64_t count, int param_type,
         for (; i < count && tab.n < kTensors; i++) {
             if (tensors[i].count == 0) continue;
             const int64_t c = (tensors[i].count + kChunk - 1) / kChunk;
-            if (c > kMaxChunks) return (int)hipErrorInvalidValue;
             if (chunks + c > kMaxChunks) break;
             tab.t[tab.n] = tensors[i];
             tab.first[tab.n++] = chunks;

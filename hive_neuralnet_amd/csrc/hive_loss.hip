@@ -27,11 +27,13 @@
 // Measured (MI355X): 16 positions 6 us, one launch; 2,048 of 60 moves on
 // average 10 us, of which the second launch, the sum of the blocks' shares,
 // takes 3 (the last block adding them: 17 in all, as every block's write-back
-// for it has to come first); 65,521 of 85 in bf16 28 us: the sums before them 9 in two launches
-// (46 us in all where every block looked back itself), the lists 17, of which
+// for it has to come first); 65,521 of 85 in bf16 28 us: the sums before them
+// 8 in two launches (46 us in all where every block looked back itself), the
+// lists 18, of which
 // the VALU is busy 12 (450 instructions a wave; a third of the slots it works
-// on hold a move); 192 x 85,834 bf16 logits 51 us: 22 for the slices, 4.5
-// TB/s, and 23 for the gradient, which finds its second read in the cache.
+// on hold a move); 192 x 85,834 bf16 logits 47 us: 22 for the slices, 4.5
+// TB/s, and 23 for the gradient, which finds its second read in the cache (26
+// where every lane joined the list's 21 slices itself).
 #include "hive_train.hpp"
 
 namespace {
@@ -506,7 +508,7 @@ __global__ void __launch_bounds__(1024) k_loss_join(Batch a, int64_t parts) {
 
 constexpr int64_t kShort = 16 * kHeld, kMiddle = 64 * kHeld;  // widths whose lists 16 lanes, a wave hold
 constexpr int64_t kSlice = 4096;                                 // moves of a slice
-constexpr int64_t kMaxBatch = (int64_t)1 << 31;
+constexpr int64_t kMaxBatch = ((int64_t)1 << 26) - 4;  // a wave a position: a grid holds under 2^32 threads
 constexpr int64_t kGridRows = 32768;  // positions of a launch over slices: a grid has 65,535 rows at most
 
 inline int64_t ranges_of(int64_t B) { return B <= kInline ? 0 : (B + kRange - 1) / kRange; }

@@ -543,10 +543,10 @@ template <typename Sh> int64_t backward_blocks(int64_t rows) {
 }
 constexpr int64_t kWideParts = 64;  // row ranges of k_norm_dw_wide
 
-// sizes a launch can hold, strides that keep rows apart, a weight type
+// sizes that a launch can hold (k_norm_join: a grid holds under 2^32 threads), types
 bool bad_sizes(int64_t rows, int64_t cols, int x_type, int w_type) {
     return rows < 0 || cols < 0 || !is_type(x_type) || !is_type(w_type) || rows > (int64_t)1 << 31 ||
-           cols > (int64_t)1 << 31;
+           cols > (int64_t)1 << 25;
 }
 
 }  // namespace

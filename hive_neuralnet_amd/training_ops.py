@@ -6,7 +6,8 @@
 
 They work in float32 inside, on float32, float16 or bfloat16 tensors, on
 torch.cuda.current_stream() without synchronising it, and raise ValueError
-for what they do not serve before anything is launched.  training.py builds
+for what they do not serve before anything is launched (RuntimeError for sizes
+past a launch's bounds, which include/hive_gpu.h names).  training.py builds
 autograd functions, an optimizer and a training step of HiveFNN on them.
 """
 from __future__ import annotations

@@ -514,7 +514,7 @@ int hg_mcts_wave_root_slots(const hg_tree* tree, const uint8_t* root_states, con
  * y = (a - mean) rstd weight + bias with rstd = 1 / sqrt(var + eps), var the
  * biased variance.  Row r of x begins at x + r * x_stride elements; y[rows][cols]
  * has x's type, weight / bias (NULL = 1 / 0) w_type, mean[rows] and rstd[rows]
- * are float. */
+ * are float.  rows <= 2^31 (2^21 of more than 16,384 values), cols <= 2^25. */
 int hg_layer_norm_forward(const void* x, int x_type, int64_t rows, int64_t cols, int64_t x_stride,
                           const void* weight, const void* bias, int w_type, float eps, int sigmoid, void* y,
                           float* mean, float* rstd, void* stream);
@@ -544,6 +544,7 @@ int hg_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int
  * Positions of weight 0, without moves, or whose logits are all -inf add
  * nothing and have gradients of 0; a sum of weights of 0 counts as 1.  Logits
  * past the positions' own have gradients of 0, moves past N are left out.
+ * B <= 2^26 - 4, width <= 2^31.
  * workspace: hg_policy_value_loss_workspace(B, width) bytes, 16-byte aligned. */
 int64_t hg_policy_value_loss_workspace(int64_t B, int64_t width);
 int hg_policy_value_loss(const void* logits, int type, int64_t N, const void* values, const int64_t* num_actions,
@@ -561,7 +562,8 @@ int hg_policy_value_loss(const void* logits, int type, int64_t N, const void* va
  * in whole blocks of HG_ADAMW_BLOCK elements, 4-byte aligned, each block with a
  * float scale: exp_avg = code * scale, exp_avg_sq = (code * scale)^2; new values
  * are rounded to a neighbouring code at random, by bits that depend on `seed`
- * and `place` + the element's index alone (place: a multiple of the block). */
+ * and `place` + the element's index alone (place: a multiple of the block).
+ * A tensor has under 2^34 elements (count <= 2^34 - 1024). */
 #define HG_ADAMW_BLOCK 256
 typedef struct hg_adamw_tensor {
     void* param;

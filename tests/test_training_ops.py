@@ -99,3 +99,22 @@ def test_adamw_refusals():
                 dict(exp_avg_sq_scale=None), dict(place=100), dict(exp_avg=p + 1), dict(bits=32, param=None)):
         assert step(**bad) == INVALID, bad
     assert step(count=0) == 0
+
+
+@needs_library
+def test_sizes_past_a_launch_are_refused():
+    """Before anything is launched: a grid of 2^32 threads, also where only a later launch or tensor has one."""
+    lib = hive_gpu.load_library()
+    buf = (ctypes.c_float * 64)()
+    p = (ctypes.addressof(buf) + 15) & ~15
+    for width in (4, 512, 5000):
+        assert lib.hg_policy_value_loss(p, 0, 4, p, p, p, 0, width, p, p, p, (1 << 26) - 3, 1.0, 1.0, p, p, p, p,
+                                        None) == INVALID, width
+    cols = (1 << 25) + 1
+    assert lib.hg_layer_norm_forward(p, 0, 1, cols, cols, p, p, 0, 1e-5, 0, p, p, p, None) == INVALID
+    assert lib.hg_layer_norm_backward(p, cols, p, 0, 1, cols, cols, p, p, p, 0, 0, p, p, None, p, None) == INVALID
+    assert lib.hg_layer_norm_forward(p, 0, (1 << 21) + 1, 20000, 20000, p, p, 0, 1e-5, 0, p, p, p, None) == INVALID
+    two = (training_ops.HgAdamwTensor * 2)()
+    two[0] = training_ops.HgAdamwTensor(p, p, p, p, p, p, 4, 0)
+    two[1] = training_ops.HgAdamwTensor(p, p, p, p, p, p, (1 << 34) - 1023, 256)
+    assert lib.hg_adamw_step(two, 2, 0, 0, 8, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, None, 0, None) == INVALID
