@@ -16,35 +16,41 @@
 // Where a position's logits begin is a sum over the positions before it.
 // Every block adds up what it needs itself: the counts before its first
 // position and all the weights, up to kInline positions read in full, past
-// them the sums of ranges of kRange positions that a first launch leaves.
+// them the sums of ranges of kRange positions that a first launch leaves.  Past
+// kLookBack positions a second launch leaves each position's begin instead
+// (10,000 positions of 2 moves: 13.2 us with it, 10.7 without; 20,000: 13.5,
+// 12.2; 40,000: 15.4, 16.9).
 //
 // Lists of up to 256 moves (16 lanes a position) and up to 1,024 (a wave) are
 // read once and held in registers.  Longer ones are cut into slices, a block
 // each, so that few positions fill the card too: one launch leaves each
 // slice's largest logit and sums, the next joins a position's slices and
-// writes the gradient from a second read.
+// writes the gradient from a second read.  All loads of a list, a slice's
+// targets and the counts before it go out before any of them is waited for.
 //
-// Measured (MI355X): 16 positions 6 us, one launch; 2,048 of 60 moves on
-// average 10 us, of which the second launch, the sum of the blocks' shares,
+// Measured (MI355X): 16 positions 5 us, one launch; 2,048 of 60 moves on
+// average 9 us, of which the second launch, the sum of the blocks' shares,
 // takes 3 (the last block adding them: 17 in all, as every block's write-back
-// for it has to come first); 65,521 of 85 in bf16 28 us: the sums before them
-// 8 in two launches (46 us in all where every block looked back itself), the
-// lists 18, of which
-// the VALU is busy 12 (450 instructions a wave; a third of the slots it works
-// on hold a move); 192 x 85,834 bf16 logits 47 us: 22 for the slices, 4.5
+// for it has to come first); 65,521 of 85 in bf16 23.5 us: the sums before them
+// 6 in two launches, the lists 15 (one load after the other, as conversions
+// inside their branches make them: 18), of which the VALU is busy 12 (a third
+// of the slots it works on hold a move; lists sorted by length among a block's
+// waves: no gain); 192 x 85,834 bf16 logits 47 us: 22 for the slices, 4.5
 // TB/s, and 23 for the gradient, which finds its second read in the cache (26
-// where every lane joined the list's 21 slices itself).
+// where every lane joined the list's 21 slices itself; slices of 8,192: 49 us,
+// of 2,048: 54).
 #include "hive_train.hpp"
 
 namespace {
 
 using namespace ht;
 
-constexpr int64_t kInline = 4096, kRange = 1024;
+constexpr int64_t kInline = 4096, kRange = 256, kLookBack = 24 * 1024;
 constexpr int kThreads = 256;
 constexpr int kHeld = 16;  // logits of a position a lane holds
+constexpr int64_t kSlice = 4096;  // moves of a slice of a long list
 
-struct Range {  // of kRange positions
+struct Range {
     int64_t moves;
     float policy, value;
 };
@@ -58,7 +64,8 @@ struct Batch {
     const float *pw, *vt, *vw;
     int64_t N, width, B;
     float value_coef, loss_scale;
-    const Range* ranges;  // nullptr: up to kInline positions
+    Range* ranges;        // of `range` positions each; nullptr: up to kInline positions
+    int64_t range;
     int64_t* begin;       // [B] where a position's logits begin, and the weights' sums (1 where they are 0);
     float* sums;          // nullptr: every block looks back itself
     float2* row_loss;     // [blocks or B]: shares of the policy loss and of the value loss
@@ -69,10 +76,23 @@ struct Batch {
 __device__ __forceinline__ int64_t clamp_count(int64_t n, int64_t width) {
     return n < 0 ? 0 : (n > width ? width : n);
 }
-template <typename V> __device__ __forceinline__ V wave_sum(V v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
+// the sum over a wave's lanes, by the moves of group_join, 32 bits at a time
+template <int kControl> __device__ __forceinline__ int64_t dpp(int64_t v) {
+    const uint32_t lo = __builtin_amdgcn_mov_dpp((int)v, kControl, 0xF, 0xF, true);
+    const uint32_t hi = __builtin_amdgcn_mov_dpp((int)(v >> 32), kControl, 0xF, 0xF, true);
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ int64_t wave_sum(int64_t v) {
+    v += dpp<0xB1>(v);
+    v += dpp<0x4E>(v);
+    v += dpp<0x141>(v);
+    v += dpp<0x140>(v);
+    auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+    auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
+    v = (int64_t)((uint64_t)hi[0] << 32 | lo[0]) + (int64_t)((uint64_t)hi[1] << 32 | lo[1]);
+    lo = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+    hi = __builtin_amdgcn_permlane32_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
+    return (int64_t)((uint64_t)hi[0] << 32 | lo[0]) + (int64_t)((uint64_t)hi[1] << 32 | lo[1]);
 }
 
 // What a block needs of the positions before its first one and of all.
@@ -83,24 +103,40 @@ struct Before {
 template <int threads> __device__ __forceinline__ Before look_back(const Batch& a, int64_t first) {
     __shared__ int64_t lds_moves[threads / 64];
     __shared__ float lds_policy[threads / 64], lds_value[threads / 64];
-    int64_t moves = 0, from = 0;
+    int64_t moves = 0;
     float policy = 0.0f, value = 0.0f;
     if (a.ranges) {
-        const int64_t all = (a.B + kRange - 1) / kRange, mine = first / kRange;
-        from = mine * kRange;
+        const int64_t all = (a.B + a.range - 1) / a.range, mine = first / a.range;
         for (int64_t i = threadIdx.x; i < all; i += threads) {
             const Range r = a.ranges[i];
             moves += i < mine ? r.moves : 0;
             policy += r.policy;
             value += r.value;
         }
+        for (int64_t i = mine * a.range + threadIdx.x; i < first; i += threads)
+            moves += clamp_count(a.num_actions[i], a.width);
     } else {
-        for (int64_t i = threadIdx.x; i < a.B; i += threads) {
-            policy += a.pw[i];
-            value += a.vw[i];
+        constexpr int n = 4;  // positions of a thread whose loads go out together
+        const int last = (int)a.B - 1;
+        for (int i = threadIdx.x; i <= last; i += n * threads) {
+            int64_t c[n];
+            float p[n], v[n];
+#pragma unroll
+            for (int k = 0; k < n; k++) {
+                const int at = min(i + k * threads, last);
+                c[k] = a.num_actions[at];
+                p[k] = a.pw[at];
+                v[k] = a.vw[at];
+            }
+#pragma unroll
+            for (int k = 0; k < n; k++) {
+                const int at = i + k * threads;
+                moves += at < first ? clamp_count(c[k], a.width) : 0;
+                policy += at <= last ? p[k] : 0.0f;
+                value += at <= last ? v[k] : 0.0f;
+            }
         }
     }
-    for (int64_t i = from + threadIdx.x; i < first; i += threads) moves += clamp_count(a.num_actions[i], a.width);
     moves = wave_sum(moves);
     policy = group_sum<64>(policy);
     value = group_sum<64>(value);
@@ -122,22 +158,17 @@ template <int threads> __device__ __forceinline__ Before look_back(const Batch& 
     return r;
 }
 
-// a block a range of kRange positions
-__global__ void __launch_bounds__(kThreads)
-k_loss_ranges(const int64_t* __restrict__ num_actions, int64_t B, int64_t width, const float* __restrict__ pw,
-              const float* __restrict__ vw, Range* __restrict__ ranges) {
-    __shared__ int64_t lds_moves[kThreads / 64];
-    __shared__ float lds[2][kThreads / 64];
+// the sums of a range, a block each
+__global__ void __launch_bounds__(kRange) k_loss_ranges(Batch a) {
+    __shared__ int64_t lds_moves[kRange / 64];
+    __shared__ float lds[2][kRange / 64];
     int64_t moves = 0;
     float policy = 0.0f, value = 0.0f;
-#pragma unroll
-    for (int k = 0; k < kRange / kThreads; k++) {
-        const int64_t i = (int64_t)blockIdx.x * kRange + k * kThreads + threadIdx.x;
-        if (i < B) {
-            moves += clamp_count(num_actions[i], width);
-            policy += pw[i];
-            value += vw[i];
-        }
+    const int64_t first = (int64_t)blockIdx.x * a.range, end = min(a.B, first + a.range);
+    for (int64_t i = first + threadIdx.x; i < end; i += kRange) {
+        moves += clamp_count(a.num_actions[i], a.width);
+        policy += a.pw[i];
+        value += a.vw[i];
     }
     moves = wave_sum(moves);
     policy = group_sum<64>(policy);
@@ -152,31 +183,38 @@ k_loss_ranges(const int64_t* __restrict__ num_actions, int64_t B, int64_t width,
     if (threadIdx.x != 0) return;
     Range r = {0, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < kThreads / 64; i++) {
+    for (int i = 0; i < kRange / 64; i++) {
         r.moves += lds_moves[i];
         r.policy += lds[0][i];
         r.value += lds[1][i];
     }
-    ranges[blockIdx.x] = r;
+    a.ranges[blockIdx.x] = r;
 }
 
-// begin and sums, a range of kRange positions a block
+// begin and sums, a range a block
 __global__ void __launch_bounds__(kRange) k_loss_begins(Batch a) {
-    __shared__ int64_t lds[kRange / 64];
-    const int64_t first = (int64_t)blockIdx.x * kRange, b = first + threadIdx.x;
+    __shared__ int64_t lds[2][kRange / 64];
+    const int64_t first = (int64_t)blockIdx.x * a.range, end = min(a.B, first + a.range);
     const Before before = look_back<kRange>(a, first);
-    const int lane = threadIdx.x & 63;
-    const int64_t n = b < a.B ? clamp_count(a.num_actions[b], a.width) : 0;
-    int64_t upto = n;
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t v = __shfl_up(upto, o, 64);
-        upto += lane >= o ? v : 0;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t begin = before.moves;
+    int turn = 0;
+    for (int64_t base = first; base < end; base += kRange, turn ^= 1) {
+        const int64_t b = base + threadIdx.x, n = b < end ? clamp_count(a.num_actions[b], a.width) : 0;
+        int64_t upto = n;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int64_t v = __shfl_up(upto, o, 64);
+            upto += lane >= o ? v : 0;
+        }
+        if (lane == 63) lds[turn][wave] = upto;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kRange / 64; i++) upto += i < wave ? lds[turn][i] : 0;
+        if (b < end) a.begin[b] = begin + upto - n;
+#pragma unroll
+        for (int i = 0; i < kRange / 64; i++) begin += lds[turn][i];
     }
-    if (lane == 63) lds[threadIdx.x >> 6] = upto;
-    __syncthreads();
-    for (int i = 0; i < (int)(threadIdx.x >> 6); i++) upto += lds[i];
-    if (b < a.B) a.begin[b] = before.moves + upto - n;
-    if (b == 0) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
         a.sums[0] = before.policy;
         a.sums[1] = before.value;
     }
@@ -198,19 +236,20 @@ __device__ __forceinline__ void load_flat(const T* p, int64_t at, int64_t all, f
 }
 
 // what a position holds besides its list, read before the list is waited for
-struct Scalars {
-    float w, u, off;  // policy weight, value weight, value less its target
+template <typename T> struct Scalars {
+    float w, u, target;  // policy weight, value weight, the value's target
+    T value;
 };
-template <typename T> __device__ __forceinline__ Scalars scalars_of(const Batch& a, int64_t b) {
-    return Scalars{a.pw[b], a.vw[b], to_f32(((const T*)a.values)[b]) - a.vt[b]};
+template <typename T> __device__ __forceinline__ Scalars<T> scalars_of(const Batch& a, int64_t b) {
+    return Scalars<T>{a.pw[b], a.vw[b], a.vt[b], ((const T*)a.values)[b]};
 }
 // the value loss of position b, and its gradient
 template <typename T>
-__device__ __forceinline__ float value_loss(const Batch& a, int64_t b, const Scalars& s, float weights) {
-    const float u = s.u / weights;
+__device__ __forceinline__ float value_loss(const Batch& a, int64_t b, const Scalars<T>& s, float weights) {
+    const float u = s.u / weights, off = to_f32(s.value) - s.target;
     const bool used = u != 0.0f;
-    ((T*)a.dvalues)[b] = from_f32<T>(used ? 2.0f * a.value_coef * u * s.off * a.loss_scale : 0.0f);
-    return used ? u * s.off * s.off : 0.0f;
+    ((T*)a.dvalues)[b] = from_f32<T>(used ? 2.0f * a.value_coef * u * off * a.loss_scale : 0.0f);
+    return used ? u * off * off : 0.0f;
 }
 __device__ __forceinline__ void store_losses(const Batch& a, float policy, float value) {
     a.losses[0] = policy + a.value_coef * value;
@@ -235,15 +274,14 @@ __global__ void __launch_bounds__(kThreads) k_loss_held(Batch a) {
     int64_t lo;
     int count = 0;
     float policy_sum, value_sum, policy = 0.0f, value = 0.0f;
-    Scalars own = {};
-    if (b < a.B) own = scalars_of<T>(a, b);
+    const int64_t here = min(b, a.B - 1);
+    const int64_t listed = a.num_actions[here];
+    const Scalars<T> own = scalars_of<T>(a, here);
     if (a.begin) {
+        lo = a.begin[here];
         policy_sum = a.sums[0];
         value_sum = a.sums[1];
-        if (b < a.B) {
-            lo = a.begin[b];
-            count = (int)clamp_count(a.num_actions[b], a.width);
-        }
+        count = (int)clamp_count(listed, a.width);
     } else {
         const Before before = look_back<kThreads>(a, first);
         policy_sum = before.policy;
@@ -262,19 +300,43 @@ __global__ void __launch_bounds__(kThreads) k_loss_held(Batch a) {
         // a position of weight 0 is taken as one without moves, but for its gradient's zeros
         const float share = own.w / policy_sum;
         const int live = own.w != 0.0f ? count : 0;
-        float x[vecs][n], pi[vecs][n];
-#pragma unroll
-        for (int k = 0; k < vecs; k++) {
-            const int c = (lane + k * kLanes) * n;
-            if (c < live) {
-                load_flat<T, n>((const T*)a.logits, lo + c, a.N, x[k]);
-                load_flat<P, n>((const P*)a.targets, b * a.width + c, a.B * a.width, pi[k]);
-            }
-        }
         // a step that no list of the wave reaches is passed by
         bool reached[vecs];
 #pragma unroll
         for (int k = 0; k < vecs; k++) reached[k] = __any(k * kLanes * n < live);
+        float x[vecs][n], pi[vecs][n];
+        const int64_t row = b * a.width;
+        const int most = live > 0 ? (live + n - 1) / n * n : n;
+        if (__all(lo + most <= a.N && row + most <= a.B * a.width)) {
+            // no vector passes the arrays' ends: all loads at once, a lane past its list's end at the list's start
+            typedef T tvec __attribute__((ext_vector_type(n), aligned(sizeof(T))));
+            typedef P pvec __attribute__((ext_vector_type(n), aligned(sizeof(P))));
+            tvec raw[vecs];
+            pvec raw_pi[vecs];
+#pragma unroll
+            for (int k = 0; k < vecs; k++) {
+                if (!reached[k]) break;
+                const int c = (lane + k * kLanes) * n, at = c < live ? c : 0;
+                raw[k] = *(const tvec*)((const T*)a.logits + lo + at);
+                raw_pi[k] = *(const pvec*)((const P*)a.targets + row + at);
+            }
+#pragma unroll
+            for (int k = 0; k < vecs; k++)
+#pragma unroll
+                for (int i = 0; i < n; i++) {
+                    x[k][i] = to_f32<T>(raw[k][i]);
+                    pi[k][i] = to_f32<P>(raw_pi[k][i]);
+                }
+        } else {
+#pragma unroll
+            for (int k = 0; k < vecs; k++) {
+                const int c = (lane + k * kLanes) * n;
+                if (c < live) {
+                    load_flat<T, n>((const T*)a.logits, lo + c, a.N, x[k]);
+                    load_flat<P, n>((const P*)a.targets, row + c, a.B * a.width, pi[k]);
+                }
+            }
+        }
         float top = -INFINITY;
 #pragma unroll
         for (int k = 0; k < vecs; k++) {
@@ -351,18 +413,36 @@ __global__ void __launch_bounds__(kThreads) k_loss_held(Batch a) {
 __device__ __forceinline__ Before begin_of(const Batch& a, int64_t b) {
     return a.begin ? Before{a.begin[b], a.sums[0], a.sums[1]} : look_back<kThreads>(a, b);
 }
-// the slice of a position: elements [from, to) of its `count` from logit lo on
+// the slice of a position: `len` elements from element `from` of its list of `count`
 struct Cut {
-    int64_t lo, count, from, to;
+    int64_t count, from;
+    int len;
 };
-__device__ __forceinline__ Cut cut_of(const Batch& a, int64_t b, int64_t begin, int64_t slice) {
-    Cut c;
-    c.lo = min(a.N, begin);
-    c.count = min(clamp_count(a.num_actions[b], a.width), a.N - c.lo);
-    c.from = min(c.count, (int64_t)blockIdx.x * slice);
-    c.to = min(c.count, c.from + slice);
-    return c;
+__device__ __forceinline__ Cut cut_of(int64_t count, int64_t slice) {
+    const int64_t from = min(count, (int64_t)blockIdx.x * slice);
+    return Cut{count, from, (int)min(slice, count - from)};
 }
+
+// A thread's share of a piece of kSlice elements, kSlice / kThreads of them in
+// vectors of n, of an array of `len` (past its end: none), as they are read.
+template <typename E, int n> struct Piece {
+    static constexpr int vecs = (int)kSlice / kThreads / n;
+    typedef E vec __attribute__((ext_vector_type(n), aligned(sizeof(E))));
+    vec v[vecs];
+    __device__ __forceinline__ void load(const E* p, int from, int len, E none) {
+#pragma unroll
+        for (int k = 0; k < vecs; k++) {
+            const int c = from + (threadIdx.x + k * kThreads) * n;
+            if (c + n <= len) {
+                v[k] = *(const vec*)(p + c);
+            } else {
+                skipped();
+#pragma unroll
+                for (int i = 0; i < n; i++) v[k][i] = c + i < len ? p[c + i] : none;
+            }
+        }
+    }
+};
 
 // the n slices of a list as one, by a wave: a lane takes every 64th, all bring theirs to the largest logit
 __device__ __forceinline__ Slice join(const Slice* slices, int n) {
@@ -390,24 +470,27 @@ __global__ void __launch_bounds__(kThreads)
 k_loss_slices(Batch a, int64_t first, int64_t slice, Slice* __restrict__ slices) {
     constexpr int n = Vector<T>::n;
     const int64_t b = first + blockIdx.y;
-    const Before before = begin_of(a, b);
-    const Cut cut = cut_of(a, b, before.moves, slice);
-    const int64_t at = cut.lo, row = b * a.width, all = a.B * a.width;
-    // one pass: each thread's largest logit so far, its sums brought to a new one as it comes
+    // where the logits begin takes a look at the positions before: the first targets are read meanwhile
+    Cut cut = cut_of(min(clamp_count(a.num_actions[b], a.width), a.N), slice);
+    const P* targets = (const P*)a.targets + b * a.width + cut.from;
+    Piece<P, n> pi;
+    pi.load(targets, 0, cut.len, (P)0.0f);
+    const int64_t lo = min(a.N, begin_of(a, b).moves);
+    cut = cut_of(min(cut.count, a.N - lo), slice);
+    const T* logits = (const T*)a.logits + lo + cut.from;
+    const int len = cut.len;
+    // one pass: each thread's largest logit so far (fmaxf passes a NaN by: it comes through the sums), its sums brought
+    // to a new one as it comes
     float top = -INFINITY, total = 0.0f, mass = 0.0f, cross = 0.0f;
-    for (int64_t c = cut.from + threadIdx.x * n; c < cut.to; c += kThreads * n) {
-        float x[n], pi[n];
-        load_flat<T, n>((const T*)a.logits, at + c, a.N, x);
-        load_flat<P, n>((const P*)a.targets, row + c, all, pi);
+    for (int at = 0; at < len; at += kSlice) {
+        Piece<T, n> x;
+        if (at) pi.load(targets, at, len, (P)0.0f);
+        x.load(logits, at, len, from_f32<T>(-INFINITY));
         float most = top;
 #pragma unroll
-        for (int i = 0; i < n; i++) {
-            if (c + i >= cut.to) {
-                x[i] = -INFINITY;
-                pi[i] = 0.0f;
-            }
-            most = fmaxf(most, x[i]);  // passes a NaN by: it comes through the sums
-        }
+        for (int k = 0; k < x.vecs; k++)
+#pragma unroll
+            for (int i = 0; i < n; i++) most = fmaxf(most, to_f32<T>(x.v[k][i]));
         if (most != top) {
             total *= exp_(top - most);  // 0 * 0 where this is the first logit above -inf
             cross = plus(cross, mass, top - most);
@@ -415,12 +498,15 @@ k_loss_slices(Batch a, int64_t first, int64_t slice, Slice* __restrict__ slices)
         }
         const float shift = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-        for (int i = 0; i < n; i++) {
-            const float z = x[i] - shift;
-            total += exp_(z);
-            mass += pi[i];
-            cross = plus(cross, pi[i], z);
-        }
+        for (int k = 0; k < x.vecs; k++)
+#pragma unroll
+            for (int i = 0; i < n; i++) {
+                const float z = to_f32<T>(x.v[k][i]) - shift;
+                const float p = at + (threadIdx.x + k * kThreads) * n + i < len ? to_f32<P>(pi.v[k][i]) : 0.0f;
+                total += exp_(z);
+                mass += p;
+                cross = plus(cross, p, z);
+            }
     }
     // the block's largest, the sums brought to it and added
     __shared__ float lds[4][kThreads / 64];
@@ -458,24 +544,42 @@ __global__ void __launch_bounds__(kThreads)
 k_loss_gradient(Batch a, int64_t first, int64_t slice, const Slice* __restrict__ slices) {
     constexpr int n = Vector<T>::n;
     const int64_t b = first + blockIdx.y;
+    Cut cut = cut_of(min(clamp_count(a.num_actions[b], a.width), a.N), slice);
+    const P* targets = (const P*)a.targets + b * a.width + cut.from;
+    Piece<P, n> pi;
+    pi.load(targets, 0, cut.len, (P)0.0f);
     const Before before = begin_of(a, b);
-    const Cut cut = cut_of(a, b, before.moves, slice);
+    const int64_t lo = min(a.N, before.moves);
+    cut = cut_of(min(cut.count, a.N - lo), slice);
+    const T* logits = (const T*)a.logits + lo + cut.from;
+    T* dlogits = (T*)a.dlogits + lo + cut.from;
+    const int len = cut.len;
+    Piece<T, n> x;
+    x.load(logits, 0, len, (T)0.0f);
     const Slice s = join(slices + b * gridDim.x, gridDim.x);
-    const Scalars own = scalars_of<T>(a, b);
+    const Scalars<T> own = scalars_of<T>(a, b);
     const float share = own.w / before.policy;
     const bool used = own.w != 0.0f && s.total != 0.0f;
     const float shift = s.top == -INFINITY ? 0.0f : s.top;
     const float scale = used ? share * a.loss_scale : 0.0f, p_scale = used ? s.mass / s.total * scale : 0.0f;
-    const int64_t at = cut.lo, row = b * a.width, all = a.B * a.width;
-    for (int64_t c = cut.from + threadIdx.x * n; c < cut.to; c += kThreads * n) {
-        float x[n], pi[n];
-        load_flat<T, n>((const T*)a.logits, at + c, a.N, x);
-        load_flat<P, n>((const P*)a.targets, row + c, all, pi);
+    for (int at = 0; at < len; at += kSlice) {
+        if (at) {
+            pi.load(targets, at, len, (P)0.0f);
+            x.load(logits, at, len, (T)0.0f);
+        }
 #pragma unroll
-        for (int i = 0; i < n; i++) x[i] = used ? fmaf(exp_(x[i] - shift), p_scale, -(pi[i] * scale)) : 0.0f;
-        store_some((T*)a.dlogits + at + c, (int)min((int64_t)n, cut.to - c), x);
+        for (int k = 0; k < x.vecs; k++) {
+            const int c = at + (threadIdx.x + k * kThreads) * n;
+            float dx[n];
+#pragma unroll
+            for (int i = 0; i < n; i++) {
+                const float p = exp_(to_f32<T>(x.v[k][i]) - shift);
+                dx[i] = used ? fmaf(p, p_scale, -(to_f32<P>(pi.v[k][i]) * scale)) : 0.0f;
+            }
+            store_some(dlogits + c, len - c, dx);
+        }
     }
-    if (b == a.B - 1 && blockIdx.x == 0) clear_rest<T>(a, cut.lo + cut.count, threadIdx.x, kThreads);
+    if (b == a.B - 1 && blockIdx.x == 0) clear_rest<T>(a, lo + cut.count, threadIdx.x, kThreads);
     if (threadIdx.x == 0 && blockIdx.x == 0)
         a.row_loss[b] = make_float2(used ? (logf(s.total) * s.mass - s.cross) * share : 0.0f,
                                     value_loss<T>(a, b, own, before.value));
@@ -507,11 +611,12 @@ __global__ void __launch_bounds__(1024) k_loss_join(Batch a, int64_t parts) {
 }
 
 constexpr int64_t kShort = 16 * kHeld, kMiddle = 64 * kHeld;  // widths whose lists 16 lanes, a wave hold
-constexpr int64_t kSlice = 4096;                                 // moves of a slice
 constexpr int64_t kMaxBatch = ((int64_t)1 << 26) - 4;  // a wave a position: a grid holds under 2^32 threads
 constexpr int64_t kGridRows = 32768;  // positions of a launch over slices: a grid has 65,535 rows at most
 
-inline int64_t ranges_of(int64_t B) { return B <= kInline ? 0 : (B + kRange - 1) / kRange; }
+// ranges of 256 positions, or 1,024 of them: every block adds up all that come before its own
+inline int64_t range_of(int64_t B) { return kRange * ((B + 1024 * kRange - 1) / (1024 * kRange)); }
+inline int64_t ranges_of(int64_t B) { return B <= kInline ? 0 : (B + range_of(B) - 1) / range_of(B); }
 // Slices of a list: of 4,096 moves, or 256 of them.  They depend on the width
 // alone, so that a position's gradient is the same in every batch.
 inline int64_t slices_of(int64_t width) {
@@ -561,6 +666,7 @@ int hg_policy_value_loss(const void* logits, int type, int64_t N, const void* va
     a.value_coef = value_coef;
     a.loss_scale = loss_scale;
     a.ranges = ranges_of(B) ? ranges : nullptr;
+    a.range = B > 0 ? range_of(B) : kRange;
     a.row_loss = (float2*)(ranges + ranges_of(B));
     a.losses = losses;
     a.dlogits = dlogits;
@@ -568,13 +674,10 @@ int hg_policy_value_loss(const void* logits, int type, int64_t N, const void* va
     Slice* slices = (Slice*)(a.row_loss + losses_of(B));
     a.begin = (int64_t*)(slices + (width > kMiddle ? B * slices_of(width) : 0));
     a.sums = (float*)(a.begin + B);
-    if (a.ranges) {
-        hipLaunchKernelGGL(k_loss_ranges, dim3((unsigned)ranges_of(B)), dim3(kThreads), 0, st, num_actions, B, width,
-                           policy_weights, value_weights, ranges);
-    }
-    // past that a slice's look back would cost more than the launch
-    if (a.ranges || (width > kMiddle && B > kThreads))
-        hipLaunchKernelGGL(k_loss_begins, dim3((unsigned)((B + kRange - 1) / kRange)), dim3(kRange), 0, st, a);
+    if (a.ranges) hipLaunchKernelGGL(k_loss_ranges, dim3((unsigned)ranges_of(B)), dim3(kRange), 0, st, a);
+    // past that the blocks' look back would cost more than the launch (a long list has a block a slice)
+    if (width <= kMiddle ? B > kLookBack : B > kThreads)
+        hipLaunchKernelGGL(k_loss_begins, dim3((unsigned)((B + a.range - 1) / a.range)), dim3(kRange), 0, st, a);
     else
         a.begin = nullptr;
     int64_t parts = 0;

@@ -341,6 +341,21 @@ def test_policy_value_loss_sums_many_positions(ext):
         _check_loss(ext, _loss_inputs(B, 16, 16, F32, F32, B))
 
 
+@pytest.mark.parametrize("B,width,longest", [(4097, 3, 3), (24 * 1024, 5, 5), (24 * 1024 + 1, 2, 2), (262145, 2, 2),
+                                             (530001, 2, 1), (4200, 1100, 20)])
+def test_policy_value_loss_finds_its_logits(ext, B, width, longest):
+    """Each way to a position's first logit: ranges of 256 positions and of more, by each block and by a launch."""
+    _check_loss(ext, _loss_inputs(B, width, longest, F32, F32, B), longest=longest)
+
+
+@pytest.mark.parametrize("width", [200, 900, 9000])
+def test_policy_value_loss_of_fewer_logits_than_counts(ext, width):
+    """Lists that the logits' end cuts, at every step of the ways lists are read, and no logits at all."""
+    args = _loss_inputs(5, width, width, F32, F32, width, full=True)
+    for left in (0, 1, 3, width - 1, width, width + 1, 2 * width + 4099 % width, 5 * width - 1):
+        _check_loss(ext, [args[0][:left].contiguous(), *args[1:]], longest=width)
+
+
 @pytest.mark.parametrize("longest", [40, 700, 20000])
 def test_policy_value_loss_masked_logits(ext, longest):
     """-inf at moves that are masked, whole positions of them, the type's lowest value, positions of weight 0
