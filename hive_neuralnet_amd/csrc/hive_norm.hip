@@ -23,8 +23,9 @@
 // Bound by memory.  Measured (MI355X, inputs not in cache): forward 16,384 x
 // 2,048 f32 45 us, 5.9 TB/s; 8,192 x 4,096 bf16 26 us, 5.2; 118,271 x 64 f32
 // with the sigmoid 13 us, 4.6; 4,096 x 5,119 bf16, rows at odd addresses, 24
-// us, 3.5.  Backward 78 us, 5.2 TB/s; 40 us, 5.0; 23 us, 3.9; 40 us, 3.1; 4 to
-// 6 us of each are the second launch.  In the backward pass the next row is
+// us, 3.6.  Backward 76 us, 5.3 TB/s; 39.5 us, 5.1; 21.5 us, 4.2; 40 us, 3.1; 2
+// to 4 us of each are the second launch (1.5 more where each of its loads
+// waited for the one before).  In the backward pass the next row is
 // read while this one is worked on (8,192 x 4,096: 61 us without) and h and dh
 // are worked out again for dx, from the row's own 16 bits, which leaves the
 // registers for it; loads wait for nothing, an end that cuts a vector is
@@ -391,8 +392,15 @@ k_norm_join(const float* __restrict__ part, int parts, int64_t cols, int w_type,
     __shared__ float lds[32][33];
     const int64_t c = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
     float s = 0.0f;
+    constexpr int n = 8;  // parts whose loads go out together
     if (c < 2 * cols)
-        for (int p = threadIdx.x >> 5; p < parts; p += 32) s += part[2 * p * cols + c];
+        for (int p = threadIdx.x >> 5; p < parts; p += 32 * n) {
+            float v[n];
+#pragma unroll
+            for (int k = 0; k < n; k++) v[k] = part[2 * (int64_t)min(p + 32 * k, parts - 1) * cols + c];
+#pragma unroll
+            for (int k = 0; k < n; k++) s += p + 32 * k < parts ? v[k] : 0.0f;
+        }
     lds[threadIdx.x >> 5][threadIdx.x & 31] = s;
     __syncthreads();
     if (threadIdx.x >= 32 || c >= 2 * cols) return;
