@@ -21,16 +21,16 @@
 // visible to another chiplet writes back its whole L2 first, for every block.)
 //
 // Bound by memory.  Measured (MI355X, inputs not in cache): forward 16,384 x
-// 2,048 f32 45 us, 5.9 TB/s; 8,192 x 4,096 bf16 26 us, 5.2; 118,271 x 64 f32
-// with the sigmoid 13 us, 4.6; 4,096 x 5,119 bf16, rows at odd addresses, 24
-// us, 3.6.  Backward 76 us, 5.3 TB/s; 39.5 us, 5.1; 21.5 us, 4.2; 40 us, 3.1; 2
+// 2,048 f32 44 us, 6.1 TB/s; 8,192 x 4,096 bf16 24.5 us, 5.5; 118,271 x 64 f32
+// with the sigmoid 13 us, 4.6; 4,096 x 5,119 bf16, rows at odd addresses, 23
+// us, 3.7.  Backward 76 us, 5.3 TB/s; 39.5 us, 5.1; 21.5 us, 4.2; 40 us, 3.1; 2
 // to 4 us of each are the second launch (1.5 more where each of its loads
-// waited for the one before).  In the backward pass the next row is
-// read while this one is worked on (8,192 x 4,096: 61 us without) and h and dh
-// are worked out again for dx, from the row's own 16 bits, which leaves the
-// registers for it; loads wait for nothing, an end that cuts a vector is
-// settled where the vector is used (4,096 x 5,119: 65 us where each load was
-// settled before the next).
+// waited for the one before).  The next row is read while this one is worked on
+// (8,192 x 4,096: 26 us without in the forward pass, 61 in the backward) and,
+// in the backward pass, h and dh are worked out again for dx, from the row's
+// own 16 bits, which leaves the registers for it; loads wait for nothing, an end
+// that cuts a vector is settled where the vector is used (4,096 x 5,119: 65 us
+// where each load was settled before the next).
 #include "hive_train.hpp"
 
 namespace {
@@ -173,14 +173,21 @@ k_norm_forward(const typename Sh::T* __restrict__ x, int64_t rows, int cols, int
         load_param<n>(w, w_type, (lane + k * Sh::kLanes) * n, cols, 1.0f, wv[k]);
         load_param<n>(b, w_type, (lane + k * Sh::kLanes) * n, cols, 0.0f, bv[k]);
     }
+    typename Vector<typename Sh::T>::type next[Sh::kVecs];
+    auto fetch = [&](int64_t row) {
+        const typename Sh::T* xr = x + (row < rows ? row * x_stride : 0);
+#pragma unroll
+        for (int k = 0; k < Sh::kVecs; k++) next[k] = load_row<Sh>(xr, lane, k, cols);
+    };
+    fetch((int64_t)blockIdx.x * Sh::kGroups + threadIdx.x / Sh::kLanes);
     // rows are taken by whole blocks: waves that share sums stay together
     for (int64_t base = (int64_t)blockIdx.x * Sh::kGroups; base < rows; base += step) {
         const int64_t row = base + threadIdx.x / Sh::kLanes;
         const bool there = row < rows;
-        const typename Sh::T* xr = x + (there ? row * x_stride : 0);
         typename Vector<typename Sh::T>::type raw[Sh::kVecs];
 #pragma unroll
-        for (int k = 0; k < Sh::kVecs; k++) raw[k] = load_row<Sh>(xr, lane, k, cols);
+        for (int k = 0; k < Sh::kVecs; k++) raw[k] = next[k];
+        if (base + step < rows) fetch(row + step);
         float a[Sh::kVecs][n];
         float s[1] = {0.0f};
 #pragma unroll
