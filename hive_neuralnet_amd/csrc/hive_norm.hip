@@ -84,7 +84,8 @@ __device__ __forceinline__ void load_param(const void* p, int type, int c, int c
     }
 }
 __device__ __forceinline__ float load_param(const void* p, int type, int64_t c, float none) {
-    return !p ? none : type == HG_F32 ? param_at<float>(p, c) : type == HG_F16 ? param_at<f16>(p, c) : param_at<bf16>(p, c);
+    if (!p) return none;
+    return type == HG_F32 ? param_at<float>(p, c) : type == HG_F16 ? param_at<f16>(p, c) : param_at<bf16>(p, c);
 }
 __device__ __forceinline__ void store_param(void* p, int type, int64_t c, float v) {
     if (type == HG_F32) ((float*)p)[c] = v;
@@ -100,7 +101,11 @@ template <typename T_, int kThreads_, int kLanes_, int kVecs_> struct Shape {
     static constexpr int kThreads = kThreads_, kGroups = kThreads / kLanes;
     static constexpr int kWaves = kLanes > 64 ? kLanes / 64 : 1;  // of a row
     // whether the backward pass has the registers to read the next row ahead
-    static constexpr bool kAhead = kThreads <= 512 || kVecs * 4 <= (kN == 4 ? 8 : 4);
+    static constexpr bool kAhead = kThreads <= 512 || kVecs * 4 <= 8;
+    // the widest rows: the columns' sums of dw and db are in LDS, each thread's its own, which leaves the registers
+    // for the rest (2,048 x 16,384: bf16 48 us, 66 with them in registers and no next row; f32 95, 152 with some in
+    // scratch)
+    static constexpr bool kSumsInLds = kThreads == 1024 && kLanes == kThreads && kVecs * kN == kValues;
 };
 
 // v, its registers' contents unknown to the optimiser: what follows from it is worked out from it again
@@ -260,6 +265,33 @@ k_norm_backward(const typename Sh::T* __restrict__ dy, int64_t dy_stride, const 
     float wv[Sh::kVecs][n], sw[Sh::kVecs][n] = {}, sb[Sh::kVecs][n] = {};
 #pragma unroll
     for (int k = 0; k < Sh::kVecs; k++) load_param<n>(w, w_type, (lane + k * Sh::kLanes) * n, cols, 1.0f, wv[k]);
+    __shared__ float4 lds_sums[2][Sh::kSumsInLds ? Sh::kVecs * n / 4 * Sh::kThreads : 1];
+    auto load_sums = [&](int k) {
+#pragma unroll
+        for (int i = 0; i < n; i += 4) {
+            const int at = (k * n + i) / 4 * Sh::kThreads + threadIdx.x;
+            const float4 p = lds_sums[0][at], q = lds_sums[1][at];
+            sw[k][i] = p.x;
+            sw[k][i + 1] = p.y;
+            sw[k][i + 2] = p.z;
+            sw[k][i + 3] = p.w;
+            sb[k][i] = q.x;
+            sb[k][i + 1] = q.y;
+            sb[k][i + 2] = q.z;
+            sb[k][i + 3] = q.w;
+        }
+    };
+    auto store_sums = [&](int k) {
+#pragma unroll
+        for (int i = 0; i < n; i += 4) {
+            const int at = (k * n + i) / 4 * Sh::kThreads + threadIdx.x;
+            lds_sums[0][at] = make_float4(sw[k][i], sw[k][i + 1], sw[k][i + 2], sw[k][i + 3]);
+            lds_sums[1][at] = make_float4(sb[k][i], sb[k][i + 1], sb[k][i + 2], sb[k][i + 3]);
+        }
+    };
+    if constexpr (Sh::kSumsInLds)
+#pragma unroll
+        for (int k = 0; k < Sh::kVecs; k++) store_sums(k);
     V next[Sh::kVecs], next_dy[Sh::kVecs];
     float next_m, next_r;
     auto fetch = [&](int64_t row) {
@@ -301,6 +333,7 @@ k_norm_backward(const typename Sh::T* __restrict__ dy, int64_t dy_stride, const 
 #pragma unroll
                 for (int i = 0; i < n; i++) a[i] = sigmoid_(a[i]);
             }
+            if constexpr (Sh::kSumsInLds) load_sums(k);
 #pragma unroll
             for (int i = 0; i < n; i++) {
                 const float h = fmaf(a[i], r, -mr);
@@ -310,6 +343,7 @@ k_norm_backward(const typename Sh::T* __restrict__ dy, int64_t dy_stride, const 
                 s[0] += dh;
                 s[1] = fmaf(dh, h, s[1]);
             }
+            if constexpr (Sh::kSumsInLds) store_sums(k);
         }
         row_sums<Sh>(s, lds, turn);
         if (!there || !dx) continue;
@@ -344,6 +378,9 @@ k_norm_backward(const typename Sh::T* __restrict__ dy, int64_t dy_stride, const 
         }
     }
     if (!part) return;
+    if constexpr (Sh::kSumsInLds)
+#pragma unroll
+        for (int k = 0; k < Sh::kVecs; k++) load_sums(k);
     // the groups of a wave, then those of the block, a vector of columns at a time
     constexpr int width = Sh::kLanes, groups = width < 64 ? all : Sh::kGroups;
     __shared__ float join[2][n][Sh::kGroups > 1 ? groups * width : 1];
@@ -535,7 +572,7 @@ template <typename T, int most, int kNarrow, int kBroad, typename F> int with_sh
     if (vecs <= 256 * most) return f(Shape<T, kBroad, 256, most>{});
     if (vecs <= 512 * most) return f(Shape<T, threads_of(512, kBroad), 512, most>{});
     if (vecs <= 1024 * most) return f(Shape<T, 1024, 1024, most>{});
-    return f(Shape<T, 1024, 1024, kValues / n>{});  // up to kMaxCols (some of the backward pass's sums in scratch)
+    return f(Shape<T, 1024, 1024, kValues / n>{});  // up to kMaxCols
 }
 template <typename T, typename F> int with_forward_shape(int64_t cols, F f) {
     return with_shape<T, kValues / Vector<T>::n, 256, 256>(cols, f);
@@ -553,7 +590,8 @@ template <typename Sh> int64_t forward_blocks(int64_t rows) {
 // sums' way through LDS and memory (2,048 x 64: 8.1 us at one row, 8.7 at two,
 // 10.7 at four; 300 x 4,096: 14.5, 12.0, 13.9)
 template <typename Sh> int64_t backward_blocks(int64_t rows) {
-    const int64_t need = (rows + 2 * Sh::kGroups - 1) / (2 * Sh::kGroups), most = (int64_t)kCus * (Sh::kVecs == 1 || Sh::kThreads > 512 ? 1024 : 512) / Sh::kThreads;
+    const int64_t need = (rows + 2 * Sh::kGroups - 1) / (2 * Sh::kGroups);
+    const int64_t most = (int64_t)kCus * (Sh::kVecs == 1 || Sh::kThreads > 512 ? 1024 : 512) / Sh::kThreads;
     return need < most ? need : most;
 }
 constexpr int64_t kWideParts = 64;  // row ranges of k_norm_dw_wide

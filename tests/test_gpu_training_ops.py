@@ -195,6 +195,14 @@ def test_layer_norm_weight_gradient_over_many_rows(ext, rows, cols, sigmoid):
         assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize("t", [F32, F16, BF16], ids=str)
+@pytest.mark.parametrize("rows,cols", [(1, 16384), (700, 16384), (1100, 9001), (600, 12290)])
+def test_layer_norm_widest_rows_of_a_block(ext, t, rows, cols):
+    """Several rows a block, its sums of the weights' gradients beside its registers."""
+    _check_norm(ext, _randn((rows, cols), 1).to(t), _randn((cols,), 3).to(t), _randn((cols,), 4).to(t),
+                _randn((rows, cols), 2).to(t), sigmoid=rows == 600)
+
+
 @pytest.mark.parametrize("sigmoid", [False, True], ids=["plain", "sigmoid"])
 def test_layer_norm_gradient_against_differences(ext, sigmoid):
     """<gradient, direction> against the difference of the forward pass on both sides.  The forward pass is
