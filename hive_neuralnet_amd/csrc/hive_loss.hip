@@ -35,10 +35,11 @@
 // 6 in two launches, the lists 15 (one load after the other, as conversions
 // inside their branches make them: 18), of which the VALU is busy 12 (a third
 // of the slots it works on hold a move; lists sorted by length among a block's
-// waves: no gain); 192 x 85,834 bf16 logits 47 us: 22 for the slices, 4.5
-// TB/s, and 23 for the gradient, which finds its second read in the cache (26
-// where every lane joined the list's 21 slices itself; slices of 8,192: 49 us,
-// of 2,048: 54).
+// waves: no gain); 192 x 85,834 bf16 logits 42.5 us: 22 for the slices, 4.5
+// TB/s, and 18 for the gradient, which finds its second read in the caches (5
+// more with stores that go through them, 1 with the slices in their order, 3
+// where every lane joined the list's 21 slices itself; slices of 8,192: 1.5
+// more, of 2,048: 6).
 #include "hive_train.hpp"
 
 namespace {
@@ -418,8 +419,8 @@ struct Cut {
     int64_t count, from;
     int len;
 };
-__device__ __forceinline__ Cut cut_of(int64_t count, int64_t slice) {
-    const int64_t from = min(count, (int64_t)blockIdx.x * slice);
+__device__ __forceinline__ Cut cut_of(int64_t count, int64_t slice, uint32_t index) {
+    const int64_t from = min(count, (int64_t)index * slice);
     return Cut{count, from, (int)min(slice, count - from)};
 }
 
@@ -443,6 +444,20 @@ template <typename E, int n> struct Piece {
         }
     }
 };
+
+// store_some past the caches: they hold what other slices have still to read
+template <typename T, int n> __device__ __forceinline__ void store_past(T* p, int live, const float v[n]) {
+    typedef T vec __attribute__((ext_vector_type(n), aligned(sizeof(T))));
+    if (live >= n) {
+        vec q;
+#pragma unroll
+        for (int i = 0; i < n; i++) q[i] = from_f32<T>(v[i]);
+        __builtin_nontemporal_store(q, (vec*)p);
+    } else {
+        skipped();
+        store_some<T, n>(p, live, v);
+    }
+}
 
 // the n slices of a list as one, by a wave: a lane takes every 64th, all bring theirs to the largest logit
 __device__ __forceinline__ Slice join(const Slice* slices, int n) {
@@ -471,12 +486,12 @@ k_loss_slices(Batch a, int64_t first, int64_t slice, Slice* __restrict__ slices)
     constexpr int n = Vector<T>::n;
     const int64_t b = first + blockIdx.y;
     // where the logits begin takes a look at the positions before: the first targets are read meanwhile
-    Cut cut = cut_of(min(clamp_count(a.num_actions[b], a.width), a.N), slice);
+    Cut cut = cut_of(min(clamp_count(a.num_actions[b], a.width), a.N), slice, blockIdx.x);
     const P* targets = (const P*)a.targets + b * a.width + cut.from;
     Piece<P, n> pi;
     pi.load(targets, 0, cut.len, (P)0.0f);
     const int64_t lo = min(a.N, begin_of(a, b).moves);
-    cut = cut_of(min(cut.count, a.N - lo), slice);
+    cut = cut_of(min(cut.count, a.N - lo), slice, blockIdx.x);
     const T* logits = (const T*)a.logits + lo + cut.from;
     const int len = cut.len;
     // one pass: each thread's largest logit so far (fmaxf passes a NaN by: it comes through the sums), its sums brought
@@ -543,14 +558,18 @@ template <typename T, typename P>
 __global__ void __launch_bounds__(kThreads)
 k_loss_gradient(Batch a, int64_t first, int64_t slice, const Slice* __restrict__ slices) {
     constexpr int n = Vector<T>::n;
-    const int64_t b = first + blockIdx.y;
-    Cut cut = cut_of(min(clamp_count(a.num_actions[b], a.width), a.N), slice);
+    // the slices that were read last come first, on the chiplet that read them: its cache holds some of them yet
+    const uint32_t linear = blockIdx.y * gridDim.x + blockIdx.x, whole = gridDim.x * gridDim.y & ~7u;
+    const uint32_t turned = linear < whole ? whole - 8 - (linear & ~7u) + (linear & 7u) : linear;
+    const uint32_t index = turned % gridDim.x;
+    const int64_t b = first + turned / gridDim.x;
+    Cut cut = cut_of(min(clamp_count(a.num_actions[b], a.width), a.N), slice, index);
     const P* targets = (const P*)a.targets + b * a.width + cut.from;
     Piece<P, n> pi;
     pi.load(targets, 0, cut.len, (P)0.0f);
     const Before before = begin_of(a, b);
     const int64_t lo = min(a.N, before.moves);
-    cut = cut_of(min(cut.count, a.N - lo), slice);
+    cut = cut_of(min(cut.count, a.N - lo), slice, index);
     const T* logits = (const T*)a.logits + lo + cut.from;
     T* dlogits = (T*)a.dlogits + lo + cut.from;
     const int len = cut.len;
@@ -576,11 +595,11 @@ k_loss_gradient(Batch a, int64_t first, int64_t slice, const Slice* __restrict__
                 const float p = exp_(to_f32<T>(x.v[k][i]) - shift);
                 dx[i] = used ? fmaf(p, p_scale, -(to_f32<P>(pi.v[k][i]) * scale)) : 0.0f;
             }
-            store_some(dlogits + c, len - c, dx);
+            store_past<T, n>(dlogits + c, len - c, dx);
         }
     }
-    if (b == a.B - 1 && blockIdx.x == 0) clear_rest<T>(a, lo + cut.count, threadIdx.x, kThreads);
-    if (threadIdx.x == 0 && blockIdx.x == 0)
+    if (b == a.B - 1 && index == 0) clear_rest<T>(a, lo + cut.count, threadIdx.x, kThreads);
+    if (threadIdx.x == 0 && index == 0)
         a.row_loss[b] = make_float2(used ? (logf(s.total) * s.mass - s.cross) * share : 0.0f,
                                     value_loss<T>(a, b, own, before.value));
 }
