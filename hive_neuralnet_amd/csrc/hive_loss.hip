@@ -29,17 +29,17 @@
 // targets and the counts before it go out before any of them is waited for.
 //
 // Measured (MI355X): 16 positions 5 us, one launch; 2,048 of 60 moves on
-// average 9 us, of which the second launch, the sum of the blocks' shares,
-// takes 3 (the last block adding them: 17 in all, as every block's write-back
-// for it has to come first); 65,521 of 85 in bf16 23.5 us: the sums before them
-// 6 in two launches, the lists 15 (one load after the other, as conversions
-// inside their branches make them: 18), of which the VALU is busy 12 (a third
-// of the slots it works on hold a move; lists sorted by length among a block's
-// waves: no gain); 192 x 85,834 bf16 logits 42.5 us: 22 for the slices, 4.5
-// TB/s, and 18 for the gradient, which finds its second read in the caches (5
-// more with stores that go through them, 1 with the slices in their order, 3
-// where every lane joined the list's 21 slices itself; slices of 8,192: 1.5
-// more, of 2,048: 6).
+// average 8 us, of which the second launch, the sum of the blocks' shares,
+// takes 2 to 3 (the last block adding them: 17 in all, as every block's
+// write-back for it has to come first); 65,521 of 85 in bf16 22.5 us: the sums
+// before them 6.5 in two launches, the lists 15 to 16 (one load after the other,
+// as conversions inside their branches make them: 19), of which the VALU is
+// busy 12.5 (a third of the slots it works on hold a move; lists sorted by length
+// among a block's waves: no gain).  192 x 85,834 bf16 logits 40.5 us: 20 for the
+// slices, 4.9 TB/s, and 20 for the gradient, 6.5 TB/s, as its second read is
+// partly in the caches (4 more with stores that go through them, 1 with the
+// slices in their order, 2 with a look back in fours, 3 where every lane joined
+// the list's 21 slices itself; slices of 8,192: 1.5 more, of 2,048: 6).
 #include "hive_train.hpp"
 
 namespace {
@@ -101,7 +101,8 @@ struct Before {
     int64_t moves;       // of the positions before `first`
     float policy, value; // sums of all weights, 1 where they are 0
 };
-template <int threads> __device__ __forceinline__ Before look_back(const Batch& a, int64_t first) {
+// (n positions of a thread, their loads together; the weights where they are wanted)
+template <int threads, int n, bool kWeights = true> __device__ __forceinline__ Before look_back(const Batch& a, int64_t first) {
     __shared__ int64_t lds_moves[threads / 64];
     __shared__ float lds_policy[threads / 64], lds_value[threads / 64];
     int64_t moves = 0;
@@ -117,7 +118,6 @@ template <int threads> __device__ __forceinline__ Before look_back(const Batch& 
         for (int64_t i = mine * a.range + threadIdx.x; i < first; i += threads)
             moves += clamp_count(a.num_actions[i], a.width);
     } else {
-        constexpr int n = 4;  // positions of a thread whose loads go out together
         const int last = (int)a.B - 1;
         for (int i = threadIdx.x; i <= last; i += n * threads) {
             int64_t c[n];
@@ -126,8 +126,8 @@ template <int threads> __device__ __forceinline__ Before look_back(const Batch& 
             for (int k = 0; k < n; k++) {
                 const int at = min(i + k * threads, last);
                 c[k] = a.num_actions[at];
-                p[k] = a.pw[at];
-                v[k] = a.vw[at];
+                p[k] = kWeights ? a.pw[at] : 0.0f;
+                v[k] = kWeights ? a.vw[at] : 0.0f;
             }
 #pragma unroll
             for (int k = 0; k < n; k++) {
@@ -139,20 +139,26 @@ template <int threads> __device__ __forceinline__ Before look_back(const Batch& 
         }
     }
     moves = wave_sum(moves);
-    policy = group_sum<64>(policy);
-    value = group_sum<64>(value);
+    if (kWeights) {
+        policy = group_sum<64>(policy);
+        value = group_sum<64>(value);
+    }
     if ((threadIdx.x & 63) == 0) {
         lds_moves[threadIdx.x >> 6] = moves;
-        lds_policy[threadIdx.x >> 6] = policy;
-        lds_value[threadIdx.x >> 6] = value;
+        if (kWeights) {
+            lds_policy[threadIdx.x >> 6] = policy;
+            lds_value[threadIdx.x >> 6] = value;
+        }
     }
     __syncthreads();
     Before r = {0, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < threads / 64; i++) {
         r.moves += lds_moves[i];
-        r.policy += lds_policy[i];
-        r.value += lds_value[i];
+        if (kWeights) {
+            r.policy += lds_policy[i];
+            r.value += lds_value[i];
+        }
     }
     if (!(r.policy > 0.0f)) r.policy = 1.0f;
     if (!(r.value > 0.0f)) r.value = 1.0f;
@@ -196,7 +202,7 @@ __global__ void __launch_bounds__(kRange) k_loss_ranges(Batch a) {
 __global__ void __launch_bounds__(kRange) k_loss_begins(Batch a) {
     __shared__ int64_t lds[2][kRange / 64];
     const int64_t first = (int64_t)blockIdx.x * a.range, end = min(a.B, first + a.range);
-    const Before before = look_back<kRange>(a, first);
+    const Before before = look_back<kRange, 4>(a, first);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int64_t begin = before.moves;
     int turn = 0;
@@ -284,7 +290,7 @@ __global__ void __launch_bounds__(kThreads) k_loss_held(Batch a) {
         value_sum = a.sums[1];
         count = (int)clamp_count(listed, a.width);
     } else {
-        const Before before = look_back<kThreads>(a, first);
+        const Before before = look_back<kThreads, 4>(a, first);
         policy_sum = before.policy;
         value_sum = before.value;
         lo = before.moves;
@@ -411,8 +417,8 @@ __global__ void __launch_bounds__(kThreads) k_loss_held(Batch a) {
 // ---- long lists: block (slice, position) -------------------------------------
 
 // what k_loss_begins left, or the block's own
-__device__ __forceinline__ Before begin_of(const Batch& a, int64_t b) {
-    return a.begin ? Before{a.begin[b], a.sums[0], a.sums[1]} : look_back<kThreads>(a, b);
+template <bool kWeights> __device__ __forceinline__ Before begin_of(const Batch& a, int64_t b) {
+    return a.begin ? Before{a.begin[b], a.sums[0], a.sums[1]} : look_back<kThreads, 1, kWeights>(a, b);
 }
 // the slice of a position: `len` elements from element `from` of its list of `count`
 struct Cut {
@@ -490,10 +496,12 @@ k_loss_slices(Batch a, int64_t first, int64_t slice, Slice* __restrict__ slices)
     const P* targets = (const P*)a.targets + b * a.width + cut.from;
     Piece<P, n> pi;
     pi.load(targets, 0, cut.len, (P)0.0f);
-    const int64_t lo = min(a.N, begin_of(a, b).moves);
+    const int64_t lo = min(a.N, begin_of<false>(a, b).moves);
+    const int listed = cut.len;
     cut = cut_of(min(cut.count, a.N - lo), slice, blockIdx.x);
     const T* logits = (const T*)a.logits + lo + cut.from;
     const int len = cut.len;
+    if (len != listed) pi.load(targets, 0, len, (P)0.0f);  // the logits' end cuts the list
     // one pass: each thread's largest logit so far (fmaxf passes a NaN by: it comes through the sums), its sums brought
     // to a new one as it comes
     float top = -INFINITY, total = 0.0f, mass = 0.0f, cross = 0.0f;
@@ -517,7 +525,7 @@ k_loss_slices(Batch a, int64_t first, int64_t slice, Slice* __restrict__ slices)
 #pragma unroll
             for (int i = 0; i < n; i++) {
                 const float z = to_f32<T>(x.v[k][i]) - shift;
-                const float p = at + (threadIdx.x + k * kThreads) * n + i < len ? to_f32<P>(pi.v[k][i]) : 0.0f;
+                const float p = to_f32<P>(pi.v[k][i]);
                 total += exp_(z);
                 mass += p;
                 cross = plus(cross, p, z);
@@ -567,7 +575,7 @@ k_loss_gradient(Batch a, int64_t first, int64_t slice, const Slice* __restrict__
     const P* targets = (const P*)a.targets + b * a.width + cut.from;
     Piece<P, n> pi;
     pi.load(targets, 0, cut.len, (P)0.0f);
-    const Before before = begin_of(a, b);
+    const Before before = begin_of<true>(a, b);
     const int64_t lo = min(a.N, before.moves);
     cut = cut_of(min(cut.count, a.N - lo), slice, index);
     const T* logits = (const T*)a.logits + lo + cut.from;
