@@ -6,6 +6,9 @@ The library is compiled with hipcc straight from csrc/*.hip into
 hive_neuralnet_amd/libhive_gpu.so (git-ignored; it travels with the tree).
 Flags: no fast-math, no FP contraction (features must be bit-exact with the
 reference's IEEE divisions), packed-FP32 instruction selection disabled.
+
+With it _train_calls.so, a CPython module over torch's headers: the training
+operators' entry points without Python's share of a call (host code alone).
 """
 from __future__ import annotations
 
@@ -20,6 +23,8 @@ LIB = os.path.join(PKG, "libhive_gpu.so")
 SOURCES = [os.path.join(PKG, "csrc", n) for n in (
     "hive_engine.hip", "hive_mcts.hip", "hive_fnn.hip", "hive_probe.hip", "hive_norm.hip", "hive_loss.hip",
     "hive_adamw.hip")]
+CALLS = os.path.join(PKG, "_train_calls.so")
+CALLS_SOURCE = os.path.join(PKG, "csrc", "train_calls.cpp")
 ARCH = os.environ.get("HIVE_GPU_ARCH", "gfx950")
 
 FLAGS = [
@@ -54,6 +59,27 @@ def build(verbose: bool = False, defines: tuple = (), out: str = LIB) -> str:
     return out
 
 
+def build_calls(out: str = CALLS) -> str:
+    """Compile the CPython module to `out`."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    tmp = out + ".tmp"
+    dirs = [os.path.join(ROOT, "include"), sysconfig.get_paths()["include"], *cpp_extension.include_paths()]
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f for d in dirs for f in ("-isystem", d)], "-o", tmp, CALLS_SOURCE,
+           *[f"-L{d}" for d in cpp_extension.library_paths()], "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError(f"g++ failed building {out}")
+    os.replace(tmp, out)
+    return out
+
+
 if __name__ == "__main__":
     import argparse
 
@@ -66,3 +92,5 @@ if __name__ == "__main__":
     if a.define and os.path.abspath(a.out) == LIB:
         ap.error("a build with --define goes to its own --out path, not the package's library")
     print(build(verbose=a.verbose, defines=tuple(a.define), out=os.path.abspath(a.out)))
+    if os.path.abspath(a.out) == LIB:
+        print(build_calls())

@@ -236,6 +236,7 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
             fn = getattr(lib, name)
             fn.argtypes = args
             fn.restype = _c_i64
+        training_ops.bind(lib)
         _lib = lib
         return lib
 

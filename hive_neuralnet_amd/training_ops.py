@@ -18,6 +18,11 @@ import math
 import numpy as np
 import torch
 
+try:  # train_calls.cpp: these entry points without Python's share of a call
+    from . import _train_calls as _calls
+except ImportError:  # not built: all of a call from here, twice the time of a small one
+    _calls = None
+
 _c_void_p = ctypes.c_void_p
 _c_i64 = ctypes.c_int64
 _c_int = ctypes.c_int
@@ -42,6 +47,14 @@ SIGS_I64 = {
     "hg_layer_norm_backward_workspace": [_c_i64, _c_i64],
     "hg_policy_value_loss_workspace": [_c_i64, _c_i64],
 }
+
+
+def bind(lib) -> None:
+    """Gives train_calls.cpp the library's functions."""
+    if _calls is not None:
+        _calls.bind(*[ctypes.cast(getattr(lib, name), _c_void_p).value for name in (
+            "hg_layer_norm_forward", "hg_layer_norm_backward", "hg_layer_norm_backward_workspace",
+            "hg_policy_value_loss", "hg_policy_value_loss_workspace", "hg_adamw_step")], _current_device, _raw_stream)
 
 
 class HgAdamwTensor(ctypes.Structure):
@@ -149,6 +162,10 @@ def layer_norm_forward(self, x: torch.Tensor, weight=None, bias=None, eps: float
     is); weight, bias [cols] of one type, or None; y has x's shape and type
     and is contiguous, mean and rstd = 1 / sqrt(var + eps) are float32
     [...]."""
+    if _calls is not None:
+        done = _calls.layer_norm_forward(x, weight, bias, eps, activation)
+        if done is not None:
+            return done
     dev = _float_tensor(x, "x")
     rows, cols, stride = _rows(x, "x")
     if not eps >= 0.0:
@@ -170,6 +187,10 @@ def layer_norm_backward(self, dy: torch.Tensor, x: torch.Tensor, mean: torch.Ten
     activation.  dweight and dbias (of the parameters' type; None for a
     parameter that is None) are sums over all rows, the same bits on every
     call; dx (x's shape and type, contiguous; None with need_dx=False)."""
+    if _calls is not None:
+        done = _calls.layer_norm_backward(dy, x, mean, rstd, weight, bias, activation, need_dx)
+        if done is not None:
+            return done
     dev = _float_tensor(x, "x")
     _place(dy, "dy")
     if dy.shape != x.shape or dy.dtype != x.dtype:
@@ -216,6 +237,11 @@ def policy_value_loss(self, logits: torch.Tensor, values: torch.Tensor, num_acti
     dlogits and dvalues are loss_scale times the gradients of the total.
     Positions of weight 0, without moves, or with no logit above -inf add
     nothing and have gradients of zero."""
+    if _calls is not None:
+        done = _calls.policy_value_loss(logits, values, num_actions, policy_targets, policy_weights, value_targets,
+                                        value_weights, value_coef, loss_scale)
+        if done is not None:
+            return done
     dev = _float_tensor(logits, "logits")
     if logits.dim() != 1 or not logits.is_contiguous():
         raise ValueError(f"logits must be one contiguous row, got {tuple(logits.shape)}")
@@ -314,6 +340,10 @@ class AdamWPlan:
         tensor of one value that multiplies the gradients (1 / the loss scale, a
         clipping factor).  seed: of the 8-bit moments' rounding; give each step
         another one."""
+        if _calls is not None and not self._partial and _calls.adamw_step(
+                self.params, grads, self._table_ptr, self._type, self.state_bits, step, lr, betas[0], betas[1], eps,
+                weight_decay, grad_scale, seed & 0xFFFFFFFF):
+            return
         if len(grads) != len(self.params):
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
         dev = self._device

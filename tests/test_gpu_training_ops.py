@@ -752,3 +752,83 @@ def test_adamw_refusals(ext):
     with pytest.raises(ValueError, match="new plan"):
         plan.step(g, 1)
     assert all(torch.equal(a, b) for a, b in zip(p, before))
+
+
+# ---- the two ways of a call ---------------------------------------------------
+
+
+def _each_entry_point(ext):
+    """What every entry point gives for plain arguments, as a list of tensors."""
+    out = []
+    for t, w_type, sigmoid in ((F32, F32, None), (BF16, F32, "sigmoid"), (F16, F16, None)):
+        wide = _randn((300, 200), 1).to(t)
+        x, dy = wide[:, 3:180], _randn((300, 177), 2).to(t)
+        w, b = _randn((177,), 3).to(w_type), _randn((177,), 4).to(w_type)
+        for weight, bias in ((w, b), (w, None), (None, b), (None, None)):
+            y, mean, rstd = ext.layer_norm_forward(x, weight, bias, 1e-5, sigmoid)
+            out += [y, mean, rstd, *ext.layer_norm_backward(dy, x, mean, rstd, weight, bias, sigmoid)]
+            out += ext.layer_norm_backward(dy, x, mean, rstd, weight, bias, sigmoid, need_dx=False)
+        deep = dy.contiguous().view(3, 100, 177)
+        out += ext.layer_norm_forward(deep, w, b)
+        out += ext.policy_value_loss(*_loss_inputs(50, 30, 30, t, F32, 2), value_coef=0.5, loss_scale=3.0)
+        args = _loss_inputs(50, 30, 30, t, F16, 2)
+        out += ext.policy_value_loss(args[0], args[1].unsqueeze(1), args[2], args[3],
+                                     *[a.unsqueeze(1) for a in args[4:]])
+        for bits in (32, 8):
+            params = [_randn((n,), n).to(t) for n in (1, 300, 4097)]
+            plan = ext.prepare_adamw(params, bits)
+            grads = [_randn((p.numel(),), 7).to(w_type) for p in params]
+            scale = torch.full((1,), 0.25, device="cuda")
+            plan.step(grads, 1, 1e-2, seed=5)
+            plan.step([grads[0], None, grads[2]], 2, 1e-2, seed=6)
+            plan.step(grads, 3, 1e-2, grad_scale=scale, seed=(1 << 40) - 3)
+            plan.step(tuple(grads), 4, 1e-2, betas=(0.5, 0.9), eps=1e-3, weight_decay=0.1, seed=8)
+            out += params + [v.float() for v in plan.state.values()]
+    return [v for v in out if v is not None], [v is None for v in out]
+
+
+def test_native_calls_give_what_python_gives(ext, monkeypatch):
+    from hive_neuralnet_amd import training_ops
+    assert training_ops._calls is not None, "built with the library"
+    native, gaps = _each_entry_point(ext)
+    monkeypatch.setattr(training_ops, "_calls", None)
+    alone, gaps_alone = _each_entry_point(ext)
+    assert gaps == gaps_alone and len(native) == len(alone)
+    for p, q in zip(native, alone):
+        assert p.shape == q.shape and p.dtype == q.dtype and p.is_contiguous() and torch.equal(p, q)
+        assert not p.requires_grad
+
+
+def test_native_calls_serve_plain_arguments_and_leave_the_rest(ext):
+    from hive_neuralnet_amd import training_ops
+    calls = training_ops._calls
+    x, w = _randn((40, 64), 1), _randn((64,), 2)
+    assert calls.layer_norm_forward(x, w, w, 1e-5, None) is not None
+    for bad in ((x.t(), w, w, 1e-5, None), (x, w[:3], w, 1e-5, None), (x, w, w.half(), 1e-5, None),
+                (x.double(), None, None, 1e-5, None), (x, w.cpu(), None, 1e-5, None), (x, w, w, -1.0, None),
+                (x, w, w, float("nan"), None), (x, w, w, 1e-5, "tanh"), (x[:, :0], None, None, 1e-5, None),
+                (x[0, 0], None, None, 1e-5, None), (x, _randn((128,), 1)[::2], None, 1e-5, None)):
+        assert calls.layer_norm_forward(*bad) is None
+    _, mean, rstd = ext.layer_norm_forward(x)
+    assert calls.layer_norm_backward(x, x, mean, rstd, w, w, None, True) is not None
+    for bad in ((x[:4], x, mean, rstd), (x.half(), x, mean, rstd), (x, x, mean[:4], rstd), (x, x, mean, rstd.double()),
+                (x, x, mean.cpu(), rstd), (x.t().contiguous().t(), x, mean, rstd)):
+        assert calls.layer_norm_backward(*bad, w, w, None, True) is None
+    args = _loss_inputs(10, 30, 30, F32, F32, 2)
+    assert calls.policy_value_loss(*args, 1.0, 1.0) is not None
+    for i, bad in ((0, args[0].double()), (0, args[0].unsqueeze(0)), (1, args[1][:3]), (1, args[1].half()),
+                   (2, args[2].int()), (3, args[3][:, ::2]), (3, args[3].double()), (4, args[4].double()),
+                   (5, args[5].cpu()), (6, args[6].unsqueeze(0)), (6, None)):
+        assert calls.policy_value_loss(*[bad if k == i else a for k, a in enumerate(args)], 1.0, 1.0) is None, i
+    p, g = [_randn((64,), 1)], [_randn((64,), 2)]
+    plan = ext.prepare_adamw(p)
+    before = p[0].clone()
+
+    def step(params=p, grads=g, number=1, beta1=0.9, eps=1e-8, scale=None):
+        return calls.adamw_step(params, grads, plan._table_ptr, 0, 32, number, 1e-3, beta1, 0.999, eps, 0.0, scale, 0)
+
+    for bad in (dict(grads=[None]), dict(grads=[g[0][:3]]), dict(grads=[g[0].double()]), dict(grads=[g[0].cpu()]),
+                dict(grads=g + g), dict(number=0), dict(number=1.5), dict(beta1=1.0), dict(eps=-1.0),
+                dict(scale=torch.ones((2,), device="cuda")), dict(scale=1.0), dict(params=[before])):
+        assert step(**bad) is None, bad
+    assert torch.equal(p[0], before) and step() is True and not torch.equal(p[0], before)

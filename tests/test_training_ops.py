@@ -6,6 +6,7 @@ import shutil
 import subprocess
 
 import pytest
+import torch
 
 from hive_neuralnet_amd import hive_gpu, training_ops
 
@@ -118,3 +119,22 @@ def test_sizes_past_a_launch_are_refused():
     two[0] = training_ops.HgAdamwTensor(p, p, p, p, p, p, 4, 0)
     two[1] = training_ops.HgAdamwTensor(p, p, p, p, p, p, (1 << 34) - 1023, 256)
     assert lib.hg_adamw_step(two, 2, 0, 0, 8, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, None, 0, None) == INVALID
+
+
+@pytest.mark.skipif(training_ops._calls is None, reason="_train_calls.so not built")
+def test_native_calls_leave_what_they_do_not_serve():
+    """None, and no error, for arguments that are not plainly right: nothing here is on a GPU."""
+    if os.path.exists(hive_gpu.LIB_PATH):
+        hive_gpu.load_library()
+    calls, x = training_ops._calls, torch.zeros((4, 8))
+    for first in (x, None, "x", 3, [x]):
+        assert calls.layer_norm_forward(first, None, None, 1e-5, None) is None
+        assert calls.layer_norm_backward(first, first, x, x, None, None, "sigmoid", True) is None
+        assert calls.policy_value_loss(first, x, x, x, x, x, x, 1.0, 1.0) is None
+        assert calls.adamw_step([first], [x], 0, 0, 32, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, None, 0) is None
+    assert calls.layer_norm_forward(x, None, None, "eps", None) is None
+    assert calls.layer_norm_forward(x) is None
+    assert calls.adamw_step([], [], 0, 0, 32, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, None, 0) is None
+    assert calls.adamw_step(x, x, 0, 0, 32, 1, 1e-3, 0.9, 0.999, 1e-8, 0.0, None, 0) is None
+    with pytest.raises(TypeError):
+        calls.bind(1, 2)
