@@ -23,7 +23,7 @@
 // Bound by memory.  Measured (MI355X, inputs not in cache): forward 16,384 x
 // 2,048 f32 44 us, 6.1 TB/s; 8,192 x 4,096 bf16 24.5 us, 5.5; 118,271 x 64 f32
 // with the sigmoid 13 us, 4.6; 4,096 x 5,119 bf16, rows at odd addresses, 23
-// us, 3.7.  Backward 76 us, 5.3 TB/s; 39.5 us, 5.1; 21.5 us, 4.2; 40 us, 3.1; 2
+// us, 3.7.  Backward 76 us, 5.3 TB/s; 39.5 us, 5.1; 20.7 us, 4.4; 40 us, 3.1; 2
 // to 4 us of each are the second launch (1.5 more where each of its loads
 // waited for the one before).  The next row is read while this one is worked on
 // (8,192 x 4,096: 26 us without in the forward pass, 61 in the backward) and,
@@ -600,11 +600,14 @@ template <typename Sh> int64_t forward_blocks(int64_t rows) {
     return need < most ? need : most;
 }
 // As many waves as the registers leave room for, 8 a CU where a lane holds two
-// vectors, else 16, and two rows a lane group at least: a block ends with its
-// sums' way through LDS and memory (2,048 x 64: 8.1 us at one row, 8.7 at two,
-// 10.7 at four; 300 x 4,096: 14.5, 12.0, 13.9)
+// vectors, else 16.  A block ends with its sums' way through LDS and memory: a
+// lane group of more than a wave takes two rows at least (300 x 4,096: 12.0 us
+// at one row, 10.1 at two, 10.9 at four); narrower groups are many in a block
+// and take one (5,928 x 113 f16: 8.4 us, 9.4 at two), but two where that saves
+// the second launch (100 x 64: 7.5 and 4.9).
 template <typename Sh> int64_t backward_blocks(int64_t rows) {
-    const int64_t need = (rows + 2 * Sh::kGroups - 1) / (2 * Sh::kGroups);
+    const int64_t two = (rows + 2 * Sh::kGroups - 1) / (2 * Sh::kGroups), one = (rows + Sh::kGroups - 1) / Sh::kGroups;
+    const int64_t need = Sh::kLanes > 64 || two == 1 ? two : one;
     const int64_t most = (int64_t)kCus * (Sh::kVecs == 1 || Sh::kThreads > 512 ? 1024 : 512) / Sh::kThreads;
     return need < most ? need : most;
 }
