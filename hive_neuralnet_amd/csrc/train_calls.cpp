@@ -19,6 +19,7 @@
 
 #include <ATen/ATen.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "hive_gpu.h"
@@ -228,12 +229,23 @@ PyObject* policy_value_loss(PyObject*, PyObject* const* a, Py_ssize_t count) {
     END_HANDLE_TH_ERRORS
 }
 
-// (params, grads, table, param type, state bits, step, lr, beta1, beta2, eps, weight_decay, grad_scale, seed) -> True.
-// `table` is the address of a plan's hg_adamw_tensor array, whose
-// gradients are entered here; none may be left out.
+// What a step writes: the bounds of `count / 2` pieces of memory in order, each's first byte and one past its last.
+struct Written {
+    const uint64_t* bounds = nullptr;
+    Py_ssize_t count = 0;
+    bool apart(const Tensor& t) const {
+        const uint64_t begin = (uint64_t)(uintptr_t)t.const_data_ptr(), end = begin + t.nbytes();
+        const Py_ssize_t i = std::upper_bound(bounds, bounds + count, begin) - bounds;
+        return begin == end || (i % 2 == 0 && (i == count || bounds[i] >= end));
+    }
+};
+
+// (params, grads, table, param type, state bits, step, lr, beta1, beta2, eps, weight_decay, grad_scale, seed[, bounds,
+// their number]) -> True.  `table` is the address of a plan's hg_adamw_tensor array, whose
+// gradients are entered here; none may be left out.  `bounds`: the address of Written's.
 PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t count) {
     HANDLE_TH_ERRORS
-    if (count != 13 || !adamw_ || !PyList_Check(a[0]) || !(PyList_Check(a[1]) || PyTuple_Check(a[1]))) Py_RETURN_NONE;
+    if ((count != 13 && count != 15) || !adamw_ || !PyList_Check(a[0]) || !(PyList_Check(a[1]) || PyTuple_Check(a[1]))) Py_RETURN_NONE;
     Place at;
     auto* table = (hg_adamw_tensor*)PyLong_AsVoidPtr(a[2]);
     const int param_type = (int)PyLong_AsLong(a[3]), bits = (int)PyLong_AsLong(a[4]);
@@ -241,6 +253,8 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const double lr = PyFloat_AsDouble(a[6]), beta1 = PyFloat_AsDouble(a[7]), beta2 = PyFloat_AsDouble(a[8]),
                  eps = PyFloat_AsDouble(a[9]), decay = PyFloat_AsDouble(a[10]);
     const uint32_t seed = (uint32_t)PyLong_AsUnsignedLongMask(a[12]);
+    Written written;
+    if (count == 15) written = {(const uint64_t*)PyLong_AsVoidPtr(a[13]), PyLong_AsSsize_t(a[14])};
     const Py_ssize_t n = PyList_GET_SIZE(a[0]);
     if (bad_number() || n == 0 || PySequence_Fast_GET_SIZE(a[1]) != n || step < 1 ||
         !at.find(tensor(PyList_GET_ITEM(a[0], 0))) ||
@@ -249,7 +263,8 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const float* scale = nullptr;
     if (a[11] != Py_None) {
         const Tensor* t = tensor(a[11]);
-        if (!t || !at.holds(*t) || t->scalar_type() != at::kFloat || t->numel() != 1) Py_RETURN_NONE;
+        if (!t || !at.holds(*t) || t->scalar_type() != at::kFloat || t->numel() != 1 || !written.apart(*t))
+            Py_RETURN_NONE;
         scale = (const float*)t->const_data_ptr();
     }
     int grad_type = -1;
@@ -260,6 +275,7 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t count) {
             Py_RETURN_NONE;
         const int type = type_of(*g);
         if (type < 0 || (i && type != grad_type)) Py_RETURN_NONE;
+        if (!written.apart(*g) && (g->const_data_ptr() != table[i].param || type != param_type)) Py_RETURN_NONE;
         grad_type = type;
         table[i].grad = g->const_data_ptr();
     }

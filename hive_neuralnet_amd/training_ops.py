@@ -12,8 +12,8 @@ autograd functions, an optimizer and a training step of HiveFNN on them.
 """
 from __future__ import annotations
 
+import bisect
 import ctypes
-import math
 
 import numpy as np
 import torch
@@ -268,6 +268,11 @@ def policy_value_loss(self, logits: torch.Tensor, values: torch.Tensor, num_acti
     return losses, dlogits, dvalues
 
 
+def _bytes(t: torch.Tensor):
+    """(first byte, one past the last) of a contiguous tensor."""
+    return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+
+
 class AdamWPlan:
     """hg_adamw_step over a fixed list of tensors, checked and laid out once.
 
@@ -277,7 +282,12 @@ class AdamWPlan:
     exp_avg_sq_scale, a float32 per 256 elements; a code stands for code *
     scale, in exp_avg_sq for the square root of the moment.  The plan enters
     the parameters by address: updates in place are seen, a parameter whose
-    memory is replaced needs a new plan."""
+    memory is replaced needs a new plan.
+
+    A step's blocks run beside each other, so nothing that it writes may be
+    written or read through another of its tensors: parameters and moments
+    that share memory, and gradients that lie in them, are refused (but a
+    gradient that is its own parameter's memory, element for element)."""
 
     def __init__(self, lib, params, state_bits: int = 32, state=None):
         params = list(params)
@@ -313,6 +323,13 @@ class AdamWPlan:
                     not v.is_contiguous():
                 raise ValueError(f"{k} must be a contiguous {t} tensor of {n} values on {dev}")
         self.state = {k: state[k] for k in want}
+        named = [(f"params[{i}]", p) for i, p in enumerate(params)] + list(self.state.items())
+        held = sorted((*_bytes(t), name) for name, t in named if t.numel())
+        for (_, end, a), (begin, _, b) in zip(held, held[1:]):
+            if begin < end:
+                raise ValueError(f"{a} and {b} share memory: a step writes both at once")
+        self._written = [x for begin, end, _ in held for x in (begin, end)]  # in order: inside one past an odd number
+        self._written_table = np.array(self._written, dtype=np.uint64)
         self._table = np.zeros((len(params),), dtype=np.dtype(HgAdamwTensor))
         at = np.array(self.places, dtype=np.uint64)
         size = np.uint64(4 if state_bits == 32 else 1)
@@ -329,8 +346,15 @@ class AdamWPlan:
         self._shapes = [p.shape for p in params]
         self._grad, self._count = self._table["grad"], self._table["count"]
         self._table_ptr = self._table.ctypes.data
+        self._written_ptr = self._written_table.ctypes.data
         self._type = TYPES[params[0].dtype]
         self._device = params[0].get_device()
+
+    def _apart(self, t: torch.Tensor) -> bool:
+        """Whether a step writes nothing of t."""
+        begin, end = _bytes(t)
+        i = bisect.bisect_right(self._written, begin)
+        return begin == end or i % 2 == 0 and (i == len(self._written) or self._written[i] >= end)
 
     def step(self, grads, step: int, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
              weight_decay: float = 0.01, grad_scale: torch.Tensor | None = None, seed: int = 0) -> None:
@@ -342,7 +366,7 @@ class AdamWPlan:
         another one."""
         if _calls is not None and not self._partial and _calls.adamw_step(
                 self.params, grads, self._table_ptr, self._type, self.state_bits, step, lr, betas[0], betas[1], eps,
-                weight_decay, grad_scale, seed & 0xFFFFFFFF):
+                weight_decay, grad_scale, seed & 0xFFFFFFFF, self._written_ptr, len(self._written)):
             return
         if len(grads) != len(self.params):
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
@@ -367,10 +391,15 @@ class AdamWPlan:
             raise ValueError(f"betas must be in [0, 1) and eps not negative, got {betas} and {eps}")
         if [p.data_ptr() for p in self.params] != self._ptrs:
             raise ValueError("a parameter's memory was replaced: make a new plan")
+        for i, (g, p) in enumerate(zip(grads, self.params)):
+            if g is not None and not self._apart(g) and (g.data_ptr() != p.data_ptr() or g.dtype != p.dtype):
+                raise ValueError(f"the gradient of params[{i}] shares memory with a parameter or moment")
         scale = None
         if grad_scale is not None:
             if grad_scale.numel() != 1 or grad_scale.dtype != torch.float32 or grad_scale.get_device() != dev:
                 raise ValueError(f"grad_scale must be one float32 value on device {dev}")
+            if not self._apart(grad_scale):
+                raise ValueError("grad_scale lies in memory that the step writes")
             scale = grad_scale.data_ptr()
         self._grad[:] = ptrs
         missing = 0 in ptrs and any(g is None for g in grads)

@@ -563,6 +563,9 @@ int hg_policy_value_loss(const void* logits, int type, int64_t N, const void* va
  * float scale: exp_avg = code * scale, exp_avg_sq = (code * scale)^2; new values
  * are rounded to a neighbouring code at random, by bits that depend on `seed`
  * and `place` + the element's index alone (place: a multiple of the block).
+ * No tensor's param and moments may share memory with another's, nor with any
+ * gradient but the param's own, element for element: the blocks that step them
+ * run beside each other.
  * A tensor has under 2^34 elements (count <= 2^34 - 1024). */
 #define HG_ADAMW_BLOCK 256
 typedef struct hg_adamw_tensor {

@@ -280,3 +280,11 @@ def test_training_command(capsys, monkeypatch):
     training.main()
     lines = capsys.readouterr().out.strip().splitlines()
     assert len(lines) == 3 and "policy" in lines[0]
+
+
+def test_optimizer_refuses_a_weight_twice():
+    """A weight that is listed twice would be stepped by two blocks at once."""
+    from hive_neuralnet_amd.training import AdamW
+    p = torch.nn.Parameter(_randn((9,), 1))
+    with pytest.warns(UserWarning, match="duplicate"), pytest.raises(ValueError, match="share memory"):
+        AdamW([p, p])

@@ -832,3 +832,41 @@ def test_native_calls_serve_plain_arguments_and_leave_the_rest(ext):
                 dict(scale=torch.ones((2,), device="cuda")), dict(scale=1.0), dict(params=[before])):
         assert step(**bad) is None, bad
     assert torch.equal(p[0], before) and step() is True and not torch.equal(p[0], before)
+
+
+@pytest.mark.parametrize("native", [True, False], ids=["native", "python"])
+def test_adamw_refuses_memory_that_a_step_writes_twice(ext, native, monkeypatch):
+    """The same weight twice, slices that overlap, one tensor as both moments, moments in a weight's memory, and
+    gradients or a scale that lie in what the step writes; nothing is launched.  Slices side by side are served, and a
+    gradient that is its own weight's memory."""
+    from hive_neuralnet_amd import training_ops
+    if not native:
+        monkeypatch.setattr(training_ops, "_calls", None)
+    flat = _randn((1024,), 1)
+    other = _randn((256,), 2)
+    zeros = torch.zeros((512,), device="cuda")
+    inside = torch.zeros((1024,), device="cuda")
+    for params, state, word in (
+            ([other, other], None, r"params\[0\] and params\[1\]"), ([flat[:300], flat[299:]], None, "share memory"),
+            ([flat[100:200], flat], None, "share memory"), ([flat, other, flat[5:6]], None, "share memory"),
+            ([flat[:300]], {"exp_avg": zeros, "exp_avg_sq": zeros}, "exp_avg_sq"),
+            ([inside[700:1000]], {"exp_avg": inside[:512], "exp_avg_sq": inside[256:768]}, "share memory"),
+            ([inside[500:800]], {"exp_avg": inside[:512], "exp_avg_sq": zeros}, r"exp_avg and params\[0\]")):
+        with pytest.raises(ValueError, match=word):
+            ext.prepare_adamw(params, 32, state)
+    p = [flat[:300], flat[300:], torch.empty((0,), device="cuda"), other]
+    plan = ext.prepare_adamw(p)
+    before = flat.clone()
+    g = [torch.ones_like(t) for t in p]
+    for grads, kw in (([flat[1:301], *g[1:]], {}), ([*g[:3], flat[:256]], {}), ([*g[:3], flat[768:]], {}),
+                      ([*g[:3], plan.state["exp_avg"][5:261]], {}), (g, {"grad_scale": flat[300:301]}),
+                      (g, {"grad_scale": plan.state["exp_avg_sq"][:1]})):
+        with pytest.raises(ValueError, match="memory"):
+            plan.step(grads, 1, **kw)
+    with pytest.raises(ValueError, match="memory"):  # at its weight's address, but not element for element
+        ext.prepare_adamw([flat]).step([flat[:512].view(BF16)], 1)
+    assert torch.equal(flat, before)
+    plan.step([p[0], g[1], g[2], p[3]], 1, **HYPER)  # a gradient that is the weight itself
+    zero = torch.zeros((1,), dtype=torch.float64, device="cuda")
+    want, _, _ = _adamw_reference(before[:300].double(), before[:300].double(), zero, zero, 1)
+    _close(p[0], want, 4 * U * before[:300].double().abs() + HYPER["lr"] * 16 * U, "own memory")
