@@ -76,19 +76,21 @@ def policy_value_loss(logits, values, num_actions, policy_targets, policy_weight
 class AdamW(torch.optim.Optimizer):
     """AdamW with decoupled weight decay, all parameters of a group and type
     in one launch, the moments in 32 bits or, with state_bits=8, in 8
-    (AdamWPlan).  A parameter without a gradient is left as it is; the step's
-    number counts the optimizer's steps.  `seed` seeds the rounding of 8-bit
-    moments; each step takes the next one."""
+    (AdamWPlan).  A parameter without a gradient is left as it is, and the
+    bias correction is that of the steps it has taken itself (parameters of
+    one group and type that have taken different numbers of them take a
+    launch each number).  `seed` seeds the rounding of 8-bit moments; each
+    step takes the next one."""
 
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
                  state_bits: int = 32, seed: int = 0):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
         self._ext = hive_gpu.load_extension()
         self.state_bits, self.seed, self.steps = state_bits, int(seed), 0
-        self._plans: list = []  # (group, plan)
+        self._plans: list = []  # (group, plan, the steps that each of its parameters has taken)
         self._make_plans(None)
 
-    def _make_plans(self, states) -> None:
+    def _make_plans(self, states, taken=None) -> None:
         plans = []
         for group in self.param_groups:
             by_type: dict = {}
@@ -100,7 +102,8 @@ class AdamW(torch.optim.Optimizer):
                     if len(plans) >= len(states):
                         raise ValueError("the saved state has fewer parameter lists than the optimizer")
                     state = {k: v.to(members[0].device, copy=True) for k, v in states[len(plans)].items()}
-                plans.append((group, self._ext.prepare_adamw(members, self.state_bits, state)))
+                plan = self._ext.prepare_adamw(members, self.state_bits, state)
+                plans.append((group, plan, [0] * len(members) if taken is None else list(taken[len(plans)])))
         if states is not None and len(states) != len(plans):
             raise ValueError(f"the saved state has {len(states)} parameter lists, the optimizer {len(plans)}")
         self._plans = plans
@@ -119,27 +122,35 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         self.steps += 1
-        for group, plan in self._plans:
+        for group, plan, taken in self._plans:
             grads = [None if p.grad is None else p.grad.contiguous() for p in plan.params]
-            plan.step(grads, self.steps, lr=group["lr"], betas=group["betas"], eps=group["eps"],
-                      weight_decay=group["weight_decay"], grad_scale=grad_scale, seed=self.seed + self.steps)
+            numbers = {n for n, g in zip(taken, grads) if g is not None}
+            for number in numbers:
+                now = grads if len(numbers) == 1 else [g if n == number else None for n, g in zip(taken, grads)]
+                plan.step(now, number + 1, lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                          weight_decay=group["weight_decay"], grad_scale=grad_scale, seed=self.seed + self.steps)
+            taken[:] = [n if g is None else n + 1 for n, g in zip(taken, grads)]
             for p, g in zip(plan.params, grads):  # autograd sees that a weight it saved has changed
                 if g is not None:
                     torch.autograd.graph.increment_version(p)
         return loss
 
     def state_dict(self):
-        """The moments as they are held, the step's number, the groups' settings."""
+        """The moments as they are held, the numbers of steps, the groups' settings."""
         groups = [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups]
         return {"state_bits": self.state_bits, "seed": self.seed, "steps": self.steps,
-                "states": [dict(plan.state) for _, plan in self._plans], "param_groups": groups}
+                "states": [dict(plan.state) for _, plan, _ in self._plans],
+                "taken": [list(taken) for _, _, taken in self._plans], "param_groups": groups}
 
     def load_state_dict(self, state_dict) -> None:
         if state_dict["state_bits"] != self.state_bits:
             raise ValueError(f"the saved moments are in {state_dict['state_bits']} bits, these in {self.state_bits}")
         if len(state_dict["param_groups"]) != len(self.param_groups):
             raise ValueError(f"{len(state_dict['param_groups'])} saved groups, {len(self.param_groups)} here")
-        self._make_plans(state_dict["states"])
+        taken = state_dict.get("taken")  # None: saved when one number served all
+        if taken is None:
+            taken = [[state_dict["steps"]] * len(plan.params) for _, plan, _ in self._plans]
+        self._make_plans(state_dict["states"], taken)
         for group, saved in zip(self.param_groups, state_dict["param_groups"]):
             group.update(saved)
         self.seed, self.steps = state_dict["seed"], state_dict["steps"]

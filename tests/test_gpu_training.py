@@ -288,3 +288,62 @@ def test_optimizer_refuses_a_weight_twice():
     p = torch.nn.Parameter(_randn((9,), 1))
     with pytest.warns(UserWarning, match="duplicate"), pytest.raises(ValueError, match="share memory"):
         AdamW([p, p])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_optimizer_counts_each_parameters_steps(bits):
+    """Parameters whose gradients come late or now and then: the bias correction is that of a parameter's own steps.
+    A first step moves a weight by lr and its decay whenever it comes (m / sqrt(v) is the gradient's sign); in 32 bits
+    all steps are compared with torch.optim.AdamW in 64 (16 u of lr and 4 u of the weight a step)."""
+    from hive_neuralnet_amd.training import AdamW
+    shapes, every = [(64, 3), (300,), (1,), (33,)], [1, 7, 3, 1]
+    a = [torch.nn.Parameter(_randn(s, i)) for i, s in enumerate(shapes)]
+    b = [torch.nn.Parameter(p.detach().double()) for p in a]
+    ours, theirs = AdamW(a, lr=1e-2, state_bits=bits), torch.optim.AdamW(b, lr=1e-2)
+    for k in range(1, 22):
+        for i, (p, q) in enumerate(zip(a, b)):
+            p.grad = _randn(p.shape, 100 * k + i) if k % every[i] == 0 else None
+            q.grad = None if p.grad is None else p.grad.double()
+        before = a[1].detach().clone()
+        ours.step()
+        theirs.step()
+        if k == 7:
+            want = before.double() * (1.0 - 1e-4) - 1e-2 * torch.sign(a[1].grad.double())
+            bound = 16 * U * 1e-2 + 4 * U * before.double().abs() + 1e-2 * 1e-8 / a[1].grad.double().abs()
+            assert ((a[1].detach().double() - want).abs() <= bound).all()
+    if bits == 32:
+        for p, q in zip(a, b):
+            bound = 21 * (16 * U * 1e-2 + 4 * U * float(q.detach().abs().max()))
+            assert float((p.detach().double() - q.detach()).abs().max()) < bound
+
+
+def test_optimizer_state_holds_each_parameters_steps():
+    """Saved and loaded, the counts go on; a state without them (one count for all) still loads."""
+    from hive_neuralnet_amd.training import AdamW
+
+    def make():
+        ps = [torch.nn.Parameter(_randn(s, i)) for i, s in enumerate([(40, 9), (300,)])]
+        return ps, AdamW(ps, lr=1e-2)
+
+    def steps(ps, opt, ks):
+        for k in ks:
+            ps[0].grad = _randn(ps[0].shape, 50 * k)
+            ps[1].grad = _randn(ps[1].shape, 50 * k + 1) if k >= 2 else None
+            opt.step()
+
+    a, opt_a = make()
+    steps(a, opt_a, range(6))
+    b, opt_b = make()
+    steps(b, opt_b, range(3))
+    saved = opt_b.state_dict()
+    c, opt_c = make()
+    for p, q in zip(c, b):
+        p.data.copy_(q.data)
+    opt_c.load_state_dict(saved)
+    steps(c, opt_c, range(3, 6))
+    for p, q in zip(a, c):
+        assert torch.equal(p, q)
+    d, opt_d = make()
+    opt_d.load_state_dict({k: saved[k] for k in ("state_bits", "seed", "steps", "states", "param_groups")})
+    assert opt_d.steps == 3
+    steps(d, opt_d, range(3, 4))
