@@ -121,18 +121,18 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        self.steps += 1
+        seed = self.seed + self.steps + 1
         for group, plan, taken in self._plans:
             grads = [None if p.grad is None else p.grad.contiguous() for p in plan.params]
-            numbers = {n for n, g in zip(taken, grads) if g is not None}
-            for number in numbers:
-                now = grads if len(numbers) == 1 else [g if n == number else None for n, g in zip(taken, grads)]
+            for number in sorted({n for n, g in zip(taken, grads) if g is not None}, reverse=True):
+                now = [g if n == number else None for n, g in zip(taken, grads)]
                 plan.step(now, number + 1, lr=group["lr"], betas=group["betas"], eps=group["eps"],
-                          weight_decay=group["weight_decay"], grad_scale=grad_scale, seed=self.seed + self.steps)
-            taken[:] = [n if g is None else n + 1 for n, g in zip(taken, grads)]
+                          weight_decay=group["weight_decay"], grad_scale=grad_scale, seed=seed)
+                taken[:] = [n if g is None else n + 1 for n, g in zip(taken, now)]
             for p, g in zip(plan.params, grads):  # autograd sees that a weight it saved has changed
                 if g is not None:
                     torch.autograd.graph.increment_version(p)
+        self.steps += 1
         return loss
 
     def state_dict(self):

@@ -347,3 +347,19 @@ def test_optimizer_state_holds_each_parameters_steps():
     opt_d.load_state_dict({k: saved[k] for k in ("state_bits", "seed", "steps", "states", "param_groups")})
     assert opt_d.steps == 3
     steps(d, opt_d, range(3, 4))
+
+
+def test_optimizer_does_not_count_a_refused_step():
+    from hive_neuralnet_amd.training import AdamW
+    p = [torch.nn.Parameter(_randn((9,), 1)), torch.nn.Parameter(_randn((4,), 2))]
+    opt = AdamW(p, lr=1e-2)
+    for t in p:
+        t.grad = torch.ones_like(t)
+    before = [t.detach().clone() for t in p]
+    with pytest.raises(ValueError, match="grad_scale"):
+        opt.step(grad_scale=torch.ones((2,), device="cuda"))
+    assert opt.steps == 0
+    opt.step()
+    for t, q in zip(p, before):  # a first step: lr and the decay
+        want = q.double() * (1.0 - 1e-4) - 1e-2
+        assert ((t.detach().double() - want).abs() <= 16 * U * 1e-2 + 4 * U * q.double().abs() + 1e-10).all()
