@@ -51,6 +51,9 @@ def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, activ
 class _PolicyValueLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, values, num_actions, targets, pw, vt, vw, value_coef, loss_scale):
+        # the gradient is held in 32 bits, so that what comes in (a scaler's factor) meets it before it is rounded
+        ctx.types = logits.dtype, values.dtype
+        logits, values = (t.float() if t.dtype in (torch.float16, torch.bfloat16) else t for t in (logits, values))
         losses, dlogits, dvalues = hive_gpu.load_extension().policy_value_loss(
             logits, values, num_actions, targets, pw, vt, vw, value_coef, loss_scale)
         ctx.save_for_backward(dlogits, dvalues)
@@ -62,13 +65,15 @@ class _PolicyValueLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, _policy, _value):
         dlogits, dvalues = ctx.saved_tensors
-        return (dlogits * grad).to(dlogits.dtype), (dvalues * grad).to(dvalues.dtype), *([None] * 7)
+        return (dlogits * grad).to(ctx.types[0]), (dvalues * grad).to(ctx.types[1]), *([None] * 7)
 
 
 def policy_value_loss(logits, values, num_actions, policy_targets, policy_weights, value_targets, value_weights,
                       value_coef: float = 1.0, loss_scale: float = 1.0):
     """(total, policy, value) of HiveGpuExtension.policy_value_loss; total is
-    differentiable in logits and values (its gradients times loss_scale)."""
+    differentiable in logits and values (its gradients times loss_scale, which
+    total itself is not multiplied by; rounded to 16 bits once, after the
+    incoming gradient, so that a scaled total needs no loss_scale)."""
     return _PolicyValueLoss.apply(logits, values, num_actions, policy_targets, policy_weights, value_targets,
                                   value_weights, value_coef, loss_scale)
 

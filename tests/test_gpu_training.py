@@ -363,3 +363,27 @@ def test_optimizer_does_not_count_a_refused_step():
     for t, q in zip(p, before):  # a first step: lr and the decay
         want = q.double() * (1.0 - 1e-4) - 1e-2
         assert ((t.detach().double() - want).abs() <= 16 * U * 1e-2 + 4 * U * q.double().abs() + 1e-10).all()
+
+
+@pytest.mark.parametrize("t", [torch.float16, torch.bfloat16], ids=str)
+def test_loss_autograd_in_16_bits_is_rounded_once(t):
+    """The gradient times what comes in, a scaler's factor, rounded to the logits' type once: 2,048 positions' shares
+    of small probabilities are below half precision's smallest numbers before the factor.  Off by half a unit of the
+    type and by what the float32 gradient is: (longest / 64 + 64) 4 u of a position's share, 8 u of a value's."""
+    from hive_neuralnet_amd.training import policy_value_loss
+    B, K, coming = 2048, 64, 3.0 * 2.0 ** 12
+    half, tiny = (2.0 ** -11, 2.0 ** -25) if t == torch.float16 else (2.0 ** -8, 2.0 ** -134)
+    n = torch.full((B,), K, device="cuda")
+    logits, values = (3.0 * _randn((B * K,), 1)).to(t).requires_grad_(), torch.tanh(_randn((B, 1), 2)).to(t).requires_grad_()
+    targets = torch.softmax(4.0 * _randn((B, K), 3), 1)
+    ones, vt = torch.ones((B,), device="cuda"), _randn((B,), 4)
+    total, _, _ = policy_value_loss(logits, values, n, targets, ones, vt, ones, 0.5)
+    dx, dv = torch.autograd.grad(coming * total, (logits, values))
+    assert dx.dtype == t and dv.dtype == t
+    x, v = logits.detach().double().view(B, K), values.detach().double().view(-1)
+    q = targets.double()
+    want = coming / B * (torch.softmax(x, 1) * q.sum(1, keepdim=True) - q).view(-1)
+    want_v = (coming / B * (v - vt.double())).view(-1, 1)
+    for got, exact, bound in ((dx, want, coming / B * (K / 64 + 64) * 4 * U), (dv, want_v, 8 * U * want_v.abs())):
+        over = (got.double() - exact).abs() - half * exact.abs() - tiny - bound
+        assert float(over.max()) <= 0.0, float(over.max())
