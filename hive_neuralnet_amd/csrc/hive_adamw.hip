@@ -85,12 +85,12 @@ __device__ __forceinline__ void store_four(T* p, int live, typename Four<T>::typ
         if (i < live) p[i] = q[i];
 }
 
-// sqrt(v) to half a unit of the last place, 0 for 0; a v below the smallest
-// normal number counts as that
+// sqrt(v) to half a unit of the last place, 0 for 0 and inf for inf (a step by
+// m / inf = 0); a v below the smallest normal number counts as that
 __device__ __forceinline__ float root(float v) {
     const float w = v < 0x1p-126f ? 0x1p-126f : v, y = __builtin_amdgcn_rsqf(w), s = w * y;
     const float r = fmaf(fmaf(-s, s, w), 0.5f * y, s);
-    return v == 0.0f ? 0.0f : r;
+    return v == 0.0f || v == INFINITY ? v : r;
 }
 // the largest of a wave's |x|, NaN if one is: their bits are in order
 __device__ __forceinline__ uint32_t size_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }

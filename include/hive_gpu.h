@@ -563,6 +563,9 @@ int hg_policy_value_loss(const void* logits, int type, int64_t N, const void* va
  * float scale: exp_avg = code * scale, exp_avg_sq = (code * scale)^2; new values
  * are rounded to a neighbouring code at random, by bits that depend on `seed`
  * and `place` + the element's index alone (place: a multiple of the block).
+ * A gradient whose square passes float's range makes v inf, its weight steps by
+ * 0 from then on; in 8 bits the scale of v is then inf and v of all 256 elements
+ * under it inf or NaN.  An inf or NaN gradient does the same to exp_avg.
  * No tensor's param and moments may share memory with another's, nor with any
  * gradient but the param's own, element for element: the blocks that step them
  * run beside each other.

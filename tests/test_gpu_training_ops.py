@@ -870,3 +870,23 @@ def test_adamw_refuses_memory_that_a_step_writes_twice(ext, native, monkeypatch)
     zero = torch.zeros((1,), dtype=torch.float64, device="cuda")
     want, _, _ = _adamw_reference(before[:300].double(), before[:300].double(), zero, zero, 1)
     _close(p[0], want, 4 * U * before[:300].double().abs() + HYPER["lr"] * 16 * U, "own memory")
+
+
+@pytest.mark.parametrize("t", [F32, BF16], ids=str)
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_of_a_square_past_float32(ext, bits, t):
+    """A finite gradient whose square is inf: the formula's update is m / inf = 0, the weight only decays; the
+    others of its 256 are stepped as ever (the terms of test_adamw_step)."""
+    p, g = _randn((600,), 1, 0.5), _randn((600,), 2).to(t)
+    g[[7, 300, 599]] = torch.tensor([1e20, -3e38, 2e19], device="cuda").to(t)
+    before = p.clone()
+    plan = ext.prepare_adamw([p], state_bits=bits)
+    plan.step([g], 1, **HYPER)
+    zero = torch.zeros((1,), dtype=torch.float64, device="cuda")
+    want, _, _ = _adamw_reference(before.double(), g.double(), zero, zero, 1)
+    keep = before.double() * (1.0 - HYPER["lr"] * HYPER["weight_decay"])
+    want = torch.where(torch.isinf(g.float() * g.float()), keep, want)
+    _close(p, want, 4 * U * before.double().abs() + HYPER["lr"] * 16 * U, "params")
+    _, v = _moments(plan.state, 0, 600)
+    assert not torch.isfinite(v[[7, 300, 599]]).any()
+    assert bits == 8 or torch.isfinite(v[[0, 6, 8, 301, 598]]).all()
