@@ -210,7 +210,7 @@ k_norm_forward(const typename Sh::T* __restrict__ x, int64_t rows, int cols, int
             for (int i = 0; i < n; i++) s[0] += a[k][i];
         }
         row_sums<Sh>(s, lds, turn);
-        const float m = s[0] * inv;
+        const float m = s[0] / (float)cols;  // a product with the rounded 1 / cols would miss a constant row's value
         s[0] = 0.0f;
 #pragma unroll
         for (int k = 0; k < Sh::kVecs; k++) {
@@ -316,7 +316,7 @@ k_norm_backward(const typename Sh::T* __restrict__ dy, int64_t dy_stride, const 
             raw[k] = next[k];
             raw_dy[k] = next_dy[k];
         }
-        const float m = next_m, r = next_r, mr = m * r;
+        const float m = next_m, r = next_r;
         if (Sh::kAhead && base + step < rows) fetch(row + step);
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
@@ -336,7 +336,7 @@ k_norm_backward(const typename Sh::T* __restrict__ dy, int64_t dy_stride, const 
             if constexpr (Sh::kSumsInLds) load_sums(k);
 #pragma unroll
             for (int i = 0; i < n; i++) {
-                const float h = fmaf(a[i], r, -mr);
+                const float h = (a[i] - m) * r;  // not a r - m r: far from zero the rounding of m r is not small
                 const float d = to_f32<typename Sh::T>(raw_dy[k][i]), dh = d * wv[k][i];
                 sw[k][i] = fmaf(d, h, sw[k][i]);
                 sb[k][i] += d;
@@ -347,7 +347,7 @@ k_norm_backward(const typename Sh::T* __restrict__ dy, int64_t dy_stride, const 
         }
         row_sums<Sh>(s, lds, turn);
         if (!there || !dx) continue;
-        const float r2 = r * r * (s[1] * inv), r1 = fmaf(m, r2, -r * (s[0] * inv));
+        const float r2 = r * r * (s[1] * inv), r1 = r * (s[0] * inv);
 #pragma unroll
         for (int k = 0; k < Sh::kVecs; k++) {
             const int c = (lane + k * Sh::kLanes) * n, live = cols - c;
@@ -368,7 +368,7 @@ k_norm_backward(const typename Sh::T* __restrict__ dy, int64_t dy_stride, const 
             }
 #pragma unroll
             for (int i = 0; i < n; i++)  // r (dh - s1 - h s2)
-                da[i] = fmaf(to_f32<typename Sh::T>(q_dy[i]), r * wv[k][i], fmaf(a[i], -r2, r1));
+                da[i] = fmaf(to_f32<typename Sh::T>(q_dy[i]), r * wv[k][i], fmaf(a[i] - m, -r2, -r1));
             if (sigmoid) {
                 skipped();
 #pragma unroll

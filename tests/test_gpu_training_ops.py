@@ -890,3 +890,39 @@ def test_adamw_of_a_square_past_float32(ext, bits, t):
     _, v = _moments(plan.state, 0, 600)
     assert not torch.isfinite(v[[7, 300, 599]]).any()
     assert bits == 8 or torch.isfinite(v[[0, 6, 8, 301, 598]]).all()
+
+
+@pytest.mark.parametrize("t", [F32, F16, BF16], ids=str)
+@pytest.mark.parametrize("cols", [7, 15, 30, 60, 61, 63, 122, 1001, 2047])
+def test_layer_norm_constant_rows(ext, cols, t):
+    """Rows of one value whose sum float32 holds exactly (a multiple of 16 below 2^28): their mean is that value,
+    so y is the bias, and what the backward pass takes from h, the weight's gradient, is 0."""
+    x = torch.tensor([10000.0, -30000.0, 16.0], device="cuda").to(t).unsqueeze(1).repeat(1, cols)
+    w, b, dy = _randn((cols,), 1), _randn((cols,), 2), _randn((3, cols), 3, 1.0, t)
+    y, mean, rstd = ext.layer_norm_forward(x, w, b)
+    assert torch.equal(mean, x[:, 0].float()) and torch.equal(y, b.to(t).expand(3, cols))
+    _close(rstd, torch.full((3,), 1e-5, dtype=torch.float64, device="cuda").rsqrt(), 4 * U * 317, "rstd")
+    dx, dw, db = ext.layer_norm_backward(dy, x, mean, rstd, w, b)
+    assert not dw.any()
+    dh = dy.double() * w.double()
+    want = rstd.double().unsqueeze(1) * (dh - dh.mean(1, keepdim=True))
+    bound = rstd.double().unsqueeze(1) * (dh.abs() + dh.abs().mean(1, keepdim=True)) * (cols / 64 + 24) * U
+    _close(dx, want, bound, "dx")
+
+
+@pytest.mark.parametrize("cols", [60, 1001, 4096])
+def test_layer_norm_backward_far_from_zero(ext, cols):
+    """h as the distance from the mean over the deviation, which far from zero the rounding of mean * rstd is not
+    part of.  Against 64 bits from the same mean and rstd: h is 3 u off, a sum of R rows (R + 6) u of its terms, a
+    row's sums (C / 64 + 24) u of theirs; dy goes along with h, so that dx has its share of h."""
+    x = _randn((3, cols), 1) + 1000.0
+    _, mean, rstd = ext.layer_norm_forward(x)
+    h = (x.double() - mean.double().unsqueeze(1)) * rstd.double().unsqueeze(1)
+    dy, w = (h + _randn((3, cols), 2, 0.1)).float(), _randn((cols,), 3, 0.1) + 1.0
+    dx, dw, _ = ext.layer_norm_backward(dy, x, mean, rstd, w, w)
+    _close(dw, (dy.double() * h).sum(0), 9 * U * (dy.double() * h).abs().sum(0), "dw")
+    dh = dy.double() * w.double()
+    s1, s2 = dh.mean(1, keepdim=True), (dh * h).mean(1, keepdim=True)
+    size = dh.abs() + dh.abs().mean(1, keepdim=True) + h.abs() * (dh * h).abs().mean(1, keepdim=True)
+    _close(dx, rstd.double().unsqueeze(1) * (dh - s1 - h * s2),
+           rstd.double().unsqueeze(1) * size * (cols / 64 + 24) * U, "dx")
