@@ -282,6 +282,10 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t count) {
     const int e =
         adamw_(table, n, param_type, grad_type, bits, step, lr, beta1, beta2, eps, decay, scale, seed, at.stream);
     if (e) return failed("adamw_step", e);
+    for (Py_ssize_t i = 0; i < n; i++) {  // autograd finds that a weight it saved has changed
+        const Tensor* p = tensor(PyList_GET_ITEM(a[0], i));
+        if (!p->is_inference()) p->unsafeGetTensorImpl()->bump_version();
+    }
     Py_RETURN_TRUE;
     END_HANDLE_TH_ERRORS
 }

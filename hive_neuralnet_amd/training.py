@@ -134,9 +134,6 @@ class AdamW(torch.optim.Optimizer):
                 plan.step(now, number + 1, lr=group["lr"], betas=group["betas"], eps=group["eps"],
                           weight_decay=group["weight_decay"], grad_scale=grad_scale, seed=seed)
                 taken[:] = [n if g is None else n + 1 for n, g in zip(taken, now)]
-            for p, g in zip(plan.params, grads):  # autograd sees that a weight it saved has changed
-                if g is not None:
-                    torch.autograd.graph.increment_version(p)
         self.steps += 1
         return loss
 

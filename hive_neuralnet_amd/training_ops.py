@@ -363,7 +363,8 @@ class AdamWPlan:
         leaves its parameter and moments as they are).  grad_scale: a float32
         tensor of one value that multiplies the gradients (1 / the loss scale, a
         clipping factor).  seed: of the 8-bit moments' rounding; give each step
-        another one."""
+        another one.  The stepped parameters' versions rise: autograd finds that
+        a weight it saved has changed."""
         if _calls is not None and not self._partial and _calls.adamw_step(
                 self.params, grads, self._table_ptr, self._type, self.state_bits, step, lr, betas[0], betas[1], eps,
                 weight_decay, grad_scale, seed & 0xFFFFFFFF, self._written_ptr, len(self._written)):
@@ -409,6 +410,9 @@ class AdamWPlan:
         _check(self._lib.hg_adamw_step(
             self._table_ptr, len(grads), self._type, TYPES[kind], self.state_bits, step, lr, betas[0], betas[1], eps,
             weight_decay, scale, seed & 0xFFFFFFFF, _raw_stream(dev)), "adamw_step")
+        for p, g in zip(self.params, grads):
+            if g is not None and not p.is_inference():
+                torch.autograd.graph.increment_version(p)
 
 
 def prepare_adamw(self, params, state_bits: int = 32, state=None) -> AdamWPlan:

@@ -926,3 +926,30 @@ def test_layer_norm_backward_far_from_zero(ext, cols):
     size = dh.abs() + dh.abs().mean(1, keepdim=True) + h.abs() * (dh * h).abs().mean(1, keepdim=True)
     _close(dx, rstd.double().unsqueeze(1) * (dh - s1 - h * s2),
            rstd.double().unsqueeze(1) * size * (cols / 64 + 24) * U, "dx")
+
+
+@pytest.mark.parametrize("native", [True, False], ids=["native", "python"])
+def test_adamw_step_raises_the_weights_versions(ext, native, monkeypatch):
+    """A weight that autograd saved before a step of the plan is known to have changed; one left out has not."""
+    from hive_neuralnet_amd import training_ops
+    if not native:
+        monkeypatch.setattr(training_ops, "_calls", None)
+    a, b = _randn((8, 8), 1), _randn((5,), 2)
+    plan = ext.prepare_adamw([a, b])
+    x = _randn((8, 8), 3).requires_grad_()
+    y, z = (x @ a).sum(), (x[0, :5] * b).sum()
+    versions = a._version, b._version
+    plan.step([torch.ones_like(a), None], 1)
+    assert a._version > versions[0] and b._version == versions[1]
+    z.backward()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    versions = a._version, b._version
+    plan.step([torch.ones_like(a), torch.ones_like(b)], 2)
+    plan.step([torch.ones_like(a), torch.ones_like(b)], 3)
+    assert a._version >= versions[0] + 2 and b._version >= versions[1] + 2
+    with torch.inference_mode():  # tensors without a version
+        c = _randn((5,), 4)
+        before = c.clone()
+        ext.prepare_adamw([c]).step([torch.ones_like(c)], 1)
+        assert not torch.equal(c, before)
