@@ -245,7 +245,9 @@ struct Written {
 // gradients are entered here; none may be left out.  `bounds`: the address of Written's.
 PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t count) {
     HANDLE_TH_ERRORS
-    if ((count != 13 && count != 15) || !adamw_ || !PyList_Check(a[0]) || !(PyList_Check(a[1]) || PyTuple_Check(a[1]))) Py_RETURN_NONE;
+    if ((count != 13 && count != 15) || !adamw_ || !PyList_Check(a[0]) ||
+        !(PyList_Check(a[1]) || PyTuple_Check(a[1])))
+        Py_RETURN_NONE;
     Place at;
     auto* table = (hg_adamw_tensor*)PyLong_AsVoidPtr(a[2]);
     const int param_type = (int)PyLong_AsLong(a[3]), bits = (int)PyLong_AsLong(a[4]);
@@ -277,8 +279,9 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t count) {
         if (type < 0 || (i && type != grad_type)) Py_RETURN_NONE;
         if (!written.apart(*g) && (g->const_data_ptr() != table[i].param || type != param_type)) Py_RETURN_NONE;
         grad_type = type;
-        table[i].grad = g->const_data_ptr();
     }
+    for (Py_ssize_t i = 0; i < n; i++)  // once all of them are served: a call that is left changes nothing
+        table[i].grad = tensor(PySequence_Fast_GET_ITEM(a[1], i))->const_data_ptr();
     const int e =
         adamw_(table, n, param_type, grad_type, bits, step, lr, beta1, beta2, eps, decay, scale, seed, at.stream);
     if (e) return failed("adamw_step", e);

@@ -953,3 +953,16 @@ def test_adamw_step_raises_the_weights_versions(ext, native, monkeypatch):
         before = c.clone()
         ext.prepare_adamw([c]).step([torch.ones_like(c)], 1)
         assert not torch.equal(c, before)
+
+
+def test_native_step_enters_no_gradient_of_a_list_it_leaves(ext):
+    """A call that is given back to Python has changed nothing, the plan's table among it."""
+    from hive_neuralnet_amd import training_ops
+    p, g = [_randn((64,), 1), _randn((9,), 2)], [_randn((64,), 3), _randn((9,), 4)]
+    plan = ext.prepare_adamw(p)
+    plan.step(g, 1)
+    held = plan._table.copy()
+    for bad in (g[1].double(), g[1].half(), g[1][:4], g[1].cpu(), None):
+        assert training_ops._calls.adamw_step(p, [g[0].clone(), bad], plan._table_ptr, 0, 32, 2, 1e-3, 0.9, 0.999, 1e-8,
+                                              0.0, None, 0) is None
+        assert (plan._table == held).all()
