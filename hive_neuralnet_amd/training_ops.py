@@ -322,6 +322,8 @@ class AdamWPlan:
             if not isinstance(v, torch.Tensor) or v.device != dev or v.dtype != t or tuple(v.shape) != (n,) or \
                     not v.is_contiguous():
                 raise ValueError(f"{k} must be a contiguous {t} tensor of {n} values on {dev}")
+            if v.data_ptr() % 4:
+                raise ValueError(f"{k} must be 4-byte aligned: codes are read four at a time")
         self.state = {k: state[k] for k in want}
         named = [(f"params[{i}]", p) for i, p in enumerate(params)] + list(self.state.items())
         held = sorted((*_bytes(t), name) for name, t in named if t.numel())

@@ -966,3 +966,13 @@ def test_native_step_enters_no_gradient_of_a_list_it_leaves(ext):
         assert training_ops._calls.adamw_step(p, [g[0].clone(), bad], plan._table_ptr, 0, 32, 2, 1e-3, 0.9, 0.999, 1e-8,
                                               0.0, None, 0) is None
         assert (plan._table == held).all()
+
+
+def test_adamw_refuses_codes_at_odd_addresses(ext):
+    """Codes are read four at a time: a state of another alignment is refused when the plan is made."""
+    p = [_randn((300,), 1)]
+    state = ext.prepare_adamw(p, state_bits=8).state
+    for key in ("exp_avg", "exp_avg_sq"):
+        odd = torch.zeros((513,), dtype=torch.float8_e4m3fn, device="cuda")[1:]
+        with pytest.raises(ValueError, match="4-byte aligned"):
+            ext.prepare_adamw(p, 8, {**state, key: odd})
