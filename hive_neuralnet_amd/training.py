@@ -18,7 +18,6 @@ of training_ops.py; AdamW is a torch.optim.Optimizer.
 from __future__ import annotations
 
 import torch
-import torch.nn.functional as F
 
 from . import hive_gpu
 from .fnn import HiveFNN
@@ -159,14 +158,18 @@ class AdamW(torch.optim.Optimizer):
 
 
 def encode(net: HiveFNN, features: torch.Tensor) -> torch.Tensor:
-    """HiveFNN.encode, the sigmoid and the layer norm in one kernel."""
-    h = layer_norm(F.linear(features, net.fc1.weight, net.fc1.bias), net.ln1.weight, net.ln1.bias, net.ln1.eps,
-                   "sigmoid")
-    return net.fc2(h)
+    """HiveFNN.encode, the sigmoid and the layer norm in one kernel (where ln1
+    is another module, or has hooks, as the module has it)."""
+    h, norm = net.fc1(features), net.ln1
+    if type(norm) is not torch.nn.LayerNorm or norm.normalized_shape != h.shape[-1:] or norm._forward_hooks or \
+            norm._forward_pre_hooks or norm._backward_hooks or norm._backward_pre_hooks:
+        return net.fc2(norm(torch.sigmoid(h)))
+    return net.fc2(layer_norm(h, norm.weight, norm.bias, norm.eps, "sigmoid"))
 
 
 def forward(net: HiveFNN, root_features, successor_features, action_to_root):
-    """HiveFNN.forward on the training operators: (action_logits [N], root_values [B, 1])."""
+    """HiveFNN.forward on the training operators: (action_logits [N],
+    root_values [B, 1]).  Hooks of the layers run, those of net itself do not."""
     root = encode(net, root_features)
     values = net.value_head(root)
     if action_to_root.shape[0] == 0:

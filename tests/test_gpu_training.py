@@ -387,3 +387,31 @@ def test_loss_autograd_in_16_bits_is_rounded_once(t):
     for got, exact, bound in ((dx, want, coming / B * (K / 64 + 64) * 4 * U), (dv, want_v, 8 * U * want_v.abs())):
         over = (got.double() - exact).abs() - half * exact.abs() - tiny - bound
         assert float(over.max()) <= 0.0, float(over.max())
+
+
+def test_train_batch_runs_the_layers_hooks():
+    """fc1 under a weight norm that a forward hook puts together, hooks on fc1 and on ln1: they take part, and the
+    gradients are those of the module's own forward pass."""
+    from hive_neuralnet_amd import hive_gpu
+    from hive_neuralnet_amd.fnn import FNNConfig, HiveFNN
+    from hive_neuralnet_amd.training import encode, synthetic_batch, train_batch
+    torch.manual_seed(3)
+    net = HiveFNN(FNNConfig.medium()).cuda()
+    net.fc1 = torch.nn.utils.weight_norm(net.fc1)
+    batch = synthetic_batch(48, 0, 80, 5)
+    optimizer = torch.optim.SGD(net.parameters(), lr=1e-2)
+    for _ in range(2):  # the weight is put together again for every step
+        train_batch(net, optimizer, batch)
+    assert all(p.grad is not None for p in net.parameters())
+    x = _randn((33, 122), 1)
+    seen = []
+    handles = [m.register_forward_hook(lambda m, i, o, k=k: seen.append(k) or 2.0 * o)
+               for k, m in (("fc1", net.fc1), ("ln1", net.ln1))]
+    got = encode(net, x)
+    assert seen == ["fc1", "ln1"]
+    _near(got.detach(), net.encode(x).detach(), 1e-5, "hooks")
+    handles[1].remove()
+    _near(encode(net, x).detach(), net.encode(x).detach(), 1e-5, "fc1's hook")
+    handles[0].remove()
+    net.ln1 = torch.nn.RMSNorm(32).cuda()  # another layer in its place
+    _near(encode(net, x).detach(), net.encode(x).detach(), 1e-5, "another norm")
