@@ -189,10 +189,8 @@ def train_batch(net: HiveFNN, optimizer, batch: FNNTrainingBatch, value_coef: fl
         logits.detach(), values.detach(), num_actions, batch.policy_targets, batch.policy_mask, batch.value_targets,
         batch.value_mask * batch.value_weights, value_coef)
     optimizer.zero_grad(set_to_none=True)
-    heads, grads = (values,), (dvalues,)
-    if logits.requires_grad:
-        heads, grads = (logits, values), (dlogits, dvalues)
-    torch.autograd.backward(heads, grads)
+    trained = [(head, grad) for head, grad in ((logits, dlogits), (values, dvalues)) if head.requires_grad]
+    torch.autograd.backward([head for head, _ in trained], [grad for _, grad in trained])
     optimizer.step()
     return losses
 

@@ -415,3 +415,25 @@ def test_train_batch_runs_the_layers_hooks():
     handles[0].remove()
     net.ln1 = torch.nn.RMSNorm(32).cuda()  # another layer in its place
     _near(encode(net, x).detach(), net.encode(x).detach(), 1e-5, "another norm")
+
+
+@pytest.mark.parametrize("trained", [("action_fc1", "action_fc2"), ("value_fc",), ("ln1",)], ids=lambda t: t[0])
+def test_train_batch_of_a_part_of_the_network(trained):
+    """Only some layers trained: the heads that depend on them give their gradients, the others none."""
+    from hive_neuralnet_amd.fnn import FNNConfig, HiveFNN
+    from hive_neuralnet_amd.training import synthetic_batch, train_batch
+    torch.manual_seed(3)
+    batch = synthetic_batch(48, 0, 80, 5)
+    torch.manual_seed(4)
+    net = HiveFNN(FNNConfig.medium()).cuda()
+    _, want, terms = _plain_step(net, batch, 1.0)
+    for k, p in net.named_parameters():
+        p.requires_grad_(k.split(".")[0] in trained)
+    train_batch(net, torch.optim.SGD(net.parameters(), lr=0.0), batch)
+    for k, p in net.named_parameters():
+        if not p.requires_grad:
+            assert p.grad is None, k
+        elif k in terms:
+            assert float((p.grad.cpu().double() - want[k]).abs().max()) <= 24 * U * terms[k], k
+        else:
+            _near(p.grad.cpu(), want[k], 5e-5, k)
