@@ -173,7 +173,7 @@ def forward(net: HiveFNN, root_features, successor_features, action_to_root):
     root = encode(net, root_features)
     values = net.value_head(root)
     if action_to_root.shape[0] == 0:
-        return root_features.new_zeros((0,)), values
+        return values.new_zeros((0,)), values
     return net.score_actions(root[action_to_root], encode(net, successor_features)), values
 
 

@@ -437,3 +437,19 @@ def test_train_batch_of_a_part_of_the_network(trained):
             assert float((p.grad.cpu().double() - want[k]).abs().max()) <= 24 * U * terms[k], k
         else:
             _near(p.grad.cpu(), want[k], 5e-5, k)
+
+
+def test_train_batch_under_autocast():
+    """bfloat16 products, also where no position has a move: logits and values have one type."""
+    from hive_neuralnet_amd.fnn import FNNConfig, HiveFNN
+    from hive_neuralnet_amd.training import synthetic_batch, train_batch
+    torch.manual_seed(3)
+    net = HiveFNN(FNNConfig.medium()).cuda()
+    batch = synthetic_batch(16, 0, 60, 5)
+    optimizer = torch.optim.SGD(net.parameters(), lr=1e-2)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        losses = train_batch(net, optimizer, batch)
+        assert torch.isfinite(losses).all() and float(losses[1]) > 0.0
+        batch.num_actions = torch.zeros_like(batch.num_actions)
+        losses = train_batch(net, optimizer, batch)
+    assert torch.isfinite(losses).all() and float(losses[1]) == 0.0
