@@ -141,13 +141,18 @@ class AdamW(torch.optim.Optimizer):
         groups = [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups]
         return {"state_bits": self.state_bits, "seed": self.seed, "steps": self.steps,
                 "states": [dict(plan.state) for _, plan, _ in self._plans],
-                "taken": [list(taken) for _, _, taken in self._plans], "param_groups": groups}
+                "taken": [list(taken) for _, _, taken in self._plans], "sizes": self._sizes(), "param_groups": groups}
+
+    def _sizes(self) -> list:
+        return [[p.numel() for p in plan.params] for _, plan, _ in self._plans]
 
     def load_state_dict(self, state_dict) -> None:
         if state_dict["state_bits"] != self.state_bits:
             raise ValueError(f"the saved moments are in {state_dict['state_bits']} bits, these in {self.state_bits}")
         if len(state_dict["param_groups"]) != len(self.param_groups):
             raise ValueError(f"{len(state_dict['param_groups'])} saved groups, {len(self.param_groups)} here")
+        if state_dict.get("sizes", self._sizes()) != self._sizes():
+            raise ValueError("the saved state is of parameters of other sizes")
         taken = state_dict.get("taken")  # None: saved when one number served all
         if taken is None:
             taken = [[state_dict["steps"]] * len(plan.params) for _, plan, _ in self._plans]

@@ -453,3 +453,14 @@ def test_train_batch_under_autocast():
         batch.num_actions = torch.zeros_like(batch.num_actions)
         losses = train_batch(net, optimizer, batch)
     assert torch.isfinite(losses).all() and float(losses[1]) == 0.0
+
+
+def test_optimizer_refuses_another_networks_state():
+    """Parameters of other sizes in as many blocks of 256."""
+    from hive_neuralnet_amd.training import AdamW
+    make = lambda shapes: AdamW([torch.nn.Parameter(_randn(s, 1)) for s in shapes])  # noqa: E731
+    saved = make([(300,), (200,)]).state_dict()
+    for shapes in ([(200,), (300,)], [(301,), (200,)], [(300,), (100,), (100,)], [(300,)]):
+        with pytest.raises(ValueError, match="sizes"):
+            make(shapes).load_state_dict(saved)
+    make([(30, 10), (200,)]).load_state_dict(saved)  # the same numbers of elements
