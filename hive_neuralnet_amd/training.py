@@ -136,6 +136,23 @@ class AdamW(torch.optim.Optimizer):
         self.steps += 1
         return loss
 
+    def __getstate__(self):
+        """For copies and pickles: what the base class has and the moments (codes as bytes: a plain pickle knows no
+        float8), from which a copy lays out its own plans."""
+        return {**super().__getstate__(), "adamw": {
+            "state_bits": self.state_bits, "seed": self.seed, "steps": self.steps,
+            "states": [{k: t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t for k, t in plan.state.items()}
+                       for _, plan, _ in self._plans],
+            "taken": [list(taken) for _, _, taken in self._plans]}}
+
+    def __setstate__(self, state) -> None:
+        own = state["adamw"]
+        super().__setstate__({k: v for k, v in state.items() if k != "adamw"})
+        self._ext = hive_gpu.load_extension()
+        self.state_bits, self.seed, self.steps = own["state_bits"], own["seed"], own["steps"]
+        self._make_plans([{k: t.view(torch.float8_e4m3fn) if t.dtype == torch.uint8 else t for k, t in held.items()}
+                          for held in own["states"]], own["taken"])
+
     def state_dict(self):
         """The moments as they are held, the numbers of steps, the groups' settings."""
         groups = [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups]

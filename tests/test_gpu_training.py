@@ -464,3 +464,33 @@ def test_optimizer_refuses_another_networks_state():
         with pytest.raises(ValueError, match="sizes"):
             make(shapes).load_state_dict(saved)
     make([(30, 10), (200,)]).load_state_dict(saved)  # the same numbers of elements
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("how", ["deepcopy", "pickle"])
+def test_optimizer_copies_go_on_alike(bits, how):
+    import copy
+    import pickle
+
+    from hive_neuralnet_amd.training import AdamW
+
+    ps = [torch.nn.Parameter(_randn(s, i)) for i, s in enumerate([(40, 9), (300,)])]
+    opt = AdamW([{"params": ps[:1], "weight_decay": 0.2}, {"params": ps[1:], "lr": 3e-3}], lr=1e-2, state_bits=bits, seed=5)
+
+    def steps(ps, opt, ks):
+        for k in ks:
+            for i, p in enumerate(ps):
+                p.grad = _randn(p.shape, 50 * k + i)
+            opt.step()
+
+    steps(ps, opt, range(3))
+    if how == "deepcopy":
+        twin_ps, twin = copy.deepcopy((ps, opt))
+    else:
+        twin_ps, twin = pickle.loads(pickle.dumps((ps, opt)))
+    steps(twin_ps, twin, range(3, 5))
+    held = [p.detach().clone() for p in ps]
+    steps(ps, opt, range(3, 5))
+    for p, q, h in zip(ps, twin_ps, held):
+        assert torch.equal(p, q) and not torch.equal(p, h)
+    assert twin.steps == opt.steps == 5 and twin.param_groups[0]["weight_decay"] == 0.2
