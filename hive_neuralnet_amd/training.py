@@ -155,15 +155,25 @@ class AdamW(torch.optim.Optimizer):
 
     def state_dict(self):
         """The moments as they are held, the numbers of steps, the groups' settings."""
+        for hook in self._optimizer_state_dict_pre_hooks.values():
+            hook(self)
         groups = [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups]
-        return {"state_bits": self.state_bits, "seed": self.seed, "steps": self.steps,
-                "states": [dict(plan.state) for _, plan, _ in self._plans],
-                "taken": [list(taken) for _, _, taken in self._plans], "sizes": self._sizes(), "param_groups": groups}
+        saved = {"state_bits": self.state_bits, "seed": self.seed, "steps": self.steps,
+                 "states": [dict(plan.state) for _, plan, _ in self._plans],
+                 "taken": [list(taken) for _, _, taken in self._plans], "sizes": self._sizes(), "param_groups": groups}
+        for hook in self._optimizer_state_dict_post_hooks.values():
+            changed = hook(self, saved)
+            saved = saved if changed is None else changed
+        return saved
 
     def _sizes(self) -> list:
         return [[p.numel() for p in plan.params] for _, plan, _ in self._plans]
 
     def load_state_dict(self, state_dict) -> None:
+        state_dict = dict(state_dict)  # a hook may change its entries
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
         if state_dict["state_bits"] != self.state_bits:
             raise ValueError(f"the saved moments are in {state_dict['state_bits']} bits, these in {self.state_bits}")
         if len(state_dict["param_groups"]) != len(self.param_groups):
@@ -177,6 +187,8 @@ class AdamW(torch.optim.Optimizer):
         for group, saved in zip(self.param_groups, state_dict["param_groups"]):
             group.update(saved)
         self.seed, self.steps = state_dict["seed"], state_dict["steps"]
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
 
 
 def encode(net: HiveFNN, features: torch.Tensor) -> torch.Tensor:

@@ -494,3 +494,17 @@ def test_optimizer_copies_go_on_alike(bits, how):
     for p, q, h in zip(ps, twin_ps, held):
         assert torch.equal(p, q) and not torch.equal(p, h)
     assert twin.steps == opt.steps == 5 and twin.param_groups[0]["weight_decay"] == 0.2
+
+
+def test_optimizer_runs_the_state_dicts_hooks():
+    from hive_neuralnet_amd.training import AdamW
+    p = torch.nn.Parameter(_randn((9,), 1))
+    opt, calls = AdamW([p]), []
+    opt.register_state_dict_pre_hook(lambda o: calls.append("pre"))
+    opt.register_state_dict_post_hook(lambda o, d: calls.append("post") or {**d, "note": 7})
+    opt.register_load_state_dict_pre_hook(lambda o, d: calls.append("load") or {**d, "steps": 41})
+    opt.register_load_state_dict_post_hook(lambda o: calls.append("loaded"))
+    saved = opt.state_dict()
+    assert calls == ["pre", "post"] and saved["note"] == 7
+    opt.load_state_dict(saved)
+    assert calls[2:] == ["load", "loaded"] and opt.steps == 41
