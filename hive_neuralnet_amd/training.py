@@ -116,6 +116,12 @@ class AdamW(torch.optim.Optimizer):
         if getattr(self, "_plans", None):
             raise ValueError("AdamW's parameters are fixed when it is made")
         super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        for key in ("lr", "eps", "weight_decay"):
+            if not group[key] >= 0.0:
+                raise ValueError(f"{key} must not be negative, got {group[key]}")
+        if not all(0.0 <= beta < 1.0 for beta in group["betas"]):
+            raise ValueError(f"betas must be in [0, 1), got {group['betas']}")
 
     @torch.no_grad()
     def step(self, closure=None, grad_scale: torch.Tensor | None = None):

@@ -508,3 +508,17 @@ def test_optimizer_runs_the_state_dicts_hooks():
     assert calls == ["pre", "post"] and saved["note"] == 7
     opt.load_state_dict(saved)
     assert calls[2:] == ["load", "loaded"] and opt.steps == 41
+
+
+def test_optimizer_refuses_settings_out_of_range():
+    from hive_neuralnet_amd.training import AdamW
+    p = torch.nn.Parameter(_randn((9,), 1))
+    nan = float("nan")
+    for bad, word in ((dict(lr=-1e-3), "lr"), (dict(lr=nan), "lr"), (dict(weight_decay=-0.1), "weight_decay"),
+                      (dict(weight_decay=nan), "weight_decay"), (dict(betas=(1.0, 0.9)), "betas"),
+                      (dict(betas=(0.9, -0.1)), "betas"), (dict(eps=-1e-8), "eps"), (dict(eps=nan), "eps")):
+        with pytest.raises(ValueError, match=word):
+            AdamW([p], **bad)
+        with pytest.raises(ValueError, match=word):
+            AdamW([{"params": [p], **bad}])
+    AdamW([p], lr=0.0, weight_decay=0.0, betas=(0.0, 0.0), eps=0.0)
