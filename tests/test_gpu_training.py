@@ -522,3 +522,49 @@ def test_optimizer_refuses_settings_out_of_range():
         with pytest.raises(ValueError, match=word):
             AdamW([{"params": [p], **bad}])
     AdamW([p], lr=0.0, weight_decay=0.0, betas=(0.0, 0.0), eps=0.0)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_graph_replays_of_a_step_and_of_long_lists_match_eager(bits):
+    """An AdamW step (the step's number as captured, gradients and their scale as they are at the replay) and the loss
+    over lists in slices, by each way to a position's first logit."""
+    from hive_neuralnet_amd import hive_gpu
+    ext = hive_gpu.load_extension()
+    shapes = [(64, 122), (64,), (5000,), (1,)]
+    a = [_randn(s, i) for i, s in enumerate(shapes)]
+    b = [t.clone() for t in a]
+    grads, scale = [_randn(s, 10 + i) for i, s in enumerate(shapes)], torch.ones((1,), device="cuda")
+    plan, twin = ext.prepare_adamw(a, bits), ext.prepare_adamw(b, bits)
+    lists = []
+    for B, width in ((5, 9001), (300, 4096), (4200, 1100)):
+        n = torch.randint(0, width + 1, (B,), generator=torch.Generator(device="cuda").manual_seed(B), device="cuda")
+        n = n if B < 4000 else n % 20
+        ones = torch.ones((B,), device="cuda")
+        lists.append([_randn((int(n.sum()),), 5), _randn((B,), 6), n, torch.softmax(_randn((B, width), 8), 1), ones,
+                      _randn((B,), 7), ones])
+
+    def work(plan):
+        plan.step(grads, 3, 1e-2, grad_scale=scale, seed=11)
+        return [t for args in lists for t in ext.policy_value_loss(*args)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work(plan)
+    torch.cuda.current_stream().wait_stream(side)
+    work(twin)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = work(plan)
+    for k in range(4):
+        for i, t in enumerate([*grads, *[args[0] for args in lists], *[args[1] for args in lists]]):
+            t.copy_(_randn(t.shape, 20 + 10 * k + i))
+        scale.fill_(0.5 ** k)
+        torch.cuda.synchronize()
+        want = [t.clone() for t in work(twin)]
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(out, want):
+            assert torch.equal(p, q), k
+        for p, q in zip([*a, *plan.state.values()], [*b, *twin.state.values()]):
+            assert torch.equal(p.view(torch.uint8), q.view(torch.uint8)), k

@@ -976,3 +976,52 @@ def test_adamw_refuses_codes_at_odd_addresses(ext):
         odd = torch.zeros((513,), dtype=torch.float8_e4m3fn, device="cuda")[1:]
         with pytest.raises(ValueError, match="4-byte aligned"):
             ext.prepare_adamw(p, 8, {**state, key: odd})
+
+
+# ---- loops that only the widest rows and longest lists take --------------------
+
+
+@pytest.mark.parametrize("xt,wt,sigmoid", [(F32, F32, False), (BF16, F32, True), (F16, F16, False)],
+                         ids=lambda t: str(t).replace("torch.", ""))
+@pytest.mark.parametrize("rows,cols,pad", [(130, 16385, 0), (200, 20001, 7)])
+def test_layer_norm_many_rows_past_a_block(ext, rows, cols, pad, xt, wt, sigmoid):
+    """More rows than there are row ranges, whole and cut from a wider tensor, with and without weight, bias and dx."""
+    x = (_randn((rows, cols + pad), 1, 2.0) + 0.5).to(xt)[:, :cols]
+    dy = _randn((rows, cols + 2 * pad), 2, 1.0, xt)[:, pad: pad + cols]
+    w, b = (1.0 + _randn((cols,), 3, 0.2)).to(wt), _randn((cols,), 4, 0.2, wt)
+    for weight, bias in ((w, b), (w, None), (None, b), (None, None)):
+        _check_norm(ext, x, weight, bias, dy, sigmoid=sigmoid)
+        act = "sigmoid" if sigmoid else None
+        _, mean, rstd = ext.layer_norm_forward(x, weight, bias, 1e-5, act)
+        _, dw, db = ext.layer_norm_backward(dy, x, mean, rstd, weight, bias, act)
+        none, dw2, db2 = ext.layer_norm_backward(dy, x, mean, rstd, weight, bias, act, need_dx=False)
+        assert none is None and (dw is None or torch.equal(dw, dw2)) and (db is None or torch.equal(db, db2))
+
+
+@pytest.mark.parametrize("xt,pt", [(F32, F32), (BF16, F16), (F16, F32)], ids=lambda t: str(t).replace("torch.", ""))
+@pytest.mark.parametrize("width", [300001, 1200007])
+def test_policy_value_loss_longest_lists(ext, width, xt, pt):
+    """More slices than a wave has lanes, and slices of two pieces: logits that rise over the list, so that every piece
+    has a larger one than those before, lists that the logits' end cuts, and long runs of masked moves.  Element by
+    element: a probability is 2 |z| + 4 u of itself off (|z| < 60), sums in chains of under 100 additions."""
+    def check(args):
+        losses, dx, _ = _check_loss(ext, args)
+        _, want, _ = _loss_reference(*args, 0.5, 1.0)
+        pi = args[3].double().view(-1)[: len(want)]
+        _close(dx, want, 300 * U * (want.abs() + pi), "dlogits")
+        return losses, dx
+
+    args = _loss_inputs(2, width, width, xt, pt, 3, full=True)
+    args[4].fill_(1.0)
+    rise = torch.linspace(-20.0, 20.0, width, device="cuda")
+    args[0] = (args[0].float().view(2, width) * 0.1 + torch.stack([rise, rise.flip(0)])).view(-1).to(xt)
+    check(args)
+    for left in (width + 1, 2 * width - 5000, 2 * width - 100):
+        check([args[0][:left].contiguous(), *args[1:]])
+    place = torch.arange(width, device="cuda")
+    for hide in (place % 4700 < 4200, place < width - 3, place != 5):
+        logits, pi = args[0].clone().view(2, width), args[3].clone()
+        logits[:, hide] = -math.inf
+        pi[:, hide] = 0.0
+        losses, dx = check([logits.view(-1), args[1], args[2], pi, *args[4:]])
+        assert torch.isfinite(losses).all() and not dx.view(2, width)[:, hide].any()
