@@ -19,7 +19,6 @@ template <typename T> __device__ __forceinline__ float to_f32(T v) { return (flo
 template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }
 
 inline bool is_type(int t) { return t == HG_F32 || t == HG_F16 || t == HG_BF16; }
-inline int size_of(int t) { return t == HG_F32 ? 4 : 2; }
 
 // Vector<T>: the elements of one 16-byte access.  Only the elements' own
 // alignment is assumed (the card takes 16-byte accesses at any of them).
@@ -127,11 +126,6 @@ template <int G> __device__ __forceinline__ float across_groups_sum(float v) {
 #pragma unroll
     for (int o = G; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
     return v;
-}
-// NaN in any lane gives NaN
-__device__ __forceinline__ float max_nan(float a, float b) { return a > b || a != a ? a : b; }
-template <int G> __device__ __forceinline__ float group_max(float v) {
-    return group_join<G>(v, [](float a, float b) { return max_nan(a, b); });
 }
 
 // f called with a value of element type `t`
