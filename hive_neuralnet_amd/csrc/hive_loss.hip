@@ -22,7 +22,8 @@
 // 12.2; 40,000: 15.4, 16.9).
 //
 // Lists of up to 256 moves (16 lanes a position) and up to 1,024 (a wave) are
-// read once and held in registers.  Longer ones are cut into slices, a block
+// read once and held in registers (4,096 positions of up to 1,024 moves f32 13.8
+// us, where the bytes at 5.4 TB/s are 4.6).  Longer ones are cut into slices, a block
 // each, so that few positions fill the card too: one launch leaves each
 // slice's largest logit and sums, the next joins a position's slices and
 // writes the gradient from a second read.  All loads of a list, a slice's
@@ -265,6 +266,8 @@ __device__ __forceinline__ void store_losses(const Batch& a, float policy, float
 }
 // s + p z, s where p is 0 whatever z is
 __device__ __forceinline__ float plus(float s, float p, float z) { return p != 0.0f ? fmaf(p, z, s) : s; }
+// Rounding z log2 e once puts the result up to |z| u of itself off (u = 2^-24; 8 u at z = -10, 58 u at -60), under 1 u of
+// the largest of a list.  An exact product would be two more operations a slot, in kernels that the VALU bounds.
 __device__ __forceinline__ float exp_(float z) { return __builtin_amdgcn_exp2f(z * 1.44269504f); }
 
 // gradients of zero for the logits that no position has

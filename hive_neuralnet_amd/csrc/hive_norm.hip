@@ -21,12 +21,13 @@
 // visible to another chiplet writes back its whole L2 first, for every block.)
 //
 // Bound by memory.  Measured (MI355X, inputs not in cache): forward 16,384 x
-// 2,048 f32 44 us, 6.1 TB/s; 8,192 x 4,096 bf16 24.5 us, 5.5; 118,271 x 64 f32
-// with the sigmoid 13 us, 4.6; 4,096 x 5,119 bf16, rows at odd addresses, 23
-// us, 3.7.  Backward 76 us, 5.3 TB/s; 39.5 us, 5.1; 20.7 us, 4.4; 40 us, 3.1; 2
+// 2,048 f32 45 us, 6.0 TB/s; 8,192 x 4,096 bf16 25 us, 5.4; 118,271 x 64 f32
+// with the sigmoid 12.4 us, 4.9; 4,096 x 5,119 bf16, rows at odd addresses, 21
+// us, 4.0.  Backward 77 us, 5.2 TB/s; 40.6 us, 5.0; 19.9 us, 4.6; 38.5 us, 3.3; 2
 // to 4 us of each are the second launch (1.5 more where each of its loads
 // waited for the one before).  The next row is read while this one is worked on
-// (8,192 x 4,096: 26 us without in the forward pass, 61 in the backward) and,
+// (8,192 x 4,096: 26 us without in the forward pass, 61 in the backward; not in
+// the backward pass of f32 rows over 8,192 values, whose registers it spills) and,
 // in the backward pass, h and dh are worked out again for dx, from the row's
 // own 16 bits, which leaves the registers for it; loads wait for nothing, an end
 // that cuts a vector is settled where the vector is used (4,096 x 5,119: 65 us
@@ -46,7 +47,9 @@ constexpr int kCus = 256;
 constexpr int kValues = 16, kBackwardVecs = 2;
 constexpr int64_t kMaxCols = 1024 * kValues;  // wider rows take kernels of their own
 
-__device__ __forceinline__ float sigmoid_(float x) {  // 0 and 1 at the infinities
+// 0 and 1 at the infinities.  Rounding x log2 e once puts e^-x up to |x| u off (u = 2^-24), the reciprocal adds 1 u: under
+// 2 u in all, and of a sigmoid near 0 |x| u of itself.  An exact product would be two more operations a value.
+__device__ __forceinline__ float sigmoid_(float x) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * x));
 }
 
@@ -473,6 +476,10 @@ k_norm_join(const float* __restrict__ part, int parts, int64_t cols, int w_type,
 }
 
 // ---- rows of more values than a block holds: a block a row, read once per use ----
+//
+// The simplest form, an element a load: 1,024 x 32,768 bf16 115 us forward and 132
+// back, f32 114 and 178, where the bytes at a copy's 5.4 TB/s are 25 and 37, 50 and
+// 75.  The row is read three times (x and dy twice, and again for the columns).
 
 constexpr int kWide = 1024;
 

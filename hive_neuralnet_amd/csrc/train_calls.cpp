@@ -12,7 +12,7 @@
 //
 // Measured (MI355X, a call's time on the host, Python alone / here): layer norm
 // forward 10.3 / 5.9 us, backward 13.7 / 6.9, the loss of 16 positions 13.1 / 6.2,
-// AdamW of 12 tensors 9.8 / 3.9; 3.7 of each hand the launch over, 0.6 make a
+// AdamW of 12 tensors 9.8 / 4.4; 3.7 of each hand the launch over, 0.6 make a
 // result tensor.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -241,8 +241,8 @@ struct Written {
 };
 
 // (params, grads, table, param type, state bits, step, lr, beta1, beta2, eps, weight_decay, grad_scale, seed[, bounds,
-// their number]) -> True.  `table` is the address of a plan's hg_adamw_tensor array, whose
-// gradients are entered here; none may be left out.  `bounds`: the address of Written's.
+// their number]) -> True.  `table` is the address of a plan's hg_adamw_tensor array, whose gradients are entered here;
+// none may be left out.  `bounds`: the address of Written's; without them nothing is looked for in what the step writes.
 PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t count) {
     HANDLE_TH_ERRORS
     if ((count != 13 && count != 15) || !adamw_ || !PyList_Check(a[0]) ||

@@ -13,7 +13,9 @@ legal lists, with its gradient -> one AdamW launch for all weights.
     python -m hive_neuralnet_amd.training --steps 50 --batch 2048     # the same on synthetic targets
 
 layer_norm and policy_value_loss are autograd functions over the entry points
-of training_ops.py; AdamW is a torch.optim.Optimizer.
+of training_ops.py, differentiable once, without rules for vmap, forward mode
+or tensors that hold no memory; AdamW is a torch.optim.Optimizer of contiguous
+parameters.
 """
 from __future__ import annotations
 

@@ -20,7 +20,7 @@ import torch
 
 try:  # train_calls.cpp: these entry points without Python's share of a call
     from . import _train_calls as _calls
-except ImportError:  # not built: all of a call from here, twice the time of a small one
+except ImportError:  # the library built by itself: all of a call from here, twice the time of a small one
     _calls = None
 
 _c_void_p = ctypes.c_void_p
@@ -229,7 +229,7 @@ def policy_value_loss(self, logits: torch.Tensor, values: torch.Tensor, num_acti
     logits [N]: each position's logits over its legal moves, the positions
     one after the other (build_forward_batch's rows); num_actions [B] int64
     (clamped to [0, width], as there); policy_targets [B, width] (the slots
-    past num_actions are not read); policy_weights, value_targets,
+    past num_actions are not used); policy_weights, value_targets,
     value_weights float32 [B] or [B, 1], the weights not negative; values
     [B] or [B, 1] of the logits' type.
     losses is float32 [total, policy, value], total = policy + value_coef
