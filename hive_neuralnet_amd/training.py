@@ -232,6 +232,8 @@ def train_batch(net: HiveFNN, optimizer, batch: FNNTrainingBatch, value_coef: fl
         batch.value_mask * batch.value_weights, value_coef)
     optimizer.zero_grad(set_to_none=True)
     trained = [(head, grad) for head, grad in ((logits, dlogits), (values, dvalues)) if head.requires_grad]
+    if not trained:
+        raise RuntimeError("nothing of the network requires a gradient")
     torch.autograd.backward([head for head, _ in trained], [grad for _, grad in trained])
     optimizer.step()
     return losses

@@ -568,3 +568,13 @@ def test_graph_replays_of_a_step_and_of_long_lists_match_eager(bits):
             assert torch.equal(p, q), k
         for p, q in zip([*a, *plan.state.values()], [*b, *twin.state.values()]):
             assert torch.equal(p.view(torch.uint8), q.view(torch.uint8)), k
+
+
+def test_train_batch_of_a_frozen_network_is_refused():
+    from hive_neuralnet_amd.fnn import FNNConfig, HiveFNN
+    from hive_neuralnet_amd.training import synthetic_batch, train_batch
+    net = HiveFNN(FNNConfig.small()).cuda()
+    optimizer = torch.optim.SGD(net.parameters(), lr=0.1)
+    net.requires_grad_(False)
+    with pytest.raises(RuntimeError, match="gradient"):
+        train_batch(net, optimizer, synthetic_batch(8, 0, 40, 5))
