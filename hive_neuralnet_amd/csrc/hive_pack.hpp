@@ -1,0 +1,98 @@
+// hive_pack.hpp -- what brings tensors into the form that hive_matrix.hpp's
+// tiles take: rows of 16-bit parts, 16-byte aligned, k along the row, zeros up
+// to a multiple of 32.
+#pragma once
+
+#include "hive_matrix.hpp"
+
+namespace hm {
+
+// the parts of a value, their sum (3 parts: exactly) the value
+template <typename T, int kParts> __device__ __forceinline__ void split(float v, T (&part)[kParts]) {
+    if constexpr (kParts == 1) {
+        part[0] = (T)v;
+    } else if constexpr (kParts == 2) {
+        part[0] = (T)v;
+        part[1] = (T)(v - (float)part[0]);
+    } else {
+        // the largest bfloat16: values that would round to inf keep to it, their other parts make up the rest.  What is inf or
+        // NaN itself has it in its first part, and zeros in the others.
+        const float top = __uint_as_float(0x7F7F0000u);
+        const bool finite = __builtin_fabsf(v) < __builtin_inff();
+        part[0] = (T)(finite ? __builtin_amdgcn_fmed3f(v, -top, top) : v);
+        const float r = finite ? v - (float)part[0] : 0.0f;
+        part[1] = (T)r;
+        part[2] = (T)(r - (float)part[1]);
+    }
+}
+// element of column c, part p, in a row of parts
+template <int kParts> __host__ __device__ __forceinline__ int64_t part_place(int64_t c, int p) {
+    return kParts == 1 ? c : (c / 32 * kParts + p) * 32 + c % 32;
+}
+__host__ __device__ inline int64_t up_to(int64_t n, int64_t unit) { return (n + unit - 1) / unit * unit; }
+// bytes of a packed row of n values
+inline int64_t packed_bytes(int64_t n, int parts) { return up_to(n, 32) * 2 * parts; }
+
+constexpr int kPackThreads = 256;
+
+// dst[r] = the parts of src[r][0..cols), zeros up to a multiple of 32.  Memory bound; a thread takes 8 values.
+template <typename S, typename T, int kParts>
+__global__ void __launch_bounds__(kPackThreads)
+k_pack(const S* __restrict__ src, int64_t src_stride, int64_t rows, int cols, T* __restrict__ dst, int64_t dst_stride) {
+    const int groups = (int)up_to(cols, 32) / 8;
+    for (int64_t i = (int64_t)blockIdx.x * kPackThreads + threadIdx.x; i < rows * groups;
+         i += (int64_t)gridDim.x * kPackThreads) {
+        const int64_t r = i / groups;
+        const int c = (int)(i % groups) * 8;
+        const S* from = src + r * src_stride + c;
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = c + k < cols ? to_f32<S>(from[k]) : 0.0f;
+        typedef T vec __attribute__((ext_vector_type(8)));
+        vec q[kParts];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            T part[kParts];
+            split<T, kParts>(v[k], part);
+#pragma unroll
+            for (int p = 0; p < kParts; p++) q[p][k] = part[p];
+        }
+#pragma unroll
+        for (int p = 0; p < kParts; p++) *(vec*)(dst + r * dst_stride + part_place<kParts>(c, p)) = q[p];
+    }
+}
+
+// dst[c] = the parts of column c of src[rows][cols], zeros up to a multiple of 32 rows: 64 x 64 pieces turned in LDS.
+template <typename S, typename T, int kParts>
+__global__ void __launch_bounds__(kPackThreads)
+k_pack_turned(const S* __restrict__ src, int64_t src_stride, int64_t rows, int cols, T* __restrict__ dst,
+              int64_t dst_stride) {
+    __shared__ float turn[64][65];
+    const int64_t r0 = (int64_t)blockIdx.x * 64;
+    const int c0 = (int)blockIdx.y * 64;
+    for (int i = threadIdx.x; i < 64 * 64; i += kPackThreads) {
+        const int64_t r = r0 + i / 64;
+        const int c = c0 + i % 64;
+        turn[i / 64][i % 64] = r < rows && c < cols ? to_f32<S>(src[r * src_stride + c]) : 0.0f;
+    }
+    __syncthreads();
+    const int64_t width = up_to(rows, 32);
+    for (int i = threadIdx.x; i < 64 * 8; i += kPackThreads) {
+        const int c = c0 + i / 8;
+        const int64_t r = r0 + i % 8 * 8;
+        if (c >= cols || r >= width) continue;
+        typedef T vec __attribute__((ext_vector_type(8)));
+        vec q[kParts];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            T part[kParts];
+            split<T, kParts>(turn[i % 8 * 8 + k][i / 8], part);
+#pragma unroll
+            for (int p = 0; p < kParts; p++) q[p][k] = part[p];
+        }
+#pragma unroll
+        for (int p = 0; p < kParts; p++) *(vec*)(dst + c * dst_stride + part_place<kParts>(r, p)) = q[p];
+    }
+}
+
+}  // namespace hm

@@ -19,7 +19,7 @@ import threading
 
 import torch
 
-from . import training_ops
+from . import network_ops, training_ops
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libhive_gpu.so")
@@ -138,8 +138,9 @@ _SIGS_I64 = {  # entry points returning a size (int64_t)
     "hg_mcts_expand_backprop_dense_workspace": [_c_i64, _c_i64],
     "hg_legal_features_actions_ordered_workspace": [_c_i64],
 }
-_SIGS.update(training_ops.SIGS)
-_SIGS_I64.update(training_ops.SIGS_I64)
+for _ops in (training_ops, network_ops):
+    _SIGS.update(_ops.SIGS)
+    _SIGS_I64.update(_ops.SIGS_I64)
 
 
 class HgTree(ctypes.Structure):
@@ -1041,8 +1042,8 @@ for _name, _fn in _mcts_methods().items():
     setattr(HiveGpuExtension, _name, _fn)
 
 
-# the training operators (layer norm, loss, AdamW): training_ops.py
-for _fn in training_ops.METHODS:
+# the training operators (layer norm, loss, AdamW): training_ops.py; those of a wider network: network_ops.py
+for _fn in training_ops.METHODS + network_ops.METHODS:
     setattr(HiveGpuExtension, _fn.__name__, _fn)
 
 _extension = None

@@ -585,6 +585,37 @@ int hg_adamw_step(const hg_adamw_tensor* tensors, int64_t count, int param_type,
                   int64_t step, double lr, double beta1, double beta2, double eps, double weight_decay,
                   const float* grad_scale, uint32_t seed, void* stream);
 
+/* ---- operators of a wider network ----
+ * Its hidden block, the update of its matrices and the choice of a move from
+ * its logits; no entry points of the reference.
+ *
+ * The gated block: gate = x Wg^T + bg, up = x Wu^T + bu, h = act(gate) up.
+ * x[rows][cols] (row r at x + r * x_stride elements), w_gate and w_up
+ * [hidden][cols], b_gate and b_up [hidden] (NULL = 0), h, gate and up
+ * [rows][hidden] are of one type; gate and up, which the backward pass needs,
+ * are both given or both NULL.  Sums are float32; float32 tensors are
+ * multiplied in three bfloat16 parts a value, 24 bits.  rows <= 2^20, cols and
+ * hidden <= 2^19.  workspace: as many bytes, 256-byte aligned (none where that
+ * is 0). */
+#define HG_SIGMOID 0
+#define HG_SILU 1  /* g sigmoid(g) */
+#define HG_GELU 2  /* g (1 + erf(g / sqrt 2)) / 2 */
+int64_t hg_gated_forward_workspace(const void* x, int type, int64_t rows, int64_t cols, int64_t x_stride,
+                                   const void* w_gate, const void* w_up, int64_t hidden);
+int hg_gated_forward(const void* x, int type, int64_t rows, int64_t cols, int64_t x_stride, const void* w_gate,
+                     const void* w_up, int64_t hidden, const void* b_gate, const void* b_up, int act, void* h, void* gate,
+                     void* up, void* workspace, void* stream);
+
+/* Its gradients from dh[rows][hidden] (rows dh_stride elements apart), of x's
+ * type, contiguous; those of the weights come together, any other is left out
+ * where it is NULL.  Sums over rows are in one order whatever runs beside them.
+ * workspace: as many bytes, 256-byte aligned. */
+int64_t hg_gated_backward_workspace(int type, int64_t rows, int64_t cols, int64_t hidden);
+int hg_gated_backward(const void* dh, int64_t dh_stride, const void* x, int type, int64_t rows, int64_t cols,
+                      int64_t x_stride, const void* w_gate, const void* w_up, int64_t hidden, const void* gate,
+                      const void* up, int act, void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up,
+                      void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
