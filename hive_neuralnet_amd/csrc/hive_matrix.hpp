@@ -185,16 +185,20 @@ __device__ __forceinline__ void multiply(const Operand& a, int m0, const Operand
     wait_all();  // the LDS is free again
 }
 
-// tile `t` of m x n tiles, in an order that keeps the tiles that run beside each other near each other: chiplet x (its
-// blocks are x, x + 8, ...) takes a range of tiles of its own, and within it bands of 8 rows, down the columns
+// block t of `all` in an order that keeps blocks that run beside each other near each other: chiplet x has the blocks x, x + 8,
+// ..., and takes a range of its own of the work
+__device__ __forceinline__ int chiplet_order(int t, int all) {
+    const int share = all / 8, extra = all % 8, x = t % 8;
+    return x * share + min(x, extra) + t / 8;
+}
+// tile t of m x n tiles: bands of 8 rows, down their columns
 struct Place {
     int m, n;
 };
-__device__ __forceinline__ Place tile_place(int t, int m, int n) {
-    const int all = m * n, share = all / 8, extra = all % 8, x = t % 8;
-    t = x * share + min(x, extra) + t / 8;
+__device__ __forceinline__ Place band_place(int t, int m, int n) {
     const int band = t / (8 * n), first = band * 8, height = min(8, m - first), in = t - band * 8 * n;
     return {first + in % height, in / height};
 }
+__device__ __forceinline__ Place tile_place(int t, int m, int n) { return band_place(chiplet_order(t, m * n), m, n); }
 
 }  // namespace hm

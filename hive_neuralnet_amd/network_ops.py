@@ -2,6 +2,8 @@
 
     ext.gated_linear                               act(x Wg^T + bg) * (x Wu^T + bu), for inference
     ext.gated_linear_forward / _backward           the same for training, and its gradients
+    ext.orthogonalize                              the Newton-Schulz iteration of a matrix or a batch of them
+    ext.prepare_muon(params).step(grads, ...)      one step of many matrices by their orthogonalised momentum
 
 They take float32, float16 or bfloat16 tensors, sum in float32, run on
 torch.cuda.current_stream() without synchronising it, and raise ValueError for
@@ -10,18 +12,24 @@ autograd functions and an optimizer on them.
 """
 from __future__ import annotations
 
+import bisect
 import ctypes
 
 import torch
 
-from .training_ops import TYPES, _check, _float_tensor, _place, _raw_stream, _rows, _vector
+from .training_ops import (TYPES, _bytes, _check, _current_device, _float_tensor, _place, _raw_stream, _rows,
+                           _vector)
 
 _c_void_p = ctypes.c_void_p
 _c_i64 = ctypes.c_int64
 _c_int = ctypes.c_int
+_c_float = ctypes.c_float
+_c_double = ctypes.c_double
 
 ACTIVATIONS = {"sigmoid": 0, "silu": 1, "gelu": 2}  # HG_SIGMOID, HG_SILU, HG_GELU
 MAX_ROWS, MAX_COLS = 1 << 20, 1 << 19
+MAX_SIDE = 1 << 17  # of a matrix that is orthogonalised
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # singular values of 0.001 and more end between 0.7 and 1.2 in five steps
 
 SIGS = {
     "hg_gated_forward": [_c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_void_p, _c_void_p, _c_i64, _c_void_p, _c_void_p,
@@ -29,8 +37,14 @@ SIGS = {
     "hg_gated_backward": [_c_void_p, _c_i64, _c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_void_p, _c_void_p, _c_i64,
                           _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                           _c_void_p, _c_void_p],
+    "hg_orthogonalize": [_c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_void_p, _c_int, _c_float,
+                         _c_void_p, _c_void_p, _c_void_p],
+    "hg_muon_step": [_c_void_p, _c_i64, _c_int, _c_int, _c_double, _c_double, _c_int, _c_double, _c_int, _c_void_p,
+                     _c_int, _c_float, _c_void_p, _c_void_p],
 }
 SIGS_I64 = {
+    "hg_orthogonalize_workspace": [_c_i64, _c_i64, _c_i64],
+    "hg_muon_step_workspace": [_c_void_p, _c_i64],
     "hg_gated_forward_workspace": [_c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_void_p, _c_void_p, _c_i64],
     "hg_gated_backward_workspace": [_c_int, _c_i64, _c_i64, _c_i64],
 }
@@ -137,4 +151,159 @@ def gated_linear_backward(self, dh: torch.Tensor, x: torch.Tensor, w_gate: torch
     return dx, *dw, *db
 
 
-METHODS = (gated_linear, gated_linear_forward, gated_linear_backward)
+def _iteration(steps, coefficients, eps):
+    """The coefficients as an array of float triples, one for all steps or one each."""
+    if not 1 <= steps <= 100:
+        raise ValueError(f"steps must be 1 to 100, got {steps}")
+    if not eps >= 0.0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    triples = [coefficients] if isinstance(coefficients[0], (int, float)) else list(coefficients)
+    if any(len(t) != 3 for t in triples):
+        raise ValueError(f"coefficients must be (a, b, c) or a list of such, got {coefficients}")
+    return (ctypes.c_float * (3 * len(triples)))(*[v for t in triples for v in t]), len(triples)
+
+
+def orthogonalize(self, u: torch.Tensor, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7) -> torch.Tensor:
+    """The Newton-Schulz iteration of each matrix of u [..., rows, cols]:
+    from X = U / (|U| + eps), |U| the root of its sum of squares, `steps` times
+    X <- a X + (b A + c A A) X with A = X X^T (X turned where U is taller than
+    wide), which takes each singular value s to a s + b s^3 + c s^5; with the
+    default coefficients all but the smallest end near 1.  coefficients:
+    (a, b, c), or a list of them, one a step (the last serves those past it).
+
+    u float32 / float16 / bfloat16, its rows contiguous, rows and matrices
+    evenly spaced; the result has its shape and type and is contiguous.  Matrices
+    are held in 22 bits a value between the products, which are summed in
+    float32."""
+    dev = _float_tensor(u, "u")
+    if u.dim() < 2 or u.shape[-1] == 0 or u.shape[-2] == 0:
+        raise ValueError(f"u must be [..., rows, cols], got {tuple(u.shape)}")
+    rows, cols = u.shape[-2:]
+    if rows > MAX_SIDE or cols > MAX_SIDE:
+        raise ValueError(f"at most {MAX_SIDE} rows and columns, got {rows} and {cols}")
+    c, triples = _iteration(steps, coefficients, eps)
+    out = torch.empty_like(u, memory_format=torch.contiguous_format)
+    if u.numel() == 0:
+        return out
+    if cols > 1 and u.stride(-1) != 1:
+        raise ValueError("u's last dimension must be contiguous")
+    try:
+        batch = u.view(-1, rows, cols) if u.dim() != 3 else u
+    except RuntimeError:
+        raise ValueError("u's matrices must be evenly spaced") from None
+    count = batch.shape[0]
+    ws = u.new_empty((self._lib.hg_orthogonalize_workspace(count, rows, cols),), dtype=torch.uint8)
+    _check(self._lib.hg_orthogonalize(u.data_ptr(), TYPES[u.dtype], count, rows, cols, batch.stride(1), batch.stride(0),
+                                      steps, c, triples, eps, out.data_ptr(), ws.data_ptr(), _raw_stream(dev)),
+           "orthogonalize")
+    return out
+
+
+class HgMuonMatrix(ctypes.Structure):
+    """C layout of `hg_muon_matrix` (include/hive_gpu.h)."""
+
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("momentum", ctypes.c_void_p),
+                ("rows", ctypes.c_int64), ("cols", ctypes.c_int64), ("scale", ctypes.c_double)]
+
+
+class MuonPlan:
+    """hg_muon_step over a fixed list of matrices, checked and laid out once.
+
+    `momentum` holds a float32 tensor of each matrix's shape.  The plan enters
+    the parameters by address: updates in place are seen, a parameter whose
+    memory is replaced needs a new plan.  Parameters and momenta that share
+    memory are refused, and gradients that lie in them."""
+
+    def __init__(self, lib, params, scale: str = "spectral", momentum=None):
+        params = list(params)
+        if not params:
+            raise ValueError("prepare_muon needs at least one matrix")
+        if scale not in ("spectral", "rms"):
+            raise ValueError(f"scale must be 'spectral' or 'rms', got {scale!r}")
+        for i, p in enumerate(params):
+            _float_tensor(p, f"params[{i}]")
+            if p.dtype != params[0].dtype:
+                raise ValueError(f"params[{i}] is {p.dtype}, params[0] {params[0].dtype}: one plan serves one type")
+            if p.dim() != 2 or p.numel() == 0 or max(p.shape) > MAX_SIDE:
+                raise ValueError(f"params[{i}] must be a matrix of 1 to {MAX_SIDE} rows and columns, got {tuple(p.shape)}")
+            if not p.is_contiguous():
+                raise ValueError(f"params[{i}] must be contiguous")
+        if momentum is None:
+            momentum = [torch.zeros_like(p, dtype=torch.float32) for p in params]
+        momentum = list(momentum)
+        if len(momentum) != len(params):
+            raise ValueError(f"{len(momentum)} momenta for {len(params)} matrices")
+        for i, (m, p) in enumerate(zip(momentum, params)):
+            if not isinstance(m, torch.Tensor) or m.device != p.device or m.dtype != torch.float32 or \
+                    m.shape != p.shape or not m.is_contiguous():
+                raise ValueError(f"momentum[{i}] must be a contiguous float32 tensor {tuple(p.shape)} on {p.device}")
+        self._lib, self.params, self.momentum = lib, params, momentum
+        held = sorted((*_bytes(t), f"{name}[{i}]") for name, ts in (("params", params), ("momentum", momentum))
+                      for i, t in enumerate(ts))
+        for (_, end, a), (begin, _, b) in zip(held, held[1:]):
+            if begin < end:
+                raise ValueError(f"{a} and {b} share memory: a step writes both")
+        self._written = [x for begin, end, _ in held for x in (begin, end)]
+        self._ptrs = [p.data_ptr() for p in params]
+        self._table = (HgMuonMatrix * len(params))()
+        for t, p, m in zip(self._table, params, momentum):
+            rows, cols = p.shape
+            t.param, t.momentum, t.rows, t.cols = p.data_ptr(), m.data_ptr(), rows, cols
+            t.scale = max(1.0, rows / cols) ** 0.5 if scale == "spectral" else 0.2 * max(rows, cols) ** 0.5
+        self._need = lib.hg_muon_step_workspace(self._table, len(params))
+        self._type = TYPES[params[0].dtype]
+        self._device = params[0].get_device()
+
+    def _apart(self, t: torch.Tensor) -> bool:
+        """Whether a step writes nothing of t."""
+        begin, end = _bytes(t)
+        i = bisect.bisect_right(self._written, begin)
+        return i % 2 == 0 and (i == len(self._written) or self._written[i] >= end)
+
+    def step(self, grads, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0,
+             steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7) -> None:
+        """m = momentum m + g; u = g + momentum m (nesterov) or m; p = p (1 - lr
+        weight_decay) - lr scale orthogonalize(u), of every matrix, in place.
+        scale: sqrt(max(1, rows / cols)) of a "spectral" plan, 0.2 sqrt(max(rows,
+        cols)) of an "rms" one.  grads: one type, contiguous, the parameters'
+        shapes; None leaves its matrix and momentum as they are.  The stepped
+        parameters' versions rise."""
+        if len(grads) != len(self.params):
+            raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
+        c, triples = _iteration(steps, coefficients, eps)
+        kind = next((g.dtype for g in grads if g is not None), torch.float32)
+        if kind not in TYPES:
+            raise ValueError(f"gradients must be float32, float16 or bfloat16, got {kind}")
+        if self._device != _current_device():
+            raise ValueError(f"the parameters are on device {self._device}, the current one is {_current_device()}")
+        for i, (g, p) in enumerate(zip(grads, self.params)):
+            if p.data_ptr() != self._ptrs[i]:
+                raise ValueError("a parameter's memory was replaced: make a new plan")
+            if g is None:
+                continue
+            if g.dtype is not kind or g.shape != p.shape or g.device != p.device or not g.is_contiguous():
+                raise ValueError(f"a gradient must be a contiguous {kind} tensor {tuple(p.shape)} on {p.device}, got "
+                                 f"{g.dtype} {tuple(g.shape)} on {g.device}")
+            if not self._apart(g):
+                raise ValueError(f"the gradient of params[{i}] shares memory with a parameter or momentum")
+        for t, g in zip(self._table, grads):
+            t.grad = None if g is None else g.data_ptr()
+        ws = torch.empty((self._need,), dtype=torch.uint8, device=self.params[0].device)
+        _check(self._lib.hg_muon_step(self._table, len(grads), self._type, TYPES[kind], lr, momentum, int(nesterov),
+                                      weight_decay, steps, c, triples, eps, ws.data_ptr(), _raw_stream(self._device)),
+               "muon_step")
+        for p, m, g in zip(self.params, self.momentum, grads):
+            if g is not None:
+                for t in (p, m):
+                    if not t.is_inference():
+                        torch.autograd.graph.increment_version(t)
+
+
+def prepare_muon(self, params, scale: str = "spectral", momentum=None) -> MuonPlan:
+    """A MuonPlan of contiguous matrices of one type.  `momentum`: those of an
+    earlier plan over matrices of the same shapes (a checkpoint), taken as they
+    are, not copied; None: zeros."""
+    return MuonPlan(self._lib, params, scale, momentum)
+
+
+METHODS = (gated_linear, gated_linear_forward, gated_linear_backward, orthogonalize, prepare_muon)

@@ -616,6 +616,40 @@ int hg_gated_backward(const void* dh, int64_t dh_stride, const void* x, int type
                       const void* up, int act, void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up,
                       void* workspace, void* stream);
 
+/* The Newton-Schulz iteration of `count` matrices u[rows][cols] (matrix i at
+ * u + i * u_step, its row r at r * u_row elements from there):
+ *   X = U / (|U| + eps), |U| the root of the sum of its squares; then `steps`
+ *   times X <- a X + (b A + c A A) X, A = X X^T (X turned where it is taller than
+ *   wide), (a, b, c) = coefficients[i] for step i, the last of the `triples` for
+ *   the steps past them (host memory, read before the call returns)
+ * out[count][rows][cols] has u's type.  Values are held in 22 bits, entries of the
+ * matrices up to 7.9 in size.  rows, cols <= 2^17, steps 1 to 100.
+ * workspace: as many bytes, 256-byte aligned. */
+int64_t hg_orthogonalize_workspace(int64_t count, int64_t rows, int64_t cols);
+int hg_orthogonalize(const void* u, int type, int64_t count, int64_t rows, int64_t cols, int64_t u_row, int64_t u_step,
+                     int steps, const float* coefficients, int triples, float eps, void* out, void* workspace,
+                     void* stream);
+
+/* One step of `count` matrices with it, in place:
+ *   m = momentum m + g;  u = g + momentum m (nesterov) or m
+ *   p = p (1 - lr weight_decay) - lr scale X(u)
+ * param, grad and momentum are contiguous [rows][cols]; a NULL grad leaves its
+ * matrix and momentum alone.  `matrices` is a host array, read before the call
+ * returns.  No param and momentum may share memory with another's, nor with any
+ * gradient.  workspace: as many bytes, 256-byte aligned; two calls that are in
+ * flight together must not share it. */
+typedef struct hg_muon_matrix {
+    void* param;
+    const void* grad;
+    float* momentum;
+    int64_t rows, cols;
+    double scale;
+} hg_muon_matrix;
+int64_t hg_muon_step_workspace(const hg_muon_matrix* matrices, int64_t count);
+int hg_muon_step(const hg_muon_matrix* matrices, int64_t count, int param_type, int grad_type, double lr, double momentum,
+                 int nesterov, double weight_decay, int steps, const float* coefficients, int triples, float eps,
+                 void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
