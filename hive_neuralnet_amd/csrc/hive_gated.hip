@@ -14,6 +14,7 @@ namespace {
 using namespace hm;
 
 constexpr int64_t kMaxRows = 1 << 20, kMaxCols = 1 << 19;
+constexpr int64_t kMaxArea = (int64_t)1 << 35;  // a launch has under 2^32 threads, 256 for a piece of 64 x 64
 
 // sigmoid(g): for 16-bit results the card's own exp2 and reciprocal, |g| 2^-24 off
 template <typename T> __device__ __forceinline__ float sigmoid_of(float g) {
@@ -396,7 +397,8 @@ int backward(const void* dh, int64_t dh_stride, const void* x, int64_t rows, int
 
 bool bad_sizes(int type, int64_t rows, int64_t cols, int64_t hidden, int act) {
     return !is_type(type) || act < HG_SIGMOID || act > HG_GELU || rows < 0 || cols < 1 || hidden < 1 || rows > kMaxRows ||
-           cols > kMaxCols || hidden > kMaxCols;
+           cols > kMaxCols || hidden > kMaxCols || rows * cols > kMaxArea || rows * hidden > kMaxArea ||
+           hidden * cols > kMaxArea;
 }
 
 template <typename T>

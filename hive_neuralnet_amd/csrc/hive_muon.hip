@@ -286,13 +286,12 @@ __global__ void __launch_bounds__(Tl::kThreads, (Tl::kThreads == 512 ? 2 : 1)) k
 
 int launched() { return (int)hipGetLastError(); }
 
-// the table's blocks: f(matrix) of each; more than a launch takes: -1
+// the table's blocks: f(matrix) of each
 template <typename F> int64_t lay_blocks(Table& tab, F f) {
     int64_t blocks = 0;
     for (int i = 0; i < tab.n; i++) {
         tab.t[i].first = (int)blocks;
         blocks += f(tab.t[i]) * tab.t[i].count;
-        if (blocks > 0x7FFFFFFF) return -1;
     }
     tab.blocks = (int)blocks;
     return blocks;
@@ -309,7 +308,6 @@ template <int kKind> int product(Table& tab, hipStream_t st) {
     auto launch = [&](auto tile, int64_t least) {
         using Tl = decltype(tile);
         const int64_t blocks = lay_blocks(tab, [](const Matrix& x) { return step_tiles<Tl>(x, kKind != kStep); });
-        if (blocks < 0) return (int)hipErrorInvalidValue;
         if (blocks < least) return -1;
         k_muon_product<kKind, Tl><<<(unsigned)blocks, Tl::kThreads, 0, st>>>(tab);
         return launched();
@@ -323,12 +321,10 @@ template <int kKind> int product(Table& tab, hipStream_t st) {
 // the iteration of the table's matrices
 int iterate(Table& tab, int steps, const float* coefficients, int64_t triples, hipStream_t st) {
     int64_t blocks = lay_blocks(tab, [](const Matrix&) { return (int64_t)kSumBlocks; });
-    if (blocks < 0) return (int)hipErrorInvalidValue;
     k_muon_sums<<<(unsigned)blocks, 256, 0, st>>>(tab);
     int e = launched();
     if (e) return e;
     blocks = lay_blocks(tab, [](const Matrix& x) { return (int64_t)((x.rows + 63) / 64) * ((x.cols + 63) / 64); });
-    if (blocks < 0) return (int)hipErrorInvalidValue;
     k_muon_pack<<<(unsigned)blocks, 256, 0, st>>>(tab);
     e = launched();
     tab.from = 0;
@@ -349,21 +345,25 @@ int iterate(Table& tab, int steps, const float* coefficients, int64_t triples, h
 bool bad_settings(int steps, const float* coefficients, int triples, float eps) {
     return steps < 1 || steps > 100 || !coefficients || triples < 1 || !(eps >= 0.0f);
 }
-bool bad_shape(int64_t rows, int64_t cols) { return rows < 1 || cols < 1 || rows > kMaxSide || cols > kMaxSide; }
+// a launch has under 2^32 threads, 256 for a piece of 64 x 64
+bool bad_shape(int64_t count, int64_t rows, int64_t cols) {
+    return rows < 1 || cols < 1 || rows > kMaxSide || cols > kMaxSide || count > 1 << 16 ||
+           count * (rows / 64 + 1) * (cols / 64 + 1) > 2049 * 2049;
+}
 
 }  // namespace
 
 extern "C" {
 
 int64_t hg_orthogonalize_workspace(int64_t count, int64_t rows, int64_t cols) {
-    if (count < 1 || bad_shape(rows, cols)) return 0;
+    if (count < 1 || bad_shape(count, rows, cols)) return 0;
     return count * layout((int)rows, (int)cols).all;
 }
 
 int hg_orthogonalize(const void* u, int type, int64_t count, int64_t rows, int64_t cols, int64_t u_row, int64_t u_step,
                      int steps, const float* coefficients, int triples, float eps, void* out, void* workspace,
                      void* stream) {
-    if (!is_type(type) || count < 0 || count > 1 << 20 || bad_shape(rows, cols) || bad_settings(steps, coefficients, triples, eps))
+    if (!is_type(type) || count < 0 || bad_shape(count, rows, cols) || bad_settings(steps, coefficients, triples, eps))
         return (int)hipErrorInvalidValue;
     if (count == 0) return 0;
     if (!u || !out || !workspace || (uintptr_t)workspace % 256) return (int)hipErrorInvalidValue;
@@ -380,7 +380,7 @@ int64_t hg_muon_step_workspace(const hg_muon_matrix* matrices, int64_t count) {
     for (int64_t i = 0; matrices && i < count; i += kMatrices) {
         int64_t bytes = 0;
         for (int64_t k = i; k < std::min(count, i + kMatrices); k++)
-            if (!bad_shape(matrices[k].rows, matrices[k].cols))
+            if (!bad_shape(1, matrices[k].rows, matrices[k].cols))
                 bytes += layout((int)matrices[k].rows, (int)matrices[k].cols).all;
         most = std::max(most, bytes);
     }
@@ -394,7 +394,7 @@ int hg_muon_step(const hg_muon_matrix* matrices, int64_t count, int param_type, 
         bad_settings(steps, coefficients, triples, eps))
         return (int)hipErrorInvalidValue;
     for (int64_t i = 0; i < count; i++)
-        if (bad_shape(matrices[i].rows, matrices[i].cols) || !matrices[i].param || !matrices[i].momentum ||
+        if (bad_shape(1, matrices[i].rows, matrices[i].cols) || !matrices[i].param || !matrices[i].momentum ||
             (uintptr_t)matrices[i].momentum % 4)
             return (int)hipErrorInvalidValue;
     if (count > 0 && (!workspace || (uintptr_t)workspace % 256)) return (int)hipErrorInvalidValue;

@@ -4,6 +4,7 @@
     ext.gated_linear_forward / _backward           the same for training, and its gradients
     ext.orthogonalize                              the Newton-Schulz iteration of a matrix or a batch of them
     ext.prepare_muon(params).step(grads, ...)      one step of many matrices by their orthogonalised momentum
+    ext.sample_actions                             a slot of each row of logits: temperature, top-k, top-p, min-p
 
 They take float32, float16 or bfloat16 tensors, sum in float32, run on
 torch.cuda.current_stream() without synchronising it, and raise ValueError for
@@ -28,6 +29,7 @@ _c_double = ctypes.c_double
 
 ACTIVATIONS = {"sigmoid": 0, "silu": 1, "gelu": 2}  # HG_SIGMOID, HG_SILU, HG_GELU
 MAX_ROWS, MAX_COLS = 1 << 20, 1 << 19
+MAX_WIDTH = 1 << 20  # slots of a row that a slot is drawn from
 MAX_SIDE = 1 << 17  # of a matrix that is orthogonalised
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # singular values of 0.001 and more end between 0.7 and 1.2 in five steps
 
@@ -41,6 +43,9 @@ SIGS = {
                          _c_void_p, _c_void_p, _c_void_p],
     "hg_muon_step": [_c_void_p, _c_i64, _c_int, _c_int, _c_double, _c_double, _c_int, _c_double, _c_int, _c_void_p,
                      _c_int, _c_float, _c_void_p, _c_void_p],
+    "hg_sample_actions": [_c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_void_p, _c_void_p, _c_void_p, _c_double,
+                          _c_void_p, _c_i64, _c_void_p, _c_double, _c_void_p, _c_double, _c_void_p, _c_void_p,
+                          _c_void_p],
 }
 SIGS_I64 = {
     "hg_orthogonalize_workspace": [_c_i64, _c_i64, _c_i64],
@@ -306,4 +311,51 @@ def prepare_muon(self, params, scale: str = "spectral", momentum=None) -> MuonPl
     return MuonPlan(self._lib, params, scale, momentum)
 
 
-METHODS = (gated_linear, gated_linear_forward, gated_linear_backward, orthogonalize, prepare_muon)
+def _setting(value, name: str, B: int, dtype: torch.dtype, dev: int):
+    """(address or None, number) of a setting: a tensor of one value a row, or a number for all."""
+    if isinstance(value, torch.Tensor):
+        return _vector(value, name, B, dtype, dev), 0
+    return None, value
+
+
+def sample_actions(self, logits: torch.Tensor, uniforms: torch.Tensor, num_actions=None, temperature=1.0, top_k=0,
+                   top_p=1.0, min_p=0.0):
+    """(actions int64 [B], log_probs float32 [B]): a slot of each row of logits
+    [B, width], drawn from uniforms [B] (float32 in [0, 1)), and the logarithm of
+    its probability among the slots kept.
+
+    logits: float32 / float16 / bfloat16, rows contiguous and evenly spaced.
+    num_actions [B] int64: a row's slots are its first ones, as the legal lists'
+    (clamped to [0, width]; None: all); slots of -inf or NaN are left out.  No
+    slot left: -1, and a log probability of 0.  Kept, in order of falling logits
+    (ties by rising slots): the first top_k (0: all); of these the fewest first
+    ones that hold top_p of their mass; of these the ones at least min_p as
+    likely as the first.  The slot drawn is the first, in order of the slots, at
+    which the running sum of exp((x - max) / temperature) passes u times the
+    whole; a temperature of 0 takes the largest logit's first slot.  Each
+    setting is a number, or a tensor of a value a row (float32; top_k int64; what
+    lies past its range counts as its end)."""
+    dev = _float_tensor(logits, "logits")
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f"logits must be [B, width], got {tuple(logits.shape)}")
+    B, width, stride = _rows(logits, "logits")
+    if width > MAX_WIDTH:
+        raise ValueError(f"rows of at most {MAX_WIDTH} slots, got {width}")
+    u = _vector(uniforms, "uniforms", B, torch.float32, dev)
+    n = None if num_actions is None else _vector(num_actions, "num_actions", B, torch.int64, dev)
+    t, t_all = _setting(temperature, "temperature", B, torch.float32, dev)
+    k, k_all = _setting(top_k, "top_k", B, torch.int64, dev)
+    p, p_all = _setting(top_p, "top_p", B, torch.float32, dev)
+    m, m_all = _setting(min_p, "min_p", B, torch.float32, dev)
+    if not t_all >= 0.0 or k_all < 0 or not 0.0 <= p_all or not 0.0 <= m_all <= 1.0:
+        raise ValueError(f"temperature, top_k and top_p must not be negative and min_p be in [0, 1], got {t_all}, {k_all}, "
+                         f"{p_all} and {m_all}")
+    actions = logits.new_empty((B,), dtype=torch.int64)
+    log_probs = logits.new_empty((B,), dtype=torch.float32)
+    _check(self._lib.hg_sample_actions(logits.data_ptr(), TYPES[logits.dtype], B, width, stride, n, u, t, t_all, k, k_all,
+                                       p, p_all, m, m_all, actions.data_ptr(), log_probs.data_ptr(), _raw_stream(dev)),
+           "sample_actions")
+    return actions, log_probs
+
+
+METHODS = (gated_linear, gated_linear_forward, gated_linear_backward, orthogonalize, prepare_muon, sample_actions)

@@ -595,7 +595,7 @@ int hg_adamw_step(const hg_adamw_tensor* tensors, int64_t count, int param_type,
  * [rows][hidden] are of one type; gate and up, which the backward pass needs,
  * are both given or both NULL.  Sums are float32; float32 tensors are
  * multiplied in three bfloat16 parts a value, 24 bits.  rows <= 2^20, cols and
- * hidden <= 2^19.  workspace: as many bytes, 256-byte aligned (none where that
+ * hidden <= 2^19, each two of them at most 2^35 together.  workspace: as many bytes, 256-byte aligned (none where that
  * is 0). */
 #define HG_SIGMOID 0
 #define HG_SILU 1  /* g sigmoid(g) */
@@ -623,7 +623,8 @@ int hg_gated_backward(const void* dh, int64_t dh_stride, const void* x, int type
  *   wide), (a, b, c) = coefficients[i] for step i, the last of the `triples` for
  *   the steps past them (host memory, read before the call returns)
  * out[count][rows][cols] has u's type.  Values are held in 22 bits, entries of the
- * matrices up to 7.9 in size.  rows, cols <= 2^17, steps 1 to 100.
+ * matrices up to 7.9 in size.  rows, cols <= 2^17, count * (rows / 64 + 1)
+ * (cols / 64 + 1) <= 2049^2, count <= 2^16, steps 1 to 100.
  * workspace: as many bytes, 256-byte aligned. */
 int64_t hg_orthogonalize_workspace(int64_t count, int64_t rows, int64_t cols);
 int hg_orthogonalize(const void* u, int type, int64_t count, int64_t rows, int64_t cols, int64_t u_row, int64_t u_step,
@@ -649,6 +650,24 @@ int64_t hg_muon_step_workspace(const hg_muon_matrix* matrices, int64_t count);
 int hg_muon_step(const hg_muon_matrix* matrices, int64_t count, int param_type, int grad_type, double lr, double momentum,
                  int nesterov, double weight_decay, int steps, const float* coefficients, int triples, float eps,
                  void* workspace, void* stream);
+
+/* A slot of each of `rows` rows of logits (row b at logits + b * stride elements),
+ * drawn from uniforms[b] in [0, 1): actions[b], and with log_probs not NULL the
+ * logarithm of its probability among what was kept.  Row b's slots are its first
+ * num_actions[b] (NULL = width; clamped to [0, width]) without those of -inf or
+ * NaN; no slot left: -1 and 0.  In order of falling logits, ties by rising slots,
+ * the first top_k stay (<= 0: all), of these the fewest first ones that hold top_p
+ * of their mass (>= 1: all; at least one), of these the ones at least min_p as
+ * likely as the first.  The slot drawn is the first, in the slots' order, at which
+ * the running sum of the weights kept, exp((x - max) / T), passes u times their
+ * whole.  T not above 0: the largest logit's first slot, of probability 1.
+ * Each setting is an array of a value a row, or where that is NULL the number
+ * beside it.  width <= 2^20, rows <= 2^25 (2^21 of more
+ * than 1,024 slots). */
+int hg_sample_actions(const void* logits, int type, int64_t rows, int64_t width, int64_t stride,
+                      const int64_t* num_actions, const float* uniforms, const float* temperatures, double temperature,
+                      const int64_t* top_ks, int64_t top_k, const float* top_ps, double top_p, const float* min_ps,
+                      double min_p, int64_t* actions, float* log_probs, void* stream);
 
 #ifdef __cplusplus
 }
