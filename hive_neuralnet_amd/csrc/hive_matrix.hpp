@@ -11,8 +11,9 @@
 //   1 part   the tensors as they are, float16 or bfloat16
 //   2 parts  float16, 22 bits of a value: A0 B0 + A0 B1 + A1 B0, the product of
 //            the last parts (2^-24 of the whole) left out
-//   3 parts  bfloat16, all 24 bits of a float over its whole range: the six
-//            products of parts whose numbers add up to at most 2
+//   3 parts  bfloat16, all 24 bits of a float from 2^-110 in size up (below that
+//            to within 2^-134): the six products of parts whose numbers add up to
+//            at most 2
 // so that float32 products run at a third or a sixth of the 16-bit rate (2.5
 // PFLOP/s), where the float32 instructions reach a sixteenth of it.
 //

@@ -7,7 +7,7 @@
 
 namespace hm {
 
-// the parts of a value, their sum (3 parts: exactly) the value
+// the parts of a value, their sum the value (3 parts: exactly, from 2^-110 in size up)
 template <typename T, int kParts> __device__ __forceinline__ void split(float v, T (&part)[kParts]) {
     if constexpr (kParts == 1) {
         part[0] = (T)v;

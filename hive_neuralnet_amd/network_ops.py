@@ -162,8 +162,10 @@ def _iteration(steps, coefficients, eps):
         raise ValueError(f"steps must be 1 to 100, got {steps}")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    triples = [coefficients] if isinstance(coefficients[0], (int, float)) else list(coefficients)
-    if any(len(t) != 3 for t in triples):
+    triples = list(coefficients)
+    if triples and isinstance(triples[0], (int, float)):
+        triples = [triples]
+    if not triples or any(len(t) != 3 for t in triples):
         raise ValueError(f"coefficients must be (a, b, c) or a list of such, got {coefficients}")
     return (ctypes.c_float * (3 * len(triples)))(*[v for t in triples for v in t]), len(triples)
 

@@ -12,10 +12,11 @@ legal lists, with its gradient -> one AdamW launch for all weights.
 
     python -m hive_neuralnet_amd.training --steps 50 --batch 2048     # the same on synthetic targets
 
-layer_norm and policy_value_loss are autograd functions over the entry points
-of training_ops.py, differentiable once, without rules for vmap, forward mode
-or tensors that hold no memory; AdamW is a torch.optim.Optimizer of contiguous
-parameters.
+layer_norm, gated_linear and policy_value_loss are autograd functions over the
+entry points of training_ops.py and network_ops.py, differentiable once, without
+rules for vmap, forward mode or tensors that hold no memory; AdamW is a
+torch.optim.Optimizer of contiguous parameters, Muon one of contiguous matrices,
+whose step is their orthogonalised momentum.
 """
 from __future__ import annotations
 
@@ -47,6 +48,36 @@ def layer_norm(x: torch.Tensor, weight=None, bias=None, eps: float = 1e-5, activ
     """Layer norm over the last dimension of x (activation="sigmoid": of
     sigmoid(x)), differentiable once in x, weight and bias."""
     return _LayerNorm.apply(x, weight, bias, eps, activation)
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, b_gate, b_up, activation):
+        h, gate, up = hive_gpu.load_extension().gated_linear_forward(x, w_gate, w_up, b_gate, b_up, activation)
+        ctx.save_for_backward(x, w_gate, w_up, gate, up)
+        ctx.activation = activation
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        x, w_gate, w_up, gate, up = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dwg, dwu, dbg, dbu = hive_gpu.load_extension().gated_linear_backward(
+            dh.contiguous(), x, w_gate, w_up, gate, up, ctx.activation, need_dx=need[0],
+            need_weights=need[1] or need[2], need_bias=need[3] or need[4])
+        return (dx, *[g if n else None for g, n in zip((dwg, dwu, dbg, dbu), need[1:5])], None)
+
+
+def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate=None, b_up=None,
+                 activation: str = "silu") -> torch.Tensor:
+    """act(x w_gate^T + b_gate) * (x w_up^T + b_up) of
+    HiveGpuExtension.gated_linear, differentiable once in all of its tensors.
+    Where no gradient is asked for, nothing is kept for one."""
+    tensors = [t for t in (x, w_gate, w_up, b_gate, b_up) if isinstance(t, torch.Tensor)]
+    if not torch.is_grad_enabled() or not any(t.requires_grad for t in tensors):
+        return hive_gpu.load_extension().gated_linear(x, w_gate, w_up, b_gate, b_up, activation)
+    return _GatedLinear.apply(x, w_gate, w_up, b_gate, b_up, activation)
 
 
 class _PolicyValueLoss(torch.autograd.Function):
@@ -199,6 +230,121 @@ class AdamW(torch.optim.Optimizer):
             hook(self)
 
 
+class Muon(torch.optim.Optimizer):
+    """Steps of matrices by their orthogonalised momentum (MuonPlan), all of a
+    group and type in one call: m = momentum m + g; u = g + momentum m (nesterov)
+    or m; p = p (1 - lr weight_decay) - lr scale X(u).  scale="spectral": sqrt(max(1,
+    rows / cols)); "rms": 0.2 sqrt(max(rows, cols)), a step as large as AdamW's.
+    Parameters are contiguous matrices; vectors, embeddings and heads of one row go
+    to another optimizer (`matrices` finds the ones of a network).  A parameter
+    without a gradient is left as it is."""
+
+    def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True,
+                 weight_decay: float = 0.0, steps: int = 5, eps: float = 1e-7, scale: str = "spectral"):
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
+                                      steps=steps, eps=eps))
+        self._ext = hive_gpu.load_extension()
+        self.scale = scale
+        self._plans: list = []  # (group, plan)
+        self._make_plans(None)
+
+    def _make_plans(self, momenta) -> None:
+        plans = []
+        for group in self.param_groups:
+            by_type: dict = {}
+            for p in group["params"]:
+                by_type.setdefault(p.dtype, []).append(p)
+            for members in by_type.values():
+                held = None
+                if momenta is not None:
+                    if len(plans) >= len(momenta):
+                        raise ValueError("the saved state has fewer parameter lists than the optimizer")
+                    held = [m.to(p.device, copy=True) for m, p in zip(momenta[len(plans)], members)]
+                    if len(momenta[len(plans)]) != len(members):
+                        raise ValueError(f"{len(momenta[len(plans)])} saved momenta for {len(members)} matrices")
+                plans.append((group, self._ext.prepare_muon(members, self.scale, held)))
+        if momenta is not None and len(momenta) != len(plans):
+            raise ValueError(f"the saved state has {len(momenta)} parameter lists, the optimizer {len(plans)}")
+        self._plans = plans
+
+    def add_param_group(self, param_group) -> None:
+        if getattr(self, "_plans", None):
+            raise ValueError("Muon's parameters are fixed when it is made")
+        super().add_param_group(param_group)
+        self._check_settings(self.param_groups[-1])
+
+    @staticmethod
+    def _check_settings(group) -> None:
+        for key in ("lr", "eps", "weight_decay"):
+            if not group[key] >= 0.0:
+                raise ValueError(f"{key} must not be negative, got {group[key]}")
+        if not 0.0 <= group["momentum"] < 1.0:
+            raise ValueError(f"momentum must be in [0, 1), got {group['momentum']}")
+        if not 1 <= group["steps"] <= 100:
+            raise ValueError(f"steps must be 1 to 100, got {group['steps']}")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """One step from the parameters' gradients."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group, plan in self._plans:
+            grads = [None if p.grad is None else p.grad.contiguous() for p in plan.params]
+            if any(g is not None for g in grads):
+                plan.step(grads, lr=group["lr"], momentum=group["momentum"], nesterov=group["nesterov"],
+                          weight_decay=group["weight_decay"], steps=group["steps"], eps=group["eps"])
+        return loss
+
+    def __getstate__(self):
+        """For copies and pickles: what the base class has and the momenta, from which a copy lays out its own plans."""
+        return {**super().__getstate__(), "muon": {"scale": self.scale,
+                                                   "momentum": [list(plan.momentum) for _, plan in self._plans]}}
+
+    def __setstate__(self, state) -> None:
+        own = state["muon"]
+        super().__setstate__({k: v for k, v in state.items() if k != "muon"})
+        self._ext = hive_gpu.load_extension()
+        self.scale = own["scale"]
+        self._make_plans(own["momentum"])
+
+    def state_dict(self):
+        """The momenta, the kind of scale, the groups' settings."""
+        for hook in self._optimizer_state_dict_pre_hooks.values():
+            hook(self)
+        saved = {"scale": self.scale, "momentum": [list(plan.momentum) for _, plan in self._plans],
+                 "param_groups": [{k: v for k, v in g.items() if k != "params"} for g in self.param_groups]}
+        for hook in self._optimizer_state_dict_post_hooks.values():
+            changed = hook(self, saved)
+            saved = saved if changed is None else changed
+        return saved
+
+    def load_state_dict(self, state_dict) -> None:
+        state_dict = dict(state_dict)  # a hook may change its entries
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
+        if state_dict["scale"] != self.scale:
+            raise ValueError(f"the saved scale is {state_dict['scale']!r}, this one {self.scale!r}")
+        if len(state_dict["param_groups"]) != len(self.param_groups):
+            raise ValueError(f"{len(state_dict['param_groups'])} saved groups, {len(self.param_groups)} here")
+        self._make_plans(state_dict["momentum"])
+        for group, saved in zip(self.param_groups, state_dict["param_groups"]):
+            group.update(saved)
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
+
+
+def matrices(net: torch.nn.Module):
+    """(matrices, others): a network's parameters that Muon takes, those of two
+    dimensions with more than one row and column, and those left to AdamW."""
+    taken, others = [], []
+    for p in net.parameters():
+        (taken if p.dim() == 2 and min(p.shape) > 1 else others).append(p)
+    return taken, others
+
+
 def encode(net: HiveFNN, features: torch.Tensor) -> torch.Tensor:
     """HiveFNN.encode, the sigmoid and the layer norm in one kernel (where ln1
     is another module, or has hooks, as the module has it)."""
@@ -221,7 +367,8 @@ def forward(net: HiveFNN, root_features, successor_features, action_to_root):
 
 def train_batch(net: HiveFNN, optimizer, batch: FNNTrainingBatch, value_coef: float = 1.0) -> torch.Tensor:
     """One training step on a sampled batch; returns [total, policy, value]
-    (float32, on the device: reading them waits for the step)."""
+    (float32, on the device: reading them waits for the step).  optimizer: one,
+    or a list of them that share the network's parameters out (Muon and AdamW)."""
     ext = hive_gpu.load_extension()
     B = int(batch.num_actions.shape[0])
     root, succ, action_to_root, num_actions = build_forward_batch(
@@ -230,12 +377,15 @@ def train_batch(net: HiveFNN, optimizer, batch: FNNTrainingBatch, value_coef: fl
     losses, dlogits, dvalues = ext.policy_value_loss(
         logits.detach(), values.detach(), num_actions, batch.policy_targets, batch.policy_mask, batch.value_targets,
         batch.value_mask * batch.value_weights, value_coef)
-    optimizer.zero_grad(set_to_none=True)
+    optimizers = optimizer if isinstance(optimizer, (list, tuple)) else [optimizer]
+    for o in optimizers:
+        o.zero_grad(set_to_none=True)
     trained = [(head, grad) for head, grad in ((logits, dlogits), (values, dvalues)) if head.requires_grad]
     if not trained:
         raise RuntimeError("nothing of the network requires a gradient")
     torch.autograd.backward([head for head, _ in trained], [grad for _, grad in trained])
-    optimizer.step()
+    for o in optimizers:
+        o.step()
     return losses
 
 
@@ -264,10 +414,16 @@ def main() -> None:
     ap.add_argument("--batch", type=int, default=2048)
     ap.add_argument("--lr", type=float, default=1e-2)
     ap.add_argument("--state-bits", type=int, default=32, choices=(32, 8))
+    ap.add_argument("--optimizer", default="adamw", choices=("adamw", "muon"),
+                    help="muon: the matrices by their orthogonalised momentum, the rest by AdamW")
     a = ap.parse_args()
     torch.manual_seed(0)
     net = HiveFNN(FNNConfig.large()).cuda()
-    optimizer = AdamW(net.parameters(), lr=a.lr, state_bits=a.state_bits)
+    if a.optimizer == "muon":
+        taken, others = matrices(net)
+        optimizer = [Muon(taken, lr=a.lr), AdamW(others, lr=a.lr, state_bits=a.state_bits)]
+    else:
+        optimizer = AdamW(net.parameters(), lr=a.lr, state_bits=a.state_bits)
     batch = synthetic_batch(a.batch)
     for i in range(a.steps):
         t = time.perf_counter()

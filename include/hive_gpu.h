@@ -594,7 +594,8 @@ int hg_adamw_step(const hg_adamw_tensor* tensors, int64_t count, int param_type,
  * [hidden][cols], b_gate and b_up [hidden] (NULL = 0), h, gate and up
  * [rows][hidden] are of one type; gate and up, which the backward pass needs,
  * are both given or both NULL.  Sums are float32; float32 tensors are
- * multiplied in three bfloat16 parts a value, 24 bits.  rows <= 2^20, cols and
+ * multiplied in three bfloat16 parts a value, 24 bits (values below 2^-110 to
+ * within 2^-134).  rows <= 2^20, cols and
  * hidden <= 2^19, each two of them at most 2^35 together.  workspace: as many bytes, 256-byte aligned (none where that
  * is 0). */
 #define HG_SIGMOID 0
