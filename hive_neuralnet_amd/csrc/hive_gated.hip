@@ -42,123 +42,102 @@ template <typename T, bool kSlope> __device__ __forceinline__ float act_of(int a
 struct Forward {
     Operand x, wg, wu;
     const void *bg, *bu;
-    void *h, *gate, *up;
+    void* h;
+    float *gate, *up;
     int hidden, act, tiles_m, tiles_n;
 };
 
 // T: the tensors' type.  A tile's columns are a wave's gates and the same hidden units' ups, in turn.
 template <typename T, typename Tl>
-__global__ void __launch_bounds__(Tl::kThreads, (Tl::kThreads == 512 ? 2 : 1)) k_gated_forward(Forward f) {
-    __shared__ __attribute__((aligned(1024))) char lds[2 * Tl::kStage];
-    constexpr int strip = Tl::kFn * 16, half = strip / 2;
+__global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_gated_forward(Forward f) {
+    __shared__ __attribute__((aligned(1024))) char lds[Tl::kLds];
     const Place t = tile_place(blockIdx.x, f.tiles_m, f.tiles_n);
     const int m0 = t.m * Tl::kM, n0 = t.n * (Tl::kN / 2);
-    Sums<Tl> s;
-    multiply<Tl>(
-        f.x, m0, f.wg, f.wu, [](int r) { return r / strip * half + r % half; }, [](int r) { return r % strip >= half; }, n0,
-        0, f.x.bytes, lds, s);
-    const int col = n0 + (int)(threadIdx.x >> 6) % Tl::kWn * half + (int)(threadIdx.x & 63) / 16 * 4;
+    Sums<Tl, 2> s;
+    multiply<Tl, 2, false, false>(f.x, m0, f.wg, f.wu, n0, 1 << 30, 0, (f.x.bytes + Tl::kRow - 1) / Tl::kRow, lds, s);
+    constexpr int share = Tl::kFn / 2, run = 4 * share;
+    const int n = n0 + s.col(), live = f.hidden - n;
+    if (live <= 0) return;
+    float bg[run], bu[run];
 #pragma unroll
-    for (int j = 0; j < Tl::kFn / 2; j++) {
-        const int n = col + j * 16, live = f.hidden - n;
-        if (live <= 0) continue;
-        float bg[4], bu[4];
+    for (int e = 0; e < run; e++) {
+        bg[e] = f.bg && e < live ? to_f32<T>(((const T*)f.bg)[n + e]) : 0.0f;
+        bu[e] = f.bu && e < live ? to_f32<T>(((const T*)f.bu)[n + e]) : 0.0f;
+    }
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            bg[e] = f.bg && e < live ? to_f32<T>(((const T*)f.bg)[n + e]) : 0.0f;
-            bu[e] = f.bu && e < live ? to_f32<T>(((const T*)f.bu)[n + e]) : 0.0f;
+    for (int i = 0; i < Tl::kFm; i++) {
+        const int64_t m = (int64_t)m0 + s.row() + i * 16;
+        if (m >= f.x.rows) continue;
+        float g[run], u[run], h[run], unused;
+#pragma unroll
+        for (int e = 0; e < run; e++) {
+            g[e] = s.acc[i][e / 4][e % 4] + bg[e];
+            u[e] = s.acc[i][share + e / 4][e % 4] + bu[e];
+            h[e] = act_of<T, false>(f.act, g[e], unused) * u[e];
         }
-#pragma unroll
-        for (int i = 0; i < Tl::kFm; i++) {
-            const int64_t m = (int64_t)m0 + s.row() + i * 16;
-            if (m >= f.x.rows) continue;
-            float g[4], u[4], h[4], unused;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                g[e] = s.acc[i][j][e] + bg[e];
-                u[e] = s.acc[i][j + Tl::kFn / 2][e] + bu[e];
-                h[e] = act_of<T, false>(f.act, g[e], unused) * u[e];
-            }
-            const int64_t to = m * f.hidden + n;
-            store_some<T, 4>((T*)f.h + to, live, h);
-            if (f.gate) {
-                store_some<T, 4>((T*)f.gate + to, live, g);
-                store_some<T, 4>((T*)f.up + to, live, u);
-            }
+        const int64_t to = m * f.hidden + n;
+        store_run<T, run>((T*)f.h + to, live, h);
+        if (f.gate) {
+            store_run<float, run>(f.gate + to, live, g);
+            store_run<float, run>(f.up + to, live, u);
         }
     }
 }
 
-// dgate and dup from dh, gate and up: rows of parts [dgate | dup] for dx, each `hidden_up` values, and turned for the
-// weights' gradients; with `sums`, the sums of each over the block's 64 rows: sums[row block][2][hidden].
+constexpr int kSlopeRows = 64;  // of a block of k_gated_slopes
+
+// dgate and dup from dh, gate and up: rows of parts [dgate | dup], each `cut` values with zeros past its own; with `sums`, the
+// sums of each over the block's rows: sums[row block][2][hidden].  Memory bound; a thread takes 8 columns of 8 rows.
 template <typename T, typename P, int kParts>
 __global__ void __launch_bounds__(256)
-k_gated_slopes(const T* __restrict__ dh, int64_t dh_stride, const T* __restrict__ gate, const T* __restrict__ up,
-               int64_t rows, int hidden, int act, P* __restrict__ flat, int64_t flat_stride, P* __restrict__ turned,
-               int64_t turned_stride, float* __restrict__ sums) {
-    __shared__ float lds[2][64][65];
-    const int64_t r0 = (int64_t)blockIdx.x * 64;
-    const int c0 = (int)blockIdx.y * 64;
-    const int hidden_up = (int)up_to(hidden, 32);
-    for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-        const int64_t r = r0 + i / 16;
-        const int c = c0 + i % 16 * 4;
-        float d[2][4];
+k_gated_slopes(const T* __restrict__ dh, int64_t dh_stride, const float* __restrict__ gate, const float* __restrict__ up,
+               int64_t rows, int hidden, int act, P* __restrict__ d, int64_t d_stride, int cut, float* __restrict__ sums) {
+    __shared__ float lds[2][8][kSlopeRows / 2 + 1][8];
+    const int64_t r0 = (int64_t)blockIdx.x * kSlopeRows;
+    const int column = threadIdx.x % 32, c = (int)blockIdx.y * 256 + column * 8, live = hidden - c;
+    float sum[2][8] = {};
+    for (int i = threadIdx.x / 32; i < kSlopeRows; i += 8) {
+        const int64_t r = r0 + i;
+        if (r >= rows || c >= cut) continue;
+        float v[8], g[8], u[8];
+        const T* from = dh + r * dh_stride + c;
+        const int64_t at = r * hidden + c;
+        load_some<T, 8>(from, live, v);
+        load_some<float, 8>(gate + at, live, g);
+        load_some<float, 8>(up + at, live, u);
+        typedef P vec __attribute__((ext_vector_type(8)));
+        vec q[2][kParts];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            d[0][k] = d[1][k] = 0.0f;
-            if (r < rows && c + k < hidden) {
-                const float g = to_f32<T>(gate[r * hidden + c + k]), u = to_f32<T>(up[r * hidden + c + k]);
-                const float v = to_f32<T>(dh[r * dh_stride + c + k]);
-                float slope;
-                const float a = act_of<T, true>(act, g, slope);
-                d[0][k] = v * u * slope;
-                d[1][k] = v * a;
-            }
-        }
+        for (int k = 0; k < 8; k++) {
+            float slope;
+            const float a = act_of<T, true>(act, g[k], slope);
+            const float both[2] = {k < live ? v[k] * u[k] * slope : 0.0f, k < live ? v[k] * a : 0.0f};
 #pragma unroll
-        for (int w = 0; w < 2; w++) {
-            typedef P vec __attribute__((ext_vector_type(4)));
-            vec q[kParts];
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                lds[w][i / 16][i % 16 * 4 + k] = d[w][k];
+            for (int w = 0; w < 2; w++) {
+                sum[w][k] += both[w];
                 P part[kParts];
-                split<P, kParts>(d[w][k], part);
+                split<P, kParts>(both[w], part);
 #pragma unroll
-                for (int p = 0; p < kParts; p++) q[p][k] = part[p];
+                for (int p = 0; p < kParts; p++) q[w][p][k] = part[p];
             }
-            if (flat && r < rows && c < hidden_up)
-#pragma unroll
-                for (int p = 0; p < kParts; p++)
-                    *(vec*)(flat + r * flat_stride + part_place<kParts>(w * hidden_up + c, p)) = q[p];
         }
+#pragma unroll
+        for (int w = 0; w < 2; w++)
+#pragma unroll
+            for (int p = 0; p < kParts; p++) *(vec*)(d + r * d_stride + part_place<kParts>(w * cut + c, p)) = q[w][p];
     }
+    if (!sums) return;
+#pragma unroll
+    for (int w = 0; w < 2; w++)
+#pragma unroll
+        for (int k = 0; k < 8; k++) lds[w][threadIdx.x / 32][column][k] = sum[w][k];
     __syncthreads();
-    const int64_t width = up_to(rows, 32);
-    if (turned)
-        for (int i = threadIdx.x; i < 2 * 64 * 8; i += 256) {
-            const int w = i / 512, c = c0 + i % 512 / 8;
-            const int64_t r = r0 + i % 8 * 8;
-            if (c >= hidden || r >= width) continue;
-            typedef P vec __attribute__((ext_vector_type(8)));
-            vec q[kParts];
+    for (int i = threadIdx.x; i < 512; i += 256) {
+        const int w = i / 256, n = (int)blockIdx.y * 256 + i % 256;
+        float all = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 8; k++) {
-                P part[kParts];
-                split<P, kParts>(lds[w][i % 8 * 8 + k][i % 512 / 8], part);
-#pragma unroll
-                for (int p = 0; p < kParts; p++) q[p][k] = part[p];
-            }
-#pragma unroll
-            for (int p = 0; p < kParts; p++)
-                *(vec*)(turned + ((int64_t)w * hidden + c) * turned_stride + part_place<kParts>(r, p)) = q[p];
-        }
-    if (sums && threadIdx.x < 128) {
-        const int w = threadIdx.x / 64, c = threadIdx.x % 64;
-        float v = 0.0f;
-        for (int r = 0; r < 64; r++) v += lds[w][r][c];
-        if (c0 + c < hidden) sums[((int64_t)blockIdx.x * 2 + w) * hidden + c0 + c] = v;
+        for (int k = 0; k < 8; k++) all += lds[w][k][i % 256 / 8][i % 8];
+        if (n < hidden) sums[((int64_t)blockIdx.x * 2 + w) * hidden + n] = all;
     }
 }
 
@@ -181,53 +160,62 @@ k_join_sums(const float* __restrict__ sums, int64_t blocks, int hidden, T* __res
     }
 }
 
-// out = A B^T: row m of the result is row m of `first` below `cut`, row m - cut of `second` from there on; with more than
-// one split (grid y) each leaves its part of the sums in `part[split][rows][n]` instead
+// out[m][n] of a turned B, and A by its rows or turned: row r of the result is row r of `first`, row cut + r row r of `second`,
+// `rows` of each; with more than one split (grid y) each leaves its part of the sums in `part[split][m][n]` instead
 struct Product {
-    Operand a, b;
+    Operand a, b, b_second;
     void *first, *second;
     float* part;
-    int cut, n, tiles_m, tiles_n, each;  // each: bytes of a row that a split takes
+    int m, n, rows, cut, cut_k;  // cut_k: the slice from which k goes on in b_second
+    int tiles_m, tiles_n, slices, each;  // each: slices that a split takes
 };
-template <typename T, typename Tl>
-__global__ void __launch_bounds__(Tl::kThreads, (Tl::kThreads == 512 ? 2 : 1)) k_product(Product f) {
-    __shared__ __attribute__((aligned(1024))) char lds[2 * Tl::kStage];
+template <typename T, typename Tl, bool kTurnedA>
+__global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_product(Product f) {
+    __shared__ __attribute__((aligned(1024))) char lds[Tl::kLds];
     const Place t = tile_place(blockIdx.x, f.tiles_m, f.tiles_n);
     const int m0 = t.m * Tl::kM, n0 = t.n * Tl::kN;
-    const int begin = (int)blockIdx.y * f.each, end = min(begin + f.each, f.a.bytes);
-    Sums<Tl> s;
-    multiply<Tl>(
-        f.a, m0, f.b, f.b, [](int r) { return r; }, [](int) { return false; }, n0, begin, end, lds, s);
+    const int begin = (int)blockIdx.y * f.each, end = min(begin + f.each, f.slices);
+    Sums<Tl, 1, true> s;
+    multiply<Tl, 1, kTurnedA, true>(f.a, m0, f.b, f.b_second, n0, f.cut_k, begin, end, lds, s);
+    constexpr int run = 4 * Tl::kFn;
+    const int n = n0 + s.col(), live = f.n - n;
+    if (live <= 0) return;
 #pragma unroll
     for (int i = 0; i < Tl::kFm; i++) {
         const int m = m0 + s.row() + i * 16;
-        if (m >= f.a.rows) continue;
+        if (m >= f.m) continue;
+        float v[run];
 #pragma unroll
-        for (int j = 0; j < Tl::kFn; j++) {
-            const int n = n0 + s.col() + j * 16, live = f.n - n;
-            if (live <= 0) continue;
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = s.acc[i][j][e];
-            if (f.part) {
-                store_some<float, 4>(f.part + ((int64_t)blockIdx.y * f.a.rows + m) * f.n + n, live, v);
-            } else {
-                T* to = m < f.cut ? (T*)f.first + (int64_t)m * f.n : (T*)f.second + (int64_t)(m - f.cut) * f.n;
-                store_some<T, 4>(to + n, live, v);
-            }
+        for (int e = 0; e < run; e++) v[e] = s.acc[i][e / 4][e % 4];
+        if (f.part) {
+            store_run<float, run>(f.part + ((int64_t)blockIdx.y * f.m + m) * f.n + n, live, v);
+        } else if (m < f.rows) {
+            store_run<T, run>((T*)f.first + (int64_t)m * f.n + n, live, v);
+        } else if (m >= f.cut && m - f.cut < f.rows) {
+            store_run<T, run>((T*)f.second + (int64_t)(m - f.cut) * f.n + n, live, v);
         }
     }
 }
 
-// the splits' parts added up
+// the splits' parts added up: 4 columns a thread, row r of `first` and, from row cut on, of `second`
 template <typename T>
 __global__ void __launch_bounds__(256)
-k_join_parts(const float* __restrict__ part, int splits, int64_t count, int64_t cut, T* __restrict__ first,
+k_join_parts(const float* __restrict__ part, int splits, int64_t m, int n, int rows, int cut, T* __restrict__ first,
              T* __restrict__ second) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
-        float v = 0.0f;
-        for (int s = 0; s < splits; s++) v += part[s * count + i];
-        (i < cut ? first[i] : second[i - cut]) = from_f32<T>(v);
+    const int across = (n + 3) / 4;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)rows * across * (second ? 2 : 1);
+         i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / across % rows;
+        const int c = (int)(i % across) * 4, live = n - c;
+        const bool of_first = i < (int64_t)rows * across;
+        float v[4] = {};
+        for (int s = 0; s < splits; s++) {
+            float p[4];
+            load_some<float, 4>(part + (s * m + (of_first ? r : cut + r)) * n + c, live, p);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] += p[e];
+        }
+        store_some<T, 4>((of_first ? first : second) + r * n + c, live, v);
     }
 }
 
@@ -255,9 +243,9 @@ struct Arena {
 
 // an operand of rows x cols values: as it is, or packed into the arena (only counted where the arena has no memory)
 template <typename T>
-int packed_rows(const void* src, int type, int64_t rows, int64_t cols, int64_t stride, Arena& ws, hipStream_t st,
-                Operand* out) {
-    if (as_it_is(src, type, rows, cols, stride)) {
+int packed_rows(const void* src, int type, int64_t rows, int64_t cols, int64_t stride, bool as_is, Arena& ws,
+                hipStream_t st, Operand* out) {
+    if (as_is) {
         *out = {src, (rows <= 1 ? cols : stride) * 2, (int)rows, (int)cols * 2};
         return 0;
     }
@@ -273,16 +261,14 @@ int packed_rows(const void* src, int type, int64_t rows, int64_t cols, int64_t s
         k_pack<T, T, 1><<<grid, kPackThreads, 0, st>>>((const T*)src, stride, rows, (int)cols, (T*)to, bytes / 2);
     return launched();
 }
+// both weights the same way: a tile takes them by one stride
 template <typename T>
-int packed_turned(const void* src, int64_t rows, int64_t cols, int64_t stride, char* to, int64_t to_stride, hipStream_t st) {
-    if (!to || rows == 0 || cols == 0) return 0;
-    const dim3 grid((unsigned)((rows + 63) / 64), (unsigned)((cols + 63) / 64));
-    if constexpr (sizeof(T) == 4)
-        k_pack_turned<float, bf16, 3>
-            <<<grid, kPackThreads, 0, st>>>((const float*)src, stride, rows, (int)cols, (bf16*)to, to_stride / 2);
-    else
-        k_pack_turned<T, T, 1><<<grid, kPackThreads, 0, st>>>((const T*)src, stride, rows, (int)cols, (T*)to, to_stride / 2);
-    return launched();
+int packed_weights(const void* wg, const void* wu, int64_t hidden, int64_t cols, Arena& ws, hipStream_t st, Operand* g,
+                   Operand* u) {
+    constexpr int type = sizeof(T) == 4 ? HG_F32 : HG_F16;
+    const bool as_is = as_it_is(wg, type, hidden, cols, cols) && as_it_is(wu, type, hidden, cols, cols);
+    const int e = packed_rows<T>(wg, type, hidden, cols, cols, as_is, ws, st, g);
+    return e ? e : packed_rows<T>(wu, type, hidden, cols, cols, as_is, ws, st, u);
 }
 
 // f called with the tile for an m x n result: the largest of which there are enough for the card's 256 compute units
@@ -290,20 +276,30 @@ template <typename T, typename F> int with_tile(int64_t m, int64_t n, F f) {
     using P = std::conditional_t<sizeof(T) == 4, bf16, T>;
     constexpr int parts = sizeof(T) == 4 ? 3 : 1;
     auto tiles = [&](int a, int b) { return ((m + a - 1) / a) * ((n + b - 1) / b); };
-    using Big = std::conditional_t<parts == 3, Tile<P, parts, 128, 256, 2, 4>, Tile<P, parts, 256, 256, 2, 4>>;
-    if (tiles(Big::kM, Big::kN) >= 192) return f(Big{});
-    if (tiles(128, 128) >= 192) return f(Tile<P, parts, 128, 128, 2, 2>{});
-    return f(Tile<P, parts, 64, 64, 2, 2>{});
+#ifdef TRY
+    if constexpr (parts == 1) {
+        if (TRY == 0) return f(Tile<P, parts, 2, 256, 256, 2, 4, 2, 1>{});
+        if (TRY == 1) return f(Tile<P, parts, 2, 128, 128, 2, 2, 2, 2>{});
+        if (TRY == 2) return f(Tile<P, parts, 2, 256, 128, 4, 2, 3, 1>{});
+    }
+#endif
+    if constexpr (parts == 1) {
+        if (tiles(256, 256) >= 192) return f(Tile<P, 1, 2, 256, 256, 2, 4, 2, 1>{});
+        if (tiles(128, 128) >= 192) return f(Tile<P, 1, 2, 128, 128, 2, 2, 2, 2>{});
+        return f(Tile<P, 1, 2, 64, 64, 2, 2, 3, 3>{});
+    } else {
+        if (tiles(128, 128) >= 192) return f(Tile<P, 3, 1, 128, 128, 2, 2, 3, 1>{});
+        return f(Tile<P, 3, 1, 64, 64, 2, 2, 3, 2>{});
+    }
 }
 
 template <typename T>
 int forward(const void* x, int64_t rows, int64_t cols, int64_t x_stride, const void* wg, const void* wu, int64_t hidden,
-            const void* bg, const void* bu, int act, void* h, void* gate, void* up, Arena& ws, hipStream_t st) {
+            const void* bg, const void* bu, int act, void* h, float* gate, float* up, Arena& ws, hipStream_t st) {
     constexpr int type = sizeof(T) == 4 ? HG_F32 : HG_F16;
     Forward f{};
-    int e = packed_rows<T>(x, type, rows, cols, x_stride, ws, st, &f.x);
-    if (!e) e = packed_rows<T>(wg, type, hidden, cols, cols, ws, st, &f.wg);
-    if (!e) e = packed_rows<T>(wu, type, hidden, cols, cols, ws, st, &f.wu);
+    int e = packed_rows<T>(x, type, rows, cols, x_stride, as_it_is(x, type, rows, cols, x_stride), ws, st, &f.x);
+    if (!e) e = packed_weights<T>(wg, wu, hidden, cols, ws, st, &f.wg, &f.wu);
     if (e || !ws.p) return e;
     f.x.bytes = std::min(f.x.bytes, std::min(f.wg.bytes, f.wu.bytes));  // a packed row's zeros have no partner in a plain one
     f.bg = bg;
@@ -322,34 +318,41 @@ int forward(const void* x, int64_t rows, int64_t cols, int64_t x_stride, const v
     });
 }
 
-// a b^T, the sum over k cut into splits where the tiles alone would leave compute units idle
-template <typename T>
-int product(const Operand& a, const Operand& b, int64_t cut, void* first, void* second, Arena& ws, hipStream_t st) {
-    return with_tile<T>(a.rows, b.rows, [&](auto tile) {
+// A B with k along B's rows, cut into splits where the tiles alone would leave compute units idle.  rows, cut, first, second:
+// Product's; k values in all, those from cut_k on of b_second.
+template <typename T, bool kTurnedA>
+int product(const Operand& a, const Operand& b, const Operand& b_second, int64_t m, int64_t k, int64_t cut_k, int64_t rows,
+            int64_t cut, void* first, void* second, int64_t n, Arena& ws, hipStream_t st) {
+    return with_tile<T>(m, n, [&](auto tile) {
         using Tl = decltype(tile);
+        constexpr int deep = 32 * Tl::kSteps;
         Product f{};
         f.a = a;
         f.b = b;
+        f.b_second = b_second;
         f.first = first;
         f.second = second;
+        f.m = (int)m;
+        f.n = (int)n;
+        f.rows = (int)rows;
         f.cut = (int)cut;
-        f.n = b.rows;
-        f.tiles_m = (a.rows + Tl::kM - 1) / Tl::kM;
-        f.tiles_n = (b.rows + Tl::kN - 1) / Tl::kN;
-        const int64_t tiles = (int64_t)f.tiles_m * f.tiles_n, slices = (a.bytes + Tl::kRow - 1) / Tl::kRow;
+        f.cut_k = (int)(cut_k / deep);
+        f.tiles_m = (int)((m + Tl::kM - 1) / Tl::kM);
+        f.tiles_n = (int)((n + Tl::kN - 1) / Tl::kN);
+        f.slices = (int)((k + deep - 1) / deep);
+        const int64_t tiles = (int64_t)f.tiles_m * f.tiles_n;
         // two blocks for each compute unit, at least 16 slices each
-        int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / tiles, slices / 16, 256}));
-        const int64_t each = (slices + splits - 1) / splits;
-        splits = (slices + each - 1) / each;
-        f.each = (int)(each * Tl::kRow);
-        const int64_t count = (int64_t)a.rows * b.rows;
-        if (splits > 1) f.part = (float*)ws.take(splits * count * 4);
+        int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / tiles, f.slices / 16, 256}));
+        f.each = (int)((f.slices + splits - 1) / splits);
+        splits = (f.slices + f.each - 1) / f.each;
+        if (splits > 1) f.part = (float*)ws.take(splits * m * n * 4);
         if (!ws.p) return 0;
-        k_product<T, Tl><<<dim3((unsigned)tiles, (unsigned)splits), Tl::kThreads, 0, st>>>(f);
+        k_product<T, Tl, kTurnedA><<<dim3((unsigned)tiles, (unsigned)splits), Tl::kThreads, 0, st>>>(f);
         int e = launched();
         if (!e && splits > 1) {
-            k_join_parts<T><<<(unsigned)std::min<int64_t>((count + 255) / 256, 4096), 256, 0, st>>>(
-                f.part, (int)splits, count, cut * b.rows, (T*)first, (T*)second);
+            const int64_t all = rows * ((n + 3) / 4) * (second ? 2 : 1);
+            k_join_parts<T><<<(unsigned)std::min<int64_t>((all + 255) / 256, 4096), 256, 0, st>>>(
+                f.part, (int)splits, m, (int)n, (int)rows, (int)cut, (T*)first, (T*)second);
             e = launched();
         }
         return e;
@@ -358,39 +361,35 @@ int product(const Operand& a, const Operand& b, int64_t cut, void* first, void* 
 
 template <typename T>
 int backward(const void* dh, int64_t dh_stride, const void* x, int64_t rows, int64_t cols, int64_t x_stride,
-             const void* wg, const void* wu, int64_t hidden, const void* gate, const void* up, int act, void* dx,
+             const void* wg, const void* wu, int64_t hidden, const float* gate, const float* up, int act, void* dx,
              void* dwg, void* dwu, void* dbg, void* dbu, Arena& ws, hipStream_t st) {
     using P = std::conditional_t<sizeof(T) == 4, bf16, T>;
-    constexpr int parts = sizeof(T) == 4 ? 3 : 1;
-    const int64_t hidden_up = up_to(hidden, 32), flat = packed_bytes(2 * hidden_up, parts), turned = packed_bytes(rows, parts);
-    const int64_t blocks = (rows + 63) / 64;
-    const bool weights = dwg != nullptr, biases = dbg || dbu;
-    char* d_flat = dx ? ws.take(rows * flat) : nullptr;
-    char* w_turned = dx ? ws.take(cols * flat) : nullptr;
-    char* d_turned = weights ? ws.take(2 * hidden * turned) : nullptr;
-    char* x_turned = weights ? ws.take(cols * turned) : nullptr;
+    constexpr int type = sizeof(T) == 4 ? HG_F32 : HG_F16, parts = sizeof(T) == 4 ? 3 : 1;
+    const int64_t cut = up_to(hidden, 64), d_bytes = packed_bytes(2 * cut, parts);  // 64: whole slices of each half
+    const int64_t blocks = (rows + kSlopeRows - 1) / kSlopeRows;
+    const bool biases = dbg || dbu;
+    char* d = ws.take(rows * d_bytes);
     float* sums = biases ? (float*)ws.take(blocks * 2 * hidden * 4) : nullptr;
     int e = 0;
     if (ws.p) {
-        k_gated_slopes<T, P, parts><<<dim3((unsigned)blocks, (unsigned)((hidden + 63) / 64)), 256, 0, st>>>(
-            (const T*)dh, dh_stride, (const T*)gate, (const T*)up, rows, (int)hidden, act, (P*)d_flat, flat / 2,
-            (P*)d_turned, turned / 2, sums);
+        k_gated_slopes<T, P, parts><<<dim3((unsigned)blocks, (unsigned)((cut + 255) / 256)), 256, 0, st>>>(
+            (const T*)dh, dh_stride, gate, up, rows, (int)hidden, act, (P*)d, d_bytes / 2, (int)cut, sums);
         e = launched();
         if (!e && biases) {
             k_join_sums<T><<<dim3((unsigned)((hidden + 63) / 64), 2), 1024, 0, st>>>(sums, blocks, (int)hidden, (T*)dbg, (T*)dbu);
             e = launched();
         }
     }
+    const Operand grads{d, d_bytes, (int)rows, (int)d_bytes};
     if (!e && dx) {
-        e = packed_turned<T>(wg, hidden, cols, cols, w_turned, flat, st);
-        if (!e) e = packed_turned<T>(wu, hidden, cols, cols, w_turned ? w_turned + hidden_up * 2 * parts : nullptr, flat, st);
-        const Operand a{d_flat, flat, (int)rows, (int)flat}, b{w_turned, flat, (int)cols, (int)flat};
-        if (!e) e = product<T>(a, b, rows, dx, nullptr, ws, st);
+        Operand g, u;
+        e = packed_weights<T>(wg, wu, hidden, cols, ws, st, &g, &u);
+        if (!e) e = product<T, false>(grads, g, u, rows, 2 * cut, cut, rows, rows, dx, nullptr, cols, ws, st);
     }
-    if (!e && weights) {
-        e = packed_turned<T>(x, rows, cols, x_stride, x_turned, turned, st);
-        const Operand a{d_turned, turned, (int)(2 * hidden), (int)turned}, b{x_turned, turned, (int)cols, (int)turned};
-        if (!e) e = product<T>(a, b, hidden, dwg, dwu, ws, st);
+    if (!e && dwg) {
+        Operand b;
+        e = packed_rows<T>(x, type, rows, cols, x_stride, as_it_is(x, type, rows, cols, x_stride), ws, st, &b);
+        if (!e) e = product<T, true>(grads, b, b, 2 * cut, rows, 1 << 30, hidden, cut, dwg, dwu, cols, ws, st);
     }
     return e;
 }
@@ -427,8 +426,8 @@ int64_t hg_gated_forward_workspace(const void* x, int type, int64_t rows, int64_
 }
 
 int hg_gated_forward(const void* x, int type, int64_t rows, int64_t cols, int64_t x_stride, const void* w_gate,
-                     const void* w_up, int64_t hidden, const void* b_gate, const void* b_up, int act, void* h, void* gate,
-                     void* up, void* workspace, void* stream) {
+                     const void* w_up, int64_t hidden, const void* b_gate, const void* b_up, int act, void* h, float* gate,
+                     float* up, void* workspace, void* stream) {
     if (bad_sizes(type, rows, cols, hidden, act) || !w_gate || !w_up || (rows > 0 && (!x || !h)) || !gate != !up)
         return (int)hipErrorInvalidValue;
     if (rows == 0) return 0;
@@ -445,16 +444,17 @@ int64_t hg_gated_backward_workspace(int type, int64_t rows, int64_t cols, int64_
     if (bad_sizes(type, rows, cols, hidden, HG_SIGMOID) || rows == 0) return 0;
     Arena ws{nullptr};
     char some[4];
+    const char* odd = (const char*)1;  // an address that nothing can be taken as it is from: the most there can be
     with_type(type, [&](auto t) {
-        return backward<decltype(t)>(nullptr, 0, nullptr, rows, cols, cols, nullptr, nullptr, hidden, nullptr, nullptr, 0,
-                                     some, some, some, some, some, ws, nullptr);
+        return backward<decltype(t)>(nullptr, 0, odd, rows, cols, cols, odd, odd, hidden, nullptr, nullptr, 0, some, some,
+                                     some, some, some, ws, nullptr);
     });
     return ws.used;
 }
 
 int hg_gated_backward(const void* dh, int64_t dh_stride, const void* x, int type, int64_t rows, int64_t cols,
-                      int64_t x_stride, const void* w_gate, const void* w_up, int64_t hidden, const void* gate,
-                      const void* up, int act, void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up,
+                      int64_t x_stride, const void* w_gate, const void* w_up, int64_t hidden, const float* gate,
+                      const float* up, int act, void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up,
                       void* workspace, void* stream) {
     if (bad_sizes(type, rows, cols, hidden, act) || !w_gate || !w_up || !dw_gate != !dw_up ||
         (rows > 0 && (!dh || !x || !gate || !up)))

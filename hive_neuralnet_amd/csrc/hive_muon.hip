@@ -15,9 +15,8 @@
 // their last parts stay above float16's smallest), and products are three
 // matrix instructions of parts (hive_matrix.hpp).
 //
-// X is held both ways, its rows for X X^T and its columns for P X, so that k
-// runs along the rows of every operand.  A and A A are symmetric: the tiles on
-// and above the diagonal are computed, and stored twice.
+// X is an operand by its rows in X X^T and by its columns in P X.  A and A A are
+// symmetric: the tiles on and above the diagonal are computed, and stored twice.
 #include <algorithm>
 #include <cmath>
 
@@ -55,7 +54,7 @@ struct Table {
 struct Layout {
     int s, l;                // the shorter and the longer side
     int64_t sb, lb;          // bytes of a packed row along each
-    int64_t x[2], xt[2], a, p, sums, all;
+    int64_t x[2], a, p, sums, all;
 };
 __host__ __device__ inline Layout layout(int rows, int cols) {
     Layout o;
@@ -64,12 +63,10 @@ __host__ __device__ inline Layout layout(int rows, int cols) {
     o.sb = up_to(o.s, 32) * 4;
     o.lb = up_to(o.l, 32) * 4;
     int64_t at = 0;
-    const int64_t x = up_to(o.s * o.lb, 256), xt = up_to(o.l * o.sb, 256), a = up_to(o.s * o.sb, 256);
+    const int64_t x = up_to(o.s * o.lb, 256), a = up_to(o.s * o.sb, 256);
     for (int i = 0; i < 2; i++) {
         o.x[i] = at;
         at += x;
-        o.xt[i] = at;
-        at += xt;
     }
     o.a = at;
     o.p = at + a;
@@ -122,7 +119,7 @@ __global__ void __launch_bounds__(256) k_muon_sums(Table tab) {
         ((double*)(x.held + matrix * o.all + o.sums))[part] = (waves[0] + waves[1]) + (waves[2] + waves[3]);
 }
 
-// X and its transpose, of parts, from the update: 64 x 64 pieces turned in LDS
+// X, of parts, from the update: 64 x 64 pieces, turned in LDS where the matrix is taller than wide
 __global__ void __launch_bounds__(256) k_muon_pack(Table tab) {
     __shared__ float turn[64][65];
     int t = blockIdx.x;
@@ -149,25 +146,20 @@ __global__ void __launch_bounds__(256) k_muon_pack(Table tab) {
         turn[i / 64][i % 64] = u;
     }
     __syncthreads();
-    // rows of the matrix as it is, and turned
     const bool tall = x.rows > x.cols;
-    f16* flat = (f16*)(held + (tall ? o.xt[0] : o.x[0]));
-    f16* turned = (f16*)(held + (tall ? o.x[0] : o.xt[0]));
-    const int64_t flat_row = up_to(x.cols, 32) * 2, turned_row = up_to(x.rows, 32) * 2;
-    for (int i = threadIdx.x; i < 2 * 64 * 8; i += 256) {
-        const bool across = i >= 512;
-        const int a = i % 512 / 8, b = i % 8 * 8;  // a row of the result and 8 of its columns
-        const int row = (across ? c0 : r0) + a, col = (across ? r0 : c0) + b;
-        if (row >= (across ? x.cols : x.rows) || col >= up_to(across ? x.rows : x.cols, 32)) continue;
+    for (int i = threadIdx.x; i < 64 * 8; i += 256) {
+        const int a = i / 8, b = i % 8 * 8;  // a row of the result and 8 of its columns
+        const int row = (tall ? c0 : r0) + a, col = (tall ? r0 : c0) + b;
+        if (row >= o.s || col >= up_to(o.l, 32)) continue;
         h8 hi, lo;
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             f16 part[2];
-            split<f16, 2>(across ? turn[b + k][a] : turn[a][b + k], part);
+            split<f16, 2>(tall ? turn[b + k][a] : turn[a][b + k], part);
             hi[k] = part[0];
             lo[k] = part[1];
         }
-        f16* to = (across ? turned + row * turned_row : flat + row * flat_row);
+        f16* to = (f16*)(held + o.x[0] + row * o.lb);
         *(h8*)(to + part_place<2>(col, 0)) = hi;
         *(h8*)(to + part_place<2>(col, 1)) = lo;
     }
@@ -175,28 +167,33 @@ __global__ void __launch_bounds__(256) k_muon_pack(Table tab) {
 
 enum Kind { kGram, kPoly, kStep };
 
-// columns c .. c + 3 (c % 4 = 0) of a row of parts
-__device__ __forceinline__ void store_parts(f16* row, int64_t c, const float v[4]) {
-    typedef f16 vec __attribute__((ext_vector_type(4)));
-    vec hi, lo;
+// the tiles of a symmetric result on and above the diagonal, each `wide` times as wide as high: row i has those from i / wide on
+__host__ __device__ inline int upper_tiles(int m, int n, int wide) {
+    int all = 0;
+    for (int i = 0; i < m; i++) all += n - i / wide;
+    return all;
+}
+
+// columns c .. c + 7 (c % 8 = 0) of a row of parts
+__device__ __forceinline__ void store_parts(f16* row, int64_t c, const float (&v)[8]) {
+    h8 hi, lo;
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
+    for (int e = 0; e < 8; e++) {
         hi[e] = (f16)v[e];
         lo[e] = (f16)(v[e] - (float)hi[e]);
     }
-    *(vec*)(row + part_place<2>(c, 0)) = hi;
-    *(vec*)(row + part_place<2>(c, 1)) = lo;
+    *(h8*)(row + part_place<2>(c, 0)) = hi;
+    *(h8*)(row + part_place<2>(c, 1)) = lo;
 }
-__device__ __forceinline__ void load_parts(const f16* row, int64_t c, float v[4]) {
-    typedef f16 vec __attribute__((ext_vector_type(4)));
-    const vec hi = *(const vec*)(row + part_place<2>(c, 0)), lo = *(const vec*)(row + part_place<2>(c, 1));
+__device__ __forceinline__ void load_parts(const f16* row, int64_t c, float (&v)[8]) {
+    const h8 hi = *(const h8*)(row + part_place<2>(c, 0)), lo = *(const h8*)(row + part_place<2>(c, 1));
 #pragma unroll
-    for (int e = 0; e < 4; e++) v[e] = (float)hi[e] + (float)lo[e];
+    for (int e = 0; e < 8; e++) v[e] = (float)hi[e] + (float)lo[e];
 }
 // the same columns, one row each, at column `c`
-__device__ __forceinline__ void store_parts_down(f16* first, int64_t row, int64_t c, int live, const float v[4]) {
+__device__ __forceinline__ void store_parts_down(f16* first, int64_t row, int64_t c, int live, const float (&v)[8]) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
+    for (int e = 0; e < 8; e++) {
         const f16 hi = (f16)v[e];
         if (e < live) {
             first[e * row + part_place<2>(c, 0)] = hi;
@@ -206,66 +203,68 @@ __device__ __forceinline__ void store_parts_down(f16* first, int64_t row, int64_
 }
 
 template <int kKind, typename Tl>
-__global__ void __launch_bounds__(Tl::kThreads, (Tl::kThreads == 512 ? 2 : 1)) k_muon_product(Table tab) {
-    __shared__ __attribute__((aligned(1024))) char lds[2 * Tl::kStage];
+__global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_muon_product(Table tab) {
+    __shared__ __attribute__((aligned(1024))) char lds[Tl::kLds];
     int t = chiplet_order(blockIdx.x, tab.blocks);
     const Matrix& x = tab.t[find(tab, t)];
     const Layout o = layout(x.rows, x.cols);
-    const int tiles_s = (o.s + Tl::kM - 1) / Tl::kM, tiles_l = (o.l + Tl::kN - 1) / Tl::kN;
-    const int per = kKind == kStep ? tiles_s * tiles_l : tiles_s * (tiles_s + 1) / 2;
+    constexpr int wide_tile = Tl::kN / Tl::kM;
+    const int tiles_s = (o.s + Tl::kM - 1) / Tl::kM, tiles_n = ((kKind == kStep ? o.l : o.s) + Tl::kN - 1) / Tl::kN;
+    const int per = kKind == kStep ? tiles_s * tiles_n : upper_tiles(tiles_s, tiles_n, wide_tile);
     const int matrix = t / per;
     t -= matrix * per;
     char* held = x.held + matrix * o.all;
     Place at;
     if (kKind == kStep) {
-        at = band_place(t, tiles_s, tiles_l);
+        at = band_place(t, tiles_s, tiles_n);
     } else {  // row by row, from the diagonal on
         at.m = 0;
-        while (t >= tiles_s - at.m) t -= tiles_s - at.m++;
-        at.n = at.m + t;
+        while (t >= tiles_n - at.m / wide_tile) t -= tiles_n - at.m++ / wide_tile;
+        at.n = at.m / wide_tile + t;
     }
     Operand a, b;
     if (kKind == kGram) a = b = {held + o.x[tab.from], o.lb, o.s, (int)o.lb};
     if (kKind == kPoly) a = b = {held + o.a, o.sb, o.s, (int)o.sb};
     if (kKind == kStep) {
         a = {held + o.p, o.sb, o.s, (int)o.sb};
-        b = {held + o.xt[tab.from], o.sb, o.l, (int)o.sb};
+        b = {held + o.x[tab.from], o.lb, o.s, (int)o.lb};
     }
     const int m0 = at.m * Tl::kM, n0 = at.n * Tl::kN;
-    Sums<Tl> s;
-    multiply<Tl>(
-        a, m0, b, b, [](int r) { return r; }, [](int) { return false; }, n0, 0, a.bytes, lds, s);
+    Sums<Tl, 1, kKind == kStep> s;
+    multiply<Tl, 1, false, kKind == kStep>(a, m0, b, b, n0, 1 << 30, 0, (a.bytes + Tl::kRow - 1) / Tl::kRow, lds, s);
+    constexpr int run = 4 * Tl::kFn;  // of a lane's columns that follow each other
     const bool tall = x.rows > x.cols;
     f16* const to = (f16*)(held + (kKind == kGram ? o.a : kKind == kPoly ? o.p : o.x[tab.from ^ 1]));
     const int wide = kKind == kStep ? o.l : o.s;              // columns of the result
     const int64_t row = (kKind == kStep ? o.lb : o.sb) / 2;   // elements of its packed rows
+    const int first = n0 + s.col();
 #pragma unroll
     for (int i = 0; i < Tl::kFm; i++) {
         const int m = m0 + s.row() + i * 16;
         if (m >= up_to(o.s, 32)) continue;
         const bool there = m < o.s;
 #pragma unroll
-        for (int j = 0; j < Tl::kFn; j++) {
-            const int n = n0 + s.col() + j * 16, live = wide - n;
+        for (int c = 0; c < run; c += 8) {
+            const int n = first + c, live = wide - n;
             if (n >= up_to(wide, 32)) continue;
-            float v[4];
+            float v[8];
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = s.acc[i][j][e] * (1.0f / kScale);
+            for (int e = 0; e < 8; e++) v[e] = s.acc[i][(c + e) / 4][e % 4] * (1.0f / kScale);
             if (kKind == kPoly) {
-                float g[4] = {};
+                float g[8] = {};
                 if (there) load_parts((const f16*)(held + o.a) + m * row, n, g);
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = fmaf(tab.c, v[e], tab.b * g[e]);
+                for (int e = 0; e < 8; e++) v[e] = fmaf(tab.c, v[e], tab.b * g[e]);
             }
             if (kKind == kStep) {
-                float g[4] = {};
+                float g[8] = {};
                 if (there) load_parts((const f16*)(held + o.x[tab.from]) + m * row, n, g);
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = fmaf(tab.a, g[e], v[e]);
+                for (int e = 0; e < 8; e++) v[e] = fmaf(tab.a, g[e], v[e]);
                 if (tab.last) {
                     if (!there) continue;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
+                    for (int e = 0; e < 8; e++) {
                         if (e >= live) break;
                         const int64_t i_out = matrix * x.out_step + (tall ? (int64_t)(n + e) * x.cols + m
                                                                           : (int64_t)m * x.cols + n + e);
@@ -275,10 +274,9 @@ __global__ void __launch_bounds__(Tl::kThreads, (Tl::kThreads == 512 ? 2 : 1)) k
                     }
                     continue;
                 }
-                store_parts_down((f16*)(held + o.xt[tab.from ^ 1]) + (int64_t)n * (o.sb / 2), o.sb / 2, m, live, v);
             }
             if (there) store_parts(to + m * row, n, v);
-            if (kKind != kStep && at.n > at.m)  // the tile's mirror image
+            if (kKind != kStep && at.n > at.m / wide_tile)  // the tile's mirror image, where no tile is
                 store_parts_down(to + n * row, row, m, live, v);
         }
     }
@@ -299,8 +297,8 @@ template <typename F> int64_t lay_blocks(Table& tab, F f) {
 
 template <typename Tl> int64_t step_tiles(const Matrix& x, bool symmetric) {
     const int s = std::min(x.rows, x.cols), l = std::max(x.rows, x.cols);
-    const int64_t ts = (s + Tl::kM - 1) / Tl::kM, tl = (l + Tl::kN - 1) / Tl::kN;
-    return symmetric ? ts * (ts + 1) / 2 : ts * tl;
+    const int m = (s + Tl::kM - 1) / Tl::kM, n = ((symmetric ? s : l) + Tl::kN - 1) / Tl::kN;
+    return symmetric ? upper_tiles(m, n, Tl::kN / Tl::kM) : (int64_t)m * n;
 }
 
 // one product of every matrix of the table, in the largest tiles of which there are enough for the card
@@ -312,9 +310,17 @@ template <int kKind> int product(Table& tab, hipStream_t st) {
         k_muon_product<kKind, Tl><<<(unsigned)blocks, Tl::kThreads, 0, st>>>(tab);
         return launched();
     };
-    int e = launch(Tile<f16, 2, 256, 256, 2, 4>{}, 192);
-    if (e < 0) e = launch(Tile<f16, 2, 128, 128, 2, 2>{}, 192);
-    if (e < 0) e = launch(Tile<f16, 2, 64, 64, 2, 2>{}, 0);
+#ifdef TRY
+    int e = -1;
+    if (TRY == 1) e = launch(Tile<f16, 2, 1, 128, 128, 2, 2, 2, 2>{}, 192);
+    if (TRY == 2) e = launch(Tile<f16, 2, 1, 128, 256, 2, 4, 3, 1>{}, 192);
+    if (TRY == 3) e = launch(Tile<f16, 2, 1, 128, 128, 2, 2, 4, 1>{}, 192);
+    if (TRY == 4) e = launch(Tile<f16, 2, 1, 128, 256, 4, 4, 3, 1>{}, 192);
+#else
+    int e = launch(Tile<f16, 2, 1, 128, 256, 2, 4, 3, 1>{}, 192);
+#endif
+    if (e < 0) e = launch(Tile<f16, 2, 1, 128, 128, 2, 2, 2, 2>{}, 192);
+    if (e < 0) e = launch(Tile<f16, 2, 1, 64, 64, 2, 2, 4, 2>{}, 0);
     return e;
 }
 

@@ -62,37 +62,4 @@ k_pack(const S* __restrict__ src, int64_t src_stride, int64_t rows, int cols, T*
     }
 }
 
-// dst[c] = the parts of column c of src[rows][cols], zeros up to a multiple of 32 rows: 64 x 64 pieces turned in LDS.
-template <typename S, typename T, int kParts>
-__global__ void __launch_bounds__(kPackThreads)
-k_pack_turned(const S* __restrict__ src, int64_t src_stride, int64_t rows, int cols, T* __restrict__ dst,
-              int64_t dst_stride) {
-    __shared__ float turn[64][65];
-    const int64_t r0 = (int64_t)blockIdx.x * 64;
-    const int c0 = (int)blockIdx.y * 64;
-    for (int i = threadIdx.x; i < 64 * 64; i += kPackThreads) {
-        const int64_t r = r0 + i / 64;
-        const int c = c0 + i % 64;
-        turn[i / 64][i % 64] = r < rows && c < cols ? to_f32<S>(src[r * src_stride + c]) : 0.0f;
-    }
-    __syncthreads();
-    const int64_t width = up_to(rows, 32);
-    for (int i = threadIdx.x; i < 64 * 8; i += kPackThreads) {
-        const int c = c0 + i / 8;
-        const int64_t r = r0 + i % 8 * 8;
-        if (c >= cols || r >= width) continue;
-        typedef T vec __attribute__((ext_vector_type(8)));
-        vec q[kParts];
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            T part[kParts];
-            split<T, kParts>(turn[i % 8 * 8 + k][i / 8], part);
-#pragma unroll
-            for (int p = 0; p < kParts; p++) q[p][k] = part[p];
-        }
-#pragma unroll
-        for (int p = 0; p < kParts; p++) *(vec*)(dst + c * dst_stride + part_place<kParts>(r, p)) = q[p];
-    }
-}
-
 }  // namespace hm

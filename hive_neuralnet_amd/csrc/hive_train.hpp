@@ -94,6 +94,19 @@ template <typename T, int n = Vector<T>::n> __device__ __forceinline__ void stor
     }
 }
 
+// n values (4 or 8) from p, zeros past the first `live`
+template <typename T, int n> __device__ __forceinline__ void load_some(const T* p, int live, float v[n]) {
+    typedef T vec __attribute__((ext_vector_type(n), aligned(sizeof(T))));
+    if (live >= n) {
+        const vec q = *(const vec*)p;
+#pragma unroll
+        for (int i = 0; i < n; i++) v[i] = to_f32<T>(q[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < n; i++) v[i] = i < live ? to_f32<T>(p[i]) : 0.0f;
+    }
+}
+
 // v of the lane that shares a lane group: 1, 2 lanes away, mirrored in 8 and
 // in 16 lanes (data-parallel moves of the VALU), the other row of 16, the
 // other half of the wave

@@ -61,12 +61,13 @@ def _activation(activation) -> int:
     return ACTIVATIONS[activation]
 
 
-def _matrix(t, name: str, shape, like: torch.Tensor) -> int:
-    """The address of a contiguous tensor of like's type and device."""
+def _matrix(t, name: str, shape, like: torch.Tensor, dtype=None) -> int:
+    """The address of a contiguous tensor on like's device, of its type or `dtype`."""
+    dtype = dtype or like.dtype
     if not isinstance(t, torch.Tensor) or t.device != like.device:
         raise ValueError(f"{name} must be a tensor on {like.device}")
-    if t.dtype != like.dtype or tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must be {tuple(shape)} {like.dtype}, got {tuple(t.shape)} {t.dtype}")
+    if t.dtype != dtype or tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {tuple(shape)} {dtype}, got {tuple(t.shape)} {t.dtype}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
     return t.data_ptr()
@@ -95,7 +96,7 @@ def _gated_forward(self, x, w_gate, w_up, b_gate, b_up, activation, keep: bool):
     bu = None if b_up is None else _vector(b_up, "b_up", hidden, x.dtype, dev)
     shape, kind = (*x.shape[:-1], hidden), TYPES[x.dtype]
     h = x.new_empty(shape)
-    gate, up = (x.new_empty(shape), x.new_empty(shape)) if keep else (None, None)
+    gate, up = (x.new_empty(shape, dtype=torch.float32) for _ in range(2)) if keep else (None, None)
     need = self._lib.hg_gated_forward_workspace(x.data_ptr(), kind, rows, cols, stride, w_gate.data_ptr(),
                                                 w_up.data_ptr(), hidden)
     ws = x.new_empty((need,), dtype=torch.uint8) if need else None
@@ -122,8 +123,9 @@ def gated_linear(self, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor
 
 def gated_linear_forward(self, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate=None, b_up=None,
                          activation="silu"):
-    """(h, gate, up): gated_linear and the two products, rounded to x's type,
-    which gated_linear_backward takes."""
+    """(h, gate, up): gated_linear and the two products in float32 (to round
+    them to 16 bits would be a third of the gradients' error), which
+    gated_linear_backward takes."""
     return _gated_forward(self, x, w_gate, w_up, b_gate, b_up, activation, True)
 
 
@@ -134,8 +136,7 @@ def gated_linear_backward(self, dh: torch.Tensor, x: torch.Tensor, w_gate: torch
     dh, the gradient of h, with the forward pass's x, weights, gate, up and
     activation; None for what is not needed.  They have x's type and are
     contiguous; sums over rows are the same bits on every call.  The gradients of
-    gate and up are rounded to x's type before they are multiplied, as gate
-    and up were."""
+    gate and up are rounded to x's type before they are multiplied."""
     act = _activation(activation)
     dev, rows, cols, stride, hidden = _gated_sizes(x, w_gate, w_up)
     shape = (*x.shape[:-1], hidden)
@@ -143,7 +144,7 @@ def gated_linear_backward(self, dh: torch.Tensor, x: torch.Tensor, w_gate: torch
     if tuple(dh.shape) != shape or dh.dtype != x.dtype:
         raise ValueError(f"dh must be {shape} {x.dtype}, got {tuple(dh.shape)} {dh.dtype}")
     dh_stride = _rows(dh, "dh")[2]
-    g, u = _matrix(gate, "gate", shape, x), _matrix(up, "up", shape, x)
+    g, u = _matrix(gate, "gate", shape, x, torch.float32), _matrix(up, "up", shape, x, torch.float32)
     dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_dx else None
     dw = (torch.empty_like(w_gate), torch.empty_like(w_up)) if need_weights else (None, None)
     db = (x.new_empty((hidden,)), x.new_empty((hidden,))) if need_bias else (None, None)

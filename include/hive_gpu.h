@@ -591,9 +591,10 @@ int hg_adamw_step(const hg_adamw_tensor* tensors, int64_t count, int param_type,
  *
  * The gated block: gate = x Wg^T + bg, up = x Wu^T + bu, h = act(gate) up.
  * x[rows][cols] (row r at x + r * x_stride elements), w_gate and w_up
- * [hidden][cols], b_gate and b_up [hidden] (NULL = 0), h, gate and up
- * [rows][hidden] are of one type; gate and up, which the backward pass needs,
- * are both given or both NULL.  Sums are float32; float32 tensors are
+ * [hidden][cols], b_gate and b_up [hidden] (NULL = 0), and h
+ * [rows][hidden] are of one type; gate and up [rows][hidden], which the backward
+ * pass needs, are float, both given or both NULL (rounding them to 16 bits would
+ * be a third of its results' error).  Sums are float32; float32 tensors are
  * multiplied in three bfloat16 parts a value, 24 bits (values below 2^-110 to
  * within 2^-134).  rows <= 2^20, cols and
  * hidden <= 2^19, each two of them at most 2^35 together.  workspace: as many bytes, 256-byte aligned (none where that
@@ -604,8 +605,8 @@ int hg_adamw_step(const hg_adamw_tensor* tensors, int64_t count, int param_type,
 int64_t hg_gated_forward_workspace(const void* x, int type, int64_t rows, int64_t cols, int64_t x_stride,
                                    const void* w_gate, const void* w_up, int64_t hidden);
 int hg_gated_forward(const void* x, int type, int64_t rows, int64_t cols, int64_t x_stride, const void* w_gate,
-                     const void* w_up, int64_t hidden, const void* b_gate, const void* b_up, int act, void* h, void* gate,
-                     void* up, void* workspace, void* stream);
+                     const void* w_up, int64_t hidden, const void* b_gate, const void* b_up, int act, void* h, float* gate,
+                     float* up, void* workspace, void* stream);
 
 /* Its gradients from dh[rows][hidden] (rows dh_stride elements apart), of x's
  * type, contiguous; those of the weights come together, any other is left out
@@ -613,8 +614,8 @@ int hg_gated_forward(const void* x, int type, int64_t rows, int64_t cols, int64_
  * workspace: as many bytes, 256-byte aligned. */
 int64_t hg_gated_backward_workspace(int type, int64_t rows, int64_t cols, int64_t hidden);
 int hg_gated_backward(const void* dh, int64_t dh_stride, const void* x, int type, int64_t rows, int64_t cols,
-                      int64_t x_stride, const void* w_gate, const void* w_up, int64_t hidden, const void* gate,
-                      const void* up, int act, void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up,
+                      int64_t x_stride, const void* w_gate, const void* w_up, int64_t hidden, const float* gate,
+                      const float* up, int act, void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up,
                       void* workspace, void* stream);
 
 /* The Newton-Schulz iteration of `count` matrices u[rows][cols] (matrix i at

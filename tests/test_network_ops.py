@@ -94,7 +94,7 @@ def test_orthogonalize_refusals():
                 dict(count=2, rows=1 << 17, cols=1 << 17)):
         assert call(**bad) == INVALID, bad
     assert call(count=0, u=None, out=None, ws=None) == 0
-    assert lib.hg_orthogonalize_workspace(3, 10, 40) >= 3 * (2 * (10 * 64 + 40 * 32) + 2 * 10 * 32) * 4
+    assert lib.hg_orthogonalize_workspace(3, 10, 40) >= 3 * (2 * 10 * 64 + 2 * 10 * 32) * 4
     assert lib.hg_orthogonalize_workspace(1, 0, 40) == 0
 
 
