@@ -2,7 +2,7 @@
 // batch of matrices, and the step of many of a network's matrices with it.
 //
 //   X = U / (|U| + eps), |U| the root of the sum of squares
-//   steps times:  A = X X^T,  P = b A + c A A,  X <- a X + P X
+//   steps times:  A = X X^T,  P = a I + b A + c A A,  X <- P X
 // which takes each singular value s to a s + b s^3 + c s^5, and with the usual
 // (a, b, c) all of them near 1.  X has the shorter side's rows: a matrix that is
 // taller than wide is turned, and turned back at the end.  A step with it:
@@ -29,6 +29,7 @@ using namespace hm;
 constexpr int kMatrices = 24;        // of a launch: their table is a kernel argument
 constexpr float kScale = 8192.0f;    // of every held matrix
 constexpr int kSumBlocks = 64;       // of a matrix's sum of squares
+constexpr int kTriples = 16;         // coefficients that a launch of the whole iteration takes
 constexpr int64_t kMaxSide = 1 << 17;
 
 // One of the step's matrices, or a batch of one shape.
@@ -48,6 +49,8 @@ struct Table {
     int g_type, out_type, update;  // update: out is a parameter
     float mu, keep, eps, a, b, c;
     int nesterov, from, last;  // from: which of the two copies of X is current
+    int steps, count;          // the iteration in one launch: its steps, and how many of them have coefficients of their own
+    float triples[3 * kTriples];
 };
 
 // where a matrix's parts lie in its workspace, in bytes
@@ -75,15 +78,6 @@ __host__ __device__ inline Layout layout(int rows, int cols) {
     return o;
 }
 
-__device__ __forceinline__ float load_any(const void* p, int type, int64_t i) {
-    return type == HG_F32 ? ((const float*)p)[i] : type == HG_F16 ? (float)((const f16*)p)[i] : (float)((const bf16*)p)[i];
-}
-__device__ __forceinline__ void store_any(void* p, int type, int64_t i, float v) {
-    if (type == HG_F32) ((float*)p)[i] = v;
-    else if (type == HG_F16) ((f16*)p)[i] = (f16)v;
-    else ((bf16*)p)[i] = (bf16)v;
-}
-
 // the matrix that block t works on, t from there on its own
 __device__ __forceinline__ int find(const Table& tab, int& t) {
     int i = 0;
@@ -92,23 +86,40 @@ __device__ __forceinline__ int find(const Table& tab, int& t) {
     return i;
 }
 
-// the momentum's step, and the sum of squares of the update in kSumBlocks parts
-__global__ void __launch_bounds__(256) k_muon_sums(Table tab) {
+// values c .. c + 7 of the update's row r, zeros past the first `live`; `m`: the momentum of the same values as it is (kStep
+// false), or before this step, which is taken and stored
+template <typename G, bool kStep>
+__device__ __forceinline__ void load_update(const Matrix& x, const Table& tab, int64_t at_g, int64_t at_m, int live,
+                                            float (&u)[8]) {
+    load_some<G, 8>((const G*)x.g + at_g, live, u);
+    if (!x.momentum) return;
+    float m[8];
+    load_some<float, 8>(x.momentum + at_m, live, m);
+    if (kStep) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) m[e] = fmaf(m[e], tab.mu, u[e]);
+        store_some<float, 4>(x.momentum + at_m, live, m);
+        store_some<float, 4>(x.momentum + at_m + 4, live - 4, m + 4);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) u[e] = tab.nesterov ? fmaf(m[e], tab.mu, u[e]) : m[e];
+}
+
+// the momentum's step, and the sum of squares of the update in kSumBlocks parts; memory bound
+template <typename G> __global__ void __launch_bounds__(256) k_muon_sums(Table tab) {
     int t = blockIdx.x;
     const Matrix& x = tab.t[find(tab, t)];
     const int matrix = t / kSumBlocks, part = t % kSumBlocks;
-    const int64_t all = (int64_t)x.rows * x.cols;
-    const int64_t each = (all + kSumBlocks - 1) / kSumBlocks, begin = part * each, end = min(begin + each, all);
+    // rows that follow each other are one
+    const bool flat = x.g_row == x.cols;
+    const int64_t cols = flat ? (int64_t)x.rows * x.cols : x.cols, across = (cols + 7) / 8, all = flat ? across : across * x.rows;
     double sum = 0.0;
-    for (int64_t i = begin + threadIdx.x; i < end; i += 256) {
-        const int64_t r = i / x.cols, c = i - r * x.cols;
-        float u = load_any(x.g, tab.g_type, matrix * x.g_step + r * x.g_row + c);
-        if (x.momentum) {
-            const float m = fmaf(x.momentum[i], tab.mu, u);
-            x.momentum[i] = m;
-            u = tab.nesterov ? fmaf(m, tab.mu, u) : m;
-        }
-        sum = fma((double)u, (double)u, sum);
+    for (int64_t i = (int64_t)part * 256 + threadIdx.x; i < all; i += kSumBlocks * 256) {
+        const int64_t r = flat ? 0 : i / across, c = (i - r * across) * 8;
+        float u[8];
+        load_update<G, true>(x, tab, matrix * x.g_step + r * x.g_row + c, r * cols + c, (int)min(cols - c, (int64_t)8), u);
+#pragma unroll
+        for (int e = 0; e < 8; e++) sum = fma((double)u[e], (double)u[e], sum);
     }
     for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
     __shared__ double waves[4];
@@ -119,8 +130,10 @@ __global__ void __launch_bounds__(256) k_muon_sums(Table tab) {
         ((double*)(x.held + matrix * o.all + o.sums))[part] = (waves[0] + waves[1]) + (waves[2] + waves[3]);
 }
 
-// X, of parts, from the update: 64 x 64 pieces, turned in LDS where the matrix is taller than wide
-__global__ void __launch_bounds__(256) k_muon_pack(Table tab) {
+__device__ __forceinline__ void store_parts(f16* row, int64_t c, const float (&v)[8]);
+
+// X, of parts, from the update: 64 x 64 pieces, turned in LDS where the matrix is taller than wide; memory bound
+template <typename G> __global__ void __launch_bounds__(256) k_muon_pack(Table tab) {
     __shared__ float turn[64][65];
     int t = blockIdx.x;
     const Matrix& x = tab.t[find(tab, t)];
@@ -132,56 +145,46 @@ __global__ void __launch_bounds__(256) k_muon_pack(Table tab) {
     for (int k = 1; k < 64; k <<= 1) sum += __shfl_xor(sum, k, 64);
     const float scale = (float)((double)kScale / (sqrt(sum) + (double)tab.eps));
     const int r0 = piece / pieces_c * 64, c0 = piece % pieces_c * 64;
-    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-        const int r = r0 + i / 64, c = c0 + i % 64;
-        float u = 0.0f;
-        if (r < x.rows && c < x.cols) {
-            u = load_any(x.g, tab.g_type, matrix * x.g_step + r * x.g_row + c);
-            if (x.momentum) {
-                const float m = x.momentum[(int64_t)r * x.cols + c];
-                u = tab.nesterov ? fmaf(m, tab.mu, u) : m;
-            }
-            u *= scale;
-        }
-        turn[i / 64][i % 64] = u;
-    }
-    __syncthreads();
     const bool tall = x.rows > x.cols;
+#pragma unroll
+    for (int i = threadIdx.x; i < 64 * 8; i += 256) {
+        const int a = i / 8, b = i % 8 * 8, r = r0 + a, c = c0 + b;
+        float u[8] = {};
+        if (r < x.rows && c < x.cols)
+            load_update<G, false>(x, tab, matrix * x.g_step + r * x.g_row + c, (int64_t)r * x.cols + c, x.cols - c, u);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            u[e] *= scale;
+            if (tall) turn[a][b + e] = u[e];
+        }
+        if (!tall && r < o.s && c < up_to(o.l, 32)) store_parts((f16*)(held + o.x[0] + r * o.lb), c, u);
+    }
+    if (!tall) return;
+    __syncthreads();
+#pragma unroll
     for (int i = threadIdx.x; i < 64 * 8; i += 256) {
         const int a = i / 8, b = i % 8 * 8;  // a row of the result and 8 of its columns
-        const int row = (tall ? c0 : r0) + a, col = (tall ? r0 : c0) + b;
-        if (row >= o.s || col >= up_to(o.l, 32)) continue;
-        h8 hi, lo;
+        if (c0 + a >= o.s || r0 + b >= up_to(o.l, 32)) continue;
+        float u[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            f16 part[2];
-            split<f16, 2>(tall ? turn[b + k][a] : turn[a][b + k], part);
-            hi[k] = part[0];
-            lo[k] = part[1];
-        }
-        f16* to = (f16*)(held + o.x[0] + row * o.lb);
-        *(h8*)(to + part_place<2>(col, 0)) = hi;
-        *(h8*)(to + part_place<2>(col, 1)) = lo;
+        for (int e = 0; e < 8; e++) u[e] = turn[b + e][a];
+        store_parts((f16*)(held + o.x[0] + (c0 + a) * o.lb), r0 + b, u);
     }
 }
 
 enum Kind { kGram, kPoly, kStep };
 
-// the tiles of a symmetric result on and above the diagonal, each `wide` times as wide as high: row i has those from i / wide on
-__host__ __device__ inline int upper_tiles(int m, int n, int wide) {
-    int all = 0;
-    for (int i = 0; i < m; i++) all += n - i / wide;
-    return all;
-}
-
-// columns c .. c + 7 (c % 8 = 0) of a row of parts
-__device__ __forceinline__ void store_parts(f16* row, int64_t c, const float (&v)[8]) {
-    h8 hi, lo;
+__device__ __forceinline__ void split_parts(const float (&v)[8], h8& hi, h8& lo) {
 #pragma unroll
     for (int e = 0; e < 8; e++) {
         hi[e] = (f16)v[e];
         lo[e] = (f16)(v[e] - (float)hi[e]);
     }
+}
+// columns c .. c + 7 (c % 8 = 0) of a row of parts
+__device__ __forceinline__ void store_parts(f16* row, int64_t c, const float (&v)[8]) {
+    h8 hi, lo;
+    split_parts(v, hi, lo);
     *(h8*)(row + part_place<2>(c, 0)) = hi;
     *(h8*)(row + part_place<2>(c, 1)) = lo;
 }
@@ -190,27 +193,48 @@ __device__ __forceinline__ void load_parts(const f16* row, int64_t c, float (&v)
 #pragma unroll
     for (int e = 0; e < 8; e++) v[e] = (float)hi[e] + (float)lo[e];
 }
-// the same columns, one row each, at column `c`
-__device__ __forceinline__ void store_parts_down(f16* first, int64_t row, int64_t c, int live, const float (&v)[8]) {
+// the first `live` of 8 values of the result, `apart` elements from each other: stored, or a parameter stepped by them
+template <bool kApart, typename P>
+__device__ __forceinline__ void store_result_of(const Matrix& x, const Table& tab, int64_t at, int64_t apart, int live,
+                                                float (&v)[8]) {
+    P* p = (P*)x.out + at;
+    if (tab.update) {
+        float old[8];
+        if (kApart) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const f16 hi = (f16)v[e];
-        if (e < live) {
-            first[e * row + part_place<2>(c, 0)] = hi;
-            first[e * row + part_place<2>(c, 1)] = (f16)(v[e] - (float)hi);
+            for (int e = 0; e < 8; e++) old[e] = e < live ? to_f32<P>(p[e * apart]) : 0.0f;
+        } else {
+            load_some<P, 8>(p, live, old);
         }
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = fmaf(-x.rate, v[e], old[e] * tab.keep);
     }
+    if (kApart) {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (e < live) p[e * apart] = from_f32<P>(v[e]);
+    } else {
+        store_some<P, 4>(p, live, v);
+        store_some<P, 4>(p + 4, live - 4, v + 4);
+    }
+}
+template <bool kApart>
+__device__ __forceinline__ void store_result(const Matrix& x, const Table& tab, int64_t at, int64_t apart, int live,
+                                             float (&v)[8]) {
+    if (tab.out_type == HG_F32) store_result_of<kApart, float>(x, tab, at, apart, live, v);
+    else if (tab.out_type == HG_F16) store_result_of<kApart, f16>(x, tab, at, apart, live, v);
+    else store_result_of<kApart, bf16>(x, tab, at, apart, live, v);
 }
 
 template <int kKind, typename Tl>
 __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_muon_product(Table tab) {
     __shared__ __attribute__((aligned(1024))) char lds[Tl::kLds];
-    int t = chiplet_order(blockIdx.x, tab.blocks);
+    int t = blockIdx.x;
     const Matrix& x = tab.t[find(tab, t)];
     const Layout o = layout(x.rows, x.cols);
-    constexpr int wide_tile = Tl::kN / Tl::kM;
     const int tiles_s = (o.s + Tl::kM - 1) / Tl::kM, tiles_n = ((kKind == kStep ? o.l : o.s) + Tl::kN - 1) / Tl::kN;
-    const int per = kKind == kStep ? tiles_s * tiles_n : upper_tiles(tiles_s, tiles_n, wide_tile);
+    const int per = kKind == kStep ? tiles_s * tiles_n : tiles_s * (tiles_s + 1) / 2;
+    t = chiplet_order(t, per * x.count);
     const int matrix = t / per;
     t -= matrix * per;
     char* held = x.held + matrix * o.all;
@@ -219,8 +243,8 @@ __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_muon_product(T
         at = band_place(t, tiles_s, tiles_n);
     } else {  // row by row, from the diagonal on
         at.m = 0;
-        while (t >= tiles_n - at.m / wide_tile) t -= tiles_n - at.m++ / wide_tile;
-        at.n = at.m / wide_tile + t;
+        while (t >= tiles_s - at.m) t -= tiles_s - at.m++;
+        at.n = at.m + t;
     }
     Operand a, b;
     if (kKind == kGram) a = b = {held + o.x[tab.from], o.lb, o.s, (int)o.lb};
@@ -238,6 +262,7 @@ __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_muon_product(T
     const int wide = kKind == kStep ? o.l : o.s;              // columns of the result
     const int64_t row = (kKind == kStep ? o.lb : o.sb) / 2;   // elements of its packed rows
     const int first = n0 + s.col();
+    const bool mirrored = at.n > at.m;  // the tile's mirror image is stored, too: no tile computes it
 #pragma unroll
     for (int i = 0; i < Tl::kFm; i++) {
         const int m = m0 + s.row() + i * 16;
@@ -254,30 +279,224 @@ __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_muon_product(T
                 float g[8] = {};
                 if (there) load_parts((const f16*)(held + o.a) + m * row, n, g);
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[e] = fmaf(tab.c, v[e], tab.b * g[e]);
+                for (int e = 0; e < 8; e++) v[e] = fmaf(tab.c, v[e], tab.b * g[e]) + (n + e == m ? tab.a * kScale : 0.0f);
             }
-            if (kKind == kStep) {
-                float g[8] = {};
-                if (there) load_parts((const f16*)(held + o.x[tab.from]) + m * row, n, g);
+            if (kKind == kStep && tab.last) {
+                if (!there) continue;
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[e] = fmaf(tab.a, g[e], v[e]);
-                if (tab.last) {
-                    if (!there) continue;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        if (e >= live) break;
-                        const int64_t i_out = matrix * x.out_step + (tall ? (int64_t)(n + e) * x.cols + m
-                                                                          : (int64_t)m * x.cols + n + e);
-                        float r = v[e] * (1.0f / kScale);
-                        if (tab.update) r = fmaf(-x.rate, r, load_any(x.out, tab.out_type, i_out) * tab.keep);
-                        store_any(x.out, tab.out_type, i_out, r);
-                    }
-                    continue;
-                }
+                for (int e = 0; e < 8; e++) v[e] *= 1.0f / kScale;
+                // a turned matrix: column n of the result is row n of X's
+                if (tall) store_result<true>(x, tab, matrix * x.out_step + (int64_t)n * x.cols + m, x.cols, live, v);
+                else store_result<false>(x, tab, matrix * x.out_step + (int64_t)m * x.cols + n, 1, live, v);
+                continue;
             }
             if (there) store_parts(to + m * row, n, v);
-            if (kKind != kStep && at.n > at.m / wide_tile)  // the tile's mirror image, where no tile is
-                store_parts_down(to + n * row, row, m, live, v);
+            if (kKind != kStep && mirrored) {
+                const int r = s.row() + i * 16, at_c = Tl::template turned_place<Tl::kN / 8>(r, (s.col() + c) / 8);
+                h8 hi, lo;
+                split_parts(v, hi, lo);
+                *(h8*)(lds + (r * Tl::kN / 8 + at_c) * 16) = hi;
+                *(h8*)(lds + Tl::kM * Tl::kN * 2 + (r * Tl::kN / 8 + at_c) * 16) = lo;
+            }
+        }
+    }
+    if constexpr (kKind != kStep) {
+        if (!mirrored) return;
+        static_assert(Tl::kLds >= Tl::kM * Tl::kN * 4 && Tl::kM == Tl::kN, "");
+        __syncthreads();
+        // 16 rows of the mirror image and 32 of their columns at a time, turned by the LDS reads
+        const int lane = threadIdx.x & 63, l = lane & 15, g = lane >> 4;
+        for (int k = threadIdx.x >> 6; k < 2 * (Tl::kN / 16) * (Tl::kM / 32); k += Tl::kThreads / 64) {
+            const int p = k & 1, piece = k / 2 % (Tl::kN / 16), block = k / 2 / (Tl::kN / 16);
+            typedef short s4 __attribute__((ext_vector_type(4)));
+            typedef short s8 __attribute__((ext_vector_type(8)));
+            typedef __attribute__((address_space(3))) s4* Lds;
+            const int r = block * 32 + g * 8 + l / 4, c = Tl::template turned_place<Tl::kN / 8>(r, piece * 2 + l % 4 / 2);
+            const char* first = lds + p * Tl::kM * Tl::kN * 2 + (r * Tl::kN / 8 + c) * 16 + l % 2 * 8;
+            const s4 u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)first);
+            const s4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(first + 4 * Tl::kN * 2));
+            const int n = n0 + piece * 16 + l, m = m0 + block * 32 + g * 8;
+            if (n < o.s) *(s8*)(to + n * row + part_place<2>(m, p)) = s8{u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
+        }
+    }
+}
+
+// The whole step of a matrix whose shorter side is at most 64 and whose longer one at most kL: a block holds X, A and P in
+// LDS and takes every product there, where the products of larger ones take three launches an iteration (15 us for the
+// self-play network's three matrices, 110 by launches).  Rows of 64 values and more, so that the 16 rows that are read
+// together can begin in 16 different places: chunk c of row r is held at place(r, c), which also spreads the rows that a
+// turned read takes.
+constexpr int kSmall = 64;
+template <int kL, typename G>
+__global__ void __launch_bounds__(1024) k_muon_small(Table tab) {
+    constexpr int kRowX = kL * 4, kRowA = kSmall * 4, kPieces = kL / 64;  // bytes; a wave's pieces of 16 x 16 of X
+    constexpr int kEach = kSmall * kL / 1024;                             // values a thread loads
+    __shared__ __attribute__((aligned(256))) char lds[kSmall * (kRowX + 2 * kRowA)];
+    __shared__ double waves[16];
+    char* const lx = lds;
+    char* const la = lds + kSmall * kRowX;
+    char* const lp = la + kSmall * kRowA;
+    auto place = [](int r, int c) { return c ^ (((r & 3) | (r >> 1 & 4)) << 1 | (r >> 2 & 1)); };
+    // byte of column c's part p in row r
+    auto byte = [&](int r, int c, int p) { return place(r, c / 32 * 8 + p * 4 + c % 32 / 8) * 16 + c % 8 * 2; };
+    int t = blockIdx.x;
+    const Matrix& x = tab.t[find(tab, t)];
+    const int matrix = t, rows = x.rows, cols = x.cols, n = rows * cols;
+    const bool tall = rows > cols;
+    const int s = tall ? cols : rows, l = tall ? rows : cols;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, row16 = lane & 15, g = lane >> 4;
+    float u[kEach], m[kEach];
+    // i / cols = the high word of i times it, rounded up: exact for i below 2^14 and cols up to 2^8
+    const uint32_t inverse = 0xFFFFFFFFu / (uint32_t)cols + 1;
+    const G* from = (const G*)x.g + matrix * x.g_step;
+    const int g_row = (int)x.g_row;
+    auto row_of = [&](int i) { return cols == 1 ? i : (int)__umulhi((uint32_t)i, inverse); };
+#pragma unroll
+    for (int k = 0; k < kEach; k++) {  // all loads under way before the first value is used
+        const int i = k * 1024 + tid, r = row_of(i);
+        u[k] = i < n ? to_f32<G>(from[(int64_t)r * g_row + i - r * cols]) : 0.0f;
+    }
+#pragma unroll
+    for (int k = 0; k < kEach; k++) {
+        const int i = k * 1024 + tid;
+        m[k] = i < n && x.momentum ? x.momentum[i] : 0.0f;
+    }
+    for (int i = tid; i < (int)sizeof(lds) / 16; i += 1024) ((float4*)lds)[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    double sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < kEach; k++) {
+        const int i = k * 1024 + tid;
+        if (x.momentum) {
+            m[k] = fmaf(m[k], tab.mu, u[k]);
+            if (i < n) x.momentum[i] = m[k];
+            u[k] = tab.nesterov ? fmaf(m[k], tab.mu, u[k]) : m[k];
+        }
+        sum = fma((double)u[k], (double)u[k], sum);
+    }
+    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) waves[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+    for (int i = 0; i < 16; i++) sum += waves[i];
+    const float scale = (float)((double)kScale / (sqrt(sum) + (double)tab.eps));
+#pragma unroll
+    for (int k = 0; k < kEach; k++) {
+        const int i = k * 1024 + tid;
+        if (i >= n) continue;
+        const int of = row_of(i), in = i - of * cols, r = tall ? in : of, c = tall ? of : in;
+        f16 part[2];
+        split<f16, 2>(u[k] * scale, part);
+        *(f16*)(lx + r * kRowX + byte(r, c, 0)) = part[0];
+        *(f16*)(lx + r * kRowX + byte(r, c, 1)) = part[1];
+    }
+    __syncthreads();
+    auto operand = [&](const char* from, int row, int piece, int k, int p) {  // rows as they are
+        const int r = piece * 16 + row16;
+        return *(const h8*)(from + r * row + place(r, k * 8 + p * 4 + g) * 16);
+    };
+    auto turned = [&](int piece, int k, int p) {  // of X: 4 k each of two reads
+        typedef short s4 __attribute__((ext_vector_type(4)));
+        typedef short s8 __attribute__((ext_vector_type(8)));
+        typedef __attribute__((address_space(3))) s4* Lds;
+        const int c = (piece / 2 * 2 + p) * 4 + piece % 2 * 2 + row16 % 4 / 2, r = k * 32 + g * 8 + row16 / 4;
+        const s4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(lx + r * kRowX + place(r, c) * 16 + row16 % 2 * 8));
+        const s4 w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(lx + (r + 4) * kRowX + place(r + 4, c) * 16 + row16 % 2 * 8));
+        return __builtin_bit_cast(h8, (s8){v[0], v[1], v[2], v[3], w[0], w[1], w[2], w[3]});
+    };
+    auto add = [](f4 c, const h8 (&a)[2], const h8 (&b)[2]) {
+        c = mfma(b[0], a[1], c);
+        c = mfma(b[1], a[0], c);
+        return mfma(b[0], a[0], c);
+    };
+    typedef f16 half4 __attribute__((ext_vector_type(4)));
+    auto keep = [&](char* to, int row, int r, int c, const float (&v)[4]) {
+        half4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            hi[e] = (f16)v[e];
+            lo[e] = (f16)(v[e] - (float)hi[e]);
+        }
+        *(half4*)(to + r * row + byte(r, c, 0)) = hi;
+        *(half4*)(to + r * row + byte(r, c, 1)) = lo;
+    };
+    const int pm = wave / 4, pn = wave % 4;  // the wave's piece of A and of P; zeros past the matrix are multiplied like the rest
+    const int r = pm * 16 + row16;
+    auto finish = [&](auto type, const f4 (&next)[kPieces]) {
+        using P = decltype(type);
+        P* out = (P*)x.out + matrix * x.out_step;
+        int at[kPieces][4];
+        float old[kPieces][4];
+#pragma unroll
+        for (int j = 0; j < kPieces; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int c = (pn + 4 * j) * 16 + g * 4 + e;
+                at[j][e] = r < s && c < l ? (tall ? c * cols + r : r * cols + c) : -1;
+                old[j][e] = tab.update && at[j][e] >= 0 ? to_f32<P>(out[at[j][e]]) : 0.0f;
+            }
+#pragma unroll
+        for (int j = 0; j < kPieces; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const float o = next[j][e] * (1.0f / kScale / kScale);
+                if (at[j][e] >= 0) out[at[j][e]] = from_f32<P>(tab.update ? fmaf(-x.rate, o, old[j][e] * tab.keep) : o);
+            }
+    };
+    for (int step = 0; step < tab.steps; step++) {
+        const float* abc = tab.triples + 3 * min(step, tab.count - 1);
+        f4 sum_a = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < kL / 32; k++) {
+            const h8 a[2] = {operand(lx, kRowX, pm, k, 0), operand(lx, kRowX, pm, k, 1)};
+            const h8 b[2] = {operand(lx, kRowX, pn, k, 0), operand(lx, kRowX, pn, k, 1)};
+            sum_a = add(sum_a, a, b);
+        }
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = sum_a[e] * (1.0f / kScale);
+        keep(la, kRowA, r, pn * 16 + g * 4, v);
+        __syncthreads();
+        f4 sum_p = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < kSmall / 32; k++) {
+            const h8 a[2] = {operand(la, kRowA, pm, k, 0), operand(la, kRowA, pm, k, 1)};
+            const h8 b[2] = {operand(la, kRowA, pn, k, 0), operand(la, kRowA, pn, k, 1)};
+            sum_p = add(sum_p, a, b);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            v[e] = fmaf(abc[2], sum_p[e] * (1.0f / kScale), abc[1] * v[e]) + (pn * 16 + g * 4 + e == r ? abc[0] * kScale : 0.0f);
+        keep(lp, kRowA, r, pn * 16 + g * 4, v);
+        __syncthreads();
+        h8 p[kSmall / 32][2];
+#pragma unroll
+        for (int k = 0; k < kSmall / 32; k++) {
+            p[k][0] = operand(lp, kRowA, pm, k, 0);
+            p[k][1] = operand(lp, kRowA, pm, k, 1);
+        }
+        f4 next[kPieces];
+#pragma unroll
+        for (int j = 0; j < kPieces; j++) {
+            next[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < kSmall / 32; k++) {
+                const h8 b[2] = {turned(pn + 4 * j, k, 0), turned(pn + 4 * j, k, 1)};
+                next[j] = add(next[j], p[k], b);
+            }
+        }
+        if (step < tab.steps - 1) {
+            __syncthreads();  // X is read
+#pragma unroll
+            for (int j = 0; j < kPieces; j++) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = next[j][e] * (1.0f / kScale);
+                keep(lx, kRowX, r, (pn + 4 * j) * 16 + g * 4, v);
+            }
+            __syncthreads();
+        } else {
+            if (tab.out_type == HG_F32) finish(float{}, next);
+            else if (tab.out_type == HG_F16) finish(f16{}, next);
+            else finish(bf16{}, next);
         }
     }
 }
@@ -298,7 +517,7 @@ template <typename F> int64_t lay_blocks(Table& tab, F f) {
 template <typename Tl> int64_t step_tiles(const Matrix& x, bool symmetric) {
     const int s = std::min(x.rows, x.cols), l = std::max(x.rows, x.cols);
     const int m = (s + Tl::kM - 1) / Tl::kM, n = ((symmetric ? s : l) + Tl::kN - 1) / Tl::kN;
-    return symmetric ? upper_tiles(m, n, Tl::kN / Tl::kM) : (int64_t)m * n;
+    return symmetric ? (int64_t)m * (m + 1) / 2 : (int64_t)m * n;
 }
 
 // one product of every matrix of the table, in the largest tiles of which there are enough for the card
@@ -310,29 +529,56 @@ template <int kKind> int product(Table& tab, hipStream_t st) {
         k_muon_product<kKind, Tl><<<(unsigned)blocks, Tl::kThreads, 0, st>>>(tab);
         return launched();
     };
-#ifdef TRY
-    int e = -1;
-    if (TRY == 1) e = launch(Tile<f16, 2, 1, 128, 128, 2, 2, 2, 2>{}, 192);
-    if (TRY == 2) e = launch(Tile<f16, 2, 1, 128, 256, 2, 4, 3, 1>{}, 192);
-    if (TRY == 3) e = launch(Tile<f16, 2, 1, 128, 128, 2, 2, 4, 1>{}, 192);
-    if (TRY == 4) e = launch(Tile<f16, 2, 1, 128, 256, 4, 4, 3, 1>{}, 192);
-#else
-    int e = launch(Tile<f16, 2, 1, 128, 256, 2, 4, 3, 1>{}, 192);
-#endif
-    if (e < 0) e = launch(Tile<f16, 2, 1, 128, 128, 2, 2, 2, 2>{}, 192);
+    int e = launch(Tile<f16, 2, 1, 128, 128, 2, 2, 2, 2>{}, 192);
     if (e < 0) e = launch(Tile<f16, 2, 1, 64, 64, 2, 2, 4, 2>{}, 0);
     return e;
 }
 
+// the matrices of the table that `small` says, their whole iteration in one launch
+template <int kL, typename F> int iterate_small(const Table& all, F small, hipStream_t st) {
+    Table tab = all;
+    tab.n = 0;
+    for (int i = 0; i < all.n; i++)
+        if (small(all.t[i])) tab.t[tab.n++] = all.t[i];
+    if (tab.n == 0) return 0;
+    const int64_t blocks = lay_blocks(tab, [](const Matrix&) { return (int64_t)1; });
+    return with_type(tab.g_type, [&](auto t) {
+        k_muon_small<kL, decltype(t)><<<(unsigned)blocks, 1024, 0, st>>>(tab);
+        return launched();
+    });
+}
+
 // the iteration of the table's matrices
-int iterate(Table& tab, int steps, const float* coefficients, int64_t triples, hipStream_t st) {
+int iterate(Table& all, int steps, const float* coefficients, int64_t triples, hipStream_t st) {
+    all.steps = steps;
+    all.count = (int)std::min<int64_t>(triples, steps);
+    auto fits = [&](const Matrix& x, int side) {
+        return std::min(x.rows, x.cols) <= kSmall && std::max(x.rows, x.cols) <= side && all.count <= kTriples;
+    };
+    for (int i = 0; i < 3 * all.count && i < 3 * kTriples; i++) all.triples[i] = coefficients[i];
+    int e = iterate_small<128>(all, [&](const Matrix& x) { return fits(x, 128); }, st);
+    if (!e) e = iterate_small<256>(all, [&](const Matrix& x) { return fits(x, 256) && !fits(x, 128); }, st);
+    if (e) return e;
+    Table tab = all;
+    tab.n = 0;
+    for (int i = 0; i < all.n; i++)
+        if (!fits(all.t[i], 256)) tab.t[tab.n++] = all.t[i];
+    if (tab.n == 0) return 0;
+    // the longest sums first: what is left at the end of a launch is short
+    std::sort(tab.t, tab.t + tab.n, [](const Matrix& a, const Matrix& b) {
+        return std::max(a.rows, a.cols) > std::max(b.rows, b.cols);
+    });
     int64_t blocks = lay_blocks(tab, [](const Matrix&) { return (int64_t)kSumBlocks; });
-    k_muon_sums<<<(unsigned)blocks, 256, 0, st>>>(tab);
-    int e = launched();
+    e = with_type(tab.g_type, [&](auto t) {
+        k_muon_sums<decltype(t)><<<(unsigned)blocks, 256, 0, st>>>(tab);
+        return launched();
+    });
     if (e) return e;
     blocks = lay_blocks(tab, [](const Matrix& x) { return (int64_t)((x.rows + 63) / 64) * ((x.cols + 63) / 64); });
-    k_muon_pack<<<(unsigned)blocks, 256, 0, st>>>(tab);
-    e = launched();
+    e = with_type(tab.g_type, [&](auto t) {
+        k_muon_pack<decltype(t)><<<(unsigned)blocks, 256, 0, st>>>(tab);
+        return launched();
+    });
     tab.from = 0;
     for (int i = 0; i < steps && !e; i++) {
         const float* c = coefficients + 3 * std::min<int64_t>(i, triples - 1);
