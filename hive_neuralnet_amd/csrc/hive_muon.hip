@@ -45,7 +45,8 @@ struct Matrix {
 };
 struct Table {
     Matrix t[kMatrices];
-    int n, blocks;
+    int n;
+    int range[9];  // chiplet x's tiles of a product: [range[x], range[x + 1])
     int g_type, out_type, update;  // update: out is a parameter
     float mu, keep, eps, a, b, c;
     int nesterov, from, last;  // from: which of the two copies of X is current
@@ -229,12 +230,13 @@ __device__ __forceinline__ void store_result(const Matrix& x, const Table& tab, 
 template <int kKind, typename Tl>
 __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_muon_product(Table tab) {
     __shared__ __attribute__((aligned(1024))) char lds[Tl::kLds];
-    int t = blockIdx.x;
+    // block b is on chiplet b % 8
+    int t = tab.range[blockIdx.x % 8] + (int)(blockIdx.x / 8);
+    if (t >= tab.range[blockIdx.x % 8 + 1]) return;
     const Matrix& x = tab.t[find(tab, t)];
     const Layout o = layout(x.rows, x.cols);
     const int tiles_s = (o.s + Tl::kM - 1) / Tl::kM, tiles_n = ((kKind == kStep ? o.l : o.s) + Tl::kN - 1) / Tl::kN;
     const int per = kKind == kStep ? tiles_s * tiles_n : tiles_s * (tiles_s + 1) / 2;
-    t = chiplet_order(t, per * x.count);
     const int matrix = t / per;
     t -= matrix * per;
     char* held = x.held + matrix * o.all;
@@ -510,8 +512,31 @@ template <typename F> int64_t lay_blocks(Table& tab, F f) {
         tab.t[i].first = (int)blocks;
         blocks += f(tab.t[i]) * tab.t[i].count;
     }
-    tab.blocks = (int)blocks;
     return blocks;
+}
+
+// Shares the tiles of a product out among the chiplets, each of which has an L2 of its own: ranges of tiles that follow each
+// other, of equal work (a tile's sum is as long as `depth` says), so that a matrix is read by one or two of them (A of
+// 24 matrices of 1,024 x 1,024 and 4,096: 0.4 GB from memory, 1.1 where every chiplet has tiles of every matrix).  Returns the
+// blocks to launch.
+template <typename F, typename D> int64_t lay_ranges(Table& tab, F tiles, D depth) {
+    int64_t work = 0, done = 0;
+    for (int i = 0; i < tab.n; i++) work += tiles(tab.t[i]) * tab.t[i].count * depth(tab.t[i]);
+    int64_t most = 0;
+    int x = 0;
+    for (int i = 0; i < tab.n; i++) {
+        const int64_t all = tiles(tab.t[i]) * tab.t[i].count, each = depth(tab.t[i]);
+        // chiplet x begins at the first tile before which x / 8 of the work is done
+        while (x < 8 && work * x <= 8 * (done + all * each)) {
+            const int64_t before = std::max<int64_t>(0, (work * x / 8 - done + each - 1) / each);
+            tab.range[x++] = tab.t[i].first + (int)std::min(before, all);
+        }
+        done += all * each;
+        tab.range[8] = tab.t[i].first + (int)all;
+    }
+    while (x < 8) tab.range[x++] = tab.range[8];
+    for (x = 0; x < 8; x++) most = std::max<int64_t>(most, tab.range[x + 1] - tab.range[x]);
+    return 8 * most;
 }
 
 template <typename Tl> int64_t step_tiles(const Matrix& x, bool symmetric) {
@@ -526,7 +551,10 @@ template <int kKind> int product(Table& tab, hipStream_t st) {
         using Tl = decltype(tile);
         const int64_t blocks = lay_blocks(tab, [](const Matrix& x) { return step_tiles<Tl>(x, kKind != kStep); });
         if (blocks < least) return -1;
-        k_muon_product<kKind, Tl><<<(unsigned)blocks, Tl::kThreads, 0, st>>>(tab);
+        const int64_t grid = lay_ranges(
+            tab, [](const Matrix& x) { return step_tiles<Tl>(x, kKind != kStep); },
+            [](const Matrix& x) { return (int64_t)(kKind == kGram ? std::max(x.rows, x.cols) : std::min(x.rows, x.cols)); });
+        k_muon_product<kKind, Tl><<<(unsigned)grid, Tl::kThreads, 0, st>>>(tab);
         return launched();
     };
     int e = launch(Tile<f16, 2, 1, 128, 128, 2, 2, 2, 2>{}, 192);

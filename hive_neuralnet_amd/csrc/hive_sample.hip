@@ -48,6 +48,7 @@ struct Row {
     int n;
     int64_t k;  // 0: all
     double t, p, min_p, u;
+    double scale;  // log2(e) / t
     bool greedy, cut_p;
 };
 __device__ __forceinline__ Row row_of(const Settings& s, int64_t b) {
@@ -63,6 +64,7 @@ __device__ __forceinline__ Row row_of(const Settings& s, int64_t b) {
     r.u = (double)s.uniforms[b];
     r.u = r.u > 0.0 ? r.u : 0.0;  // NaN: 0
     r.greedy = !(r.t > 0.0);
+    r.scale = 1.4426950408889634 / r.t;
     r.cut_p = r.p < 1.0;
     return r;
 }
@@ -76,11 +78,27 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
-// exp((x - top) / t), 1 for x = top whatever it is
-__device__ __forceinline__ double weight_of(uint32_t key, uint32_t top, double t) {
+// exp((x - top) / t) = 2^(scale (x - top)), scale = log2(e) / t; 1 for x = top whatever it is.  A series of 2^f, |f| <= 1/2,
+// to f^11: 2^-47 of the whole left out, with the rounding of scale and of the product under 2^-45, a weight's own rounding.
+__device__ __forceinline__ double weight_of(uint32_t key, uint32_t top, double scale) {
     if (key == top) return 1.0;
-    const double w = key ? exp(((double)value_of(key) - (double)value_of(top)) / t) : 0.0;
-    return w <= 1.0 ? w : 0.0;  // NaN: a logit below one of inf at a temperature of inf
+    if (!key) return 0.0;
+    // NaN (a logit below one of inf at a temperature of inf) and -inf: 0
+    const double y = fmax(((double)value_of(key) - (double)value_of(top)) * scale, -1200.0), n = rint(y);
+    const double f = (y - n) * 0.6931471805599453;
+    double s = 1.0 / 39916800.0;
+    s = fma(s, f, 1.0 / 3628800.0);
+    s = fma(s, f, 1.0 / 362880.0);
+    s = fma(s, f, 1.0 / 40320.0);
+    s = fma(s, f, 1.0 / 5040.0);
+    s = fma(s, f, 1.0 / 720.0);
+    s = fma(s, f, 1.0 / 120.0);
+    s = fma(s, f, 1.0 / 24.0);
+    s = fma(s, f, 1.0 / 6.0);
+    s = fma(s, f, 0.5);
+    s = fma(s, f, 1.0);
+    s = fma(s, f, 1.0);
+    return ldexp(s, (int)n);
 }
 // keys of slots c .. c + 3 of n
 template <typename T> __device__ __forceinline__ void load_keys(const T* row, int c, int n, uint32_t key[4]) {
@@ -95,26 +113,46 @@ template <typename T> __device__ __forceinline__ void load_keys(const T* row, in
     }
 }
 
-template <typename V, typename F> __device__ __forceinline__ V wave_join(V v, F f) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v = f(v, (V)__shfl_xor(v, o, 64));
-    return v;
-}
-template <typename V> __device__ __forceinline__ V wave_sum(V v) {
-    return wave_join(v, [](V a, V b) { return a + b; });
-}
-__device__ __forceinline__ uint32_t wave_most(uint32_t v) {
-    return wave_join(v, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
-}
-// the sum of the lanes up to this one
-template <typename V> __device__ __forceinline__ V wave_scan(V v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const V w = __shfl_up(v, o, 64);
-        if (lane >= o) v += w;
+// v of the lane that DPP control `kControl` names, 0 where it names none or its row of 16 is not in kRows
+template <int kControl, int kRows = 0xF, typename V> __device__ __forceinline__ V moved(V v) {
+    if constexpr (sizeof(V) == 8) {
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, kControl, kRows, 0xF, false);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), kControl, kRows, 0xF, false);
+        return __builtin_bit_cast(V, (uint64_t)hi << 32 | lo);
+    } else {
+        return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kControl, kRows, 0xF, false));
     }
+}
+// the sum of the lanes up to this one: within rows of 16, then the rows before
+template <typename V> __device__ __forceinline__ V wave_scan(V v) {
+    v += moved<0x111>(v);       // row_shr 1, 2, 4, 8
+    v += moved<0x112>(v);
+    v += moved<0x114>(v);
+    v += moved<0x118>(v);
+    v += moved<0x142, 0xA>(v);  // the end of row 0 to row 1, of row 2 to row 3
+    v += moved<0x143, 0xC>(v);  // the end of row 1 to rows 2 and 3
     return v;
+}
+template <typename V> __device__ __forceinline__ V from_lane(V v, int lane) {  // the same for all lanes
+    if constexpr (sizeof(V) == 8) {
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+        return __builtin_bit_cast(V, (uint64_t)hi << 32 | lo);
+    } else {
+        return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+    }
+}
+template <typename V> __device__ __forceinline__ V wave_sum(V v) { return from_lane(wave_scan(v), 63); }
+__device__ __forceinline__ uint32_t wave_most(uint32_t v) {
+    v = max(v, moved<0x111>(v));
+    v = max(v, moved<0x112>(v));
+    v = max(v, moved<0x114>(v));
+    v = max(v, moved<0x118>(v));
+    v = max(v, moved<0x142, 0xA>(v));
+    v = max(v, moved<0x143, 0xC>(v));
+    return from_lane(v, 63);
 }
 __device__ __forceinline__ int lanes_below(uint64_t mask) {
     return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
@@ -154,7 +192,7 @@ template <int kPer> struct Held {
                     const uint64_t middle = __ballot((in >> (threadIdx.x & 63) & 1) && lanes_below(in) == __popcll(in) / 2);
                     const int lane = __ffsll((unsigned long long)middle) - 1;
                     pivot = __builtin_amdgcn_readlane(k, lane);
-                    if (!kCount) each = __shfl(v, lane, 64);
+                    if (!kCount) each = from_lane(v, lane);
                     found = true;
                 }
             }
@@ -215,6 +253,68 @@ template <int kPer> struct Held {
     }
 };
 
+// The draw from a wave's row, whose largest key is `top`: its place among the slots held, and the logarithm of its
+// probability.  `all_live`: the weights of the row's live slots, where they are not all held (0: they are).
+template <int kPer>
+__device__ __forceinline__ int draw(Held<kPer>& h, const Row& r, uint32_t top, double all_live, double& log_prob) {
+    int live = 0, action = -1;
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+        h.w[i] = rint(weight_of(h.key[i], top, r.scale) * kWaveOne);
+        live += __popcll(__ballot(h.key[i] != 0));
+    }
+    if (r.k && r.k < live) h.keep(h.template cut_at<true>((double)r.k));
+    if (r.cut_p) {
+        double all = 0.0;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) all += h.w[i];
+        all = wave_sum(all);
+        const double want = ceil(r.p * (all_live > 0.0 ? all_live : all));
+        h.keep(h.template cut_at<false>(want < 1.0 ? 1.0 : want));
+    }
+    const double least = r.min_p * kWaveOne;
+    double part[kPer / 4], all = 0.0;  // a lane's sums in each chunk
+#pragma unroll
+    for (int i = 0; i < kPer; i += 4) {
+        part[i / 4] = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            h.w[i + e] = h.w[i + e] >= least ? h.w[i + e] : 0.0;
+            part[i / 4] += h.w[i + e];
+        }
+        all += part[i / 4];
+    }
+    all = wave_sum(all);
+    const double border = fmin(r.u * all, all - 1.0);  // u at or past 1: the last
+    double before = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPer; i += 4) {
+        if (action >= 0) continue;
+        const double upto = wave_scan(part[i / 4]) + before;
+        const uint64_t past = __ballot(upto > border);
+        if (past) {
+            const int first = __ffsll((unsigned long long)past) - 1;
+            double run = upto - part[i / 4];
+            int mine = -1;
+            uint32_t key = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                run += h.w[i + e];
+                if (mine < 0 && run > border) {
+                    mine = e;
+                    key = h.key[i + e];
+                }
+            }
+            action = i * 64 + first * 4 + from_lane(mine, first);
+            key = from_lane(key, first);
+            log_prob = (key == top ? 0.0 : ((double)value_of(key) - (double)value_of(top)) / r.t) - log(all / kWaveOne);
+        } else {
+            before = from_lane(upto, 63);
+        }
+    }
+    return action;
+}
+
 template <typename T, int kPer> __global__ void __launch_bounds__(256) k_sample_held(Settings s) {
     const int lane = threadIdx.x & 63;
     const int64_t b = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -230,7 +330,7 @@ template <typename T, int kPer> __global__ void __launch_bounds__(256) k_sample_
         for (int e = 0; e < 4; e++) top = max(top, h.key[i + e]);
     }
     top = wave_most(top);
-    int64_t action = -1;
+    int action = -1;
     double log_prob = 0.0;
     if (top && r.greedy) {
 #pragma unroll
@@ -242,67 +342,11 @@ template <typename T, int kPer> __global__ void __launch_bounds__(256) k_sample_
             const uint64_t have = __ballot(mine < 4);
             if (have) {
                 const int first = __ffsll((unsigned long long)have) - 1;
-                action = i * 64 + first * 4 + __shfl(mine, first, 64);
+                action = i * 64 + first * 4 + from_lane(mine, first);
             }
         }
     } else if (top) {
-        int live = 0;
-#pragma unroll
-        for (int i = 0; i < kPer; i++) {
-            h.w[i] = rint(weight_of(h.key[i], top, r.t) * kWaveOne);
-            live += __popcll(__ballot(h.key[i] != 0));
-        }
-        if (r.k && r.k < live) h.keep(h.template cut_at<true>((double)r.k));
-        if (r.cut_p) {
-            double all = 0.0;
-#pragma unroll
-            for (int i = 0; i < kPer; i++) all += h.w[i];
-            all = wave_sum(all);
-            const double want = ceil(r.p * all);
-            h.keep(h.template cut_at<false>(want < 1.0 ? 1.0 : want));
-        }
-        const double least = r.min_p * kWaveOne;
-        double part[kPer / 4], all = 0.0;  // a lane's sums in each chunk
-#pragma unroll
-        for (int i = 0; i < kPer; i += 4) {
-            part[i / 4] = 0.0;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                h.w[i + e] = h.w[i + e] >= least ? h.w[i + e] : 0.0;
-                part[i / 4] += h.w[i + e];
-            }
-            all += part[i / 4];
-        }
-        all = wave_sum(all);
-        const double border = fmin(r.u * all, all - 1.0);  // u at or past 1: the last
-        double before = 0.0;
-        bool found = false;
-#pragma unroll
-        for (int i = 0; i < kPer; i += 4) {
-            if (found) continue;
-            const double upto = wave_scan(part[i / 4]) + before;
-            const uint64_t past = __ballot(upto > border);
-            if (past) {
-                const int first = __ffsll((unsigned long long)past) - 1;
-                double run = upto - part[i / 4];
-                int mine = -1;
-                uint32_t key = 0;
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    run += h.w[i + e];
-                    if (mine < 0 && run > border) {
-                        mine = e;
-                        key = h.key[i + e];
-                    }
-                }
-                action = i * 64 + first * 4 + __shfl(mine, first, 64);
-                key = __shfl(key, first, 64);
-                log_prob = (key == top ? 0.0 : ((double)value_of(key) - (double)value_of(top)) / r.t) - log(all / kWaveOne);
-                found = true;
-            } else {
-                before = __shfl(upto, 63, 64);
-            }
-        }
+        action = draw(h, r, top, 0.0, log_prob);
     }
     if (lane == 0) {
         s.actions[b] = action;
@@ -395,7 +439,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) k_sample_long(
         }
         return;
     }
-    auto weight = [&](uint32_t key) { return (unsigned long long)rint(weight_of(key, top, r.t) * kBlockOne); };
+    auto weight = [&](uint32_t key) { return (unsigned long long)rint(weight_of(key, top, r.scale) * kBlockOne); };
     auto clear = [&] {
         for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
         __syncthreads();
@@ -442,12 +486,12 @@ template <typename T> __global__ void __launch_bounds__(kThreads) k_sample_long(
     }
     // the sums of 256 slots each, what equals the cut's key counted apart
     const double least = r.min_p;
-    const unsigned long long same = weight_of(cut.key, top, r.t) >= least ? weight(cut.key) : 0;
+    const unsigned long long same = weight_of(cut.key, top, r.scale) >= least ? weight(cut.key) : 0;
     const int parts = (r.n + 255) / 256;
     unsigned long long* sums = sh.bins;
     auto kept = [&](uint32_t key) {
         if (key <= cut.key) return 0ull;
-        const double w = weight_of(key, top, r.t);
+        const double w = weight_of(key, top, r.scale);
         return w >= least ? (unsigned long long)rint(w * kBlockOne) : 0ull;
     };
     __syncthreads();
@@ -486,7 +530,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) k_sample_long(
         sum += of_part(p, before);
         before += sh.equal[p];
     }
-    const unsigned long long upto = wave_scan(sum), all = __shfl(upto, 63, 64);
+    const unsigned long long upto = wave_scan(sum), all = from_lane(upto, 63);
     const double passed = floor(r.u * (double)all);
     const unsigned long long border = passed >= (double)all ? all - 1 : (unsigned long long)passed;
     const int at = __ffsll((unsigned long long)__ballot(upto > border)) - 1;
@@ -499,9 +543,9 @@ template <typename T> __global__ void __launch_bounds__(kThreads) k_sample_long(
         total += w;
         before += sh.equal[part];
     }
-    part = __shfl(part, at, 64);
-    total = __shfl(total, at, 64);
-    before = __shfl(before, at, 64);
+    part = from_lane(part, at);
+    total = from_lane(total, at);
+    before = from_lane(before, at);
     uint32_t key[4];
     load_keys(row, part * 256 + lane * 4, r.n, key);
     unsigned long long w[4], mine = 0;
