@@ -15,9 +15,11 @@
 // Cuts are (key, count): all slots above the key and the first `count` that
 // equal it; keys are the logits' bits in unsigned order, 0 for what is not
 // live (NaN, too).  Rows up to 1,024 slots are held by a wave's registers, and a
-// cut is found by pivots, the middle one of what is left; longer rows are read
-// by a block, cuts found by three digits of the key, whose counts or weights are
-// added up in LDS.
+// cut is found by pivots.  Longer rows are read by a block: once for the largest
+// and, with top_k, the counts of each 11-bit digit of the keys, once more for the
+// weights of each digit with top_p alone, and once for the slots that these or
+// min_p leave, which a wave draws from where they are 1,024 or less.  Where they
+// are more, cuts are found by all three digits of the key.
 #include <cmath>
 
 #include "hive_train.hpp"
@@ -78,27 +80,52 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float value_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
-// exp((x - top) / t) = 2^(scale (x - top)), scale = log2(e) / t; 1 for x = top whatever it is.  A series of 2^f, |f| <= 1/2,
-// to f^11: 2^-47 of the whole left out, with the rounding of scale and of the product under 2^-45, a weight's own rounding.
+// exp((x - top) / t) = 2^(scale (x - top)), scale = log2(e) / t, of n slots; 1 for x = top whatever it is, 0 for what is not
+// live.  A series of 2^f, |f| <= 1/2, to f^11: 2^-47 of the whole left out, with the rounding of scale and of the product
+// under 2^-45, a weight's own rounding.  Slot by slot within a term, so that its coefficient is loaded once.
+template <int n>
+__device__ __forceinline__ void weights_of(const uint32_t (&key)[n], uint32_t top, double scale, double (&w)[n]) {
+    constexpr double term[12] = {1.0 / 39916800.0, 1.0 / 3628800.0, 1.0 / 362880.0, 1.0 / 40320.0, 1.0 / 5040.0, 1.0 / 720.0,
+                                 1.0 / 120.0,      1.0 / 24.0,      1.0 / 6.0,      0.5,           1.0,          1.0};
+    const double x_top = (double)value_of(top);
+    double f[n];
+    int exponent[n];
+#pragma unroll
+    for (int i = 0; i < n; i++) {
+        // NaN (a logit below one of inf at a temperature of inf) and -inf: 0
+        const double y = fmax(((double)value_of(key[i]) - x_top) * scale, -1200.0), whole = rint(y);
+        f[i] = (y - whole) * 0.6931471805599453;
+        exponent[i] = (int)whole;
+        w[i] = term[0];
+    }
+#pragma unroll
+    for (int k = 1; k < 12; k++)
+#pragma unroll
+        for (int i = 0; i < n; i++) w[i] = fma(w[i], f[i], term[k]);
+#pragma unroll
+    for (int i = 0; i < n; i++) {
+        w[i] = ldexp(w[i], exponent[i]);
+        w[i] = key[i] == top ? 1.0 : key[i] ? w[i] : 0.0;
+    }
+}
 __device__ __forceinline__ double weight_of(uint32_t key, uint32_t top, double scale) {
-    if (key == top) return 1.0;
-    if (!key) return 0.0;
-    // NaN (a logit below one of inf at a temperature of inf) and -inf: 0
-    const double y = fmax(((double)value_of(key) - (double)value_of(top)) * scale, -1200.0), n = rint(y);
-    const double f = (y - n) * 0.6931471805599453;
-    double s = 1.0 / 39916800.0;
-    s = fma(s, f, 1.0 / 3628800.0);
-    s = fma(s, f, 1.0 / 362880.0);
-    s = fma(s, f, 1.0 / 40320.0);
-    s = fma(s, f, 1.0 / 5040.0);
-    s = fma(s, f, 1.0 / 720.0);
-    s = fma(s, f, 1.0 / 120.0);
-    s = fma(s, f, 1.0 / 24.0);
-    s = fma(s, f, 1.0 / 6.0);
-    s = fma(s, f, 0.5);
-    s = fma(s, f, 1.0);
-    s = fma(s, f, 1.0);
-    return ldexp(s, (int)n);
+    const uint32_t one[1] = {key};
+    double w[1];
+    weights_of<1>(one, top, scale, w);
+    return w[0];
+}
+// The logarithm of key's weight over `all` of them: log m = 2 z (1 + z^2 / 3 + ...), z = (m - 1) / (m + 1), m between the roots
+// of 1/2 and 2: 2^-27 of it left out.
+__device__ __forceinline__ double log_share(uint32_t key, uint32_t top, double scale, double all) {
+    int e;
+    double m = frexp(all, &e);
+    if (m < 0.7071067811865476) {
+        m *= 2.0;
+        e--;
+    }
+    const double z = (m - 1.0) / (m + 1.0), q = z * z;
+    const double log_all = 2.0 * z * fma(q, fma(q, fma(q, fma(q, 1.0 / 9.0, 1.0 / 7.0), 0.2), 1.0 / 3.0), 1.0) + e * 0.6931471805599453;
+    return (key == top ? 0.0 : ((double)value_of(key) - (double)value_of(top)) * (scale * 0.6931471805599453)) - log_all;
 }
 // keys of slots c .. c + 3 of n
 template <typename T> __device__ __forceinline__ void load_keys(const T* row, int c, int n, uint32_t key[4]) {
@@ -114,14 +141,18 @@ template <typename T> __device__ __forceinline__ void load_keys(const T* row, in
 }
 
 // v of the lane that DPP control `kControl` names, 0 where it names none or its row of 16 is not in kRows
+template <int kControl, int kRows = 0xF> __device__ __forceinline__ int moved_word(int v) {
+    if constexpr (kRows == 0xF) return __builtin_amdgcn_mov_dpp(v, kControl, 0xF, 0xF, true);
+    else return __builtin_amdgcn_update_dpp(0, v, kControl, kRows, 0xF, false);
+}
 template <int kControl, int kRows = 0xF, typename V> __device__ __forceinline__ V moved(V v) {
     if constexpr (sizeof(V) == 8) {
         const uint64_t b = __builtin_bit_cast(uint64_t, v);
-        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, kControl, kRows, 0xF, false);
-        const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), kControl, kRows, 0xF, false);
+        const uint32_t lo = (uint32_t)moved_word<kControl, kRows>((int)(uint32_t)b);
+        const uint32_t hi = (uint32_t)moved_word<kControl, kRows>((int)(uint32_t)(b >> 32));
         return __builtin_bit_cast(V, (uint64_t)hi << 32 | lo);
     } else {
-        return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kControl, kRows, 0xF, false));
+        return __builtin_bit_cast(V, moved_word<kControl, kRows>(__builtin_bit_cast(int, v)));
     }
 }
 // the sum of the lanes up to this one: within rows of 16, then the rows before
@@ -168,64 +199,90 @@ template <int kPer> struct Held {
     uint32_t key[kPer];
     double w[kPer];
 
-    // the cut at which a sum over the keys above, of counts or of weights, first reaches `want` (at most their whole)
-    template <bool kCount> __device__ __forceinline__ Cut cut_at(double want) const {
-        uint32_t low = 1, high = 0xFFFFFFFFu;
-        for (int round = 0; round < 64 * kPer; round++) {
-            // the pivot: the middle lane of those that hold a key between
-            uint32_t pivot = 0;
-            double each = 1.0;
-            bool found = false;
+    uint8_t bin[kPer];  // four an octave of weight, falling; the last holds the rest
+    __device__ __forceinline__ void share_out(uint32_t top, float scale) {
+        const float x = value_of(top);
 #pragma unroll
-            for (int j = 0; j < kPer; j++) {
-                if (found) continue;
-                const int at = (j + round) % kPer;
-                uint32_t k = key[0];
-                double v = w[0];
+        for (int i = 0; i < kPer; i++) {
+            const float y = (x - value_of(key[i])) * scale * 4.0f;
+            bin[i] = (uint8_t)(y < 63.0f ? (int)y : 63);  // NaN, too
+        }
+    }
+
+    // The cut at which a sum over the keys above, of counts or of weights, first reaches `want`; {0, 0}, which cuts nothing,
+    // where their whole does not.  Counts or weights (here in 2^-22) added up by bins in LDS say in which bin the cut is; in it,
+    // a round takes the key that some lane holds between the bounds as pivot, the first lane past a place that changes
+    // from round to round, so that rows in order are halved like others.  Rounds are settled by sums in float32 where
+    // these are far from `want`, about one a row by exact ones.  Where the bins' rounding has said a wrong one, its keys come
+    // to an end, and all are searched.
+    template <bool kCount> __device__ __forceinline__ Cut cut_at(double want, uint32_t* bins) const {
+        const int lane = threadIdx.x & 63;
+        float wf[kPer], far = 0.0f;
+        const float want_f = (float)want;
+        bins[lane] = 0;
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                for (int i = 1; i < kPer; i++) {
-                    k = at == i ? key[i] : k;
-                    v = at == i ? w[i] : v;
+        for (int i = 0; i < kPer; i++) {
+            wf[i] = kCount ? (key[i] ? 1.0f : 0.0f) : (float)w[i] * (float)(0x1p22 / kWaveOne);
+            far += wf[i];
+            if (key[i]) atomicAdd(&bins[bin[i]], (uint32_t)wf[i]);
+        }
+        // the float sums' rounding: a chain of kPer + 6 additions, 2^-24 of the whole each, and that of the terms and of `want`
+        far = kCount ? 0.0f : wave_sum(far) * (float)(kWaveOne / 0x1p22) * 0x1p-18f;
+        __builtin_amdgcn_wave_barrier();
+        const uint32_t upto = wave_scan(bins[lane]);
+        const uint64_t past = __ballot((double)upto >= (kCount ? want : want * (0x1p22 / kWaveOne)));
+        const int cut_bin = past ? __ffsll((unsigned long long)past) - 1 : 64;
+#pragma unroll 1
+        for (int all = cut_bin > 63; all < 2; all++) {
+            uint32_t low = 1, high = 0xFFFFFFFFu;
+            for (int round = 0; round < 64 * kPer && low <= high; round++) {
+                uint32_t pivot = 0;
+                double each = 1.0;
+                uint64_t in = 0;
+#pragma unroll
+                for (int j = 0; j < kPer; j++) {
+                    const uint64_t here = __ballot(key[j] - low <= high - low && (all || bin[j] == cut_bin));
+                    if (__popcll(here) > __popcll(in)) {
+                        in = here;
+                        const uint64_t later = here & ~0ull << (round * 23 + 32 & 63);
+                        const int at = __ffsll((unsigned long long)(later ? later : here)) - 1;
+                        pivot = from_lane(key[j], at);
+                        if (!kCount) each = from_lane(w[j], at);
+                    }
                 }
-                const uint64_t in = __ballot(k >= low && k <= high);
-                if (in) {
-                    const uint64_t middle = __ballot((in >> (threadIdx.x & 63) & 1) && lanes_below(in) == __popcll(in) / 2);
-                    const int lane = __ffsll((unsigned long long)middle) - 1;
-                    pivot = __builtin_amdgcn_readlane(k, lane);
-                    if (!kCount) each = from_lane(v, lane);
-                    found = true;
-                }
-            }
-            if (!found) break;
-            int equal = 0;
-            double above;
-            if constexpr (kCount) {
-                int c = 0;
+                if (!in) break;
+                int equal = 0, count = 0;
+                float near = 0.0f;
 #pragma unroll
                 for (int i = 0; i < kPer; i++) {
-                    c += __popcll(__ballot(key[i] > pivot));
                     equal += __popcll(__ballot(key[i] == pivot));
+                    if (kCount) count += __popcll(__ballot(key[i] > pivot));
+                    else near += key[i] > pivot ? wf[i] : 0.0f;
                 }
-                above = c;
-            } else {
-                double s = 0.0;
+                double above = count;
+                if (!kCount) {
+                    near = wave_sum(near) * (float)(kWaveOne / 0x1p22);
+                    above = near;
+                    const float upto = near + equal * (float)each;
+                    if (near <= want_f + far && upto >= want_f - far) {
+                        double s = 0.0;
 #pragma unroll
-                for (int i = 0; i < kPer; i++) {
-                    s += key[i] > pivot ? w[i] : 0.0;
-                    equal += __popcll(__ballot(key[i] == pivot));
+                        for (int i = 0; i < kPer; i++) s += key[i] > pivot ? w[i] : 0.0;
+                        above = wave_sum(s);
+                    }
                 }
-                above = wave_sum(s);
-            }
-            if (above >= want) {
-                low = pivot + 1;
-            } else if (above + equal * each < want) {
-                high = pivot - 1;
-            } else {
-                const double more = kCount ? want - above : ceil((want - above) / each);
-                return {pivot, (int64_t)more};
+                if (above >= want) {
+                    low = pivot + 1;
+                } else if (above + equal * each < want) {
+                    high = pivot - 1;
+                } else {
+                    const double more = kCount ? want - above : ceil((want - above) / each);
+                    return {pivot, (int64_t)more};
+                }
             }
         }
-        return {0, 0};  // not reached: `want` is at most the whole
+        return {0, 0};
     }
     // what is past the cut leaves
     __device__ __forceinline__ void keep(Cut c) {
@@ -254,70 +311,72 @@ template <int kPer> struct Held {
 };
 
 // The draw from a wave's row, whose largest key is `top`: its place among the slots held, and the logarithm of its
-// probability.  `all_live`: the weights of the row's live slots, where they are not all held (0: they are).
+// probability.  `all_live`: the weights of the row's live slots, where they are not all held (0: they are).  `bins`: 64 words
+// of LDS, the wave's own.
 template <int kPer>
-__device__ __forceinline__ int draw(Held<kPer>& h, const Row& r, uint32_t top, double all_live, double& log_prob) {
+__device__ __forceinline__ int draw(Held<kPer>& h, const Row& r, uint32_t top, double all_live, uint32_t* bins,
+                                    double& log_prob) {
     int live = 0, action = -1;
+    weights_of<kPer>(h.key, top, r.scale, h.w);
 #pragma unroll
     for (int i = 0; i < kPer; i++) {
-        h.w[i] = rint(weight_of(h.key[i], top, r.scale) * kWaveOne);
+        h.w[i] = rint(h.w[i] * kWaveOne);
         live += __popcll(__ballot(h.key[i] != 0));
     }
-    if (r.k && r.k < live) h.keep(h.template cut_at<true>((double)r.k));
+    const bool cut_k = r.k && r.k < live;
+    if (cut_k || r.cut_p) h.share_out(top, (float)r.scale);
+    if (cut_k) h.keep(h.template cut_at<true>((double)r.k, bins));
     if (r.cut_p) {
         double all = 0.0;
 #pragma unroll
         for (int i = 0; i < kPer; i++) all += h.w[i];
         all = wave_sum(all);
         const double want = ceil(r.p * (all_live > 0.0 ? all_live : all));
-        h.keep(h.template cut_at<false>(want < 1.0 ? 1.0 : want));
+        h.keep(h.template cut_at<false>(want < 1.0 ? 1.0 : want, bins));
     }
     const double least = r.min_p * kWaveOne;
-    double part[kPer / 4], all = 0.0;  // a lane's sums in each chunk
+    double upto[kPer / 4], all = 0.0;  // the sums up to a lane's last slot of each chunk
 #pragma unroll
     for (int i = 0; i < kPer; i += 4) {
-        part[i / 4] = 0.0;
+        double part = 0.0;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             h.w[i + e] = h.w[i + e] >= least ? h.w[i + e] : 0.0;
-            part[i / 4] += h.w[i + e];
+            part += h.w[i + e];
         }
-        all += part[i / 4];
+        upto[i / 4] = wave_scan(part) + all;
+        all = from_lane(upto[i / 4], 63);
     }
-    all = wave_sum(all);
     const double border = fmin(r.u * all, all - 1.0);  // u at or past 1: the last
-    double before = 0.0;
 #pragma unroll
     for (int i = 0; i < kPer; i += 4) {
         if (action >= 0) continue;
-        const double upto = wave_scan(part[i / 4]) + before;
-        const uint64_t past = __ballot(upto > border);
+        const uint64_t past = __ballot(upto[i / 4] > border);
         if (past) {
             const int first = __ffsll((unsigned long long)past) - 1;
-            double run = upto - part[i / 4];
-            int mine = -1;
-            uint32_t key = 0;
+            double run = upto[i / 4];  // back from the lane's last slot: the first whose sum is past the border
+            int mine = 3;
+            uint32_t key = h.key[i + 3];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                run += h.w[i + e];
-                if (mine < 0 && run > border) {
+            for (int e = 2; e >= 0; e--) {
+                run -= h.w[i + e + 1];
+                if (run > border) {
                     mine = e;
                     key = h.key[i + e];
                 }
             }
             action = i * 64 + first * 4 + from_lane(mine, first);
-            key = from_lane(key, first);
-            log_prob = (key == top ? 0.0 : ((double)value_of(key) - (double)value_of(top)) / r.t) - log(all / kWaveOne);
-        } else {
-            before = from_lane(upto, 63);
+            log_prob = log_share(from_lane(key, first), top, r.scale, all / kWaveOne);
         }
     }
     return action;
 }
 
 template <typename T, int kPer> __global__ void __launch_bounds__(256) k_sample_held(Settings s) {
+    __shared__ uint32_t bins[4][64];
     const int lane = threadIdx.x & 63;
-    const int64_t b = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    // the same for the wave's lanes, and known to be: its settings come by scalar loads, all at once
+    const int64_t b = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (b >= s.rows) return;
     const Row r = row_of(s, b);
     const T* row = (const T*)s.logits + b * s.stride;
@@ -346,7 +405,7 @@ template <typename T, int kPer> __global__ void __launch_bounds__(256) k_sample_
             }
         }
     } else if (top) {
-        action = draw(h, r, top, 0.0, log_prob);
+        action = draw(h, r, top, 0.0, bins[threadIdx.x >> 6], log_prob);
     }
     if (lane == 0) {
         s.actions[b] = action;
@@ -360,9 +419,9 @@ constexpr int kParts = (int)(kMaxWidth / 256);
 struct Shared {
     unsigned long long bins[kParts];  // the first kBins: of a digit; then all: the sums of 256 slots each
     uint32_t equal[kParts];
-    unsigned long long above, all;
-    uint32_t most[kWaves];
-    int bin;
+    unsigned long long above, all, most[kWaves];
+    int bin, left;
+    uint32_t wave_bins[64];
 };
 
 // the bin, from the top, at which the sum reaches `want`, and the sum above it; by wave 0, for all
@@ -393,57 +452,149 @@ template <typename T> __global__ void __launch_bounds__(kThreads) k_sample_long(
     const Row r = row_of(s, b);
     const T* row = (const T*)s.logits + b * s.stride;
     auto each = [&](auto f) {
-        for (int c = tid * 4; c < r.n; c += kThreads * 4) {
-            uint32_t key[4];
-            load_keys(row, c, r.n, key);
+        for (int c = tid * 4; c - lane * 4 < r.n; c += 4 * kThreads * 4) {  // whole waves: f may ask all lanes
+            uint32_t key[4][4];  // four loads under way
 #pragma unroll
-            for (int e = 0; e < 4; e++) f(key[e], c + e);
+            for (int k = 0; k < 4; k++) load_keys(row, c + k * kThreads * 4, r.n, key[k]);
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) f(key[k][e], c + k * kThreads * 4 + e);
         }
     };
-    uint32_t top = 0;
+    auto clear = [&] {
+        for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
+        __syncthreads();
+    };
+    const bool by_count = r.k && !r.greedy;
+    if (by_count) clear();
+    // the largest key and its first slot as one number, and how many are live
+    unsigned long long best = 0;
     int live = 0;
-    each([&](uint32_t key, int) {
-        top = max(top, key);
+    each([&](uint32_t key, int i) {
+        const unsigned long long one = (unsigned long long)key << 32 | (uint32_t)~i;
+        best = key && one > best ? one : best;
         live += key != 0;
+        if (by_count && key) atomicAdd(&sh.bins[key >> 21], 1ull);
     });
-    top = wave_most(top);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned long long other = __shfl_xor(best, o, 64);
+        best = other > best ? other : best;
+    }
     live = wave_sum(live);
     if (lane == 0) {
-        sh.most[wave] = top;
+        sh.most[wave] = best;
         sh.equal[wave] = live;
     }
     __syncthreads();
     live = 0;
     for (int i = 0; i < kWaves; i++) {
-        top = max(top, sh.most[i]);
+        best = sh.most[i] > best ? sh.most[i] : best;
         live += sh.equal[i];
     }
     __syncthreads();
-    if (!top) {
+    const uint32_t top = (uint32_t)(best >> 32);
+    if (!top || r.greedy) {
         if (tid == 0) {
-            s.actions[b] = -1;
-            if (s.log_probs) s.log_probs[b] = 0.0f;
-        }
-        return;
-    }
-    if (r.greedy) {
-        if (tid == 0) sh.bin = r.n;
-        __syncthreads();
-        int first = r.n;
-        each([&](uint32_t key, int i) { first = key == top && i < first ? i : first; });
-        if (first < r.n) atomicMin(&sh.bin, first);
-        __syncthreads();
-        if (tid == 0) {
-            s.actions[b] = sh.bin;
+            s.actions[b] = top ? (int64_t)(uint32_t)~(uint32_t)best : -1;
             if (s.log_probs) s.log_probs[b] = 0.0f;
         }
         return;
     }
     auto weight = [&](uint32_t key) { return (unsigned long long)rint(weight_of(key, top, r.scale) * kBlockOne); };
-    auto clear = [&] {
-        for (int i = tid; i < kBins; i += kThreads) sh.bins[i] = 0;
+    // What has to be at or above `floor` to be kept.  By top_k, the digit in which the k-th is; by top_p without it, that in which
+    // the mass is reached; by min_p, a weight a little below it (the logit's rounding to float32 and that of the logarithm).
+    const bool cut_k = r.k && r.k < live;
+    uint32_t floor_key = 1;
+    unsigned long long all_live = 0;
+    if (cut_k) {
+        find_bin(sh, (unsigned long long)r.k);
+        floor_key = max(1u, (uint32_t)sh.bin << 21);
+    } else if (r.cut_p) {
         __syncthreads();
-    };
+        clear();
+        each([&](uint32_t key, int) {
+            if (const unsigned long long w = key ? weight(key) : 0) atomicAdd(&sh.bins[key >> 21], w);
+        });
+        __syncthreads();
+        if (wave == 0) {
+            unsigned long long sum = 0;
+            for (int i = lane; i < kBins; i += 64) sum += sh.bins[i];
+            sum = wave_sum(sum);
+            if (lane == 0) sh.all = sum;
+        }
+        __syncthreads();
+        all_live = sh.all;
+        const double part = ceil(r.p * (double)all_live);
+        find_bin(sh, part < 1.0 ? 1ull : part < (double)all_live ? (unsigned long long)part : all_live);
+        floor_key = max(1u, (uint32_t)sh.bin << 21);
+    }
+    if (r.min_p > 0.0 && !(cut_k && r.cut_p)) {  // top_p of the k largest needs them all
+        const double x = (double)value_of(top), raw = x + r.t * log(r.min_p), at = raw - 1e-6 * (fabs(x) + fabs(raw) + r.t);
+        const float least = at > -3.4028234663852886e38 ? (float)at : -__builtin_inff();  // NaN: none
+        floor_key = max(floor_key, key_of(least));
+    }
+    if (tid == 0) sh.left = 0;
+    __syncthreads();
+    // the slots left, in any order, then in the row's
+    uint32_t* const left_key = (uint32_t*)sh.bins;
+    uint32_t* const left_slot = left_key + kHeld;
+    uint32_t* const key_in_order = left_slot + kHeld;
+    uint32_t* const slot_in_order = key_in_order + kHeld;
+    const bool few = floor_key > 1 || live <= kHeld;
+    if (few)
+        each([&](uint32_t key, int i) {
+            const uint64_t these = __ballot(key >= floor_key);
+            if (!these) return;
+            int first = 0;
+            if (lane == __ffsll((unsigned long long)these) - 1) first = atomicAdd(&sh.left, __popcll(these));
+            const int at = from_lane(first, __ffsll((unsigned long long)these) - 1) + lanes_below(these);
+            if (key >= floor_key && at < kHeld) {
+                left_key[at] = key;
+                left_slot[at] = i;
+            }
+        });
+    __syncthreads();
+    const int left = sh.left;
+    if (few && left <= kHeld) {
+        if (tid < kHeld - left) left_slot[left + tid] = 0xFFFFFFFFu;
+        key_in_order[tid] = 0;
+        __syncthreads();
+        if (tid < left) {
+            const uint32_t mine = left_slot[tid];
+            int rank = 0;
+            for (int i = 0; i < left; i += 4) {
+                const uint4 q = *(const uint4*)(left_slot + i);
+                rank += (q.x < mine) + (q.y < mine) + (q.z < mine) + (q.w < mine);
+            }
+            key_in_order[rank] = left_key[tid];
+            slot_in_order[rank] = mine;
+        }
+        __syncthreads();
+        if (wave != 0) return;
+        double log_prob = 0.0;
+        const double whole = (double)all_live * (kWaveOne / kBlockOne);
+        auto drawn = [&](auto h) {
+            constexpr int per = (int)(sizeof(h.key) / 4);
+#pragma unroll
+            for (int i = 0; i < per; i += 4) {
+                const uint4 q = *(const uint4*)(key_in_order + i * 64 + lane * 4);
+                h.key[i] = q.x;
+                h.key[i + 1] = q.y;
+                h.key[i + 2] = q.z;
+                h.key[i + 3] = q.w;
+            }
+            return draw(h, r, top, whole, sh.wave_bins, log_prob);
+        };
+        const int place = left <= 256 ? drawn(Held<4>{}) : drawn(Held<kHeld / 64>{});
+        if (lane == 0) {
+            s.actions[b] = slot_in_order[place];
+            if (s.log_probs) s.log_probs[b] = (float)log_prob;
+        }
+        return;
+    }
+    __syncthreads();
     // the cut at which the sum of `of` over the keys reaches `want`, by digits of 11, 11 and 10 bits; `last`: keys that
     // equal it are counted by `extra` alone
     auto cut_at = [&](unsigned long long want, auto of, uint32_t last, unsigned long long extra) {
@@ -467,7 +618,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) k_sample_long(
         return Cut{prefix, (int64_t)((want + one - 1) / one)};
     };
     Cut cut{1, (int64_t)1 << 40};  // nothing is cut
-    if (r.k && r.k < live) cut = cut_at((unsigned long long)r.k, [](uint32_t) { return 1ull; }, 0, 0);
+    if (cut_k) cut = cut_at((unsigned long long)r.k, [](uint32_t) { return 1ull; }, 0, 0);
     if (r.cut_p) {
         unsigned long long sum = 0;
         each([&](uint32_t key, int) {
@@ -570,8 +721,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) k_sample_long(
     s.actions[b] = (int64_t)part * 256 + lane * 4 + e;
     if (s.log_probs) {
         const uint32_t k = key[e];
-        s.log_probs[b] = (float)((k == top ? 0.0 : ((double)value_of(k) - (double)value_of(top)) / r.t) -
-                                 log((double)all / kBlockOne));
+        s.log_probs[b] = (float)log_share(k, top, r.scale, (double)all / kBlockOne);
     }
 }
 
