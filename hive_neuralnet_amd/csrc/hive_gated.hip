@@ -84,20 +84,28 @@ __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_gated_forward(
     }
 }
 
-constexpr int kSlopeRows = 64;  // of a block of k_gated_slopes
+// k_gated_slopes: threads across a row, 8 columns each
+inline int slope_across(int64_t cut) { return cut >= 256 ? 32 : cut >= 128 ? 16 : 8; }
+inline int slope_each(int64_t rows, int64_t cut) {  // rows a thread takes: 8, or fewer where blocks would be few
+    int each = 8;
+    while (each > 1 && rows * cut < (int64_t)1024 * 2048 * each) each /= 2;
+    return each;
+}
 
 // dgate and dup from dh, gate and up: rows of parts [dgate | dup], each `cut` values with zeros past its own; with `sums`, the
-// sums of each over the block's rows: sums[row block][2][hidden].  Memory bound; a thread takes 8 columns of 8 rows.
+// sums of each over the block's rows: sums[row block][2][hidden].  Memory bound; a thread takes 8 columns of `each` rows.
 template <typename T, typename P, int kParts>
 __global__ void __launch_bounds__(256)
 k_gated_slopes(const T* __restrict__ dh, int64_t dh_stride, const float* __restrict__ gate, const float* __restrict__ up,
-               int64_t rows, int hidden, int act, P* __restrict__ d, int64_t d_stride, int cut, float* __restrict__ sums) {
-    __shared__ float lds[2][8][kSlopeRows / 2 + 1][8];
-    const int64_t r0 = (int64_t)blockIdx.x * kSlopeRows;
-    const int column = threadIdx.x % 32, c = (int)blockIdx.y * 256 + column * 8, live = hidden - c;
+               int64_t rows, int hidden, int act, P* __restrict__ d, int64_t d_stride, int cut, int across, int each,
+               float* __restrict__ sums) {
+    __shared__ float lds[2][256][9];
+    const int groups = 256 / across, group = threadIdx.x / across, c0 = (int)blockIdx.y * across * 8;
+    const int c = c0 + threadIdx.x % across * 8, live = hidden - c;
+    const int64_t r0 = (int64_t)blockIdx.x * groups * each;
     float sum[2][8] = {};
-    for (int i = threadIdx.x / 32; i < kSlopeRows; i += 8) {
-        const int64_t r = r0 + i;
+    for (int i = 0; i < each; i++) {
+        const int64_t r = r0 + i * groups + group;
         if (r >= rows || c >= cut) continue;
         float v[8], g[8], u[8];
         const T* from = dh + r * dh_stride + c;
@@ -130,14 +138,13 @@ k_gated_slopes(const T* __restrict__ dh, int64_t dh_stride, const float* __restr
 #pragma unroll
     for (int w = 0; w < 2; w++)
 #pragma unroll
-        for (int k = 0; k < 8; k++) lds[w][threadIdx.x / 32][column][k] = sum[w][k];
+        for (int k = 0; k < 8; k++) lds[w][threadIdx.x][k] = sum[w][k];
     __syncthreads();
-    for (int i = threadIdx.x; i < 512; i += 256) {
-        const int w = i / 256, n = (int)blockIdx.y * 256 + i % 256;
+    for (int i = threadIdx.x; i < 2 * across * 8; i += 256) {
+        const int w = i / (across * 8), n = i % (across * 8);
         float all = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 8; k++) all += lds[w][k][i % 256 / 8][i % 8];
-        if (n < hidden) sums[((int64_t)blockIdx.x * 2 + w) * hidden + n] = all;
+        for (int k = 0; k < groups; k++) all += lds[w][k * across + n / 8][n % 8];
+        if (c0 + n < hidden) sums[((int64_t)blockIdx.x * 2 + w) * hidden + c0 + n] = all;
     }
 }
 
@@ -149,6 +156,7 @@ k_join_sums(const float* __restrict__ sums, int64_t blocks, int hidden, T* __res
     const int c = (int)blockIdx.x * 64 + (threadIdx.x & 63), w = blockIdx.y, wave = threadIdx.x >> 6;
     float v = 0.0f;
     if (c < hidden)
+#pragma unroll 8
         for (int64_t b = wave; b < blocks; b += 16) v += sums[(b * 2 + w) * hidden + c];
     lds[wave][threadIdx.x & 63] = v;
     __syncthreads();
@@ -197,26 +205,41 @@ __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_product(Produc
     }
 }
 
-// the splits' parts added up: 4 columns a thread, row r of `first` and, from row cut on, of `second`
-template <typename T>
+// the splits' parts added up: 4 columns a thread, kLanes threads for the same ones where there are many parts; row r of `first`
+// and, from row cut on, of `second`
+template <typename T, int kLanes>
 __global__ void __launch_bounds__(256)
 k_join_parts(const float* __restrict__ part, int splits, int64_t m, int n, int rows, int cut, T* __restrict__ first,
              T* __restrict__ second) {
-    const int across = (n + 3) / 4;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < (int64_t)rows * across * (second ? 2 : 1);
-         i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / across % rows;
-        const int c = (int)(i % across) * 4, live = n - c;
-        const bool of_first = i < (int64_t)rows * across;
-        float v[4] = {};
-        for (int s = 0; s < splits; s++) {
+    constexpr int each = 256 / kLanes;
+    __shared__ float lds[kLanes > 1 ? kLanes : 1][kLanes > 1 ? each : 1][4];
+    const int across = (n + 3) / 4, lane = threadIdx.x / each, at = threadIdx.x % each;
+    const int64_t all = (int64_t)rows * across * (second ? 2 : 1), i = (int64_t)blockIdx.x * each + at;
+    const int64_t r = i / across % rows;
+    const int c = (int)(i % across) * 4, live = n - c;
+    const bool of_first = i < (int64_t)rows * across;
+    float v[4] = {};
+    if (i < all) {
+        const float* from = part + (of_first ? r : cut + r) * n + c;
+#pragma unroll 4
+        for (int s = lane; s < splits; s += kLanes) {
             float p[4];
-            load_some<float, 4>(part + (s * m + (of_first ? r : cut + r)) * n + c, live, p);
+            load_some<float, 4>(from + s * m * n, live, p);
 #pragma unroll
             for (int e = 0; e < 4; e++) v[e] += p[e];
         }
-        store_some<T, 4>((of_first ? first : second) + r * n + c, live, v);
     }
+    if constexpr (kLanes > 1) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) lds[lane][at][e] = v[e];
+        __syncthreads();
+        if (lane) return;
+#pragma unroll
+        for (int k = 1; k < kLanes; k++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[e] += lds[k][at][e];
+    }
+    if (i < all) store_some<T, 4>((of_first ? first : second) + r * n + c, live, v);
 }
 
 // ---- host -------------------------------------------------------------------
@@ -241,66 +264,91 @@ struct Arena {
     }
 };
 
-// an operand of rows x cols values: as it is, or packed into the arena (only counted where the arena has no memory)
+// `count` operands of rows x cols values, as they are, or, where one of them cannot be taken so, packed into the arena (only
+// counted where the arena has no memory): a tile takes two by one stride
 template <typename T>
-int packed_rows(const void* src, int type, int64_t rows, int64_t cols, int64_t stride, bool as_is, Arena& ws,
-                hipStream_t st, Operand* out) {
-    if (as_is) {
-        *out = {src, (rows <= 1 ? cols : stride) * 2, (int)rows, (int)cols * 2};
-        return 0;
-    }
+int operands(const void* const* src, int count, int64_t rows, int64_t cols, int64_t stride, Arena& ws, hipStream_t st,
+             Operand* out) {
+    constexpr int type = sizeof(T) == 4 ? HG_F32 : HG_F16;
+    bool as_is = true;
+    for (int i = 0; i < count; i++) as_is = as_is && as_it_is(src[i], type, rows, cols, stride);
     const int parts = parts_of(type);
     const int64_t bytes = packed_bytes(cols, parts);
-    char* to = ws.take(rows * bytes);
-    *out = {to, bytes, (int)rows, (int)bytes};
-    if (!to || rows == 0) return 0;
-    const unsigned grid = (unsigned)std::min<int64_t>((rows * (up_to(cols, 32) / 8) + kPackThreads - 1) / kPackThreads, 8192);
-    if constexpr (sizeof(T) == 4)
-        k_pack<float, bf16, 3><<<grid, kPackThreads, 0, st>>>((const float*)src, stride, rows, (int)cols, (bf16*)to, bytes / 2);
-    else
-        k_pack<T, T, 1><<<grid, kPackThreads, 0, st>>>((const T*)src, stride, rows, (int)cols, (T*)to, bytes / 2);
+    Packing f{};
+    for (int i = 0; i < count; i++) {
+        if (as_is) {
+            out[i] = {src[i], (rows <= 1 ? cols : stride) * 2, (int)rows, (int)cols * 2};
+        } else {
+            f.src[i] = src[i];
+            f.dst[i] = ws.take(rows * bytes);
+            out[i] = {f.dst[i], bytes, (int)rows, (int)bytes};
+        }
+    }
+    if (as_is || !ws.p || rows == 0) return 0;
+    f.src_stride = stride;
+    f.dst_stride = bytes / 2;
+    f.rows = rows;
+    f.cols = (int)cols;
+    const int64_t threads = rows * (up_to(cols, 32) / 8);
+    const dim3 grid((unsigned)std::min<int64_t>((threads + kPackThreads - 1) / kPackThreads, 1 << 20), count);
+    if constexpr (sizeof(T) == 4) k_pack<float, bf16, 3><<<grid, kPackThreads, 0, st>>>(f);
+    else k_pack<T, T, 1><<<grid, kPackThreads, 0, st>>>(f);
     return launched();
 }
-// both weights the same way: a tile takes them by one stride
-template <typename T>
-int packed_weights(const void* wg, const void* wu, int64_t hidden, int64_t cols, Arena& ws, hipStream_t st, Operand* g,
-                   Operand* u) {
-    constexpr int type = sizeof(T) == 4 ? HG_F32 : HG_F16;
-    const bool as_is = as_it_is(wg, type, hidden, cols, cols) && as_it_is(wu, type, hidden, cols, cols);
-    const int e = packed_rows<T>(wg, type, hidden, cols, cols, as_is, ws, st, g);
-    return e ? e : packed_rows<T>(wu, type, hidden, cols, cols, as_is, ws, st, u);
-}
 
-// f called with the tile for an m x n result: the largest of which there are enough for the card's 256 compute units
-template <typename T, typename F> int with_tile(int64_t m, int64_t n, F f) {
+// What a tile of a product costs: a slice's time with every compute unit at work (a block's, with its neighbours on the same
+// one), and the time around its slices, in nanoseconds, as measured at 8,192 x 8,192 x 8,192 and the like.
+template <typename Tl> struct Cost {
+    static constexpr double slice = Tl::kParts == 3 ? (Tl::kM == 128 ? 1900 : 1100) : Tl::kM == 256 ? 1650 : Tl::kM == 128 ? 1000 : 700;
+    static constexpr double around = Tl::kM == 256 ? 6000 : Tl::kM == 128 ? 4000 : 2500;
+};
+// The least time of an m x n result with `slices` of 64 k (32 of floats') over the ways to cut k into splits (`most` of them),
+// whose parts are added up in a launch of their own.
+struct Plan {
+    double time;
+    int64_t splits;
+};
+template <typename Tl> Plan plan_of(int64_t m, int64_t n, int64_t slices, int64_t most) {
+    const int64_t tiles = ((m + Tl::kM - 1) / Tl::kM) * ((n + Tl::kN - 1) / Tl::kN), room = 256 * Tl::kBlocks;
+    Plan best{1e300, 1};
+    for (int64_t s = 1; s <= most && (s == 1 || slices / s >= 4); s = s < 8 ? s + 1 : s * 5 / 4) {
+        const int64_t each = (slices + s - 1) / s, blocks = tiles * ((slices + each - 1) / each);
+        // a compute unit with fewer blocks than it holds takes each of them in less time, down to half
+        const int64_t rounds = (blocks + room - 1) / room;
+        const double full = blocks >= room ? 1.0 : std::max(0.5, (double)((blocks + 255) / 256) / Tl::kBlocks);
+        double time = rounds * (each * Cost<Tl>::slice * full + Cost<Tl>::around);
+        if (s > 1) time += 4000.0 + 2.0 * s * m * n * 4.0 / 4000.0;  // written and read at 4 TB/s
+        if (time < best.time) best = {time, s};
+    }
+    return best;
+}
+// f called with the tile, and the number of splits, that take the least time
+template <typename T, typename F> int with_tile(int64_t m, int64_t n, int64_t k, int64_t most, F f) {
     using P = std::conditional_t<sizeof(T) == 4, bf16, T>;
-    constexpr int parts = sizeof(T) == 4 ? 3 : 1;
-    auto tiles = [&](int a, int b) { return ((m + a - 1) / a) * ((n + b - 1) / b); };
-#ifdef TRY
-    if constexpr (parts == 1) {
-        if (TRY == 0) return f(Tile<P, parts, 2, 256, 256, 2, 4, 2, 1>{});
-        if (TRY == 1) return f(Tile<P, parts, 2, 128, 128, 2, 2, 2, 2>{});
-        if (TRY == 2) return f(Tile<P, parts, 2, 256, 128, 4, 2, 3, 1>{});
+    constexpr bool parts = sizeof(T) == 4;
+    using Middle = std::conditional_t<parts, Tile<P, 3, 1, 128, 128, 2, 2, 3, 1>, Tile<P, 1, 2, 128, 128, 2, 2, 2, 2>>;
+    using Small = std::conditional_t<parts, Tile<P, 3, 1, 64, 64, 2, 2, 3, 2>, Tile<P, 1, 2, 64, 64, 2, 2, 3, 3>>;
+    const int64_t slices = std::max<int64_t>(1, (k + 32 * Small::kSteps - 1) / (32 * Small::kSteps));
+    const Plan middle = plan_of<Middle>(m, n, slices, most), small = plan_of<Small>(m, n, slices, most);
+    if constexpr (!parts) {
+        using Large = Tile<P, 1, 2, 256, 256, 2, 4, 2, 1>;
+        const Plan large = plan_of<Large>(m, n, slices, most);
+        if (large.time <= middle.time && large.time <= small.time) return f(Large{}, large.splits);
     }
-#endif
-    if constexpr (parts == 1) {
-        if (tiles(256, 256) >= 192) return f(Tile<P, 1, 2, 256, 256, 2, 4, 2, 1>{});
-        if (tiles(128, 128) >= 192) return f(Tile<P, 1, 2, 128, 128, 2, 2, 2, 2>{});
-        return f(Tile<P, 1, 2, 64, 64, 2, 2, 3, 3>{});
-    } else {
-        if (tiles(128, 128) >= 192) return f(Tile<P, 3, 1, 128, 128, 2, 2, 3, 1>{});
-        return f(Tile<P, 3, 1, 64, 64, 2, 2, 3, 2>{});
-    }
+    return middle.time <= small.time ? f(Middle{}, middle.splits) : f(Small{}, small.splits);
 }
 
 template <typename T>
 int forward(const void* x, int64_t rows, int64_t cols, int64_t x_stride, const void* wg, const void* wu, int64_t hidden,
             const void* bg, const void* bu, int act, void* h, float* gate, float* up, Arena& ws, hipStream_t st) {
-    constexpr int type = sizeof(T) == 4 ? HG_F32 : HG_F16;
     Forward f{};
-    int e = packed_rows<T>(x, type, rows, cols, x_stride, as_it_is(x, type, rows, cols, x_stride), ws, st, &f.x);
-    if (!e) e = packed_weights<T>(wg, wu, hidden, cols, ws, st, &f.wg, &f.wu);
+    const void* const weights[2] = {wg, wu};
+    Operand w[2];
+    int e = operands<T>(&x, 1, rows, cols, x_stride, ws, st, &f.x);
+    if (!e) e = operands<T>(weights, 2, hidden, cols, cols, ws, st, w);
     if (e || !ws.p) return e;
+    f.wg = w[0];
+    f.wu = w[1];
     f.x.bytes = std::min(f.x.bytes, std::min(f.wg.bytes, f.wu.bytes));  // a packed row's zeros have no partner in a plain one
     f.bg = bg;
     f.bu = bu;
@@ -309,7 +357,7 @@ int forward(const void* x, int64_t rows, int64_t cols, int64_t x_stride, const v
     f.up = up;
     f.hidden = (int)hidden;
     f.act = act;
-    return with_tile<T>(rows, 2 * hidden, [&](auto tile) {
+    return with_tile<T>(rows, 2 * hidden, cols, 1, [&](auto tile, int64_t) {
         using Tl = decltype(tile);
         f.tiles_m = (int)((rows + Tl::kM - 1) / Tl::kM);
         f.tiles_n = (int)((hidden + Tl::kN / 2 - 1) / (Tl::kN / 2));
@@ -323,7 +371,7 @@ int forward(const void* x, int64_t rows, int64_t cols, int64_t x_stride, const v
 template <typename T, bool kTurnedA>
 int product(const Operand& a, const Operand& b, const Operand& b_second, int64_t m, int64_t k, int64_t cut_k, int64_t rows,
             int64_t cut, void* first, void* second, int64_t n, Arena& ws, hipStream_t st) {
-    return with_tile<T>(m, n, [&](auto tile) {
+    return with_tile<T>(m, n, k, 256, [&](auto tile, int64_t splits) {
         using Tl = decltype(tile);
         constexpr int deep = 32 * Tl::kSteps;
         Product f{};
@@ -341,8 +389,6 @@ int product(const Operand& a, const Operand& b, const Operand& b_second, int64_t
         f.tiles_n = (int)((n + Tl::kN - 1) / Tl::kN);
         f.slices = (int)((k + deep - 1) / deep);
         const int64_t tiles = (int64_t)f.tiles_m * f.tiles_n;
-        // two blocks for each compute unit, at least 16 slices each
-        int64_t splits = std::max<int64_t>(1, std::min<int64_t>({512 / tiles, f.slices / 16, 256}));
         f.each = (int)((f.slices + splits - 1) / splits);
         splits = (f.slices + f.each - 1) / f.each;
         if (splits > 1) f.part = (float*)ws.take(splits * m * n * 4);
@@ -351,8 +397,12 @@ int product(const Operand& a, const Operand& b, const Operand& b_second, int64_t
         int e = launched();
         if (!e && splits > 1) {
             const int64_t all = rows * ((n + 3) / 4) * (second ? 2 : 1);
-            k_join_parts<T><<<(unsigned)std::min<int64_t>((all + 255) / 256, 4096), 256, 0, st>>>(
-                f.part, (int)splits, m, (int)n, (int)rows, (int)cut, (T*)first, (T*)second);
+            if (splits >= 8)
+                k_join_parts<T, 16><<<(unsigned)((all + 15) / 16), 256, 0, st>>>(f.part, (int)splits, m, (int)n, (int)rows,
+                                                                                (int)cut, (T*)first, (T*)second);
+            else
+                k_join_parts<T, 1><<<(unsigned)((all + 255) / 256), 256, 0, st>>>(f.part, (int)splits, m, (int)n, (int)rows,
+                                                                                 (int)cut, (T*)first, (T*)second);
             e = launched();
         }
         return e;
@@ -364,16 +414,17 @@ int backward(const void* dh, int64_t dh_stride, const void* x, int64_t rows, int
              const void* wg, const void* wu, int64_t hidden, const float* gate, const float* up, int act, void* dx,
              void* dwg, void* dwu, void* dbg, void* dbu, Arena& ws, hipStream_t st) {
     using P = std::conditional_t<sizeof(T) == 4, bf16, T>;
-    constexpr int type = sizeof(T) == 4 ? HG_F32 : HG_F16, parts = sizeof(T) == 4 ? 3 : 1;
+    constexpr int parts = sizeof(T) == 4 ? 3 : 1;
     const int64_t cut = up_to(hidden, 64), d_bytes = packed_bytes(2 * cut, parts);  // 64: whole slices of each half
-    const int64_t blocks = (rows + kSlopeRows - 1) / kSlopeRows;
+    const int across = slope_across(cut), each = slope_each(rows, cut), deep = 256 / across * each;
+    const int64_t blocks = (rows + deep - 1) / deep;
     const bool biases = dbg || dbu;
     char* d = ws.take(rows * d_bytes);
     float* sums = biases ? (float*)ws.take(blocks * 2 * hidden * 4) : nullptr;
     int e = 0;
     if (ws.p) {
-        k_gated_slopes<T, P, parts><<<dim3((unsigned)blocks, (unsigned)((cut + 255) / 256)), 256, 0, st>>>(
-            (const T*)dh, dh_stride, gate, up, rows, (int)hidden, act, (P*)d, d_bytes / 2, (int)cut, sums);
+        k_gated_slopes<T, P, parts><<<dim3((unsigned)blocks, (unsigned)((cut + across * 8 - 1) / (across * 8))), 256, 0, st>>>(
+            (const T*)dh, dh_stride, gate, up, rows, (int)hidden, act, (P*)d, d_bytes / 2, (int)cut, across, each, sums);
         e = launched();
         if (!e && biases) {
             k_join_sums<T><<<dim3((unsigned)((hidden + 63) / 64), 2), 1024, 0, st>>>(sums, blocks, (int)hidden, (T*)dbg, (T*)dbu);
@@ -382,13 +433,14 @@ int backward(const void* dh, int64_t dh_stride, const void* x, int64_t rows, int
     }
     const Operand grads{d, d_bytes, (int)rows, (int)d_bytes};
     if (!e && dx) {
-        Operand g, u;
-        e = packed_weights<T>(wg, wu, hidden, cols, ws, st, &g, &u);
-        if (!e) e = product<T, false>(grads, g, u, rows, 2 * cut, cut, rows, rows, dx, nullptr, cols, ws, st);
+        const void* const weights[2] = {wg, wu};
+        Operand w[2];
+        e = operands<T>(weights, 2, hidden, cols, cols, ws, st, w);
+        if (!e) e = product<T, false>(grads, w[0], w[1], rows, 2 * cut, cut, rows, rows, dx, nullptr, cols, ws, st);
     }
     if (!e && dwg) {
         Operand b;
-        e = packed_rows<T>(x, type, rows, cols, x_stride, as_it_is(x, type, rows, cols, x_stride), ws, st, &b);
+        e = operands<T>(&x, 1, rows, cols, x_stride, ws, st, &b);
         if (!e) e = product<T, true>(grads, b, b, 2 * cut, rows, 1 << 30, hidden, cut, dwg, dwu, cols, ws, st);
     }
     return e;

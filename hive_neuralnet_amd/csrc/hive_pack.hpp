@@ -35,19 +35,24 @@ inline int64_t packed_bytes(int64_t n, int parts) { return up_to(n, 32) * 2 * pa
 
 constexpr int kPackThreads = 256;
 
+// What a launch packs: up to two tensors of one shape, grid y.
+struct Packing {
+    const void* src[2];
+    void* dst[2];
+    int64_t src_stride, dst_stride, rows;
+    int cols;
+};
 // dst[r] = the parts of src[r][0..cols), zeros up to a multiple of 32.  Memory bound; a thread takes 8 values.
-template <typename S, typename T, int kParts>
-__global__ void __launch_bounds__(kPackThreads)
-k_pack(const S* __restrict__ src, int64_t src_stride, int64_t rows, int cols, T* __restrict__ dst, int64_t dst_stride) {
-    const int groups = (int)up_to(cols, 32) / 8;
-    for (int64_t i = (int64_t)blockIdx.x * kPackThreads + threadIdx.x; i < rows * groups;
+template <typename S, typename T, int kParts> __global__ void __launch_bounds__(kPackThreads) k_pack(Packing f) {
+    const int groups = (int)up_to(f.cols, 32) / 8;
+    const S* const src = (const S*)f.src[blockIdx.y];
+    T* const dst = (T*)f.dst[blockIdx.y];
+    for (int64_t i = (int64_t)blockIdx.x * kPackThreads + threadIdx.x; i < f.rows * groups;
          i += (int64_t)gridDim.x * kPackThreads) {
-        const int64_t r = i / groups;
-        const int c = (int)(i % groups) * 8;
-        const S* from = src + r * src_stride + c;
+        const int64_t r = f.rows < 1 << 20 && groups < 1 << 11 ? (int64_t)((uint32_t)i / (uint32_t)groups) : i / groups;
+        const int c = (int)(i - r * groups) * 8;
         float v[8];
-#pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = c + k < cols ? to_f32<S>(from[k]) : 0.0f;
+        load_some<S, 8>(src + r * f.src_stride + c, f.cols - c, v);
         typedef T vec __attribute__((ext_vector_type(8)));
         vec q[kParts];
 #pragma unroll
@@ -58,7 +63,7 @@ k_pack(const S* __restrict__ src, int64_t src_stride, int64_t rows, int cols, T*
             for (int p = 0; p < kParts; p++) q[p][k] = part[p];
         }
 #pragma unroll
-        for (int p = 0; p < kParts; p++) *(vec*)(dst + r * dst_stride + part_place<kParts>(c, p)) = q[p];
+        for (int p = 0; p < kParts; p++) *(vec*)(dst + r * f.dst_stride + part_place<kParts>(c, p)) = q[p];
     }
 }
 
