@@ -299,8 +299,10 @@ int operands(const void* const* src, int count, int64_t rows, int64_t cols, int6
 // What a tile of a product costs: a slice's time with every compute unit at work (a block's, with its neighbours on the same
 // one), and the time around its slices, in nanoseconds, as measured at 8,192 x 8,192 x 8,192 and the like.
 template <typename Tl> struct Cost {
-    static constexpr double slice = Tl::kParts == 3 ? (Tl::kM == 128 ? 1900 : 1100) : Tl::kM == 256 ? 1650 : Tl::kM == 128 ? 1000 : 700;
-    static constexpr double around = Tl::kM == 256 ? 6000 : Tl::kM == 128 ? 4000 : 2500;
+    static constexpr int size = Tl::kM * Tl::kN;
+    static constexpr double slice = Tl::kParts == 3 ? (size == 128 * 128 ? 1900 : size == 64 * 128 ? 1500 : 1100)
+                                                    : (size == 256 * 256 ? 1650 : size == 128 * 128 ? 1000 : 700);
+    static constexpr double around = size == 256 * 256 ? 6000 : size == 128 * 128 ? 4000 : 2500;
 };
 // The least time of an m x n result with `slices` of 64 k (32 of floats') over the ways to cut k into splits (`most` of them),
 // whose parts are added up in a launch of their own.
@@ -330,11 +332,10 @@ template <typename T, typename F> int with_tile(int64_t m, int64_t n, int64_t k,
     using Small = std::conditional_t<parts, Tile<P, 3, 1, 64, 64, 2, 2, 3, 2>, Tile<P, 1, 2, 64, 64, 2, 2, 3, 3>>;
     const int64_t slices = std::max<int64_t>(1, (k + 32 * Small::kSteps - 1) / (32 * Small::kSteps));
     const Plan middle = plan_of<Middle>(m, n, slices, most), small = plan_of<Small>(m, n, slices, most);
-    if constexpr (!parts) {
-        using Large = Tile<P, 1, 2, 256, 256, 2, 4, 2, 1>;
-        const Plan large = plan_of<Large>(m, n, slices, most);
-        if (large.time <= middle.time && large.time <= small.time) return f(Large{}, large.splits);
-    }
+    // floats: 64 x 128 tiles, of which a compute unit holds two; 16-bit tensors: 256 x 256, which read the least
+    using Third = std::conditional_t<parts, Tile<P, 3, 1, 64, 128, 2, 2, 2, 2>, Tile<P, 1, 2, 256, 256, 2, 4, 2, 1>>;
+    const Plan third = plan_of<Third>(m, n, slices, most);
+    if (third.time <= middle.time && third.time <= small.time) return f(Third{}, third.splits);
     return middle.time <= small.time ? f(Middle{}, middle.splits) : f(Small{}, small.splits);
 }
 
