@@ -1,18 +1,18 @@
-// train_calls.cpp -- the training operators' entry points from Python without
-// Python's share of a call.
+// train_calls.cpp -- the training operators' entry points, and the draw of a
+// slot from each row of logits, from Python without Python's share of a call.
 //
 // A small norm, loss or step spends 2 to 6 us on the device and 4 in handing a
 // launch over; checks of its arguments, the result tensors and the C call, taken
 // one by one from Python, came to 6 to 10 more.  Each function here does for
-// one entry point what training_ops.py does for arguments that are plainly
+// one entry point what training_ops.py or network_ops.py does for arguments that are plainly
 // right -- the same conditions, results and C call -- and returns None, having
-// done nothing, for any other: training_ops.py then finds what it serves
+// done nothing, for any other: the Python module then finds what it serves
 // besides (rows of more dimensions that are evenly spaced, gradients left out)
 // or the words of the refusal.
 //
 // Measured (MI355X, a call's time on the host, Python alone / here): layer norm
 // forward 10.3 / 5.9 us, backward 13.7 / 6.9, the loss of 16 positions 13.1 / 6.2,
-// AdamW of 12 tensors 9.8 / 4.4; 3.7 of each hand the launch over, 0.6 make a
+// AdamW of 12 tensors 9.8 / 4.4, a draw from one row 9.8 / SAMPLE; 3.7 of each hand the launch over, 0.6 make a
 // result tensor.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -21,6 +21,7 @@
 
 #include <algorithm>
 #include <cstdint>
+#include <limits>
 
 #include "hive_gpu.h"
 
@@ -34,6 +35,7 @@ decltype(&hg_layer_norm_backward_workspace) norm_workspace_;
 decltype(&hg_policy_value_loss) loss_;
 decltype(&hg_policy_value_loss_workspace) loss_workspace_;
 decltype(&hg_adamw_step) adamw_;
+decltype(&hg_sample_actions) sample_;
 
 // torch's: the current device, a device's current stream
 PyObject *current_device_, *current_stream_;
@@ -293,6 +295,64 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t count) {
     END_HANDLE_TH_ERRORS
 }
 
+// A setting of a draw: a tensor of a value a row, or a number for all.
+struct Setting {
+    const void* each = nullptr;
+    double all = 0.0;
+    // false: neither, or a number that is refused
+    bool find(PyObject* o, const Place& at, int64_t rows, at::ScalarType type, double most) {
+        if (const Tensor* t = tensor(o)) {
+            if (!is_vector(t, at, rows, type)) return false;
+            each = t->const_data_ptr();
+            return true;
+        }
+        all = PyFloat_AsDouble(o);
+        return !bad_number() && all >= 0.0 && all <= most;
+    }
+};
+
+// (logits, uniforms, num_actions, temperature, top_k, top_p, min_p) -> (actions, log_probs)
+PyObject* sample_actions(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    HANDLE_TH_ERRORS
+    if (count != 7 || !sample_) Py_RETURN_NONE;
+    Place at;
+    const Tensor *logits = tensor(a[0]), *uniforms = tensor(a[1]), *counts = tensor(a[2]);
+    if (!at.find(logits) || type_of(*logits) < 0 || logits->dim() != 2 || logits->size(1) == 0 ||
+        logits->size(1) > 1 << 20 || (logits->stride(1) != 1 && logits->size(1) > 1) || logits->numel() == 0)
+        return not_here();
+    const int64_t rows = logits->size(0), width = logits->size(1);
+    constexpr double any = std::numeric_limits<double>::infinity();
+    Setting t, p, min_p, k;
+    if (!is_vector(uniforms, at, rows, at::kFloat) || (a[2] != Py_None && !is_vector(counts, at, rows, at::kLong)) ||
+        !t.find(a[3], at, rows, at::kFloat, any) || !p.find(a[5], at, rows, at::kFloat, any) ||
+        !min_p.find(a[6], at, rows, at::kFloat, 1.0) || (!tensor(a[4]) && !PyLong_Check(a[4])) ||
+        !k.find(a[4], at, rows, at::kLong, 0x1p62))
+        return not_here();
+    Tensor actions = at::empty({rows}, logits->options().dtype(at::kLong));
+    Tensor log_probs = at::empty({rows}, logits->options().dtype(at::kFloat));
+    const int e = sample_(logits->const_data_ptr(), type_of(*logits), rows, width, logits->stride(0),
+                          a[2] == Py_None ? nullptr : (const int64_t*)counts->const_data_ptr(),
+                          (const float*)uniforms->const_data_ptr(), (const float*)t.each, t.all, (const int64_t*)k.each,
+                          (int64_t)k.all, (const float*)p.each, p.all, (const float*)min_p.each, min_p.all,
+                          (int64_t*)actions.mutable_data_ptr(), (float*)log_probs.mutable_data_ptr(), at.stream);
+    if (e) return failed("sample_actions", e);
+    PyObject* both = PyTuple_New(2);
+    if (!both) return nullptr;
+    PyTuple_SET_ITEM(both, 0, wrap(std::move(actions)));
+    PyTuple_SET_ITEM(both, 1, wrap(std::move(log_probs)));
+    return both;
+    END_HANDLE_TH_ERRORS
+}
+
+// (the address of libhive_gpu.so's hg_sample_actions), after bind
+PyObject* bind_network(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    if (count != 1) return PyErr_Format(PyExc_TypeError, "bind_network takes 1 address");
+    void* f = PyLong_AsVoidPtr(a[0]);
+    if (PyErr_Occurred()) return nullptr;
+    sample_ = (decltype(sample_))f;
+    Py_RETURN_NONE;
+}
+
 // (the addresses of libhive_gpu.so's functions, in the order below, torch's two)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
     if (count != 8) return PyErr_Format(PyExc_TypeError, "bind takes 6 addresses and 2 functions");
@@ -314,7 +374,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
 
 #define CALL(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {CALL(layer_norm_forward), CALL(layer_norm_backward), CALL(policy_value_loss),
-                         CALL(adamw_step),         CALL(bind),                {nullptr, nullptr, 0, nullptr}};
+                         CALL(adamw_step),         CALL(bind),                CALL(sample_actions),
+                         CALL(bind_network),       {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_train_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

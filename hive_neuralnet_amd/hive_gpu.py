@@ -238,6 +238,7 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
             fn.argtypes = args
             fn.restype = _c_i64
         training_ops.bind(lib)
+        network_ops.bind(lib)
         _lib = lib
         return lib
 

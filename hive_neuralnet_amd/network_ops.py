@@ -18,7 +18,7 @@ import ctypes
 
 import torch
 
-from .training_ops import (TYPES, _bytes, _check, _current_device, _float_tensor, _place, _raw_stream, _rows,
+from .training_ops import (TYPES, _bytes, _calls, _check, _current_device, _float_tensor, _place, _raw_stream, _rows,
                            _vector)
 
 _c_void_p = ctypes.c_void_p
@@ -53,6 +53,12 @@ SIGS_I64 = {
     "hg_gated_forward_workspace": [_c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_void_p, _c_void_p, _c_i64],
     "hg_gated_backward_workspace": [_c_int, _c_i64, _c_i64, _c_i64],
 }
+
+
+def bind(lib) -> None:
+    """Gives train_calls.cpp the library's function (training_ops.bind comes first)."""
+    if _calls is not None:
+        _calls.bind_network(ctypes.cast(lib.hg_sample_actions, _c_void_p).value)
 
 
 def _activation(activation) -> int:
@@ -338,6 +344,10 @@ def sample_actions(self, logits: torch.Tensor, uniforms: torch.Tensor, num_actio
     whole; a temperature of 0 takes the largest logit's first slot.  Each
     setting is a number, or a tensor of a value a row (float32; top_k int64; what
     lies past its range counts as its end)."""
+    if _calls is not None:
+        done = _calls.sample_actions(logits, uniforms, num_actions, temperature, top_k, top_p, min_p)
+        if done is not None:
+            return done
     dev = _float_tensor(logits, "logits")
     if logits.dim() != 2 or logits.shape[1] == 0:
         raise ValueError(f"logits must be [B, width], got {tuple(logits.shape)}")
