@@ -89,12 +89,14 @@ struct Operand {
     int rows, bytes;
 };
 
-template <typename T_, int kParts_, int kSteps_, int kM_, int kN_, int kWm_, int kWn_, int kStages_, int kBlocks_>
+template <typename T_, int kParts_, int kSteps_, int kM_, int kN_, int kWm_, int kWn_, int kStages_, int kBlocks_,
+          bool kAhead_ = true>
 struct Tile {
     using T = T_;
     using V = typename Fragment<T>::type;
     static constexpr int kParts = kParts_, kSteps = kSteps_, kM = kM_, kN = kN_, kWm = kWm_, kWn = kWn_, kStages = kStages_;
     static constexpr int kBlocks = kBlocks_;                          // that a compute unit holds
+    static constexpr bool kAhead = kAhead_;                           // operands are read a step ahead
     static constexpr int kThreads = 64 * kWm * kWn, kWavesEach = kBlocks * kThreads / 256;  // of a block; on a SIMD
     static constexpr int kRow = 64 * kParts * kSteps;                 // bytes of a slice's row
     static constexpr int kChunks = kRow / 16;
@@ -234,7 +236,7 @@ __device__ __forceinline__ void multiply(const Operand& a, int m0, const Operand
     const int l = lane & 15, g = lane >> 4;
     const int wave_m = wave / Tl::kWn * Tl::kFm, wave_n = wave % Tl::kWn * Tl::kFn;  // in pieces of 16
     const char* const lds_b = lds + Tl::kM * Tl::kRow;
-    V va[2][Tl::kParts][Tl::kFm], vb[2][Tl::kParts][Tl::kFn];
+    V va[Tl::kAhead ? 2 : 1][Tl::kParts][Tl::kFm], vb[Tl::kAhead ? 2 : 1][Tl::kParts][Tl::kFn];
     auto straight = [&](const char* from, int piece, int p, int step) {
         return *(const V*)(from + (piece * 16 + l) * Tl::kRow + Tl::place(l, (step * Tl::kParts + p) * 4 + g) * 16);
     };
@@ -267,6 +269,39 @@ __device__ __forceinline__ void multiply(const Operand& a, int m0, const Operand
             else va[half][p][i] = straight(from, wave_m + i, p, step);
         }
     };
+    if constexpr (!Tl::kAhead) {
+        static_assert(Tl::kSteps == 1, "");
+#pragma unroll
+        for (int n = 0; n < Tl::kStages - 1; n++) {
+            const From f = from(begin + n);
+#pragma unroll
+            for (int i = 0; i < Tl::kLoads; i++) fetch(i, f, n);
+        }
+        int stage = 0;
+        for (int k = begin; k < end; k++) {
+            wait_loads<(Tl::kStages - 2) * Tl::kLoads>();
+            const From f = from(k + Tl::kStages - 1);
+            const int free = stage == 0 ? Tl::kStages - 1 : stage - 1;
+#pragma unroll
+            for (int r = 0; r < Tl::kReads; r++) read(r, 0, stage, 0);
+            int n = 0;
+#pragma unroll
+            for (int sum = Tl::kParts - 1; sum >= 0; sum--)
+#pragma unroll
+                for (int p = 0; p <= sum; p++)
+#pragma unroll
+                    for (int i = 0; i < Tl::kFm; i++, n++) {
+#pragma unroll
+                        for (int j = 0; j < Tl::kFn; j++)
+                            s.acc[i][j] = mfma(vb[0][sum - p][j], va[0][p][i], s.acc[i][j]);
+#pragma unroll
+                        for (int i2 = 0; i2 < Tl::kLoads; i2++)
+                            if (i2 * Tl::kGroups / (2 * Tl::kLoads) == n) fetch(i2, f, free);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+            stage = stage + 1 == Tl::kStages ? 0 : stage + 1;
+        }
+    } else {
 #pragma unroll
     for (int n = 0; n < Tl::kStages; n++) {
         const From f = from(begin + n);
@@ -320,6 +355,7 @@ __device__ __forceinline__ void multiply(const Operand& a, int m0, const Operand
             multiply_step(k, zero{}, zero{});
             if (k + 1 < end) multiply_step(k + 1, zero{}, one{});
         }
+    }
     }
     wait_loads<0>();  // the LDS is free again
     if constexpr (kTurnedB) s.regroup();

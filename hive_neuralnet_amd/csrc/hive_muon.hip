@@ -557,7 +557,9 @@ template <int kKind> int product(Table& tab, hipStream_t st) {
         k_muon_product<kKind, Tl><<<(unsigned)grid, Tl::kThreads, 0, st>>>(tab);
         return launched();
     };
-    int e = launch(Tile<f16, 2, 1, 128, 128, 2, 2, 2, 2>{}, 192);
+    int e = -1;
+    if constexpr (kKind == kStep) e = launch(Tile<f16, 2, 1, 256, 256, 2, 4, 2, 1, false>{}, 192);
+    if (e < 0) e = launch(Tile<f16, 2, 1, 128, 128, 2, 2, 2, 2>{}, 192);
     if (e < 0) e = launch(Tile<f16, 2, 1, 64, 64, 2, 2, 4, 2>{}, 0);
     return e;
 }
