@@ -56,8 +56,7 @@ __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_gated_forward(
     Sums<Tl, 2> s;
     multiply<Tl, 2, false, false>(f.x, m0, f.wg, f.wu, n0, 1 << 30, 0, (f.x.bytes + Tl::kRow - 1) / Tl::kRow, lds, s);
     constexpr int share = Tl::kFn / 2, run = 4 * share;
-    const int n = n0 + s.col(), live = f.hidden - n;
-    if (live <= 0) return;
+    const int n = n0 + s.col(), live = f.hidden - n, first = n0 + s.first_col();
     float bg[run], bu[run];
 #pragma unroll
     for (int e = 0; e < run; e++) {
@@ -75,11 +74,11 @@ __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_gated_forward(
             u[e] = s.acc[i][share + e / 4][e % 4] + bu[e];
             h[e] = act_of<T, false>(f.act, g[e], unused) * u[e];
         }
-        const int64_t to = m * f.hidden + n;
-        store_run<T, run>((T*)f.h + to, live, h);
+        const int64_t to = m * f.hidden + first;
+        store_row<T, run>((T*)f.h + to, f.hidden - first, h);
         if (f.gate) {
-            store_run<float, run>(f.gate + to, live, g);
-            store_run<float, run>(f.up + to, live, u);
+            store_row<float, run>(f.gate + to, f.hidden - first, g);
+            store_row<float, run>(f.up + to, f.hidden - first, u);
         }
     }
 }
@@ -186,8 +185,7 @@ __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_product(Produc
     Sums<Tl, 1, true> s;
     multiply<Tl, 1, kTurnedA, true>(f.a, m0, f.b, f.b_second, n0, f.cut_k, begin, end, lds, s);
     constexpr int run = 4 * Tl::kFn;
-    const int n = n0 + s.col(), live = f.n - n;
-    if (live <= 0) return;
+    const int n = n0 + s.first_col(), live = f.n - n;
 #pragma unroll
     for (int i = 0; i < Tl::kFm; i++) {
         const int m = m0 + s.row() + i * 16;
@@ -196,11 +194,11 @@ __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_product(Produc
 #pragma unroll
         for (int e = 0; e < run; e++) v[e] = s.acc[i][e / 4][e % 4];
         if (f.part) {
-            store_run<float, run>(f.part + ((int64_t)blockIdx.y * f.m + m) * f.n + n, live, v);
+            store_row<float, run>(f.part + ((int64_t)blockIdx.y * f.m + m) * f.n + n, live, v);
         } else if (m < f.rows) {
-            store_run<T, run>((T*)f.first + (int64_t)m * f.n + n, live, v);
+            store_row<T, run>((T*)f.first + (int64_t)m * f.n + n, live, v);
         } else if (m >= f.cut && m - f.cut < f.rows) {
-            store_run<T, run>((T*)f.second + (int64_t)(m - f.cut) * f.n + n, live, v);
+            store_row<T, run>((T*)f.second + (int64_t)(m - f.cut) * f.n + n, live, v);
         }
     }
 }

@@ -127,11 +127,9 @@ template <typename Tl, int kHalves, bool kTurnedB = false> struct Sums {
     static constexpr int kShare = Tl::kFn / kHalves;
     f4 acc[Tl::kFm][Tl::kFn];
     __device__ __forceinline__ int row() const { return (int)(threadIdx.x >> 6) / Tl::kWn * Tl::kFm * 16 + (threadIdx.x & 15); }
-    __device__ __forceinline__ int col() const {
-        const int first = (int)(threadIdx.x >> 6) % Tl::kWn * kShare * 16, q = (int)(threadIdx.x & 63) / 16;
-        if constexpr (kTurnedB && Tl::kFn == 2) return first + (q & 1) * 16 + (q >> 1) * 8;
-        return first + q * 4 * kShare;
-    }
+    // of the wave's part, and of the lane's columns
+    __device__ __forceinline__ int first_col() const { return (int)(threadIdx.x >> 6) % Tl::kWn * kShare * 16; }
+    __device__ __forceinline__ int col() const { return first_col() + (int)(threadIdx.x & 63) / 16 * 4 * kShare; }
     // row r of a tile of B: its column of C, and which half it is of
     static __device__ __forceinline__ int column(int r) {
         return r / (Tl::kFn * 16) * kShare * 16 + r % 16 / 4 * 4 * kShare + r / 16 % kShare * 4 + r % 4;
@@ -149,6 +147,11 @@ template <typename Tl, int kHalves, bool kTurnedB = false> struct Sums {
                 for (int j = 0; j < Tl::kFn; j++) v[j] = acc[i][j][e];
 #pragma unroll
                 for (int j = 0; j < Tl::kFn; j += 2) {
+                    if constexpr (Tl::kFn == 2) {
+                        const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[0]), __float_as_uint(v[1]), false, false);
+                        v[0] = __uint_as_float(p[0]);
+                        v[1] = __uint_as_float(p[1]);
+                    }
                     const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[j]), __float_as_uint(v[j + 1]), false, false);
                     v[j] = __uint_as_float(p[0]);
                     v[j + 1] = __uint_as_float(p[1]);
@@ -361,12 +364,70 @@ __device__ __forceinline__ void multiply(const Operand& a, int m0, const Operand
     if constexpr (kTurnedB) s.regroup();
 }
 
-// the first `live` of n values to p, 16 bytes at a time
-template <typename T, int n> __device__ __forceinline__ void store_run(T* p, int live, const float (&v)[n]) {
-    constexpr int each = n < Vector<T>::n ? n : Vector<T>::n;
-#pragma unroll
-    for (int i = 0; i < n; i += each) store_some<T, each>(p + i, live - i, v + i);
+// words a and b of the four lanes that share a row changed round: where lane q held pieces 2 q and 2 q + 1 of eight, it holds
+// pieces q and 4 + q
+__device__ __forceinline__ void spread(uint32_t& a, uint32_t& b) {
+    const auto p = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    const auto q = __builtin_amdgcn_permlane32_swap(p[0], p[1], false, false);
+    a = q[0];
+    b = q[1];
 }
+// The n values of each of the four lanes that share a row of C to that row: lane q's are those of columns n q .. n q + n - 1,
+// `p` the row's place of the first of all, `live` what there are of it (the same for the four).  Pieces of 16 bytes change
+// lanes first, so that a store writes 64 bytes that follow each other (8,192 rows of gate and up, 8,192 wide, with their
+// product: 190 us where it wrote 16 of every 32, FIGURE so).
+template <typename T, int n> __device__ __forceinline__ void store_row(T* p, int live, const float (&v)[n]) {
+    const int q = (int)(threadIdx.x & 63) / 16;
+    if constexpr (n < Vector<T>::n) {
+        store_some<T, n>(p + q * n, live - q * n, v);
+    } else {
+        constexpr int each = Vector<T>::n, pieces = n / each;
+        static_assert(n % each == 0 && (pieces == 1 || pieces == 2 || pieces == 4), "");
+        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+        typedef typename Vector<T>::type vec;
+        u4 w[pieces];
+#pragma unroll
+        for (int i = 0; i < pieces; i++) {
+            vec x;
+#pragma unroll
+            for (int e = 0; e < each; e++) x[e] = from_f32<T>(v[i * each + e]);
+            w[i] = __builtin_bit_cast(u4, x);
+        }
+        if constexpr (pieces >= 2)
+#pragma unroll
+            for (int i = 0; i < pieces; i += 2)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    uint32_t a = w[i][k], b = w[i + 1][k];
+                    spread(a, b);
+                    w[i][k] = a;
+                    w[i + 1][k] = b;
+                }
+        if constexpr (pieces == 4)  // lane q held pieces 4 q .. 4 q + 3; now the halves of w[0] and w[2], of w[1] and w[3]
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const auto h = __builtin_amdgcn_permlane32_swap(w[i][k], w[i + 2][k], false, false);
+                    w[i][k] = h[0];
+                    w[i + 2][k] = h[1];
+                }
+#pragma unroll
+        for (int i = 0; i < pieces; i++) {
+            const int piece = q + 4 * (pieces == 4 ? (i & 1) * 2 + i / 2 : i);
+            const vec x = __builtin_bit_cast(vec, w[i]);
+            T* to = p + piece * each;
+            const int left = live - piece * each;
+            if (left >= each) {
+                *(vec*)to = x;
+            } else {
+#pragma unroll
+                for (int e = 0; e < each; e++)
+                    if (e < left) to[e] = x[e];
+            }
+        }
+        }
+    }
 
 // block t of `all` in an order that keeps blocks that run beside each other near each other: chiplet x has the blocks x, x + 8,
 // ..., and takes a range of its own of the work

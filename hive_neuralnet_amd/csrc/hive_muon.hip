@@ -264,27 +264,28 @@ __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_muon_product(T
     const int wide = kKind == kStep ? o.l : o.s;              // columns of the result
     const int64_t row = (kKind == kStep ? o.lb : o.sb) / 2;   // elements of its packed rows
     const int first = n0 + s.col();
+    const int across = (int)(threadIdx.x & 63) / 16;  // the lane's place among the four that share a row
     const bool mirrored = at.n > at.m;  // the tile's mirror image is stored, too: no tile computes it
 #pragma unroll
     for (int i = 0; i < Tl::kFm; i++) {
         const int m = m0 + s.row() + i * 16;
-        if (m >= up_to(o.s, 32)) continue;
         const bool there = m < o.s;
+        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+        u4 parts[2][run / 8];  // of 8 columns each
 #pragma unroll
         for (int c = 0; c < run; c += 8) {
             const int n = first + c, live = wide - n;
-            if (n >= up_to(wide, 32)) continue;
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = s.acc[i][(c + e) / 4][e % 4] * (1.0f / kScale);
             if (kKind == kPoly) {
                 float g[8] = {};
-                if (there) load_parts((const f16*)(held + o.a) + m * row, n, g);
+                if (there && live > 0) load_parts((const f16*)(held + o.a) + m * row, n, g);
 #pragma unroll
                 for (int e = 0; e < 8; e++) v[e] = fmaf(tab.c, v[e], tab.b * g[e]) + (n + e == m ? tab.a * kScale : 0.0f);
             }
             if (kKind == kStep && tab.last) {
-                if (!there) continue;
+                if (!there || live <= 0) continue;
 #pragma unroll
                 for (int e = 0; e < 8; e++) v[e] *= 1.0f / kScale;
                 // a turned matrix: column n of the result is row n of X's
@@ -292,13 +293,32 @@ __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_muon_product(T
                 else store_result<false>(x, tab, matrix * x.out_step + (int64_t)m * x.cols + n, 1, live, v);
                 continue;
             }
-            if (there) store_parts(to + m * row, n, v);
+            h8 hi, lo;
+            split_parts(v, hi, lo);
+            parts[0][c / 8] = __builtin_bit_cast(u4, hi);
+            parts[1][c / 8] = __builtin_bit_cast(u4, lo);
             if (kKind != kStep && mirrored) {
                 const int r = s.row() + i * 16, at_c = Tl::template turned_place<Tl::kN / 8>(r, (s.col() + c) / 8);
-                h8 hi, lo;
-                split_parts(v, hi, lo);
                 *(h8*)(lds + (r * Tl::kN / 8 + at_c) * 16) = hi;
                 *(h8*)(lds + Tl::kM * Tl::kN * 2 + (r * Tl::kN / 8 + at_c) * 16) = lo;
+            }
+        }
+        if (kKind == kStep && tab.last) continue;
+        // 16 columns a lane: the four lanes' pieces change round, so that a store writes the 64 bytes of a part of 32 columns
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+            if constexpr (run == 16)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    uint32_t a = parts[p][0][k], b = parts[p][1][k];
+                    spread(a, b);
+                    parts[p][0][k] = a;
+                    parts[p][1][k] = b;
+                }
+#pragma unroll
+            for (int k = 0; k < run / 8; k++) {
+                const int group = n0 + s.first_col() + k * 32;  // its first column
+                if (there && group < wide) *(u4*)(to + m * row + part_place<2>(group, p) + across * 8) = parts[p][k];
             }
         }
     }
