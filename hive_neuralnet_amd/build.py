@@ -22,7 +22,7 @@ ROOT = os.path.dirname(PKG)
 LIB = os.path.join(PKG, "libhive_gpu.so")
 SOURCES = [os.path.join(PKG, "csrc", n) for n in (
     "hive_engine.hip", "hive_mcts.hip", "hive_fnn.hip", "hive_probe.hip", "hive_norm.hip", "hive_loss.hip",
-    "hive_adamw.hip")]
+    "hive_adamw.hip", "hive_gated.hip", "hive_muon.hip", "hive_sample.hip")]
 CALLS = os.path.join(PKG, "_train_calls.so")
 CALLS_SOURCE = os.path.join(PKG, "csrc", "train_calls.cpp")
 ARCH = os.environ.get("HIVE_GPU_ARCH", "gfx950")
