@@ -66,10 +66,12 @@ __device__ __forceinline__ i4 buffer(const void* p) {
     return d;
 }
 
-// 16 bytes a lane from the buffer at offset + step into LDS at lds + 16 * lane.  Nothing waits for it: wait_all() does.
+// 16 bytes a lane from the buffer at offset + step into LDS at lds + 16 * lane.  Nothing waits for it: wait_loads() does.  The
+// instruction reads m0 one wait state after its write, and scalar registers five after a write by a lane read at the
+// earliest, which the compiler does not see to in a block of its own.
 __device__ __forceinline__ void load_to_lds(i4 from, uint32_t offset, uint32_t step, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(offset), "s"(from),
-                 "s"(step)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(offset),
+                 "s"(from), "s"(step)
                  : "memory");
 }
 // all but this wave's newest `kNewer` loads have landed and its LDS reads are done, and so it is for the block's other waves
@@ -375,7 +377,7 @@ __device__ __forceinline__ void spread(uint32_t& a, uint32_t& b) {
 // The n values of each of the four lanes that share a row of C to that row: lane q's are those of columns n q .. n q + n - 1,
 // `p` the row's place of the first of all, `live` what there are of it (the same for the four).  Pieces of 16 bytes change
 // lanes first, so that a store writes 64 bytes that follow each other (8,192 rows of gate and up, 8,192 wide, with their
-// product: 190 us where it wrote 16 of every 32, FIGURE so).
+// product: 190 us where it wrote 16 of every 32, 182 so).
 template <typename T, int n> __device__ __forceinline__ void store_row(T* p, int live, const float (&v)[n]) {
     const int q = (int)(threadIdx.x & 63) / 16;
     if constexpr (n < Vector<T>::n) {
