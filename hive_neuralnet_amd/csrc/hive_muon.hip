@@ -700,16 +700,17 @@ int hg_muon_step(const hg_muon_matrix* matrices, int64_t count, int param_type, 
             (uintptr_t)matrices[i].momentum % 4)
             return (int)hipErrorInvalidValue;
     if (count > 0 && (!workspace || (uintptr_t)workspace % 256)) return (int)hipErrorInvalidValue;
-    for (int64_t i = 0; i < count;) {
+    // the same kMatrices matrices a launch as the workspace is sized for, whichever of them have a gradient
+    for (int64_t i = 0; i < count; i += kMatrices) {
         Table tab{};
         char* held = (char*)workspace;
-        for (; i < count && tab.n < kMatrices; i++) {
-            const hg_muon_matrix& m = matrices[i];
+        for (int64_t k = i; k < std::min(count, i + kMatrices); k++) {
+            const hg_muon_matrix& m = matrices[k];
             if (!m.grad) continue;
             tab.t[tab.n++] = {m.grad, m.momentum, m.param, held, m.cols, 0, 0, (float)(lr * m.scale), (int)m.rows, (int)m.cols, 1, 0};
             held += layout((int)m.rows, (int)m.cols).all;
         }
-        if (tab.n == 0) break;
+        if (tab.n == 0) continue;
         tab.g_type = grad_type;
         tab.out_type = param_type;
         tab.update = 1;

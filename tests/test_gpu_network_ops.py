@@ -10,6 +10,7 @@ one, each taken as off by a unit in the last place (they may cut instead of
 rounding): (parts K / 16 + 80) u sum |terms|.  16-bit products are exact in 32
 bits.  What is rounded to 16 bits between (the gradients of gate and up) is off by half
 a unit of its type."""
+import ctypes
 import math
 
 import pytest
@@ -533,6 +534,32 @@ def test_muon_refusals(ext):
                       ([g.long(), g.long()], {}), ([g, g], dict(coefficients=(1.0,)))):
         with pytest.raises(ValueError):
             plan.step(grads, **kw)
+def test_muon_step_workspace_with_gradients_left_out(ext):
+    """Whichever matrices have a gradient, a step stays within its workspace: the first twelve have none, and as many as a
+    launch takes of large ones follow."""
+    shapes = [(10, 12)] * 12 + [(140, 190)] * 24 + [(12, 10)] * 12
+    params = [_randn(s, i) for i, s in enumerate(shapes)]
+    grads = [None if i < 12 else _randn(s, 90 + i) for i, s in enumerate(shapes)]
+    plan = ext.prepare_muon(params)
+    need = ext._lib.hg_muon_step_workspace(plan._table, len(shapes))
+    assert need == ext._lib.hg_muon_step_workspace(plan._table, 24)  # twelve large ones and twelve small ones
+    ws = torch.full((need + (1 << 24),), 0x5A, dtype=torch.uint8, device="cuda")
+    for t, g in zip(plan._table, grads):
+        t.grad = None if g is None else g.data_ptr()
+    before = [p.clone() for p in params]
+    coefficients = (ctypes.c_float * 3)(3.4445, -4.7750, 2.0315)
+    assert ext._lib.hg_muon_step(plan._table, len(shapes), 0, 0, 0.02, 0.95, 1, 0.0, 5, coefficients, 1, 1e-7, ws.data_ptr(),
+                                 torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert bool((ws[need:] == 0x5A).all())
+    for i, (p, g, b) in enumerate(zip(params, grads, before)):
+        if g is None:
+            assert torch.equal(p, b)
+        else:
+            want, _, error = _muon_reference(b, g, torch.zeros_like(b), 0.02, 0.95, True, 0.0, "spectral")
+            assert float((p.double() - want).norm()) <= error * 1.1 + 5 * U * float(want.norm()) + 4 * U * 0.02 * 40
+
+
     assert all(torch.equal(a, b) for a, b in zip([p, q, *plan.momentum], before))
     plan.step([g, g])  # one gradient for two parameters
     plan.step([None, None])
