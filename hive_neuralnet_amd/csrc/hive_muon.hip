@@ -27,7 +27,8 @@ namespace {
 using namespace hm;
 
 constexpr int kMatrices = 24;        // of a launch: their table is a kernel argument
-constexpr float kScale = 8192.0f;    // of every held matrix
+constexpr float kScale = 8192.0f;    // of X and A as they are held: entries up to 7.9
+constexpr float kScaleP = 1024.0f;   // of P, which has a on its diagonal: up to 63
 constexpr int kSumBlocks = 64;       // of a matrix's sum of squares
 constexpr int kTriples = 16;         // coefficients that a launch of the whole iteration takes
 constexpr int64_t kMaxSide = 1 << 17;
@@ -277,12 +278,13 @@ __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_muon_product(T
             const int n = first + c, live = wide - n;
             float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = s.acc[i][(c + e) / 4][e % 4] * (1.0f / kScale);
+            for (int e = 0; e < 8; e++) v[e] = s.acc[i][(c + e) / 4][e % 4] * (1.0f / (kKind == kStep ? kScaleP : kScale));
             if (kKind == kPoly) {
                 float g[8] = {};
                 if (there && live > 0) load_parts((const f16*)(held + o.a) + m * row, n, g);
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[e] = fmaf(tab.c, v[e], tab.b * g[e]) + (n + e == m ? tab.a * kScale : 0.0f);
+                for (int e = 0; e < 8; e++)
+                    v[e] = fmaf(tab.c, v[e], tab.b * g[e]) * (kScaleP / kScale) + (n + e == m ? tab.a * kScaleP : 0.0f);
             }
             if (kKind == kStep && tab.last) {
                 if (!there || live <= 0) continue;
@@ -371,12 +373,11 @@ __global__ void __launch_bounds__(1024) k_muon_small(Table tab) {
     // i / cols = the high word of i times it, rounded up: exact for i below 2^14 and cols up to 2^8
     const uint32_t inverse = 0xFFFFFFFFu / (uint32_t)cols + 1;
     const G* from = (const G*)x.g + matrix * x.g_step;
-    const int g_row = (int)x.g_row;
     auto row_of = [&](int i) { return cols == 1 ? i : (int)__umulhi((uint32_t)i, inverse); };
 #pragma unroll
     for (int k = 0; k < kEach; k++) {  // all loads under way before the first value is used
         const int i = k * 1024 + tid, r = row_of(i);
-        u[k] = i < n ? to_f32<G>(from[(int64_t)r * g_row + i - r * cols]) : 0.0f;
+        u[k] = i < n ? to_f32<G>(from[r * x.g_row + i - r * cols]) : 0.0f;
     }
 #pragma unroll
     for (int k = 0; k < kEach; k++) {
@@ -460,7 +461,7 @@ __global__ void __launch_bounds__(1024) k_muon_small(Table tab) {
         for (int j = 0; j < kPieces; j++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float o = next[j][e] * (1.0f / kScale / kScale);
+                const float o = next[j][e] * (1.0f / kScaleP / kScale);
                 if (at[j][e] >= 0) out[at[j][e]] = from_f32<P>(tab.update ? fmaf(-x.rate, o, old[j][e] * tab.keep) : o);
             }
     };
@@ -487,7 +488,8 @@ __global__ void __launch_bounds__(1024) k_muon_small(Table tab) {
         }
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            v[e] = fmaf(abc[2], sum_p[e] * (1.0f / kScale), abc[1] * v[e]) + (pn * 16 + g * 4 + e == r ? abc[0] * kScale : 0.0f);
+            v[e] = fmaf(abc[2], sum_p[e] * (1.0f / kScale), abc[1] * v[e]) * (kScaleP / kScale) +
+                   (pn * 16 + g * 4 + e == r ? abc[0] * kScaleP : 0.0f);
         keep(lp, kRowA, r, pn * 16 + g * 4, v);
         __syncthreads();
         h8 p[kSmall / 32][2];
@@ -511,7 +513,7 @@ __global__ void __launch_bounds__(1024) k_muon_small(Table tab) {
 #pragma unroll
             for (int j = 0; j < kPieces; j++) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = next[j][e] * (1.0f / kScale);
+                for (int e = 0; e < 4; e++) v[e] = next[j][e] * (1.0f / kScaleP);
                 keep(lx, kRowX, r, (pn + 4 * j) * 16 + g * 4, v);
             }
             __syncthreads();
@@ -707,8 +709,9 @@ int hg_muon_step(const hg_muon_matrix* matrices, int64_t count, int param_type, 
         for (int64_t k = i; k < std::min(count, i + kMatrices); k++) {
             const hg_muon_matrix& m = matrices[k];
             if (!m.grad) continue;
-            tab.t[tab.n++] = {m.grad, m.momentum, m.param, held, m.cols, 0, 0, (float)(lr * m.scale), (int)m.rows, (int)m.cols, 1, 0};
-            held += layout((int)m.rows, (int)m.cols).all;
+            const int rows = (int)m.rows, cols = (int)m.cols;
+            tab.t[tab.n++] = {m.grad, m.momentum, m.param, held, m.cols, 0, 0, (float)(lr * m.scale), rows, cols, 1, 0};
+            held += layout(rows, cols).all;
         }
         if (tab.n == 0) continue;
         tab.g_type = grad_type;

@@ -188,7 +188,8 @@ def orthogonalize(self, u: torch.Tensor, steps: int = 5, coefficients=COEFFICIEN
     u float32 / float16 / bfloat16, its rows contiguous, rows and matrices
     evenly spaced; the result has its shape and type and is contiguous.  Matrices
     are held in 22 bits a value between the products, which are summed in
-    float32."""
+    float32; a, b and c may be such that X's entries stay below 7.9 in size and
+    those of a I + b A + c A A below 63."""
     dev = _float_tensor(u, "u")
     if u.dim() < 2 or u.shape[-1] == 0 or u.shape[-2] == 0:
         raise ValueError(f"u must be [..., rows, cols], got {tuple(u.shape)}")

@@ -443,6 +443,11 @@ def test_orthogonalize_refusals(ext):
         with pytest.raises(ValueError):
             call()
 
+    # a schedule whose first steps lift small singular values most: a is past X's own range
+    lifting = [(8.2, -23.0, 16.8), (4.1, -2.9, 0.55), (3.9, -2.85, 0.53), (2.0, -1.5, 0.5)]
+    _check_orthogonal(ext.orthogonalize(u, steps=4, coefficients=lifting), u, 4, lifting)
+    big = _randn((130, 400), 61)
+    _check_orthogonal(ext.orthogonalize(big, steps=4, coefficients=lifting), big, 4, lifting)
 
 def _muon_reference(p, g, m, lr, mu, nesterov, decay, scale, steps=5):
     g = g.double()
