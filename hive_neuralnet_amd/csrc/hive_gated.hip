@@ -21,21 +21,22 @@ template <typename T> __device__ __forceinline__ float sigmoid_of(float g) {
     if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g));
     return 1.0f / (1.0f + expf(-g));
 }
-// act(g) and its slope
+// act(g) and its slope, at infinite g as well: a unit whose bias is -inf is off.  The slope's own factor g is held to +-200,
+// past which what it multiplies is 0 in float32.
 template <typename T, bool kSlope> __device__ __forceinline__ float act_of(int act, float g, float& slope) {
+    const float held = __builtin_amdgcn_fmed3f(g, -200.0f, 200.0f);
     if (act == HG_GELU) {
         skipped();
         const float share = 0.5f * erfcf(-0.70710678f * g);  // of the tail itself: 1 + erf would cancel there
-        if (kSlope) slope = share + 0.39894228f * g * expf(-0.5f * g * g);
-        return g * share;
+        if (kSlope) slope = share + 0.39894228f * held * expf(-0.5f * held * held);
+        return g == -__builtin_inff() ? 0.0f : g * share;
     }
     const float share = sigmoid_of<T>(g);
     if (act == HG_SIGMOID) {
         if (kSlope) slope = share * (1.0f - share);
         return share;
     }
-    if (kSlope) slope = share * (1.0f + g * (1.0f - share));
-    // far below zero the product is of inf and 0 where g is -inf: 0, as silu's limit
+    if (kSlope) slope = share * (1.0f + held * (1.0f - share));
     return g == -__builtin_inff() ? 0.0f : g * share;
 }
 
@@ -244,7 +245,6 @@ k_join_parts(const float* __restrict__ part, int splits, int64_t m, int n, int r
 
 int launched() { return (int)hipGetLastError(); }
 
-int64_t esize(int type) { return type == HG_F32 ? 4 : 2; }
 int parts_of(int type) { return type == HG_F32 ? 3 : 1; }
 // whether the tiles can take rows as they are
 bool as_it_is(const void* p, int type, int64_t rows, int64_t cols, int64_t stride) {

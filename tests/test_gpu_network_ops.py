@@ -180,6 +180,53 @@ def test_gated_far_values(ext, t):
         _check_gated(ext, x, wg, wu, None, None, torch.ones((4, 9), device="cuda", dtype=t), act)
 
 
+@pytest.mark.parametrize("act", ["sigmoid", "silu", "gelu"])
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_gated_units_that_a_bias_turns_off(ext, t, act):
+    """A bias of -inf: the unit's output and all that comes back through it are 0."""
+    x, wg, wu, bg, bu, dh = _gated(50, 40, 36, t, 13)
+    bg[[3, 35]] = float("-inf")
+    h, gate, up = ext.gated_linear_forward(x, wg, wu, bg, bu, act)
+    assert torch.isfinite(h).all() and not h[:, [3, 35]].any() and torch.isneginf(gate[:, [3, 35]]).all()
+    got = ext.gated_linear_backward(dh, x, wg, wu, gate, up, act)
+    for g in got[1:]:
+        assert not g[[3, 35]].any()
+    off = dh.clone()
+    off[:, [3, 35]] = 0
+    bg[[3, 35]] = 0
+    _, gate, up = ext.gated_linear_forward(x, wg, wu, bg, bu, act)
+    for a, b in zip(got, ext.gated_linear_backward(off, x, wg, wu, gate, up, act)):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+
+
+def test_sample_top_k_of_any_size(ext):
+    x, u = _randn((4, 70), 3), torch.tensor([0.1, 0.4, 0.7, 0.999], device="cuda")
+    for a, b in zip(ext.sample_actions(x, u, top_k=2 ** 64), ext.sample_actions(x, u)):
+        assert torch.equal(a, b)
+
+
+def test_rows_more_than_31_bits_apart(ext):
+    """Offsets and strides of tensors of more than 2^31 values."""
+    apart = 2 ** 31 + 24
+    store = torch.zeros((2 * apart + 512,), dtype=F16, device="cuda")
+    for cols in (48, 200):
+        wide = store.as_strided((3, cols), (apart, 1), 0)
+        wide.copy_(_randn((3, cols), cols, 1.0, F16))
+        x = wide.contiguous()
+        assert torch.equal(ext.orthogonalize(wide), ext.orthogonalize(x))
+        assert torch.equal(ext.orthogonalize(store.as_strided((3, 2, cols // 2), (apart, cols // 2, 1))),
+                           ext.orthogonalize(x.view(3, 2, cols // 2)))
+        _, wg, wu, bg, bu, dh = _gated(3, cols, 40, F16, 7)
+        h, gate, up = ext.gated_linear_forward(wide, wg, wu, bg, bu)
+        again = ext.gated_linear_forward(x, wg, wu, bg, bu)
+        assert all(torch.equal(a, b) for a, b in zip((h, gate, up), again))
+        grads = [ext.gated_linear_backward(dh, v, wg, wu, gate, up) for v in (wide, x)]
+        assert all(torch.equal(a, b) for a, b in zip(*grads))
+        u = torch.tensor([0.1, 0.5, 0.9], device="cuda")
+        for a, b in zip(ext.sample_actions(wide, u, top_k=9), ext.sample_actions(x, u, top_k=9)):
+            assert torch.equal(a, b)
+
+
 def test_gated_float32_keeps_its_range(ext):
     """Values near the largest and the smallest floats: parts neither overflow nor vanish.  bfloat16's smallest step is
     2^-133, so the parts of a value hold it to 2^-134 (1e-38 has 7 of its bits left), which meets the other factor:
