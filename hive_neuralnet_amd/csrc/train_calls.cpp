@@ -12,7 +12,7 @@
 //
 // Measured (MI355X, a call's time on the host, Python alone / here): layer norm
 // forward 10.3 / 5.9 us, backward 13.7 / 6.9, the loss of 16 positions 13.1 / 6.2,
-// AdamW of 12 tensors 9.8 / 4.4, a draw from one row 9.8 / SAMPLE; 3.7 of each hand the launch over, 0.6 make a
+// AdamW of 12 tensors 9.8 / 4.4, a draw from one row 9.8 / 5.5; 3.7 of each hand the launch over, 0.6 make a
 // result tensor.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>

@@ -325,6 +325,8 @@ def _setting(value, name: str, B: int, dtype: torch.dtype, dev: int):
     """(address or None, number) of a setting: a tensor of one value a row, or a number for all."""
     if isinstance(value, torch.Tensor):
         return _vector(value, name, B, dtype, dev), 0
+    if dtype is torch.int64 and not isinstance(value, int) or not isinstance(value, (int, float)):
+        raise ValueError(f"{name} must be a number or a tensor of one a row, got {value!r}")
     return None, value
 
 
@@ -366,8 +368,9 @@ def sample_actions(self, logits: torch.Tensor, uniforms: torch.Tensor, num_actio
                          f"{p_all} and {m_all}")
     actions = logits.new_empty((B,), dtype=torch.int64)
     log_probs = logits.new_empty((B,), dtype=torch.float32)
-    _check(self._lib.hg_sample_actions(logits.data_ptr(), TYPES[logits.dtype], B, width, stride, n, u, t, t_all, k, k_all,
-                                       p, p_all, m, m_all, actions.data_ptr(), log_probs.data_ptr(), _raw_stream(dev)),
+    _check(self._lib.hg_sample_actions(logits.data_ptr(), TYPES[logits.dtype], B, width, stride, n, u, t, t_all, k,
+                                       min(k_all, width), p, p_all, m, m_all, actions.data_ptr(), log_probs.data_ptr(),
+                                       _raw_stream(dev)),
            "sample_actions")
     return actions, log_probs
 

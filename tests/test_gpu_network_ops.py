@@ -443,6 +443,11 @@ def test_orthogonalize_settings(ext):
     schedule = [(3.0, -3.2, 1.2), (1.875, -1.25, 0.375)]
     _check_orthogonal(ext.orthogonalize(u, steps=4, coefficients=schedule), u, 4, schedule)
     _check_orthogonal(ext.orthogonalize(u, eps=1.0), u, eps=1.0)
+    # a schedule whose first steps lift small singular values most: a is past X's own range
+    lifting = [(8.2, -23.0, 16.8), (4.1, -2.9, 0.55), (3.9, -2.85, 0.53), (2.0, -1.5, 0.5)]
+    _check_orthogonal(ext.orthogonalize(u, steps=4, coefficients=lifting), u, 4, lifting)
+    big = _randn((130, 400), 61)
+    _check_orthogonal(ext.orthogonalize(big, steps=4, coefficients=lifting), big, 4, lifting)
     quintic = (1.875, -1.25, 0.375)  # converges: the result is orthogonal
     q = ext.orthogonalize(u, steps=30, coefficients=quintic).double()
     assert float((q @ q.t() - torch.eye(48, device="cuda")).abs().max()) < 1e-5
@@ -490,11 +495,6 @@ def test_orthogonalize_refusals(ext):
         with pytest.raises(ValueError):
             call()
 
-    # a schedule whose first steps lift small singular values most: a is past X's own range
-    lifting = [(8.2, -23.0, 16.8), (4.1, -2.9, 0.55), (3.9, -2.85, 0.53), (2.0, -1.5, 0.5)]
-    _check_orthogonal(ext.orthogonalize(u, steps=4, coefficients=lifting), u, 4, lifting)
-    big = _randn((130, 400), 61)
-    _check_orthogonal(ext.orthogonalize(big, steps=4, coefficients=lifting), big, 4, lifting)
 
 def _muon_reference(p, g, m, lr, mu, nesterov, decay, scale, steps=5):
     g = g.double()
@@ -532,6 +532,32 @@ def test_muon_step(ext, pt, gt, scale):
             assert off <= error * 1.1 + (HALF_ULP[pt] + 4 * U) * float(want.norm()) + 4 * U * 0.05 * float(want.norm() + 8) + \
                 TINY[pt] * math.sqrt(want.numel()), (i, off, error)
             moms[i] = plan.momentum[i].clone()
+
+
+def test_muon_step_workspace_with_gradients_left_out(ext):
+    """Whichever matrices have a gradient, a step stays within its workspace: the first twelve have none, and as many as a
+    launch takes of large ones follow."""
+    shapes = [(10, 12)] * 12 + [(140, 190)] * 24 + [(12, 10)] * 12
+    params = [_randn(s, i) for i, s in enumerate(shapes)]
+    grads = [None if i < 12 else _randn(s, 90 + i) for i, s in enumerate(shapes)]
+    plan = ext.prepare_muon(params)
+    need = ext._lib.hg_muon_step_workspace(plan._table, len(shapes))
+    assert need == ext._lib.hg_muon_step_workspace(plan._table, 24)  # twelve large ones and twelve small ones
+    ws = torch.full((need + (1 << 24),), 0x5A, dtype=torch.uint8, device="cuda")
+    for t, g in zip(plan._table, grads):
+        t.grad = None if g is None else g.data_ptr()
+    before = [p.clone() for p in params]
+    coefficients = (ctypes.c_float * 3)(3.4445, -4.7750, 2.0315)
+    assert ext._lib.hg_muon_step(plan._table, len(shapes), 0, 0, 0.02, 0.95, 1, 0.0, 5, coefficients, 1, 1e-7, ws.data_ptr(),
+                                 torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert bool((ws[need:] == 0x5A).all())
+    for i, (p, g, b) in enumerate(zip(params, grads, before)):
+        if g is None:
+            assert torch.equal(p, b)
+        else:
+            want, _, error = _muon_reference(b, g, torch.zeros_like(b), 0.02, 0.95, True, 0.0, "spectral")
+            assert float((p.double() - want).norm()) <= error * 1.1 + 5 * U * float(want.norm()) + 4 * U * 0.02 * 40
 
 
 def test_muon_step_in_a_graph(ext):
@@ -586,32 +612,6 @@ def test_muon_refusals(ext):
                       ([g.long(), g.long()], {}), ([g, g], dict(coefficients=(1.0,)))):
         with pytest.raises(ValueError):
             plan.step(grads, **kw)
-def test_muon_step_workspace_with_gradients_left_out(ext):
-    """Whichever matrices have a gradient, a step stays within its workspace: the first twelve have none, and as many as a
-    launch takes of large ones follow."""
-    shapes = [(10, 12)] * 12 + [(140, 190)] * 24 + [(12, 10)] * 12
-    params = [_randn(s, i) for i, s in enumerate(shapes)]
-    grads = [None if i < 12 else _randn(s, 90 + i) for i, s in enumerate(shapes)]
-    plan = ext.prepare_muon(params)
-    need = ext._lib.hg_muon_step_workspace(plan._table, len(shapes))
-    assert need == ext._lib.hg_muon_step_workspace(plan._table, 24)  # twelve large ones and twelve small ones
-    ws = torch.full((need + (1 << 24),), 0x5A, dtype=torch.uint8, device="cuda")
-    for t, g in zip(plan._table, grads):
-        t.grad = None if g is None else g.data_ptr()
-    before = [p.clone() for p in params]
-    coefficients = (ctypes.c_float * 3)(3.4445, -4.7750, 2.0315)
-    assert ext._lib.hg_muon_step(plan._table, len(shapes), 0, 0, 0.02, 0.95, 1, 0.0, 5, coefficients, 1, 1e-7, ws.data_ptr(),
-                                 torch.cuda.current_stream().cuda_stream) == 0
-    torch.cuda.synchronize()
-    assert bool((ws[need:] == 0x5A).all())
-    for i, (p, g, b) in enumerate(zip(params, grads, before)):
-        if g is None:
-            assert torch.equal(p, b)
-        else:
-            want, _, error = _muon_reference(b, g, torch.zeros_like(b), 0.02, 0.95, True, 0.0, "spectral")
-            assert float((p.double() - want).norm()) <= error * 1.1 + 5 * U * float(want.norm()) + 4 * U * 0.02 * 40
-
-
     assert all(torch.equal(a, b) for a, b in zip([p, q, *plan.momentum], before))
     plan.step([g, g])  # one gradient for two parameters
     plan.step([None, None])
@@ -848,6 +848,7 @@ def test_sample_refusals(ext):
                  lambda: ext.sample_actions(x, u, top_p=-0.1), lambda: ext.sample_actions(x, u, min_p=1.5),
                  lambda: ext.sample_actions(x, u, temperature=float("nan")),
                  lambda: ext.sample_actions(x, u, temperature=u.double()),
+                 lambda: ext.sample_actions(x, u, top_k=2.5), lambda: ext.sample_actions(x, u, top_p=None),
                  lambda: ext.sample_actions(x, u, top_k=u), lambda: ext.sample_actions(x, u, top_p=u[:2])):
         with pytest.raises(ValueError):
             call()
