@@ -241,6 +241,296 @@ k_join_parts(const float* __restrict__ part, int splits, int64_t m, int n, int r
     if (i < all) store_some<T, 4>((of_first ? first : second) + r * n + c, live, v);
 }
 
+// ---- narrow blocks: up to 128 columns and 64 hidden units --------------------
+//
+// The weights' parts fit a compute unit's LDS and a tile spans the whole of a row, so each pass reads its rows once, as they
+// are, splits them in registers and writes its results: nothing is packed, and dgate and dup stay where they are used.  A
+// product's operands lie in fragments: 16 of its rows by 32 k of one part, 16 bytes a lane in the lanes' order.
+constexpr int kNarrowCols = 128, kNarrowHidden = 64, kNarrowThreads = 512, kNarrowBlocks = 256;
+
+struct Narrow {
+    const void *x, *wg, *wu, *bg, *bu, *dh;
+    void *h, *dx;
+    float *gate, *up, *part, *sums;
+    int64_t rows, x_stride, dh_stride;
+    int cols, hidden, act;
+};
+template <typename T> struct Split {
+    using P = std::conditional_t<sizeof(T) == 4, bf16, T>;
+    using V = typename Fragment<P>::type;
+    static constexpr int n = sizeof(T) == 4 ? 3 : 1;
+    V part[n];
+    __device__ __forceinline__ void set(const float (&v)[8]) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            P q[n];
+            split<P, n>(v[k], q);
+#pragma unroll
+            for (int p = 0; p < n; p++) part[p][k] = q[p];
+        }
+    }
+    // fragment `piece` of eight of k step `step`
+    static __device__ __forceinline__ V* place(V* held, int step, int p, int piece) { return held + ((step * n + p) * 8 + piece) * 64; }
+    __device__ __forceinline__ void put(V* held, int step, int piece, int lane) const {
+#pragma unroll
+        for (int p = 0; p < n; p++) place(held, step, p, piece)[lane] = part[p];
+    }
+};
+// acc[j] += the products of this lane's row of A with pieces 0..7 of B
+template <typename T> __device__ __forceinline__ void narrow_step(typename Split<T>::V* held, int step, const Split<T>& a, f4 (&acc)[8]) {
+    using S = Split<T>;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int sum = S::n - 1; sum >= 0; sum--)
+#pragma unroll
+        for (int p = 0; p <= sum; p++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) acc[j] = mfma(S::place(held, step, sum - p, j)[lane], a.part[p], acc[j]);
+}
+// piece j's row i, so that lane l's sums are 16 columns that follow each other of each half of the pieces
+__device__ __forceinline__ int narrow_column(int j, int i) { return j / 4 * 64 + i / 4 * 16 + j % 4 * 4 + i % 4; }
+
+template <typename T> __global__ void __launch_bounds__(kNarrowThreads, 2) k_narrow_forward(Narrow f) {
+    using S = Split<T>;
+    __shared__ __attribute__((aligned(16))) typename S::V held[4 * S::n * 8 * 64];
+    const int tid = threadIdx.x, l = tid & 15, q = (tid & 63) / 16, steps = (f.cols + 31) / 32;
+    const T* const x = (const T*)f.x;
+    const int64_t tiles = (f.rows + 15) / 16, stride = (int64_t)gridDim.x * 8;
+    int64_t t = (int64_t)blockIdx.x * 8 + tid / 64;
+    float v[4][8];
+    auto load = [&](int64_t tile) {
+        const int64_t r = tile * 16 + l;
+        if (r >= f.rows) return;
+#pragma unroll
+        for (int s = 0; s < 4; s++)
+            if (s < steps) load_some<T, 8>(x + r * f.x_stride + s * 32 + q * 8, f.cols - s * 32 - q * 8, v[s]);
+    };
+#pragma unroll
+    for (int s = 0; s < 4; s++)
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[s][k] = 0.0f;
+    load(t);
+    for (int i = tid; i < 128 * 4 * steps; i += kNarrowThreads) {
+        const int r = i / (4 * steps), c = i % (4 * steps) * 8, n = narrow_column(r / 16, r % 16), unit = n % 64;
+        float w[8] = {};
+        if (unit < f.hidden) load_some<T, 8>((const T*)(n < 64 ? f.wg : f.wu) + (int64_t)unit * f.cols + c, f.cols - c, w);
+        S a;
+        a.set(w);
+        a.put(held, c / 32, r / 16, c % 32 / 8 * 16 + r % 16);
+    }
+    float bg[16], bu[16];
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        const int n = q * 16 + e;
+        bg[e] = f.bg && n < f.hidden ? to_f32<T>(((const T*)f.bg)[n]) : 0.0f;
+        bu[e] = f.bu && n < f.hidden ? to_f32<T>(((const T*)f.bu)[n]) : 0.0f;
+    }
+    __syncthreads();
+    for (; t < tiles; t += stride) {
+        f4 acc[8];
+        S a[4];
+#pragma unroll
+        for (int j = 0; j < 8; j++) acc[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < 4; s++) a[s].set(v[s]);
+        load(t + stride);
+#pragma unroll
+        for (int s = 0; s < 4; s++)
+            if (s < steps) narrow_step<T>(held, s, a[s], acc);
+        const int64_t m = t * 16 + l;
+        if (m >= f.rows) continue;
+        float g[16], u[16], h[16], unused;
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            g[e] = acc[e / 4][e % 4] + bg[e];
+            u[e] = acc[4 + e / 4][e % 4] + bu[e];
+            h[e] = act_of<T, false>(f.act, g[e], unused) * u[e];
+        }
+        store_row<T, 16>((T*)f.h + m * f.hidden, f.hidden, h);
+        if (f.gate) {
+            store_row<float, 16>(f.gate + m * f.hidden, f.hidden, g);
+            store_row<float, 16>(f.up + m * f.hidden, f.hidden, u);
+        }
+    }
+}
+
+// dgate and dup of 8 values
+template <typename T>
+__device__ __forceinline__ void slopes_of(int act, const float (&dh)[8], const float (&g)[8], const float (&u)[8], float (&dg)[8],
+                                          float (&du)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        float slope;
+        const float a = act_of<T, true>(act, g[k], slope);
+        dg[k] = dh[k] * u[k] * slope;
+        du[k] = dh[k] * a;
+    }
+}
+
+template <typename T> __global__ void __launch_bounds__(kNarrowThreads, 2) k_narrow_dx(Narrow f) {
+    using S = Split<T>;
+    __shared__ __attribute__((aligned(16))) typename S::V held[4 * S::n * 8 * 64];
+    const int tid = threadIdx.x, l = tid & 15, q = (tid & 63) / 16;
+    const int64_t tiles = (f.rows + 15) / 16, stride = (int64_t)gridDim.x * 8;
+    int64_t t = (int64_t)blockIdx.x * 8 + tid / 64;
+    float d[2][8], g[2][8], u[2][8];
+    auto load = [&](int64_t tile) {
+        const int64_t r = tile * 16 + l;
+        if (r >= f.rows) return;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const int c = s * 32 + q * 8, live = f.hidden - c;
+            load_some<T, 8>((const T*)f.dh + r * f.dh_stride + c, live, d[s]);
+            load_some<float, 8>(f.gate + r * f.hidden + c, live, g[s]);
+            load_some<float, 8>(f.up + r * f.hidden + c, live, u[s]);
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < 2; s++)
+#pragma unroll
+        for (int k = 0; k < 8; k++) d[s][k] = g[s][k] = u[s][k] = 0.0f;
+    load(t);
+    // B's rows are x's columns, k the hidden units: gate's 64, then up's
+    for (int i = tid; i < 128 * 16; i += kNarrowThreads) {
+        const int n = i % 128, k = i / 128 * 8, unit = k % 64;
+        const T* from = (const T*)(k < 64 ? f.wg : f.wu) + (int64_t)unit * f.cols + n;
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[e] = n < f.cols && unit + e < f.hidden ? to_f32<T>(from[e * f.cols]) : 0.0f;
+        S a;
+        a.set(w);
+        a.put(held, k / 32, n / 64 * 4 + n % 16 / 4, k % 32 / 8 * 16 + n % 64 / 16 * 4 + n % 4);
+    }
+    __syncthreads();
+    for (; t < tiles; t += stride) {
+        f4 acc[8];
+        S a[4];
+#pragma unroll
+        for (int j = 0; j < 8; j++) acc[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            float dg[8], du[8];
+            slopes_of<T>(f.act, d[s], g[s], u[s], dg, du);
+            a[s].set(dg);
+            a[2 + s].set(du);
+        }
+        load(t + stride);
+#pragma unroll
+        for (int s = 0; s < 4; s++)
+            if (s % 2 * 32 < f.hidden) narrow_step<T>(held, s, a[s], acc);
+        const int64_t m = t * 16 + l;
+        if (m >= f.rows) continue;
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; e++) v[e] = acc[half * 4 + e / 4][e % 4];
+            store_row<T, 16>((T*)f.dx + m * f.cols + half * 64, f.cols - half * 64, v);
+        }
+    }
+}
+
+// The weights' gradients over the block's rows, part[block][gate's 64 units, then up's][cols], and the sums of dgate and dup,
+// sums[block][2][hidden]; either may be left out.  64 rows at a time: a wave brings 32 rows of 16 units and of 32 columns into
+// LDS, a lane 8 rows of one, and takes a piece of 64 x 32 of the result.
+template <typename T> __global__ void __launch_bounds__(kNarrowThreads, 2) k_narrow_dw(Narrow f) {
+    using S = Split<T>;
+    __shared__ __attribute__((aligned(16))) typename S::V held[2][2 * S::n * 8 * 64];
+    const int tid = threadIdx.x, lane = tid & 63, l = lane & 15, q = lane / 16, wave = tid / 64, piece = wave % 4, step = wave / 4;
+    const int unit = piece * 16 + l, col = piece * 32 + l;
+    float d[8], g[8], u[8], x[2][8], sum_g = 0.0f, sum_u = 0.0f;
+    auto load = [&](int64_t slab) {
+        const int64_t r0 = slab * 64 + step * 32 + q * 8;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int64_t r = r0 + e;
+            const bool in = r < f.rows && unit < f.hidden;
+            d[e] = in ? to_f32<T>(((const T*)f.dh)[r * f.dh_stride + unit]) : 0.0f;
+            g[e] = in ? f.gate[r * f.hidden + unit] : 0.0f;
+            u[e] = in ? f.up[r * f.hidden + unit] : 0.0f;
+            if (f.part)
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    x[i][e] = r < f.rows && col + 16 * i < f.cols ? to_f32<T>(((const T*)f.x)[r * f.x_stride + col + 16 * i]) : 0.0f;
+        }
+    };
+    f4 acc[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) acc[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int64_t slabs = (f.rows + 63) / 64;
+    load(blockIdx.x);
+    for (int64_t slab = blockIdx.x; slab < slabs; slab += gridDim.x) {
+        float dg[8], du[8];
+        slopes_of<T>(f.act, d, g, u, dg, du);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            sum_g += dg[e];
+            sum_u += du[e];
+        }
+        if (f.part) {
+            S a;
+            a.set(dg);
+            a.put(held[0], step, piece, lane);
+            a.set(du);
+            a.put(held[0], step, 4 + piece, lane);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                a.set(x[i]);
+                a.put(held[1], step, piece * 2 + i, lane);
+            }
+        }
+        load(slab + gridDim.x);
+        if (!f.part) continue;
+        __syncthreads();
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            typename S::V vb[S::n][2];
+#pragma unroll
+            for (int p = 0; p < S::n; p++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) vb[p][j] = S::place(held[1], s, p, piece * 2 + j)[lane];
+#pragma unroll
+            for (int p = S::n - 1; p >= 0; p--) {
+                typename S::V va[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) va[i] = S::place(held[0], s, p, step * 4 + i)[lane];
+#pragma unroll
+                for (int o = S::n - 1 - p; o >= 0; o--)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int j = 0; j < 2; j++) acc[i][j] = mfma(vb[o][j], va[i], acc[i][j]);
+            }
+        }
+        __syncthreads();
+    }
+    if (f.part)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int m = (step * 4 + i) * 16 + l, n = (piece * 2 + j) * 16 + q * 4;
+                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                store_some<float, 4>(f.part + ((int64_t)blockIdx.x * 128 + m) * f.cols + n, f.cols - n, v);
+            }
+    if (!f.sums) return;
+    float* const lds = (float*)held;  // its products are read
+    lds[tid] = sum_g;
+    lds[kNarrowThreads + tid] = sum_u;
+    __syncthreads();
+    if (tid < 128) {
+        const int w = tid / 64, n = tid % 64;
+        float all = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) all += lds[w * kNarrowThreads + (s * 4 + n / 16) * 64 + k * 16 + n % 16];
+        if (n < f.hidden) f.sums[((int64_t)blockIdx.x * 2 + w) * f.hidden + n] = all;
+    }
+}
+
 // ---- host -------------------------------------------------------------------
 
 int launched() { return (int)hipGetLastError(); }
@@ -337,9 +627,35 @@ template <typename T, typename F> int with_tile(int64_t m, int64_t n, int64_t k,
     return middle.time <= small.time ? f(Middle{}, middle.splits) : f(Small{}, small.splits);
 }
 
+bool is_narrow(int64_t cols, int64_t hidden) { return cols <= kNarrowCols && hidden <= kNarrowHidden; }
+
+template <typename T>
+int join_parts(const float* part, int64_t splits, int64_t m, int64_t n, int64_t rows, int64_t cut, void* first, void* second,
+               hipStream_t st) {
+    const int64_t all = rows * ((n + 3) / 4) * (second ? 2 : 1);
+    if (splits >= 8)
+        k_join_parts<T, 16><<<(unsigned)((all + 15) / 16), 256, 0, st>>>(part, (int)splits, m, (int)n, (int)rows, (int)cut,
+                                                                        (T*)first, (T*)second);
+    else
+        k_join_parts<T, 1><<<(unsigned)((all + 255) / 256), 256, 0, st>>>(part, (int)splits, m, (int)n, (int)rows, (int)cut,
+                                                                         (T*)first, (T*)second);
+    return launched();
+}
+template <typename T> int join_sums(const float* sums, int64_t blocks, int64_t hidden, void* dbg, void* dbu, hipStream_t st) {
+    k_join_sums<T><<<dim3((unsigned)((hidden + 63) / 64), 2), 1024, 0, st>>>(sums, blocks, (int)hidden, (T*)dbg, (T*)dbu);
+    return launched();
+}
+
 template <typename T>
 int forward(const void* x, int64_t rows, int64_t cols, int64_t x_stride, const void* wg, const void* wu, int64_t hidden,
             const void* bg, const void* bu, int act, void* h, float* gate, float* up, Arena& ws, hipStream_t st) {
+    if (is_narrow(cols, hidden)) {
+        if (!ws.p) return 0;
+        const Narrow f{x, wg, wu, bg, bu, nullptr, h, nullptr, gate, up, nullptr, nullptr, rows, x_stride, 0, (int)cols,
+                       (int)hidden, act};
+        k_narrow_forward<T><<<(unsigned)std::min<int64_t>((rows + 127) / 128, kNarrowBlocks), kNarrowThreads, 0, st>>>(f);
+        return launched();
+    }
     Forward f{};
     const void* const weights[2] = {wg, wu};
     Operand w[2];
@@ -395,14 +711,7 @@ int product(const Operand& a, const Operand& b, const Operand& b_second, int64_t
         k_product<T, Tl, kTurnedA><<<dim3((unsigned)tiles, (unsigned)splits), Tl::kThreads, 0, st>>>(f);
         int e = launched();
         if (!e && splits > 1) {
-            const int64_t all = rows * ((n + 3) / 4) * (second ? 2 : 1);
-            if (splits >= 8)
-                k_join_parts<T, 16><<<(unsigned)((all + 15) / 16), 256, 0, st>>>(f.part, (int)splits, m, (int)n, (int)rows,
-                                                                                (int)cut, (T*)first, (T*)second);
-            else
-                k_join_parts<T, 1><<<(unsigned)((all + 255) / 256), 256, 0, st>>>(f.part, (int)splits, m, (int)n, (int)rows,
-                                                                                 (int)cut, (T*)first, (T*)second);
-            e = launched();
+            e = join_parts<T>(f.part, splits, m, n, rows, cut, first, second, st);
         }
         return e;
     });
@@ -412,6 +721,25 @@ template <typename T>
 int backward(const void* dh, int64_t dh_stride, const void* x, int64_t rows, int64_t cols, int64_t x_stride,
              const void* wg, const void* wu, int64_t hidden, const float* gate, const float* up, int act, void* dx,
              void* dwg, void* dwu, void* dbg, void* dbu, Arena& ws, hipStream_t st) {
+    if (is_narrow(cols, hidden)) {
+        const int64_t blocks = std::min<int64_t>((rows + 63) / 64, kNarrowBlocks);
+        Narrow f{x, wg, wu, nullptr, nullptr, dh, nullptr, dx, (float*)gate, (float*)up, nullptr, nullptr, rows, x_stride,
+                 dh_stride, (int)cols, (int)hidden, act};
+        if (dwg) f.part = (float*)ws.take(blocks * 2 * kNarrowHidden * cols * 4);
+        if (dbg || dbu) f.sums = (float*)ws.take(blocks * 2 * hidden * 4);
+        if (!ws.p) return 0;
+        int e = 0;
+        if (dx) {
+            k_narrow_dx<T><<<(unsigned)std::min<int64_t>((rows + 127) / 128, kNarrowBlocks), kNarrowThreads, 0, st>>>(f);
+            e = launched();
+        }
+        if (!e && (f.part || f.sums)) {
+            k_narrow_dw<T><<<(unsigned)blocks, kNarrowThreads, 0, st>>>(f);
+            e = launched();
+        }
+        if (!e && f.part) e = join_parts<T>(f.part, blocks, 2 * kNarrowHidden, cols, hidden, kNarrowHidden, dwg, dwu, st);
+        return e || !f.sums ? e : join_sums<T>(f.sums, blocks, hidden, dbg, dbu, st);
+    }
     using P = std::conditional_t<sizeof(T) == 4, bf16, T>;
     constexpr int parts = sizeof(T) == 4 ? 3 : 1;
     const int64_t cut = up_to(hidden, 64), d_bytes = packed_bytes(2 * cut, parts);  // 64: whole slices of each half
@@ -425,10 +753,7 @@ int backward(const void* dh, int64_t dh_stride, const void* x, int64_t rows, int
         k_gated_slopes<T, P, parts><<<dim3((unsigned)blocks, (unsigned)((cut + across * 8 - 1) / (across * 8))), 256, 0, st>>>(
             (const T*)dh, dh_stride, gate, up, rows, (int)hidden, act, (P*)d, d_bytes / 2, (int)cut, across, each, sums);
         e = launched();
-        if (!e && biases) {
-            k_join_sums<T><<<dim3((unsigned)((hidden + 63) / 64), 2), 1024, 0, st>>>(sums, blocks, (int)hidden, (T*)dbg, (T*)dbu);
-            e = launched();
-        }
+        if (!e && biases) e = join_sums<T>(sums, blocks, hidden, dbg, dbu, st);
     }
     const Operand grads{d, d_bytes, (int)rows, (int)d_bytes};
     if (!e && dx) {
