@@ -66,11 +66,13 @@ __device__ __forceinline__ i4 buffer(const void* p) {
     return d;
 }
 
-// 16 bytes a lane from the buffer at offset + step into LDS at lds + 16 * lane.  Nothing waits for it: wait_loads() does.  The
-// instruction reads m0 one wait state after its write, and scalar registers five after a write by a lane read at the
-// earliest, which the compiler does not see to in a block of its own.
-__device__ __forceinline__ void load_to_lds(i4 from, uint32_t offset, uint32_t step, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(offset),
+// Scalar operands of load_to_lds: vector memory may read a scalar register five wait states after a lane's value was written
+// to it at the earliest, which the compiler does not see to for a block of its own.
+__device__ __forceinline__ void settle(i4& from, int& step) { asm("s_nop 4" : "+s"(from), "+s"(step)); }
+// 16 bytes a lane from the buffer at offset + step into LDS at lds + 16 * lane.  Nothing waits for it: wait_loads() does.
+// from and step are settled; m0 is read one wait state after its write.
+__device__ __forceinline__ void load_to_lds(i4 from, uint32_t offset, int step, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(offset),
                  "s"(from), "s"(step)
                  : "memory");
 }
@@ -215,9 +217,15 @@ __device__ __forceinline__ void multiply(const Operand& a, int m0, const Operand
         const int n_b = second ? n - cut : n;
         f.b0 = buffer((const char*)(second ? b1.p : b0.p) +
                       (kTurnedB ? (int64_t)n_b * deep * b0.stride + n0 * 2 * Tl::kParts : n0 * b0.stride));
-        f.b1 = kHalves == 2 ? buffer((const char*)b1.p + n0 * b1.stride) : f.b0;
         f.step_a = kTurnedA ? 0 : n * Tl::kRow;
         f.step_b = kTurnedB ? 0 : n * Tl::kRow;
+        settle(f.a, f.step_a);
+        settle(f.b0, f.step_b);
+        f.b1 = f.b0;
+        if constexpr (kHalves == 2) {
+            f.b1 = buffer((const char*)b1.p + n0 * b1.stride);
+            settle(f.b1, f.step_b);
+        }
         // a slice past the end is loaded, too, as zeros: a wait counts on it
         f.most_a = n >= end ? 0 : kTurnedA ? a.rows - n * deep : a.bytes - n * Tl::kRow;
         f.most_b = n >= end ? 0 : kTurnedB ? b0.rows - n_b * deep : b0.bytes - n * Tl::kRow;
