@@ -16,14 +16,15 @@ using namespace hm;
 constexpr int64_t kMaxRows = 1 << 20, kMaxCols = 1 << 19;
 constexpr int64_t kMaxArea = (int64_t)1 << 35;  // a launch has under 2^32 threads, 256 for a piece of 64 x 64
 
-// sigmoid(g): for 16-bit results the card's own exp2 and reciprocal, |g| 2^-24 off
-template <typename T> __device__ __forceinline__ float sigmoid_of(float g) {
-    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g));
-    return 1.0f / (1.0f + expf(-g));
+// sigmoid(g) by the card's own exp2 and reciprocal, (|g| + 4) 2^-24 of itself off: the rounding of gate's sum is of that
+// size.  (With expf and a division, 118,271 rows of 122 floats to 64 units took 48 us instead of 44 forward, 107 instead of
+// 102 backward.)
+__device__ __forceinline__ float sigmoid_of(float g) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g));
 }
 // act(g) and its slope, at infinite g as well: a unit whose bias is -inf is off.  The slope's own factor g is held to +-200,
 // past which what it multiplies is 0 in float32.
-template <typename T, bool kSlope> __device__ __forceinline__ float act_of(int act, float g, float& slope) {
+template <bool kSlope> __device__ __forceinline__ float act_of(int act, float g, float& slope) {
     const float held = __builtin_amdgcn_fmed3f(g, -200.0f, 200.0f);
     if (act == HG_GELU) {
         skipped();
@@ -31,7 +32,7 @@ template <typename T, bool kSlope> __device__ __forceinline__ float act_of(int a
         if (kSlope) slope = share + 0.39894228f * held * expf(-0.5f * held * held);
         return g == -__builtin_inff() ? 0.0f : g * share;
     }
-    const float share = sigmoid_of<T>(g);
+    const float share = sigmoid_of(g);
     if (act == HG_SIGMOID) {
         if (kSlope) slope = share * (1.0f - share);
         return share;
@@ -73,7 +74,7 @@ __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_gated_forward(
         for (int e = 0; e < run; e++) {
             g[e] = s.acc[i][e / 4][e % 4] + bg[e];
             u[e] = s.acc[i][share + e / 4][e % 4] + bu[e];
-            h[e] = act_of<T, false>(f.act, g[e], unused) * u[e];
+            h[e] = act_of<false>(f.act, g[e], unused) * u[e];
         }
         const int64_t to = m * f.hidden + first;
         store_row<T, run>((T*)f.h + to, f.hidden - first, h);
@@ -118,7 +119,7 @@ k_gated_slopes(const T* __restrict__ dh, int64_t dh_stride, const float* __restr
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             float slope;
-            const float a = act_of<T, true>(act, g[k], slope);
+            const float a = act_of<true>(act, g[k], slope);
             const float both[2] = {k < live ? v[k] * u[k] * slope : 0.0f, k < live ? v[k] * a : 0.0f};
 #pragma unroll
             for (int w = 0; w < 2; w++) {
@@ -241,94 +242,91 @@ k_join_parts(const float* __restrict__ part, int splits, int64_t m, int n, int r
     if (i < all) store_some<T, 4>((of_first ? first : second) + r * n + c, live, v);
 }
 
-// ---- narrow blocks: up to 128 columns and 64 hidden units --------------------
+// ---- float32 blocks of up to 128 columns and 64 hidden units -----------------
 //
 // The weights' parts fit a compute unit's LDS and a tile spans the whole of a row, so each pass reads its rows once, as they
-// are, splits them in registers and writes its results: nothing is packed, and dgate and dup stay where they are used.  A
-// product's operands lie in fragments: 16 of its rows by 32 k of one part, 16 bytes a lane in the lanes' order.
+// are, splits them in registers and writes its results: nothing is packed, and dgate and dup are held nowhere.  A product's
+// operands lie in fragments: 16 of its rows by 32 k of one part, 16 bytes a lane in the lanes' order.
 constexpr int kNarrowCols = 128, kNarrowHidden = 64, kNarrowThreads = 512, kNarrowBlocks = 256;
 
 struct Narrow {
-    const void *x, *wg, *wu, *bg, *bu, *dh;
-    void *h, *dx;
-    float *gate, *up, *part, *sums;
+    const float *x, *wg, *wu, *bg, *bu, *dh;
+    float *h, *dx, *gate, *up, *part, *sums;
     int64_t rows, x_stride, dh_stride;
     int cols, hidden, act;
 };
-template <typename T> struct Split {
-    using P = std::conditional_t<sizeof(T) == 4, bf16, T>;
-    using V = typename Fragment<P>::type;
-    static constexpr int n = sizeof(T) == 4 ? 3 : 1;
-    V part[n];
+struct Parts {
+    b8 part[3];
     __device__ __forceinline__ void set(const float (&v)[8]) {
 #pragma unroll
         for (int k = 0; k < 8; k++) {
-            P q[n];
-            split<P, n>(v[k], q);
+            bf16 q[3];
+            split<bf16, 3>(v[k], q);
 #pragma unroll
-            for (int p = 0; p < n; p++) part[p][k] = q[p];
+            for (int p = 0; p < 3; p++) part[p][k] = q[p];
         }
     }
     // fragment `piece` of eight of k step `step`
-    static __device__ __forceinline__ V* place(V* held, int step, int p, int piece) { return held + ((step * n + p) * 8 + piece) * 64; }
-    __device__ __forceinline__ void put(V* held, int step, int piece, int lane) const {
+    static __device__ __forceinline__ b8* place(b8* held, int step, int p, int piece) {
+        return held + ((step * 3 + p) * 8 + piece) * 64;
+    }
+    __device__ __forceinline__ void put(b8* held, int step, int piece) const {
 #pragma unroll
-        for (int p = 0; p < n; p++) place(held, step, p, piece)[lane] = part[p];
+        for (int p = 0; p < 3; p++) place(held, step, p, piece)[threadIdx.x & 63] = part[p];
     }
 };
+// 8 values of row r from column c on, zeros past its `cols`
+__device__ __forceinline__ void load_row(const float* p, int64_t r, int64_t stride, int c, int cols, float (&v)[8]) {
+    load_some<float, 8>(p + r * stride + c, cols - c, v);
+}
 // acc[j] += the products of this lane's row of A with pieces 0..7 of B
-template <typename T> __device__ __forceinline__ void narrow_step(typename Split<T>::V* held, int step, const Split<T>& a, f4 (&acc)[8]) {
-    using S = Split<T>;
-    const int lane = threadIdx.x & 63;
+__device__ __forceinline__ void narrow_step(b8* held, int step, const Parts& a, f4 (&acc)[8]) {
 #pragma unroll
-    for (int sum = S::n - 1; sum >= 0; sum--)
+    for (int sum = 2; sum >= 0; sum--)
 #pragma unroll
         for (int p = 0; p <= sum; p++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) acc[j] = mfma(S::place(held, step, sum - p, j)[lane], a.part[p], acc[j]);
+            for (int j = 0; j < 8; j++) acc[j] = mfma(Parts::place(held, step, sum - p, j)[threadIdx.x & 63], a.part[p], acc[j]);
 }
-// piece j's row i, so that lane l's sums are 16 columns that follow each other of each half of the pieces
-__device__ __forceinline__ int narrow_column(int j, int i) { return j / 4 * 64 + i / 4 * 16 + j % 4 * 4 + i % 4; }
 
-template <typename T> __global__ void __launch_bounds__(kNarrowThreads, 2) k_narrow_forward(Narrow f) {
-    using S = Split<T>;
-    __shared__ __attribute__((aligned(16))) typename S::V held[4 * S::n * 8 * 64];
-    const int tid = threadIdx.x, l = tid & 15, q = (tid & 63) / 16, steps = (f.cols + 31) / 32;
-    const T* const x = (const T*)f.x;
+// a wave takes 16 rows at a time and reads its next ones meanwhile
+__global__ void __launch_bounds__(kNarrowThreads, 2) k_narrow_forward(Narrow f) {
+    __shared__ __attribute__((aligned(16))) b8 held[4 * 3 * 8 * 64];
+    const int tid = threadIdx.x, l = tid & 15, q = (tid & 63) / 16, wave = tid / 64, steps = (f.cols + 31) / 32;
     const int64_t tiles = (f.rows + 15) / 16, stride = (int64_t)gridDim.x * 8;
-    int64_t t = (int64_t)blockIdx.x * 8 + tid / 64;
-    float v[4][8];
+    int64_t t = (int64_t)blockIdx.x * 8 + wave;
+    float v[4][8] = {};
     auto load = [&](int64_t tile) {
         const int64_t r = tile * 16 + l;
         if (r >= f.rows) return;
 #pragma unroll
         for (int s = 0; s < 4; s++)
-            if (s < steps) load_some<T, 8>(x + r * f.x_stride + s * 32 + q * 8, f.cols - s * 32 - q * 8, v[s]);
+            if (s < steps) load_row(f.x, r, f.x_stride, s * 32 + q * 8, f.cols, v[s]);
     };
+    load(t);
+    // B's rows: gate's 64 units, then up's
+    float w[4][8] = {};
 #pragma unroll
     for (int s = 0; s < 4; s++)
-#pragma unroll
-        for (int k = 0; k < 8; k++) v[s][k] = 0.0f;
-    load(t);
-    for (int i = tid; i < 128 * 4 * steps; i += kNarrowThreads) {
-        const int r = i / (4 * steps), c = i % (4 * steps) * 8, n = narrow_column(r / 16, r % 16), unit = n % 64;
-        float w[8] = {};
-        if (unit < f.hidden) load_some<T, 8>((const T*)(n < 64 ? f.wg : f.wu) + (int64_t)unit * f.cols + c, f.cols - c, w);
-        S a;
-        a.set(w);
-        a.put(held, c / 32, r / 16, c % 32 / 8 * 16 + r % 16);
-    }
+        if (s < steps)
+            load_row(wave < 4 ? f.wg : f.wu, min(wave % 4 * 16 + l, f.hidden - 1), f.cols, s * 32 + q * 8, f.cols, w[s]);
     float bg[16], bu[16];
 #pragma unroll
     for (int e = 0; e < 16; e++) {
-        const int n = q * 16 + e;
-        bg[e] = f.bg && n < f.hidden ? to_f32<T>(((const T*)f.bg)[n]) : 0.0f;
-        bu[e] = f.bu && n < f.hidden ? to_f32<T>(((const T*)f.bu)[n]) : 0.0f;
+        const int n = min(e / 4 * 16 + q * 4 + e % 4, f.hidden - 1);
+        bg[e] = f.bg ? f.bg[n] : 0.0f;
+        bu[e] = f.bu ? f.bu[n] : 0.0f;
+    }
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+        Parts a;
+        a.set(w[s]);
+        a.put(held, s, wave);
     }
     __syncthreads();
     for (; t < tiles; t += stride) {
         f4 acc[8];
-        S a[4];
+        Parts a[4];
 #pragma unroll
         for (int j = 0; j < 8; j++) acc[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -336,123 +334,130 @@ template <typename T> __global__ void __launch_bounds__(kNarrowThreads, 2) k_nar
         load(t + stride);
 #pragma unroll
         for (int s = 0; s < 4; s++)
-            if (s < steps) narrow_step<T>(held, s, a[s], acc);
+            if (s < steps) narrow_step(held, s, a[s], acc);
         const int64_t m = t * 16 + l;
         if (m >= f.rows) continue;
-        float g[16], u[16], h[16], unused;
+        const int64_t to = m * f.hidden + q * 4;
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            g[e] = acc[e / 4][e % 4] + bg[e];
-            u[e] = acc[4 + e / 4][e % 4] + bu[e];
-            h[e] = act_of<T, false>(f.act, g[e], unused) * u[e];
-        }
-        store_row<T, 16>((T*)f.h + m * f.hidden, f.hidden, h);
-        if (f.gate) {
-            store_row<float, 16>(f.gate + m * f.hidden, f.hidden, g);
-            store_row<float, 16>(f.up + m * f.hidden, f.hidden, u);
+        for (int j = 0; j < 4; j++) {
+            const int live = f.hidden - j * 16 - q * 4;
+            float g[4], u[4], h[4], unused;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                g[e] = acc[j][e] + bg[j * 4 + e];
+                u[e] = acc[4 + j][e] + bu[j * 4 + e];
+                h[e] = act_of<false>(f.act, g[e], unused) * u[e];
+            }
+            store_some<float, 4>(f.h + to + j * 16, live, h);
+            if (f.gate) {
+                store_some<float, 4>(f.gate + to + j * 16, live, g);
+                store_some<float, 4>(f.up + to + j * 16, live, u);
+            }
         }
     }
 }
 
 // dgate and dup of 8 values
-template <typename T>
-__device__ __forceinline__ void slopes_of(int act, const float (&dh)[8], const float (&g)[8], const float (&u)[8], float (&dg)[8],
-                                          float (&du)[8]) {
+__device__ __forceinline__ void slopes_of(int act, const float (&dh)[8], const float (&g)[8], const float (&u)[8],
+                                          float (&dg)[8], float (&du)[8]) {
 #pragma unroll
     for (int k = 0; k < 8; k++) {
         float slope;
-        const float a = act_of<T, true>(act, g[k], slope);
+        const float a = act_of<true>(act, g[k], slope);
         dg[k] = dh[k] * u[k] * slope;
         du[k] = dh[k] * a;
     }
 }
 
-template <typename T> __global__ void __launch_bounds__(kNarrowThreads, 2) k_narrow_dx(Narrow f) {
-    using S = Split<T>;
-    __shared__ __attribute__((aligned(16))) typename S::V held[4 * S::n * 8 * 64];
-    const int tid = threadIdx.x, l = tid & 15, q = (tid & 63) / 16;
+__global__ void __launch_bounds__(kNarrowThreads, 2) k_narrow_dx(Narrow f) {
+    __shared__ __attribute__((aligned(16))) b8 held[4 * 3 * 8 * 64];
+    const int tid = threadIdx.x, l = tid & 15, q = (tid & 63) / 16, wave = tid / 64;
     const int64_t tiles = (f.rows + 15) / 16, stride = (int64_t)gridDim.x * 8;
-    int64_t t = (int64_t)blockIdx.x * 8 + tid / 64;
-    float d[2][8], g[2][8], u[2][8];
+    int64_t t = (int64_t)blockIdx.x * 8 + wave;
+    float d[2][8] = {}, g[2][8] = {}, u[2][8] = {};
     auto load = [&](int64_t tile) {
         const int64_t r = tile * 16 + l;
         if (r >= f.rows) return;
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            const int c = s * 32 + q * 8, live = f.hidden - c;
-            load_some<T, 8>((const T*)f.dh + r * f.dh_stride + c, live, d[s]);
-            load_some<float, 8>(f.gate + r * f.hidden + c, live, g[s]);
-            load_some<float, 8>(f.up + r * f.hidden + c, live, u[s]);
+            const int c = s * 32 + q * 8;
+            load_row(f.dh, r, f.dh_stride, c, f.hidden, d[s]);
+            load_row(f.gate, r, f.hidden, c, f.hidden, g[s]);
+            load_row(f.up, r, f.hidden, c, f.hidden, u[s]);
         }
     };
-#pragma unroll
-    for (int s = 0; s < 2; s++)
-#pragma unroll
-        for (int k = 0; k < 8; k++) d[s][k] = g[s][k] = u[s][k] = 0.0f;
     load(t);
     // B's rows are x's columns, k the hidden units: gate's 64, then up's
-    for (int i = tid; i < 128 * 16; i += kNarrowThreads) {
-        const int n = i % 128, k = i / 128 * 8, unit = k % 64;
-        const T* from = (const T*)(k < 64 ? f.wg : f.wu) + (int64_t)unit * f.cols + n;
-        float w[8];
+    const int n = min(wave * 16 + l, f.cols - 1);
+    float w[4][8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) w[e] = n < f.cols && unit + e < f.hidden ? to_f32<T>(from[e * f.cols]) : 0.0f;
-        S a;
-        a.set(w);
-        a.put(held, k / 32, n / 64 * 4 + n % 16 / 4, k % 32 / 8 * 16 + n % 64 / 16 * 4 + n % 4);
+    for (int s = 0; s < 4; s++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int unit = s % 2 * 32 + q * 8 + e;
+            const float x = (s < 2 ? f.wg : f.wu)[min(unit, f.hidden - 1) * f.cols + n];
+            w[s][e] = unit < f.hidden ? x : 0.0f;
+        }
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+        Parts a;
+        a.set(w[s]);
+        a.put(held, s, wave);
     }
     __syncthreads();
     for (; t < tiles; t += stride) {
         f4 acc[8];
-        S a[4];
+        Parts a[4];
 #pragma unroll
         for (int j = 0; j < 8; j++) acc[j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             float dg[8], du[8];
-            slopes_of<T>(f.act, d[s], g[s], u[s], dg, du);
+            slopes_of(f.act, d[s], g[s], u[s], dg, du);
             a[s].set(dg);
             a[2 + s].set(du);
         }
         load(t + stride);
 #pragma unroll
         for (int s = 0; s < 4; s++)
-            if (s % 2 * 32 < f.hidden) narrow_step<T>(held, s, a[s], acc);
+            if (s % 2 * 32 < f.hidden) narrow_step(held, s, a[s], acc);
         const int64_t m = t * 16 + l;
         if (m >= f.rows) continue;
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-            float v[16];
-#pragma unroll
-            for (int e = 0; e < 16; e++) v[e] = acc[half * 4 + e / 4][e % 4];
-            store_row<T, 16>((T*)f.dx + m * f.cols + half * 64, f.cols - half * 64, v);
+        for (int j = 0; j < 8; j++) {
+            const float v[4] = {acc[j][0], acc[j][1], acc[j][2], acc[j][3]};
+            store_some<float, 4>(f.dx + m * f.cols + j * 16 + q * 4, f.cols - j * 16 - q * 4, v);
         }
     }
 }
 
 // The weights' gradients over the block's rows, part[block][gate's 64 units, then up's][cols], and the sums of dgate and dup,
 // sums[block][2][hidden]; either may be left out.  64 rows at a time: a wave brings 32 rows of 16 units and of 32 columns into
-// LDS, a lane 8 rows of one, and takes a piece of 64 x 32 of the result.
-template <typename T> __global__ void __launch_bounds__(kNarrowThreads, 2) k_narrow_dw(Narrow f) {
-    using S = Split<T>;
-    __shared__ __attribute__((aligned(16))) typename S::V held[2][2 * S::n * 8 * 64];
+// LDS, a lane 8 rows of one, and takes a piece of 64 x 32 of the result.  Units and columns past the last are the last's
+// again; nothing of theirs is stored.
+__global__ void __launch_bounds__(kNarrowThreads, 2) k_narrow_dw(Narrow f) {
+    __shared__ __attribute__((aligned(16))) b8 held[2][2 * 3 * 8 * 64];
     const int tid = threadIdx.x, lane = tid & 63, l = lane & 15, q = lane / 16, wave = tid / 64, piece = wave % 4, step = wave / 4;
-    const int unit = piece * 16 + l, col = piece * 32 + l;
+    const int unit = min(piece * 16 + l, f.hidden - 1), col[2] = {min(piece * 32 + l, f.cols - 1), min(piece * 32 + 16 + l, f.cols - 1)};
     float d[8], g[8], u[8], x[2][8], sum_g = 0.0f, sum_u = 0.0f;
     auto load = [&](int64_t slab) {
-        const int64_t r0 = slab * 64 + step * 32 + q * 8;
+        const int64_t r = slab * 64 + step * 32 + q * 8;
+        const float *at_d = f.dh + r * f.dh_stride + unit, *at_g = f.gate + r * f.hidden + unit, *at_u = f.up + r * f.hidden + unit;
+        const float *at_x[2] = {f.x + r * f.x_stride + col[0], f.x + r * f.x_stride + col[1]};
+        auto rows = [&](auto whole) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int64_t r = r0 + e;
-            const bool in = r < f.rows && unit < f.hidden;
-            d[e] = in ? to_f32<T>(((const T*)f.dh)[r * f.dh_stride + unit]) : 0.0f;
-            g[e] = in ? f.gate[r * f.hidden + unit] : 0.0f;
-            u[e] = in ? f.up[r * f.hidden + unit] : 0.0f;
-            if (f.part)
+            for (int e = 0; e < 8; e++) {
+                const bool in = decltype(whole)::value || r + e < f.rows;
+                d[e] = in ? at_d[e * f.dh_stride] : 0.0f;
+                g[e] = in ? at_g[e * f.hidden] : 0.0f;
+                u[e] = in ? at_u[e * f.hidden] : 0.0f;
+                if (f.part)
 #pragma unroll
-                for (int i = 0; i < 2; i++)
-                    x[i][e] = r < f.rows && col + 16 * i < f.cols ? to_f32<T>(((const T*)f.x)[r * f.x_stride + col + 16 * i]) : 0.0f;
-        }
+                    for (int i = 0; i < 2; i++) x[i][e] = in ? at_x[i][e * f.x_stride] : 0.0f;
+            }
+        };
+        if (slab * 64 + 64 <= f.rows) rows(std::true_type{});
+        else rows(std::false_type{});
     };
     f4 acc[4][2];
 #pragma unroll
@@ -463,41 +468,41 @@ template <typename T> __global__ void __launch_bounds__(kNarrowThreads, 2) k_nar
     load(blockIdx.x);
     for (int64_t slab = blockIdx.x; slab < slabs; slab += gridDim.x) {
         float dg[8], du[8];
-        slopes_of<T>(f.act, d, g, u, dg, du);
+        slopes_of(f.act, d, g, u, dg, du);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             sum_g += dg[e];
             sum_u += du[e];
         }
         if (f.part) {
-            S a;
+            Parts a;
             a.set(dg);
-            a.put(held[0], step, piece, lane);
+            a.put(held[0], step, piece);
             a.set(du);
-            a.put(held[0], step, 4 + piece, lane);
+            a.put(held[0], step, 4 + piece);
 #pragma unroll
             for (int i = 0; i < 2; i++) {
                 a.set(x[i]);
-                a.put(held[1], step, piece * 2 + i, lane);
+                a.put(held[1], step, piece * 2 + i);
             }
         }
-        load(slab + gridDim.x);
+        if (slab + gridDim.x < slabs) load(slab + gridDim.x);
         if (!f.part) continue;
         __syncthreads();
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            typename S::V vb[S::n][2];
+            b8 vb[3][2];
 #pragma unroll
-            for (int p = 0; p < S::n; p++)
+            for (int p = 0; p < 3; p++)
 #pragma unroll
-                for (int j = 0; j < 2; j++) vb[p][j] = S::place(held[1], s, p, piece * 2 + j)[lane];
+                for (int j = 0; j < 2; j++) vb[p][j] = Parts::place(held[1], s, p, piece * 2 + j)[lane];
 #pragma unroll
-            for (int p = S::n - 1; p >= 0; p--) {
-                typename S::V va[4];
+            for (int p = 2; p >= 0; p--) {
+                b8 va[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) va[i] = S::place(held[0], s, p, step * 4 + i)[lane];
+                for (int i = 0; i < 4; i++) va[i] = Parts::place(held[0], s, p, step * 4 + i)[lane];
 #pragma unroll
-                for (int o = S::n - 1 - p; o >= 0; o--)
+                for (int o = 2 - p; o >= 0; o--)
 #pragma unroll
                     for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -627,7 +632,12 @@ template <typename T, typename F> int with_tile(int64_t m, int64_t n, int64_t k,
     return middle.time <= small.time ? f(Middle{}, middle.splits) : f(Small{}, small.splits);
 }
 
-bool is_narrow(int64_t cols, int64_t hidden) { return cols <= kNarrowCols && hidden <= kNarrowHidden; }
+// Where the kernels of whole rows take over (floats, us forward / both gradients, they and the tiles): 8,192 x 122 -> 64 13 / 32
+// and 15 / 36, 118,271 rows of the same 40 / 102 and 80 / 170; below, building the weights' parts in every compute unit costs
+// more than packing does (1,000 rows 15 / 29 and 12 / 26).  16-bit tensors gain nothing: theirs are no larger packed.
+template <typename T> bool is_narrow(int64_t rows, int64_t cols, int64_t hidden) {
+    return sizeof(T) == 4 && rows >= 8192 && cols <= kNarrowCols && hidden <= kNarrowHidden;
+}
 
 template <typename T>
 int join_parts(const float* part, int64_t splits, int64_t m, int64_t n, int64_t rows, int64_t cut, void* first, void* second,
@@ -649,11 +659,11 @@ template <typename T> int join_sums(const float* sums, int64_t blocks, int64_t h
 template <typename T>
 int forward(const void* x, int64_t rows, int64_t cols, int64_t x_stride, const void* wg, const void* wu, int64_t hidden,
             const void* bg, const void* bu, int act, void* h, float* gate, float* up, Arena& ws, hipStream_t st) {
-    if (is_narrow(cols, hidden)) {
+    if (is_narrow<T>(rows, cols, hidden)) {
         if (!ws.p) return 0;
-        const Narrow f{x, wg, wu, bg, bu, nullptr, h, nullptr, gate, up, nullptr, nullptr, rows, x_stride, 0, (int)cols,
-                       (int)hidden, act};
-        k_narrow_forward<T><<<(unsigned)std::min<int64_t>((rows + 127) / 128, kNarrowBlocks), kNarrowThreads, 0, st>>>(f);
+        const Narrow f{(const float*)x, (const float*)wg, (const float*)wu, (const float*)bg, (const float*)bu, nullptr, (float*)h,
+                       nullptr, gate, up, nullptr, nullptr, rows, x_stride, 0, (int)cols, (int)hidden, act};
+        k_narrow_forward<<<(unsigned)std::min<int64_t>((rows + 127) / 128, kNarrowBlocks), kNarrowThreads, 0, st>>>(f);
         return launched();
     }
     Forward f{};
@@ -721,20 +731,20 @@ template <typename T>
 int backward(const void* dh, int64_t dh_stride, const void* x, int64_t rows, int64_t cols, int64_t x_stride,
              const void* wg, const void* wu, int64_t hidden, const float* gate, const float* up, int act, void* dx,
              void* dwg, void* dwu, void* dbg, void* dbu, Arena& ws, hipStream_t st) {
-    if (is_narrow(cols, hidden)) {
+    if (is_narrow<T>(rows, cols, hidden)) {
         const int64_t blocks = std::min<int64_t>((rows + 63) / 64, kNarrowBlocks);
-        Narrow f{x, wg, wu, nullptr, nullptr, dh, nullptr, dx, (float*)gate, (float*)up, nullptr, nullptr, rows, x_stride,
-                 dh_stride, (int)cols, (int)hidden, act};
+        Narrow f{(const float*)x, (const float*)wg, (const float*)wu, nullptr, nullptr, (const float*)dh, nullptr, (float*)dx,
+                 (float*)gate, (float*)up, nullptr, nullptr, rows, x_stride, dh_stride, (int)cols, (int)hidden, act};
         if (dwg) f.part = (float*)ws.take(blocks * 2 * kNarrowHidden * cols * 4);
         if (dbg || dbu) f.sums = (float*)ws.take(blocks * 2 * hidden * 4);
         if (!ws.p) return 0;
         int e = 0;
         if (dx) {
-            k_narrow_dx<T><<<(unsigned)std::min<int64_t>((rows + 127) / 128, kNarrowBlocks), kNarrowThreads, 0, st>>>(f);
+            k_narrow_dx<<<(unsigned)std::min<int64_t>((rows + 127) / 128, kNarrowBlocks), kNarrowThreads, 0, st>>>(f);
             e = launched();
         }
         if (!e && (f.part || f.sums)) {
-            k_narrow_dw<T><<<(unsigned)blocks, kNarrowThreads, 0, st>>>(f);
+            k_narrow_dw<<<(unsigned)blocks, kNarrowThreads, 0, st>>>(f);
             e = launched();
         }
         if (!e && f.part) e = join_parts<T>(f.part, blocks, 2 * kNarrowHidden, cols, hidden, kNarrowHidden, dwg, dwu, st);

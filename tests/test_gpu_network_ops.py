@@ -133,6 +133,65 @@ def test_gated_large(ext, rows, cols, hidden, t):
     _check_gated(ext, *_gated(rows, cols, hidden, t, 5), "silu")
 
 
+@pytest.mark.parametrize("act", ["sigmoid", "silu", "gelu"])
+@pytest.mark.parametrize("rows,cols,hidden", [(8192, 122, 64), (8191, 122, 64), (8193, 1, 1), (9001, 128, 64), (20011, 33, 17),
+                                              (40000, 64, 8), (10000, 127, 33), (8200, 129, 64), (8200, 128, 65)])
+def test_gated_many_rows_of_a_narrow_block(ext, rows, cols, hidden, act):
+    """Up to 128 columns and 64 units, which float32 tensors of many rows have kernels of their own for, and one past them."""
+    _check_gated(ext, *_gated(rows, cols, hidden, F32, cols, bias=hidden != 33), act)
+
+
+def test_gated_many_rows_of_a_narrow_block_cut_from_wider_tensors(ext):
+    x, wg, wu, bg, bu, dh = _gated(8500, 101, 50, F32, 9)
+    wide, wide_dh = _randn((8500, 130), 20), _randn((8500, 57), 21, 0.1)
+    _check_gated(ext, wide[:, 3:104], wg, wu, bg, None, wide_dh[:, 7:], "silu")
+    _check_gated(ext, wide[:1, :101].expand(8500, 101), wg, wu, None, bu, dh, "sigmoid")
+    _check_gated(ext, x.view(85, 100, 101), wg, wu, bg, bu, dh[:1].expand(8500, 50).view(85, 100, 50), "gelu")
+
+
+def test_gated_many_rows_of_a_narrow_block_on_their_own(ext):
+    """A row's NaN and inf stay in it, what is not needed is not given and changes nothing else, a call repeats its bits in a
+    graph and beside another, a unit that is off stays off."""
+    x, wg, wu, bg, bu, dh = _gated(9000, 122, 64, F32, 4)
+    h, gate, up = ext.gated_linear_forward(x, wg, wu, bg, bu)
+    assert torch.equal(h, ext.gated_linear(x, wg, wu, bg, bu))
+    whole = ext.gated_linear_backward(dh, x, wg, wu, gate, up)
+    for need in ((True, False, False), (False, True, False), (False, False, True), (True, True, False)):
+        some = ext.gated_linear_backward(dh, x, wg, wu, gate, up, need_dx=need[0], need_weights=need[1], need_bias=need[2])
+        for a, b, n in zip(some, whole, (need[0], need[1], need[1], need[2], need[2])):
+            assert torch.equal(a, b) if n else a is None
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    outs = []
+    for s in streams:  # two at once
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs.append((ext.gated_linear(x, wg, wu, bg, bu), *ext.gated_linear_backward(dh, x, wg, wu, gate, up)))
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        held = (ext.gated_linear(x, wg, wu, bg, bu), *ext.gated_linear_backward(dh, x, wg, wu, gate, up))
+    for _ in range(3):
+        for t in held:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        outs.append([t.clone() for t in held])
+    for o in outs:
+        assert all(torch.equal(a, b) for a, b in zip(o, (h, *whole)))
+    bad = x.clone()
+    bad[7, 3], bad[8999, 121] = float("nan"), float("inf")
+    rest = torch.ones((9000,), dtype=torch.bool, device="cuda")
+    rest[[7, 8999]] = False
+    out = ext.gated_linear(bad, wg, wu, bg, bu)
+    assert torch.equal(out[rest], h[rest]) and torch.isnan(out[7]).all() and not torch.isfinite(out[8999]).all()
+    off = bg.clone()
+    off[5] = float("-inf")
+    h, gate, up = ext.gated_linear_forward(x, wg, wu, off, bu)
+    dx, dwg, dwu, dbg, dbu = ext.gated_linear_backward(dh, x, wg, wu, gate, up)
+    assert not h[:, 5].any() and torch.isfinite(dx).all()
+    assert not any(t[5].any() for t in (dwg, dwu, dbg, dbu)) and torch.isfinite(dwg).all()
+
+
 @pytest.mark.parametrize("t", TYPES, ids=str)
 @pytest.mark.parametrize("first,pad", [(0, 8), (1, 7), (8, 0), (3, 61)])
 def test_gated_rows_cut_from_a_wider_tensor(ext, t, first, pad):
