@@ -94,18 +94,20 @@ struct Operand {
 };
 
 template <typename T_, int kParts_, int kSteps_, int kM_, int kN_, int kWm_, int kWn_, int kStages_, int kBlocks_,
-          bool kAhead_ = true>
+          bool kAhead_ = true, int kTeams_ = 1>
 struct Tile {
     using T = T_;
     using V = typename Fragment<T>::type;
     static constexpr int kParts = kParts_, kSteps = kSteps_, kM = kM_, kN = kN_, kWm = kWm_, kWn = kWn_, kStages = kStages_;
     static constexpr int kBlocks = kBlocks_;                          // that a compute unit holds
     static constexpr bool kAhead = kAhead_;                           // operands are read a step ahead
-    static constexpr int kThreads = 64 * kWm * kWn, kWavesEach = kBlocks * kThreads / 256;  // of a block; on a SIMD
+    static constexpr int kTeams = kTeams_;                            // of a block, which share out the slices
+    static constexpr int kThreads = 64 * kWm * kWn, kBlock = kTeams * kThreads;  // of a team; of a block
+    static constexpr int kWavesEach = kBlocks * kBlock / 256;         // on a SIMD
     static constexpr int kRow = 64 * kParts * kSteps;                 // bytes of a slice's row
     static constexpr int kChunks = kRow / 16;
     static constexpr int kStage = (kM + kN) * kRow;                   // bytes of a slice
-    static constexpr int kLds = kStages * kStage;
+    static constexpr int kLds = kTeams * kStages * kStage;
     static constexpr int kFm = kM / kWm / 16, kFn = kN / kWn / 16;    // a wave's 16 x 16 pieces
     static constexpr int kLoads = (kM + kN) * kChunks / kThreads;     // 16-byte loads a lane makes for a slice
     static constexpr int kLoadsA = kM * kChunks / kThreads;
@@ -130,9 +132,10 @@ struct Tile {
 template <typename Tl, int kHalves, bool kTurnedB = false> struct Sums {
     static constexpr int kShare = Tl::kFn / kHalves;
     f4 acc[Tl::kFm][Tl::kFn];
-    __device__ __forceinline__ int row() const { return (int)(threadIdx.x >> 6) / Tl::kWn * Tl::kFm * 16 + (threadIdx.x & 15); }
+    static __device__ __forceinline__ int wave() { return (int)(threadIdx.x % Tl::kThreads >> 6); }
+    __device__ __forceinline__ int row() const { return wave() / Tl::kWn * Tl::kFm * 16 + (threadIdx.x & 15); }
     // of the wave's part, and of the lane's columns
-    __device__ __forceinline__ int first_col() const { return (int)(threadIdx.x >> 6) % Tl::kWn * kShare * 16; }
+    __device__ __forceinline__ int first_col() const { return wave() % Tl::kWn * kShare * 16; }
     __device__ __forceinline__ int col() const { return first_col() + (int)(threadIdx.x & 63) / 16 * 4 * kShare; }
     // row r of a tile of B: its column of C, and which half it is of
     static __device__ __forceinline__ int column(int r) {
@@ -175,7 +178,8 @@ template <typename Tl, int kHalves, bool kTurnedB = false> struct Sums {
 };
 
 // The product over slices [begin, end) of rows m0.. of A and rows n0.. of B (columns, where they are turned).  With two halves
-// of B, b0 and b1, the same rows of both; a turned B goes on in b1 from slice `cut` on.
+// of B, b0 and b1, the same rows of both; a turned B goes on in b1 from slice `cut` on.  Of more than one team the first has
+// the sums in the end, and the others are done.
 template <typename Tl, int kHalves, bool kTurnedA, bool kTurnedB>
 __device__ __forceinline__ void multiply(const Operand& a, int m0, const Operand& b0, const Operand& b1, int n0, int cut,
                                          int begin, int end, char* lds, Sums<Tl, kHalves, kTurnedB>& s) {
@@ -183,7 +187,18 @@ __device__ __forceinline__ void multiply(const Operand& a, int m0, const Operand
     constexpr int across_a = Tl::kM * Tl::kParts / 8, across_b = Tl::kN * Tl::kParts / 8;  // chunks of a turned slice's rows
     constexpr int deep = 32 * Tl::kSteps;                                                 // k of a slice
     static_assert(!kTurnedB || kHalves == 1, "");
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int tid = threadIdx.x % Tl::kThreads, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    int stop = end;
+    char* const all = lds;
+    constexpr int team_lds = Tl::kLds / Tl::kTeams;
+    const int team = Tl::kTeams == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x / Tl::kThreads);
+    if constexpr (Tl::kTeams > 1) {
+        // the same number of slices each, as they wait for each other: those past the end are zeros
+        const int each = (end - begin + Tl::kTeams - 1) / Tl::kTeams;
+        begin += team * each;
+        stop = begin + each;
+        lds += team * team_lds;
+    }
     uint32_t offset[Tl::kLoads];
     int at[Tl::kLoads];  // the chunk's place in its row in bytes, or its k
 #pragma unroll
@@ -245,7 +260,7 @@ __device__ __forceinline__ void multiply(const Operand& a, int m0, const Operand
     for (int i = 0; i < Tl::kFm; i++)
 #pragma unroll
         for (int j = 0; j < Tl::kFn; j++) s.acc[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (begin >= end) return;
+    if (begin >= stop) return;
     const int l = lane & 15, g = lane >> 4;
     const int wave_m = wave / Tl::kWn * Tl::kFm, wave_n = wave % Tl::kWn * Tl::kFn;  // in pieces of 16
     const char* const lds_b = lds + Tl::kM * Tl::kRow;
@@ -291,7 +306,7 @@ __device__ __forceinline__ void multiply(const Operand& a, int m0, const Operand
             for (int i = 0; i < Tl::kLoads; i++) fetch(i, f, n);
         }
         int stage = 0;
-        for (int k = begin; k < end; k++) {
+        for (int k = begin; k < stop; k++) {
             wait_loads<(Tl::kStages - 2) * Tl::kLoads>();
             const From f = from(k + Tl::kStages - 1);
             const int free = stage == 0 ? Tl::kStages - 1 : stage - 1;
@@ -359,18 +374,29 @@ __device__ __forceinline__ void multiply(const Operand& a, int m0, const Operand
     using zero = std::integral_constant<int, 0>;
     using one = std::integral_constant<int, 1>;
     if constexpr (Tl::kSteps == 2) {
-        for (int k = begin; k < end; k++) {
+        for (int k = begin; k < stop; k++) {
             multiply_step(k, zero{}, zero{});
             multiply_step(k, one{}, one{});
         }
     } else {
-        for (int k = begin; k < end; k += 2) {
+        for (int k = begin; k < stop; k += 2) {
             multiply_step(k, zero{}, zero{});
-            if (k + 1 < end) multiply_step(k + 1, zero{}, one{});
+            if (k + 1 < stop) multiply_step(k + 1, zero{}, one{});
         }
     }
     }
     wait_loads<0>();  // the LDS is free again
+    if constexpr (Tl::kTeams > 1) {
+        static_assert(Tl::kFm * Tl::kFn * Tl::kThreads * 16 <= team_lds, "");
+#pragma unroll
+        for (int i = 0; i < Tl::kFm * Tl::kFn; i++)
+            if (team > 0) ((f4*)lds)[i * Tl::kThreads + tid] = s.acc[i / Tl::kFn][i % Tl::kFn];
+        __syncthreads();
+        for (int t = 1; t < Tl::kTeams && team == 0; t++)
+#pragma unroll
+            for (int i = 0; i < Tl::kFm * Tl::kFn; i++)
+                s.acc[i / Tl::kFn][i % Tl::kFn] += ((const f4*)(all + t * team_lds))[i * Tl::kThreads + tid];
+    }
     if constexpr (kTurnedB) s.regroup();
 }
 
