@@ -20,6 +20,11 @@
 // weights of each digit with top_p alone, and once for the slots that these or
 // min_p leave, which a wave draws from where they are 1,024 or less.  Where they
 // are more, cuts are found by all three digits of the key.
+//
+// Measured (MI355X): 65,521 lists of up to 256 slots with top_p 53 us (a wave each; the sums and pivots of a cut bound
+// it, not the 35 MB), 192 rows of 85,834 bfloat16 with top_k and top_p 42 us, one row of as many float32 with
+// min_p 28 where at most 1,024 slots pass it: a block reads its row two or three times at what one compute unit reads, 45 GB/s
+// a row and 0.8 TB/s in all; one short list 3 us, 5.5 with the call.
 #include <cmath>
 
 #include "hive_train.hpp"
