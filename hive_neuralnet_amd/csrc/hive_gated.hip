@@ -573,33 +573,37 @@ struct Arena {
     }
 };
 
-// `count` operands of rows x cols values, as they are, or, where one of them cannot be taken so, packed into the arena (only
-// counted where the arena has no memory): a tile takes two by one stride
+// `count` operands of rows x cols values, as they are, or, where one of them cannot be taken so, added to what `packing` packs
+// into the arena: a tile takes two by one stride
 template <typename T>
-int operands(const void* const* src, int count, int64_t rows, int64_t cols, int64_t stride, Arena& ws, hipStream_t st,
-             Operand* out) {
+void operands(const void* const* src, int count, int64_t rows, int64_t cols, int64_t stride, Arena& ws, Packing& packing,
+              Operand* out) {
     constexpr int type = sizeof(T) == 4 ? HG_F32 : HG_F16;
     bool as_is = true;
     for (int i = 0; i < count; i++) as_is = as_is && as_it_is(src[i], type, rows, cols, stride);
-    const int parts = parts_of(type);
-    const int64_t bytes = packed_bytes(cols, parts);
-    Packing f{};
+    const int64_t bytes = packed_bytes(cols, parts_of(type));
     for (int i = 0; i < count; i++) {
         if (as_is) {
             out[i] = {src[i], (rows <= 1 ? cols : stride) * 2, (int)rows, (int)cols * 2};
         } else {
-            f.src[i] = src[i];
-            f.dst[i] = ws.take(rows * bytes);
-            out[i] = {f.dst[i], bytes, (int)rows, (int)bytes};
+            const int k = packing.count++;
+            packing.src[k] = src[i];
+            packing.dst[k] = ws.take(rows * bytes);
+            packing.src_stride[k] = stride;
+            packing.rows[k] = rows;
+            out[i] = {packing.dst[k], bytes, (int)rows, (int)bytes};
         }
     }
-    if (as_is || !ws.p || rows == 0) return 0;
-    f.src_stride = stride;
-    f.dst_stride = bytes / 2;
-    f.rows = rows;
-    f.cols = (int)cols;
-    const int64_t threads = rows * (up_to(cols, 32) / 8);
-    const dim3 grid((unsigned)std::min<int64_t>((threads + kPackThreads - 1) / kPackThreads, 1 << 20), count);
+    packing.dst_stride = bytes / 2;
+    packing.cols = (int)cols;
+}
+// all of them in one launch (5 us each alone for 3,000 rows of 1,237 and its weights)
+template <typename T> int pack(const Packing& f, hipStream_t st) {
+    int64_t rows = 0;
+    for (int i = 0; i < f.count; i++) rows = std::max(rows, f.rows[i]);
+    if (rows == 0) return 0;
+    const int64_t threads = rows * (up_to(f.cols, 32) / 8);
+    const dim3 grid((unsigned)std::min<int64_t>((threads + kPackThreads - 1) / kPackThreads, 1 << 20), f.count);
     if constexpr (sizeof(T) == 4) k_pack<float, bf16, 3><<<grid, kPackThreads, 0, st>>>(f);
     else k_pack<T, T, 1><<<grid, kPackThreads, 0, st>>>(f);
     return launched();
@@ -613,6 +617,9 @@ template <typename Tl> struct Cost {
                                                     : (size == 256 * 256 ? 1650 : size == 128 * 128 ? 1000 : 700);
     static constexpr double around = size == 256 * 256 ? 6000 : size == 128 * 128 ? 4000 : 2500;
 };
+template <typename Tl> int64_t blocks_of(int64_t m, int64_t n) {
+    return ((m + Tl::kM - 1) / Tl::kM) * ((n + Tl::kN - 1) / Tl::kN);
+}
 // The least time of an m x n result with `slices` of 64 k (32 of floats') over the ways to cut k into splits (`most` of them),
 // whose parts are added up in a launch of their own.
 struct Plan {
@@ -620,7 +627,7 @@ struct Plan {
     int64_t splits;
 };
 template <typename Tl> Plan plan_of(int64_t m, int64_t n, int64_t slices, int64_t most) {
-    const int64_t tiles = ((m + Tl::kM - 1) / Tl::kM) * ((n + Tl::kN - 1) / Tl::kN), room = 256 * Tl::kBlocks;
+    const int64_t tiles = blocks_of<Tl>(m, n), room = 256 * Tl::kBlocks;
     Plan best{1e300, 1};
     for (int64_t s = 1; s <= most && (s == 1 || slices / s >= 4); s = s < 8 ? s + 1 : s * 5 / 4) {
         const int64_t each = (slices + s - 1) / s, blocks = tiles * ((slices + each - 1) / each);
@@ -645,6 +652,12 @@ template <typename T, typename F> int with_tile(int64_t m, int64_t n, int64_t k,
     using Third = std::conditional_t<parts, Tile<P, 3, 1, 64, 128, 2, 2, 2, 2>, Tile<P, 1, 2, 256, 256, 2, 4, 2, 1>>;
     const Plan third = plan_of<Third>(m, n, slices, most);
     if (third.time <= middle.time && third.time <= small.time) return f(Third{}, third.splits);
+    if constexpr (!parts) {
+        // a block a compute unit at most: twice the slices in flight (2,999 rows of 1,237 float16 to 515 units forward 29.1 us
+        // -> 25.6; two teams 27.7)
+        using Alone = Tile<P, 1, 2, 128, 128, 2, 2, 4, 1>;
+        if (middle.time <= small.time && blocks_of<Middle>(m, n) * middle.splits <= 256) return f(Alone{}, middle.splits);
+    }
     return middle.time <= small.time ? f(Middle{}, middle.splits) : f(Small{}, small.splits);
 }
 
@@ -685,9 +698,12 @@ int forward(const void* x, int64_t rows, int64_t cols, int64_t x_stride, const v
     Forward f{};
     const void* const weights[2] = {wg, wu};
     Operand w[2];
-    int e = operands<T>(&x, 1, rows, cols, x_stride, ws, st, &f.x);
-    if (!e) e = operands<T>(weights, 2, hidden, cols, cols, ws, st, w);
-    if (e || !ws.p) return e;
+    Packing packing{};
+    operands<T>(&x, 1, rows, cols, x_stride, ws, packing, &f.x);
+    operands<T>(weights, 2, hidden, cols, cols, ws, packing, w);
+    if (!ws.p) return 0;
+    const int e = pack<T>(packing, st);
+    if (e) return e;
     f.wg = w[0];
     f.wu = w[1];
     f.x.bytes = std::min(f.x.bytes, std::min(f.wg.bytes, f.wu.bytes));  // a packed row's zeros have no partner in a plain one
@@ -782,17 +798,14 @@ int backward(const void* dh, int64_t dh_stride, const void* x, int64_t rows, int
         if (!e && biases) e = join_sums<T>(sums, blocks, hidden, dbg, dbu, st);
     }
     const Operand grads{d, d_bytes, (int)rows, (int)d_bytes};
-    if (!e && dx) {
-        const void* const weights[2] = {wg, wu};
-        Operand w[2];
-        e = operands<T>(weights, 2, hidden, cols, cols, ws, st, w);
-        if (!e) e = product<T, false>(grads, w[0], w[1], rows, 2 * cut, cut, rows, rows, dx, nullptr, cols, ws, st);
-    }
-    if (!e && dwg) {
-        Operand b;
-        e = operands<T>(&x, 1, rows, cols, x_stride, ws, st, &b);
-        if (!e) e = product<T, true>(grads, b, b, 2 * cut, rows, 1 << 30, hidden, cut, dwg, dwu, cols, ws, st);
-    }
+    const void* const weights[2] = {wg, wu};
+    Operand w[2], b;
+    Packing packing{};
+    if (dx) operands<T>(weights, 2, hidden, cols, cols, ws, packing, w);
+    if (dwg) operands<T>(&x, 1, rows, cols, x_stride, ws, packing, &b);
+    if (!e && ws.p) e = pack<T>(packing, st);
+    if (!e && dx) e = product<T, false>(grads, w[0], w[1], rows, 2 * cut, cut, rows, rows, dx, nullptr, cols, ws, st);
+    if (!e && dwg) e = product<T, true>(grads, b, b, 2 * cut, rows, 1 << 30, hidden, cut, dwg, dwu, cols, ws, st);
     return e;
 }
 

@@ -35,24 +35,25 @@ inline int64_t packed_bytes(int64_t n, int parts) { return up_to(n, 32) * 2 * pa
 
 constexpr int kPackThreads = 256;
 
-// What a launch packs: up to two tensors of one shape, grid y.
+// What a launch packs: up to three tensors of rows of one width, grid y.
 struct Packing {
-    const void* src[2];
-    void* dst[2];
-    int64_t src_stride, dst_stride, rows;
-    int cols;
+    const void* src[3];
+    void* dst[3];
+    int64_t src_stride[3], rows[3], dst_stride;
+    int cols, count;
 };
 // dst[r] = the parts of src[r][0..cols), zeros up to a multiple of 32.  Memory bound; a thread takes 8 values.
 template <typename S, typename T, int kParts> __global__ void __launch_bounds__(kPackThreads) k_pack(Packing f) {
     const int groups = (int)up_to(f.cols, 32) / 8;
     const S* const src = (const S*)f.src[blockIdx.y];
     T* const dst = (T*)f.dst[blockIdx.y];
-    for (int64_t i = (int64_t)blockIdx.x * kPackThreads + threadIdx.x; i < f.rows * groups;
+    const int64_t rows = f.rows[blockIdx.y], src_stride = f.src_stride[blockIdx.y];
+    for (int64_t i = (int64_t)blockIdx.x * kPackThreads + threadIdx.x; i < rows * groups;
          i += (int64_t)gridDim.x * kPackThreads) {
-        const int64_t r = f.rows < 1 << 20 && groups < 1 << 11 ? (int64_t)((uint32_t)i / (uint32_t)groups) : i / groups;
+        const int64_t r = rows < 1 << 20 && groups < 1 << 11 ? (int64_t)((uint32_t)i / (uint32_t)groups) : i / groups;
         const int c = (int)(i - r * groups) * 8;
         float v[8];
-        load_some<S, 8>(src + r * f.src_stride + c, f.cols - c, v);
+        load_some<S, 8>(src + r * src_stride + c, f.cols - c, v);
         typedef T vec __attribute__((ext_vector_type(8)));
         vec q[kParts];
 #pragma unroll
