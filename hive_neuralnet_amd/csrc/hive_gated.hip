@@ -14,8 +14,8 @@
 // Measured (MI355X): 8,192 rows of 1,024 bfloat16 to 4,096 units forward 184 us with gate and up stored, 128 without (1,070
 // TFLOP/s; a plain product of that size by the library 125 to 130), slopes 125 (540 MB, 4.3 TB/s), dx 166, dW 160 (830 and
 // 860 TFLOP/s: operands that are turned as they are read from LDS come at half the rate; straight ones would make dx 121).
-// One row of 2,048 to 8,192 units 12 us, 5.6 TB/s of weights.  2,999 rows of 1,237 float16 to 515 units 29 forward, 12
-// slopes, 20 dx, 27 dW, 19 to lay out what 16-byte loads cannot take.
+// One row of 2,048 to 8,192 units 12 us, 5.6 TB/s of weights.  2,999 rows of 1,237 float16 to 515 units 22.5 forward, 10
+// slopes, 19 dx, 27 dW, 13.5 to lay out what 16-byte loads cannot take.
 #include <algorithm>
 
 #include "hive_pack.hpp"
@@ -33,14 +33,29 @@ constexpr int64_t kMaxArea = (int64_t)1 << 35;  // a launch has under 2^32 threa
 __device__ __forceinline__ float sigmoid_of(float g) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g));
 }
+// The share (1 + erf(g / sqrt 2)) / 2 of gelu, and bell = exp(-g^2 / 2).  The share of the tail, erfc(|g| / sqrt 2) / 2, is
+// t q(t) bell with t = 1 / (1 + 0.4 |g| / sqrt 2) and q a polynomial: a least-squares fit, over t, to exp(x^2) erfc(x) / (2 t),
+// 2e-8 of itself off; bell's argument has g^2 2^-24 of rounding.  Of the tail itself, as 1 + erf would cancel there.  (With erfcf
+// and expf, forward and slopes of 2,999 rows of 1,237 float16 to 515 units took 25.2 and 12.3 us instead of 22.5 and 9.6.)
+__device__ __forceinline__ float gelu_share(float g, float& bell) {
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.282842712f, __builtin_fabsf(g), 1.0f));
+    bell = __builtin_amdgcn_exp2f(-0.72134752f * g * g);
+    constexpr float c[11] = {0.112837918f, 0.112837933f, 0.103806868f, 0.0858696325f, 0.0595041775f, 0.0419581384f,
+                             -0.0234474856f, 0.0687806085f, -0.117763579f, 0.0702233465f, -0.0146075571f};
+    float q = c[10];
+#pragma unroll
+    for (int i = 9; i >= 0; i--) q = fmaf(q, t, c[i]);
+    const float tail = t * q * bell;
+    return g < 0.0f ? tail : 1.0f - tail;
+}
 // act(g) and its slope, at infinite g as well: a unit whose bias is -inf is off.  The slope's own factor g is held to +-200,
 // past which what it multiplies is 0 in float32.
 template <bool kSlope> __device__ __forceinline__ float act_of(int act, float g, float& slope) {
     const float held = __builtin_amdgcn_fmed3f(g, -200.0f, 200.0f);
     if (act == HG_GELU) {
-        skipped();
-        const float share = 0.5f * erfcf(-0.70710678f * g);  // of the tail itself: 1 + erf would cancel there
-        if (kSlope) slope = share + 0.39894228f * held * expf(-0.5f * held * held);
+        float bell;
+        const float share = gelu_share(g, bell);
+        if (kSlope) slope = share + 0.39894228f * held * bell;
         return g == -__builtin_inff() ? 0.0f : g * share;
     }
     const float share = sigmoid_of(g);

@@ -286,6 +286,23 @@ def test_rows_more_than_31_bits_apart(ext):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("act", ["sigmoid", "silu", "gelu"])
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_gated_activations_over_their_range(ext, t, act):
+    """Gates from -12 to 12, each to what the card's own functions, polynomials and rounding allow of itself, tails too.  The
+    weights' gradients are left out: sums of x silu(x) come to 9,001 / 2 * 12^2 / 3 = 216,000, past float16's 65,504."""
+    x = torch.linspace(-12.0, 12.0, 9001, device="cuda").to(t).unsqueeze(1)
+    one = torch.ones((1, 1), device="cuda", dtype=t)
+    h, gate, up = ext.gated_linear_forward(x, one, one * 0, None, one[0], act)
+    assert torch.equal(gate, x.float()) and bool((up == 1).all())
+    dx = ext.gated_linear_backward(torch.ones_like(x), x, one, one * 0, gate, up, act, need_weights=False)[0]
+    g = x.double()
+    a, slope, _ = _act(act, g)
+    d_eval = (g.square() + g.abs() + 16) * U
+    _close(h, a, (d_eval + 2 * U) * a.abs(), "h")
+    _close(dx, slope, 2 * d_eval * (slope.abs() + a.abs()) + (HALF_ULP[t] + _chain(64, t)) * slope.abs() * 1.01 + TINY[t], "dx")
+
+
 def test_gated_float32_keeps_its_range(ext):
     """Values near the largest and the smallest floats: parts neither overflow nor vanish.  bfloat16's smallest step is
     2^-133, so the parts of a value hold it to 2^-134 (1e-38 has 7 of its bits left), which meets the other factor:
