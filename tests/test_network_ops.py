@@ -146,3 +146,11 @@ def test_python_refuses_what_is_not_on_a_gpu():
                  lambda: ext.gated_linear_backward(x, x, w, w, x, x)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_every_kernel_source_is_built():
+    """The library is linked from all of the package's sources: a missing one would leave entry points out."""
+    import glob
+
+    from hive_neuralnet_amd import build
+    assert sorted(build.SOURCES) == sorted(glob.glob(os.path.join(build.PKG, "csrc", "*.hip")))
