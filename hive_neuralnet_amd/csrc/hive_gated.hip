@@ -276,7 +276,7 @@ k_join_parts(const float* __restrict__ part, int splits, int64_t m, int n, int r
 // operands lie in fragments: 16 of its rows by 32 k of one part, 16 bytes a lane in the lanes' order.
 //
 // 118,271 rows of 122 values to 64 units (the tiles in parentheses): forward 42 us (65 and 33 to lay out x), dx 43 (45 and
-// 36 for the slopes), both dW with the biases' 54 (55 and 33), 13 to join the blocks' parts.  They move 148 MB each (3.5
+// 36 for the slopes), both dW with the biases' 52 (55 and 33), 13 to join the blocks' parts.  They move 148 MB each (3.5
 // TB/s in the forward pass), and the matrix cores are busy for 9 us, the LDS reads of the weights take as long and the
 // activations and the splitting 15 to 20: two waves a SIMD, all that registers and LDS hold, overlap these in part.
 constexpr int kNarrowCols = 128, kNarrowHidden = 64, kNarrowThreads = 512, kNarrowBlocks = 256;

@@ -16,14 +16,14 @@
 // equal it; keys are the logits' bits in unsigned order, 0 for what is not
 // live (NaN, too).  Rows up to 1,024 slots are held by a wave's registers, and a
 // cut is found by pivots.  Longer rows are read by a block: once for the largest
-// and, with top_k, the counts of each 11-bit digit of the keys, once more for the
-// weights of each digit with top_p alone, and once for the slots that these or
+// (each thread's own, of which the top_k-th bounds the row's), once more for the
+// weights of each 11-bit digit of the keys with top_p alone, and once for the slots that these or
 // min_p leave, which a wave draws from where they are 1,024 or less.  Where they
 // are more, cuts are found by all three digits of the key.
 //
 // Measured (MI355X): 65,521 lists of up to 256 slots with top_p 53 us (a wave each; the sums and pivots of a cut bound
-// it, not the 35 MB), 192 rows of 85,834 bfloat16 with top_k and top_p 42 us, one row of as many float32 with
-// min_p 28 where at most 1,024 slots pass it: a block reads its row two or three times at what one compute unit reads, 45 GB/s
+// it, not the 35 MB), 192 rows of 85,834 bfloat16 with top_k and top_p 37 us, one row of as many float32 with
+// min_p 22 where at most 1,024 slots pass it: a block reads its row two or three times at what one compute unit reads, 45 GB/s
 // a row and 0.8 TB/s in all; one short list 3 us, 5.5 with the call.
 #include <cmath>
 
@@ -425,6 +425,7 @@ struct Shared {
     unsigned long long bins[kParts];  // the first kBins: of a digit; then all: the sums of 256 slots each
     uint32_t equal[kParts];
     unsigned long long above, all, most[kWaves];
+    int holders[kWaves];
     int bin, left;
     uint32_t wave_bins[64];
 };
@@ -473,15 +474,17 @@ template <typename T> __global__ void __launch_bounds__(kThreads) k_sample_long(
     };
     const bool by_count = r.k && !r.greedy;
     if (by_count) clear();
-    // the largest key and its first slot as one number, and how many are live
-    unsigned long long best = 0;
-    int live = 0;
+    // the largest key and its first slot, then as one number, and how many are live
+    uint32_t own = 0;
+    int live = 0, slot = 0;
     each([&](uint32_t key, int i) {
-        const unsigned long long one = (unsigned long long)key << 32 | (uint32_t)~i;
-        best = key && one > best ? one : best;
+        slot = key > own ? i : slot;
+        own = max(key, own);
         live += key != 0;
-        if (by_count && key) atomicAdd(&sh.bins[key >> 21], 1ull);
     });
+    if (by_count && own) atomicAdd(&sh.bins[own >> 21], 1ull);
+    unsigned long long best = own ? (unsigned long long)own << 32 | (uint32_t)~slot : 0;
+    const int holders = wave_sum(own != 0 ? 1 : 0);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const unsigned long long other = __shfl_xor(best, o, 64);
@@ -491,12 +494,15 @@ template <typename T> __global__ void __launch_bounds__(kThreads) k_sample_long(
     if (lane == 0) {
         sh.most[wave] = best;
         sh.equal[wave] = live;
+        sh.holders[wave] = holders;
     }
     __syncthreads();
     live = 0;
+    int all_holders = 0;  // threads with a live slot
     for (int i = 0; i < kWaves; i++) {
         best = sh.most[i] > best ? sh.most[i] : best;
         live += sh.equal[i];
+        all_holders += sh.holders[i];
     }
     __syncthreads();
     const uint32_t top = (uint32_t)(best >> 32);
@@ -508,14 +514,31 @@ template <typename T> __global__ void __launch_bounds__(kThreads) k_sample_long(
         return;
     }
     auto weight = [&](uint32_t key) { return (unsigned long long)rint(weight_of(key, top, r.scale) * kBlockOne); };
-    // What has to be at or above `floor` to be kept.  By top_k, the digit in which the k-th is; by top_p without it, that in which
-    // the mass is reached; by min_p, a weight a little below it (the logit's rounding to float32 and that of the logarithm).
+    // What has to be at or above `floor` to be kept.  By top_k, the two digits in which the k-th largest of the threads' own
+    // largest is, at or above which there are k at least (to count every key's digit took 42 us instead of 37 for 192 rows of
+    // 85,834 and the 50 largest: the digits are few, and what adds to one waits for the others), or, where fewer threads hold
+    // any, the digit of the k-th of all keys; by top_p without it, that in which the mass is reached; by min_p, a weight a little below it (the logit's rounding to float32 and that of the logarithm).
     const bool cut_k = r.k && r.k < live;
     uint32_t floor_key = 1;
     unsigned long long all_live = 0;
     if (cut_k) {
+        if (r.k > all_holders) {
+            clear();
+            each([&](uint32_t key, int) {
+                if (key) atomicAdd(&sh.bins[key >> 21], 1ull);
+            });
+            __syncthreads();
+        }
         find_bin(sh, (unsigned long long)r.k);
-        floor_key = max(1u, (uint32_t)sh.bin << 21);
+        const uint32_t bin = sh.bin;
+        floor_key = max(1u, bin << 21);
+        if (r.k <= all_holders) {  // the next digit as well
+            const unsigned long long want = (unsigned long long)r.k - sh.above;
+            clear();
+            if (own >> 21 == bin && own) atomicAdd(&sh.bins[own >> 10 & 2047], 1ull);
+            find_bin(sh, want);
+            floor_key = max(1u, bin << 21 | (uint32_t)sh.bin << 10);
+        }
     } else if (r.cut_p) {
         __syncthreads();
         clear();

@@ -874,6 +874,20 @@ def test_sample_sorted_rows(ext, K):
         _check_sample(ext, x, _uniforms(len(x), 8), **kw)
 
 
+@pytest.mark.parametrize("t", [F32, BF16], ids=str)
+@pytest.mark.parametrize("K", [1025, 2300, 4097, 9000])
+def test_sample_the_largest_of_a_long_row(ext, K, t):
+    """As many as there are threads, fewer and more, than a wave holds, and than there are: at random, in order, all but alike,
+    with most of the row masked."""
+    x = _logits(4, K, K, t)
+    x[1] = x[1].sort().values
+    x[2] = (x[2] * 0.5).round()
+    x[3, torch.randperm(K, generator=_gen(5), device="cuda")[: K * 7 // 8]] = float("-inf")
+    for k in (1, 50, 256, 257, 575, 576, 1023, 1024, 1025, 1200, K - 1, K):
+        _check_sample(ext, x, _uniforms(4, k), k=k)
+    _check_sample(ext, x, _uniforms(4, 3), k=300, p=0.9, min_p=0.01, t=2.0)
+
+
 def test_sample_strides_and_types(ext):
     """Rows cut from wider ones, every other row, a broadcast row, odd addresses."""
     for t in TYPES:
