@@ -23,8 +23,9 @@
 //
 // Measured (MI355X): 65,521 lists of up to 256 slots with top_p 53 us (a wave each; the sums and pivots of a cut bound
 // it, not the 35 MB), 192 rows of 85,834 bfloat16 with top_k and top_p 37 us, one row of as many float32 with
-// min_p 22 where at most 1,024 slots pass it: a block reads its row two or three times at what one compute unit reads, 45 GB/s
-// a row and 0.8 TB/s in all; one short list 3 us, 5.5 with the call.
+// min_p 22 where at most 1,024 slots pass it, 162 with a top_p of 0.9, whose thousands of slots take four passes of weights
+// (their 64-bit series, 40 us a pass of what one compute unit adds up, bounds these; 233 where each cut began at its first
+// digit); one short list 3 us, 5.5 with the call.
 #include <cmath>
 
 #include "hive_train.hpp"
@@ -521,6 +522,13 @@ template <typename T> __global__ void __launch_bounds__(kThreads) k_sample_long(
     const bool cut_k = r.k && r.k < live;
     uint32_t floor_key = 1;
     unsigned long long all_live = 0;
+    // the cut's first digit and what is above it, where all keys were added up by it
+    int digit = -1;
+    unsigned long long above = 0;
+    auto settled = [&] {
+        digit = sh.bin;
+        above = sh.above;
+    };
     if (cut_k) {
         if (r.k > all_holders) {
             clear();
@@ -532,7 +540,9 @@ template <typename T> __global__ void __launch_bounds__(kThreads) k_sample_long(
         find_bin(sh, (unsigned long long)r.k);
         const uint32_t bin = sh.bin;
         floor_key = max(1u, bin << 21);
-        if (r.k <= all_holders) {  // the next digit as well
+        if (r.k > all_holders) {
+            settled();
+        } else {  // the next digit as well
             const unsigned long long want = (unsigned long long)r.k - sh.above;
             clear();
             if (own >> 21 == bin && own) atomicAdd(&sh.bins[own >> 10 & 2047], 1ull);
@@ -557,6 +567,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads) k_sample_long(
         const double part = ceil(r.p * (double)all_live);
         find_bin(sh, part < 1.0 ? 1ull : part < (double)all_live ? (unsigned long long)part : all_live);
         floor_key = max(1u, (uint32_t)sh.bin << 21);
+        settled();
     }
     if (r.min_p > 0.0 && !(cut_k && r.cut_p)) {  // top_p of the k largest needs them all
         const double x = (double)value_of(top), raw = x + r.t * log(r.min_p), at = raw - 1e-6 * (fabs(x) + fabs(raw) + r.t);
@@ -624,11 +635,16 @@ template <typename T> __global__ void __launch_bounds__(kThreads) k_sample_long(
     }
     __syncthreads();
     // the cut at which the sum of `of` over the keys reaches `want`, by digits of 11, 11 and 10 bits; `last`: keys that
-    // equal it are counted by `extra` alone
+    // equal it are counted by `extra` alone.  The first digit is `digit`, if that is known.
     auto cut_at = [&](unsigned long long want, auto of, uint32_t last, unsigned long long extra) {
         uint32_t prefix = 0, mask = 0;
         const int shifts[3] = {21, 10, 0};
-        for (int d = 0; d < 3; d++) {
+        if (digit >= 0) {
+            prefix = (uint32_t)digit << 21;
+            mask = 0x7FFu << 21;
+            want -= above;
+        }
+        for (int d = digit >= 0 ? 1 : 0; d < 3; d++) {
             const int shift = shifts[d];
             clear();
             each([&](uint32_t key, int) {
@@ -646,19 +662,25 @@ template <typename T> __global__ void __launch_bounds__(kThreads) k_sample_long(
         return Cut{prefix, (int64_t)((want + one - 1) / one)};
     };
     Cut cut{1, (int64_t)1 << 40};  // nothing is cut
-    if (cut_k) cut = cut_at((unsigned long long)r.k, [](uint32_t) { return 1ull; }, 0, 0);
+    if (cut_k) {
+        cut = cut_at((unsigned long long)r.k, [](uint32_t) { return 1ull; }, 0, 0);
+        digit = -1;
+    }
     if (r.cut_p) {
-        unsigned long long sum = 0;
-        each([&](uint32_t key, int) {
-            if (key > cut.key) sum += weight(key);
-        });
-        sum = wave_sum(sum);
-        if (tid == 0) sh.all = 0;
-        __syncthreads();
-        if (lane == 0) atomicAdd(&sh.all, sum);
-        __syncthreads();
-        const unsigned long long extra = cut.key > 1 ? (unsigned long long)cut.count * weight(cut.key) : 0;
-        const unsigned long long all = sh.all + extra;
+        unsigned long long extra = 0, all = all_live;
+        if (cut_k) {
+            unsigned long long sum = 0;
+            each([&](uint32_t key, int) {
+                if (key > cut.key) sum += weight(key);
+            });
+            sum = wave_sum(sum);
+            if (tid == 0) sh.all = 0;
+            __syncthreads();
+            if (lane == 0) atomicAdd(&sh.all, sum);
+            __syncthreads();
+            extra = cut.key > 1 ? (unsigned long long)cut.count * weight(cut.key) : 0;
+            all = sh.all + extra;
+        }
         const double part = ceil(r.p * (double)all);
         const unsigned long long want = part < 1.0 ? 1ull : part < (double)all ? (unsigned long long)part : all;
         cut = cut_at(want, weight, cut.key, extra);
