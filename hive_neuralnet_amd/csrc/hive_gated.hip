@@ -25,6 +25,9 @@ namespace {
 
 using namespace hm;
 
+// whether the gradients of gate and up are held times a power of two: k_gated_most
+template <typename T> constexpr bool is_scaled = std::is_same_v<T, f16>;
+
 constexpr int64_t kMaxRows = 1 << 20, kMaxCols = 1 << 19;
 constexpr int64_t kMaxArea = (int64_t)1 << 35;  // a launch has under 2^32 threads, 256 for a piece of 64 x 64
 
@@ -66,6 +69,18 @@ template <bool kSlope> __device__ __forceinline__ float act_of(int act, float g,
     }
     if (kSlope) slope = share * (1.0f + held * (1.0f - share));
     return g == -__builtin_inff() ? 0.0f : g * share;
+}
+
+// dgate and dup of 8 values
+__device__ __forceinline__ void slopes_of(int act, const float (&dh)[8], const float (&g)[8], const float (&u)[8],
+                                          float (&dg)[8], float (&du)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        float slope;
+        const float a = act_of<true>(act, g[k], slope);
+        dg[k] = dh[k] * u[k] * slope;
+        du[k] = dh[k] * a;
+    }
 }
 
 struct Forward {
@@ -120,14 +135,75 @@ inline int slope_each(int64_t rows, int64_t cut) {  // rows a thread takes: 8, o
     return each;
 }
 
+// The largest finite dgate or dup in size, one of each block's share.  Memory bound.
+//
+// dgate and dup go into their products in the tensors' 16 bits, once rounded: dx and dW are 1.35 to 1.4 times as far from the
+// exact ones as they would be by float32 (which their own rounding leaves 1), a second part of 16 bits would double both
+// products' time.  bfloat16 has float32's range.  Of float16 a scaled loss's dh up passes 65,504, and an unscaled one's is
+// under 6e-8, where dx and dW are neither: they are held times the power of two that takes the largest to 2^14 .. 2^15, which
+// leaves 29 octaves at full precision below it, and the products' sums are multiplied back.  It has to be known before the
+// first of them is rounded: a pass of its own over dh, gate and up.
+constexpr int kMostBlocks = 1024;
+template <typename T>
+__global__ void __launch_bounds__(256)
+k_gated_most(const T* __restrict__ dh, int64_t dh_stride, const float* __restrict__ gate, const float* __restrict__ up,
+             int64_t rows, int hidden, int act, float* __restrict__ most) {
+    const int across = (hidden + 7) / 8;
+    const bool small = rows * across < (int64_t)1 << 31;
+    float own = 0.0f;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * across; i += kMostBlocks * 256) {
+        const int64_t r = small ? (int64_t)((uint32_t)i / (uint32_t)across) : i / across;
+        const int c = (int)(i - r * across) * 8, live = hidden - c;
+        float v[8], g[8], u[8], both[2][8];
+        load_some<T, 8>(dh + r * dh_stride + c, live, v);
+        load_some<float, 8>(gate + r * hidden + c, live, g);
+        load_some<float, 8>(up + r * hidden + c, live, u);
+        slopes_of(act, v, g, u, both[0], both[1]);
+#pragma unroll
+        for (int w = 0; w < 2; w++)
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const float size = __builtin_fabsf(both[w][k]);
+                own = k < live && size < __builtin_inff() && size > own ? size : own;
+            }
+    }
+    own = group_join<64>(own, [](float a, float b) { return fmaxf(a, b); });
+    __shared__ float waves[4];
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = own;
+    __syncthreads();
+    if (threadIdx.x == 0) most[blockIdx.x] = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
+}
+// the power of two that takes the largest of them to 2^14 .. 2^15, the same in all threads of a block of 256
+__device__ __forceinline__ int most_exponent(const float* most) {
+    float own = 0.0f;
+    for (int i = threadIdx.x; i < kMostBlocks; i += 256) own = fmaxf(own, most[i]);
+    own = group_join<64>(own, [](float a, float b) { return fmaxf(a, b); });
+    __shared__ float waves[4];
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = own;
+    __syncthreads();
+    own = fmaxf(fmaxf(waves[0], waves[1]), fmaxf(waves[2], waves[3]));
+    int e = 15;
+    if (own > 0.0f) frexpf(own, &e);
+    return max(-113, min(15 - e, 100));
+}
+
 // dgate and dup from dh, gate and up: rows of parts [dgate | dup], each `cut` values with zeros past its own; with `sums`, the
-// sums of each over the block's rows: sums[row block][2][hidden].  Memory bound; a thread takes 8 columns of `each` rows.
+// sums of each over the block's rows: sums[row block][2][hidden].  With `most`, times 2^e of it, and 2^-e to `back`.  Memory
+// bound; a thread takes 8 columns of `each` rows.
 template <typename T, typename P, int kParts>
 __global__ void __launch_bounds__(256)
 k_gated_slopes(const T* __restrict__ dh, int64_t dh_stride, const float* __restrict__ gate, const float* __restrict__ up,
                int64_t rows, int hidden, int act, P* __restrict__ d, int64_t d_stride, int cut, int across, int each,
-               float* __restrict__ sums) {
+               float* __restrict__ sums, const float* __restrict__ most, float* __restrict__ back) {
     __shared__ float lds[2][256][9];
+    float factor = 1.0f;
+    if constexpr (is_scaled<T>) {
+        if (most) {
+            const int e = most_exponent(most);
+            factor = ldexpf(1.0f, e);
+            if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *back = ldexpf(1.0f, -e);
+        }
+    }
     const int groups = 256 / across, group = threadIdx.x / across, c0 = (int)blockIdx.y * across * 8;
     const int c = c0 + threadIdx.x % across * 8, live = hidden - c;
     const int64_t r0 = (int64_t)blockIdx.x * groups * each;
@@ -152,7 +228,7 @@ k_gated_slopes(const T* __restrict__ dh, int64_t dh_stride, const float* __restr
             for (int w = 0; w < 2; w++) {
                 sum[w][k] += both[w];
                 P part[kParts];
-                split<P, kParts>(both[w], part);
+                split<P, kParts>(is_scaled<T> ? both[w] * factor : both[w], part);
 #pragma unroll
                 for (int p = 0; p < kParts; p++) q[w][p][k] = part[p];
             }
@@ -197,11 +273,13 @@ k_join_sums(const float* __restrict__ sums, int64_t blocks, int hidden, T* __res
 }
 
 // out[m][n] of a turned B, and A by its rows or turned: row r of the result is row r of `first`, row cut + r row r of `second`,
-// `rows` of each; with more than one split (grid y) each leaves its part of the sums in `part[split][m][n]` instead
+// `rows` of each; with more than one split (grid y) each leaves its part of the sums in `part[split][m][n]` instead.  back:
+// what the sums of float16 are multiplied by.
 struct Product {
     Operand a, b, b_second;
     void *first, *second;
     float* part;
+    const float* back;
     int m, n, rows, cut, cut_k;  // cut_k: the slice from which k goes on in b_second
     int tiles_m, tiles_n, slices, each;  // each: slices that a split takes
 };
@@ -215,13 +293,14 @@ __global__ void __launch_bounds__(Tl::kThreads, Tl::kWavesEach) k_product(Produc
     multiply<Tl, 1, kTurnedA, true>(f.a, m0, f.b, f.b_second, n0, f.cut_k, begin, end, lds, s);
     constexpr int run = 4 * Tl::kFn;
     const int n = n0 + s.first_col(), live = f.n - n;
+    const float back = is_scaled<T> ? *f.back : 1.0f;
 #pragma unroll
     for (int i = 0; i < Tl::kFm; i++) {
         const int m = m0 + s.row() + i * 16;
         if (m >= f.m) continue;
         float v[run];
 #pragma unroll
-        for (int e = 0; e < run; e++) v[e] = s.acc[i][e / 4][e % 4];
+        for (int e = 0; e < run; e++) v[e] = is_scaled<T> ? s.acc[i][e / 4][e % 4] * back : s.acc[i][e / 4][e % 4];
         if (f.part) {
             store_row<float, run>(f.part + ((int64_t)blockIdx.y * f.m + m) * f.n + n, live, v);
         } else if (m < f.rows) {
@@ -386,18 +465,6 @@ __global__ void __launch_bounds__(kNarrowThreads, 2) k_narrow_forward(Narrow f) 
                 store_some<float, 4>(f.up + to + j * 16, live, u);
             }
         }
-    }
-}
-
-// dgate and dup of 8 values
-__device__ __forceinline__ void slopes_of(int act, const float (&dh)[8], const float (&g)[8], const float (&u)[8],
-                                          float (&dg)[8], float (&du)[8]) {
-#pragma unroll
-    for (int k = 0; k < 8; k++) {
-        float slope;
-        const float a = act_of<true>(act, g[k], slope);
-        dg[k] = dh[k] * u[k] * slope;
-        du[k] = dh[k] * a;
     }
 }
 
@@ -743,7 +810,7 @@ int forward(const void* x, int64_t rows, int64_t cols, int64_t x_stride, const v
 // Product's; k values in all, those from cut_k on of b_second.
 template <typename T, bool kTurnedA>
 int product(const Operand& a, const Operand& b, const Operand& b_second, int64_t m, int64_t k, int64_t cut_k, int64_t rows,
-            int64_t cut, void* first, void* second, int64_t n, Arena& ws, hipStream_t st) {
+            int64_t cut, void* first, void* second, int64_t n, const float* back, Arena& ws, hipStream_t st) {
     return with_tile<T>(m, n, k, 256, [&](auto tile, int64_t splits) {
         using Tl = decltype(tile);
         constexpr int deep = 32 * Tl::kSteps;
@@ -753,6 +820,7 @@ int product(const Operand& a, const Operand& b, const Operand& b_second, int64_t
         f.b_second = b_second;
         f.first = first;
         f.second = second;
+        f.back = back;
         f.m = (int)m;
         f.n = (int)n;
         f.rows = (int)rows;
@@ -806,10 +874,18 @@ int backward(const void* dh, int64_t dh_stride, const void* x, int64_t rows, int
     const bool biases = dbg || dbu;
     char* d = ws.take(rows * d_bytes);
     float* sums = biases ? (float*)ws.take(blocks * 2 * hidden * 4) : nullptr;
+    float* const most = is_scaled<T> && (dx || dwg) ? (float*)ws.take((kMostBlocks + 1) * 4) : nullptr;
+    float* const back = most ? most + kMostBlocks : nullptr;
     int e = 0;
-    if (ws.p) {
+    if constexpr (is_scaled<T>) {
+        if (ws.p && most) {
+            k_gated_most<T><<<kMostBlocks, 256, 0, st>>>((const T*)dh, dh_stride, gate, up, rows, (int)hidden, act, most);
+            e = launched();
+        }
+    }
+    if (ws.p && !e) {
         k_gated_slopes<T, P, parts><<<dim3((unsigned)blocks, (unsigned)((cut + across * 8 - 1) / (across * 8))), 256, 0, st>>>(
-            (const T*)dh, dh_stride, gate, up, rows, (int)hidden, act, (P*)d, d_bytes / 2, (int)cut, across, each, sums);
+            (const T*)dh, dh_stride, gate, up, rows, (int)hidden, act, (P*)d, d_bytes / 2, (int)cut, across, each, sums, most, back);
         e = launched();
         if (!e && biases) e = join_sums<T>(sums, blocks, hidden, dbg, dbu, st);
     }
@@ -820,8 +896,8 @@ int backward(const void* dh, int64_t dh_stride, const void* x, int64_t rows, int
     if (dx) operands<T>(weights, 2, hidden, cols, cols, ws, packing, w);
     if (dwg) operands<T>(&x, 1, rows, cols, x_stride, ws, packing, &b);
     if (!e && ws.p) e = pack<T>(packing, st);
-    if (!e && dx) e = product<T, false>(grads, w[0], w[1], rows, 2 * cut, cut, rows, rows, dx, nullptr, cols, ws, st);
-    if (!e && dwg) e = product<T, true>(grads, b, b, 2 * cut, rows, 1 << 30, hidden, cut, dwg, dwu, cols, ws, st);
+    if (!e && dx) e = product<T, false>(grads, w[0], w[1], rows, 2 * cut, cut, rows, rows, dx, nullptr, cols, back, ws, st);
+    if (!e && dwg) e = product<T, true>(grads, b, b, 2 * cut, rows, 1 << 30, hidden, cut, dwg, dwu, cols, back, ws, st);
     return e;
 }
 
