@@ -16,13 +16,14 @@ template <typename T, int kParts> __device__ __forceinline__ void split(float v,
         part[1] = (T)(v - (float)part[0]);
     } else {
         // the largest bfloat16: values that would round to inf keep to it, their other parts make up the rest.  What is inf or
-        // NaN itself has it in its first part, and zeros in the others.
+        // NaN itself has it in its last part, which meets the other factor's first alone, and that is 0 only where the factor
+        // is (its other parts may be, and inf times them NaN); 1 of its sign in its first, which the other's own inf meets.
         const float top = __uint_as_float(0x7F7F0000u);
         const bool finite = __builtin_fabsf(v) < __builtin_inff();
-        part[0] = (T)(finite ? __builtin_amdgcn_fmed3f(v, -top, top) : v);
+        part[0] = (T)(finite ? __builtin_amdgcn_fmed3f(v, -top, top) : __builtin_copysignf(1.0f, v));
         const float r = finite ? v - (float)part[0] : 0.0f;
         part[1] = (T)r;
-        part[2] = (T)(r - (float)part[1]);
+        part[2] = (T)(finite ? r - (float)part[1] : v);
     }
 }
 // element of column c, part p, in a row of parts

@@ -596,7 +596,7 @@ int hg_adamw_step(const hg_adamw_tensor* tensors, int64_t count, int param_type,
  * pass needs, are float, both given or both NULL (rounding them to 16 bits would
  * be a third of its results' error).  Sums are float32; float32 tensors are
  * multiplied in three bfloat16 parts a value, 24 bits (values below 2^-110 to
- * within 2^-134).  rows <= 2^20, cols and
+ * within 2^-134; an infinity times one below 2^-126 may be NaN).  rows <= 2^20, cols and
  * hidden <= 2^19, each two of them at most 2^35 together.  workspace: as many bytes, 256-byte aligned (none where that
  * is 0). */
 #define HG_SIGMOID 0

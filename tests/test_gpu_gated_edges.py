@@ -1,12 +1,72 @@
-"""The gated block at the ends of its numbers: float16
-gradients past its range.  References and tolerances:
+"""The gated block at the ends of its numbers: infinities of float32 tensors,
+float16 gradients past its range.  References and tolerances:
 test_gpu_network_ops.py."""
+import math
+
 import pytest
 import torch
 
-from test_gpu_network_ops import F16, U, _act, _gated, ext  # noqa: F401
+from test_gpu_network_ops import BF16, F16, F32, U, _act, _gated, _randn, ext  # noqa: F401
 
 pytestmark = pytest.mark.gpu
+
+
+def _same_kind(got, want, what):
+    """inf, -inf and NaN where `want` has them, and nowhere else."""
+    got, want = got.double(), want.double()
+    assert torch.equal(got.isnan(), want.isnan()), (what, "nan")
+    assert torch.equal(got.isposinf(), want.isposinf()), (what, "inf")
+    assert torch.equal(got.isneginf(), want.isneginf()), (what, "-inf")
+    some = want.isfinite()
+    # 6 (K / 16) + 80 roundings of sums of under 512 terms that are a few times the result's size at most, here loosely
+    assert not some.any() or float((got - want)[some].abs().max()) <= 2.0 ** -14 * max(1.0, float(want[some].abs().max())), what
+
+
+@pytest.mark.parametrize("rows,cols,hidden", [(40, 122, 70), (3, 9, 5), (8192, 122, 64), (1, 300, 40)])
+def test_infinities_of_float32(ext, rows, cols, hidden):  # noqa: F811
+    """An infinity times a number is an infinity of its sign and times 0 NaN, as of 16-bit tensors: in x, in the weights, in
+    both, in a sum with one of the other sign."""
+    x, wg, wu, _, _, _ = _gated(rows, cols, hidden, F32, 5)
+    x[rows // 2, cols - 1] = math.inf
+    wg[:, cols - 1], wu[:, cols - 1] = 0.5, -0.5  # whose second and third parts are 0
+    wu[hidden - 1, cols - 1] = 0.0
+    wg[hidden // 2, cols - 1] = -0.75
+    wu[0, 2], wg[1, 1] = -math.inf, math.inf
+    x[0, 2] = math.inf
+    if rows > 2:
+        x[2, 2], x[1, 1] = 0.0, -2.0
+    _, gate, up = ext.gated_linear_forward(x, wg, wu, activation="sigmoid")
+    for got, w, what in ((gate, wg, "gate"), (up, wu, "up")):
+        _same_kind(got, _products(x, w), what)
+    h = ext.gated_linear(x, wg, wu, activation="sigmoid")
+    _same_kind(h, torch.sigmoid(_products(x, wg)) * _products(x, wu), "h")
+
+
+def _products(x, w):
+    """x w^T in 64 bits, each product for itself, so that infinities meet nothing but their own factor."""
+    return torch.stack([(x.double() * one).sum(1) for one in w.double()], 1)
+
+
+@pytest.mark.parametrize("rows,cols,hidden", [(40, 122, 70), (8192, 122, 64)])
+def test_infinities_of_float32_gradients(ext, rows, cols, hidden):  # noqa: F811
+    """An infinite gradient of one unit of one row: the infinities of its row of dx, of its unit's weights, and no others."""
+    x, wg, wu, bg, bu, dh = _gated(rows, cols, hidden, F32, 6)
+    x[7] = x[7].bfloat16().float()  # one part each
+    x[7, 5] = 0.0
+    wg[9], wu[9] = wg[9].bfloat16().float(), wu[9].bfloat16().float()
+    _, gate, up = ext.gated_linear_forward(x, wg, wu, bg, bu)
+    dh[7, 9] = math.inf
+    dx, dwg, dwu, dbg, dbu = ext.gated_linear_backward(dh, x, wg, wu, gate, up)
+    a, slope, _ = _act("silu", gate.double())
+    dgate, dup = dh.double() * up.double() * slope, dh.double() * a
+    rest = torch.arange(rows, device="cuda") != 7
+    assert dx[rest].isfinite().all()
+    _same_kind(dx[7], (dgate[7].unsqueeze(1) * wg.double()).sum(0) + (dup[7].unsqueeze(1) * wu.double()).sum(0), "dx")
+    for got, d, what in ((dwg, dgate, "dw_gate"), (dwu, dup, "dw_up")):
+        one = torch.arange(hidden, device="cuda") == 9
+        assert got[~one].isfinite().all(), what
+        _same_kind(got[9], (d[:, 9:10] * x.double()).sum(0), what)
+    assert dbg[9] == dgate[7, 9] and dbu[9] == dup[7, 9]
 
 
 def _float16_case(rows, scale_dh, scale_x, scale_w, gate_bias, up_bias, seed):
