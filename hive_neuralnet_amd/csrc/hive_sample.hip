@@ -66,14 +66,14 @@ __device__ __forceinline__ Row row_of(const Settings& s, int64_t b) {
     r.t = s.temperatures ? (double)s.temperatures[b] : s.temperature;
     r.p = s.top_ps ? (double)s.top_ps[b] : s.top_p;
     r.min_p = s.min_ps ? (double)s.min_ps[b] : s.min_p;
-    r.min_p = r.min_p > 1.0 ? 1.0 : r.min_p;  // the largest always stays
+    r.min_p = r.min_p > 0.0 ? fmin(r.min_p, 1.0) : 0.0;  // the largest always stays; NaN: 0
     const int64_t k = s.top_ks ? s.top_ks[b] : s.top_k;
     r.k = k > 0 ? k : 0;
     r.u = (double)s.uniforms[b];
     r.u = r.u > 0.0 ? r.u : 0.0;  // NaN: 0
-    r.greedy = !(r.t > 0.0);
+    r.greedy = !(r.t > 0.0);  // NaN, too
     r.scale = 1.4426950408889634 / r.t;
-    r.cut_p = r.p < 1.0;
+    r.cut_p = r.p < 1.0;  // NaN: no cut
     return r;
 }
 

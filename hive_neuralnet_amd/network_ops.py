@@ -348,7 +348,8 @@ def sample_actions(self, logits: torch.Tensor, uniforms: torch.Tensor, num_actio
     which the running sum of exp((x - max) / temperature) passes u times the
     whole; a temperature of 0 takes the largest logit's first slot.  Each
     setting is a number, or a tensor of a value a row (float32; top_k int64; what
-    lies past its range counts as its end)."""
+    lies past its range counts as its end; NaN as a temperature of 0, a top_p of 1,
+    a min_p or uniform number of 0)."""
     if _calls is not None:
         done = _calls.sample_actions(logits, uniforms, num_actions, temperature, top_k, top_p, min_p)
         if done is not None:

@@ -670,7 +670,8 @@ int hg_muon_step(const hg_muon_matrix* matrices, int64_t count, int param_type, 
  * the running sum of the weights kept, exp((x - max) / T), passes u times their
  * whole.  T not above 0: the largest logit's first slot, of probability 1.
  * Each setting is an array of a value a row, or where that is NULL the number
- * beside it.  width <= 2^20, rows <= 2^25 (2^21 of more
+ * beside it.  NaN: a temperature takes the largest, top_p and min_p leave all, a
+ * uniform number is 0.  width <= 2^20, rows <= 2^25 (2^21 of more
  * than 1,024 slots). */
 int hg_sample_actions(const void* logits, int type, int64_t rows, int64_t width, int64_t stride,
                       const int64_t* num_actions, const float* uniforms, const float* temperatures, double temperature,
