@@ -12,8 +12,11 @@
 // first steps, and with them what rounding has put in their place: at 16-bit
 // rounding that would be the result.  Every matrix is held as two float16 parts a
 // value, 22 bits, times 2^13 (entries are below 2 in size and mostly far below 1;
-// their last parts stay above float16's smallest), and products are three
-// matrix instructions of parts (hive_matrix.hpp).
+// the last parts of those above 2^-15 stay above float16's smallest, which holds
+// the others to within 2^-38), and products are three matrix instructions of parts
+// (hive_matrix.hpp).  |U| far below eps makes all of X small: a matrix is held times
+// the power of two that takes its norm to between 1/2 and 1, and P takes that share
+// of b and c, and of itself where the next X is held times less (Size).
 //
 // Measured (MI355X): 16 matrices of 1,024 x 1,024 and 8 of 4,096 x 1,024, an iteration A 190 us, P 115, P X 298 (270, 220 and
 // 350 TFLOP/s, three times that of float16 instructions, 810, 670 and 1,040; large library products reach 1,100 to 1,520),
@@ -36,6 +39,7 @@ constexpr float kScale = 8192.0f;    // of X and A as they are held: entries up 
 constexpr float kScaleP = 1024.0f;   // of P, which has a on its diagonal: up to 63
 constexpr int kSumBlocks = 64;       // of a matrix's sum of squares
 constexpr int kTriples = 16;         // coefficients that a launch of the whole iteration takes
+constexpr int kMostSteps = 100;
 constexpr int64_t kMaxSide = 1 << 17;
 
 // One of the step's matrices, or a batch of one shape.
@@ -55,16 +59,22 @@ struct Table {
     int range[9];  // chiplet x's tiles of a product: [range[x], range[x + 1])
     int g_type, out_type, update;  // update: out is a parameter
     float mu, keep, eps, a, b, c;
-    int nesterov, from, last;  // from: which of the two copies of X is current
+    int nesterov, from, step, last;  // from: which of the two copies of X is current
     int steps, count;          // the iteration in one launch: its steps, and how many of them have coefficients of their own
     float triples[3 * kTriples];
 };
 
-// where a matrix's parts lie in its workspace, in bytes
+// How a matrix is held at a step: X 2^e, of norm `most` or less.
+struct Size {
+    int e;
+    float most;
+};
+
+// where a matrix's parts lie in its workspace, in bytes; sizes: a Size of each step
 struct Layout {
     int s, l;                // the shorter and the longer side
     int64_t sb, lb;          // bytes of a packed row along each
-    int64_t x[2], a, p, sums, all;
+    int64_t x[2], a, p, sums, sizes, all;
 };
 __host__ __device__ inline Layout layout(int rows, int cols) {
     Layout o;
@@ -81,8 +91,39 @@ __host__ __device__ inline Layout layout(int rows, int cols) {
     o.a = at;
     o.p = at + a;
     o.sums = at + 2 * a;
-    o.all = o.sums + up_to(kSumBlocks * 8, 256);
+    o.sizes = o.sums + up_to(kSumBlocks * 8, 256);
+    o.all = o.sizes + up_to((kMostSteps + 1) * sizeof(Size), 256);
     return o;
+}
+
+// X = U / (norm + eps) at first: its share of 1, a power of two and what is left of it
+__device__ __forceinline__ Size first_size(double norm, double eps) {
+    const double share = norm / (norm + eps);
+    int k = 0;
+    if (share > 0.0 && share < 1.0) frexp(share, &k);  // NaN: as it is
+    return {-k, 1.0f};
+}
+// ... and after a step: |P| is at most |a| + |b| t^2 + |c| t^4, t = |X|.  A matrix that is held as it is (e = 0) is not held
+// times less, however large the bound.
+__device__ __forceinline__ Size next_size(Size x, float a, float b, float c) {
+    const float t = ldexpf(x.most, -x.e), q = t * t;
+    const float most = x.most * (__builtin_fabsf(a) + __builtin_fabsf(b) * q + __builtin_fabsf(c) * q * q);
+    int k = 0;
+    if (most > 0.0f && most < __builtin_inff()) frexpf(most, &k);
+    k = min(k, x.e);
+    return {x.e - k, ldexpf(most, -k)};
+}
+// what U is multiplied by, times kScale and x's power of two: v * by 2^e, which no size of U takes past float32's range
+struct Factor {
+    float by;
+    int e;
+    __device__ __forceinline__ float operator()(float v) const { return ldexpf(v, e) * by; }
+};
+__device__ __forceinline__ Factor factor_of(double norm, double eps, Size x) {
+    const double all = (double)kScale / (norm + eps);
+    int k = 0;
+    const double by = all < __builtin_inf() ? frexp(all, &k) : all;  // inf of a norm and an eps of 0, NaN
+    return {(float)by, k + x.e};
 }
 
 // the matrix that block t works on, t from there on its own
@@ -150,7 +191,9 @@ template <typename G> __global__ void __launch_bounds__(256) k_muon_pack(Table t
     char* held = x.held + matrix * o.all;
     double sum = ((const double*)(held + o.sums))[threadIdx.x & 63];
     for (int k = 1; k < 64; k <<= 1) sum += __shfl_xor(sum, k, 64);
-    const float scale = (float)((double)kScale / (sqrt(sum) + (double)tab.eps));
+    const Size size = first_size(sqrt(sum), tab.eps);
+    const Factor scaled = factor_of(sqrt(sum), tab.eps, size);
+    if (piece == 0 && threadIdx.x == 0) *(Size*)(held + o.sizes) = size;
     const int r0 = piece / pieces_c * 64, c0 = piece % pieces_c * 64;
     const bool tall = x.rows > x.cols;
 #pragma unroll
@@ -161,7 +204,7 @@ template <typename G> __global__ void __launch_bounds__(256) k_muon_pack(Table t
             load_update<G, false>(x, tab, matrix * x.g_step + r * x.g_row + c, (int64_t)r * x.cols + c, x.cols - c, u);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            u[e] *= scale;
+            u[e] = scaled(u[e]);
             if (tall) turn[a][b + e] = u[e];
         }
         if (!tall && r < o.s && c < up_to(o.l, 32)) store_parts((f16*)(held + o.x[0] + r * o.lb), c, u);
@@ -262,6 +305,7 @@ __global__ void __launch_bounds__(Tl::kBlock, Tl::kWavesEach) k_muon_product(Tab
         b = {held + (tab.from ? o.x[1] : o.x[0]), o.lb, o.s, (int)o.lb};
     }
     const int m0 = at.m * Tl::kM, n0 = at.n * Tl::kN;
+    Size* const sizes = (Size*)(held + o.sizes) + tab.step;
     Sums<Tl, 1, kKind == kStep> s;
     multiply<Tl, 1, false, kKind == kStep>(a, m0, b, b, n0, 1 << 30, 0, (a.bytes + Tl::kRow - 1) / Tl::kRow, lds, s);
     if (Tl::kTeams > 1 && threadIdx.x >= Tl::kThreads) return;
@@ -273,6 +317,16 @@ __global__ void __launch_bounds__(Tl::kBlock, Tl::kWavesEach) k_muon_product(Tab
     const int first = n0 + s.col();
     const int across = (int)(threadIdx.x & 63) / 16;  // the lane's place among the four that share a row
     const bool mirrored = at.n > at.m;  // the tile's mirror image is stored, too: no tile computes it
+    float pa = 0.0f, pb = 0.0f, pc = 0.0f;  // P's coefficients of what is held
+    int last_e = 0;
+    if (kKind == kPoly) {
+        const int e = sizes[0].e, less = e - sizes[1].e;
+        pa = ldexpf(tab.a, -less);
+        pb = ldexpf(tab.b, -2 * e - less);
+        pc = ldexpf(tab.c, -4 * e - less);
+    }
+    if (kKind == kStep && tab.last) last_e = sizes[1].e;
+    if (kKind == kGram && at.n == 0 && threadIdx.x == 0) sizes[1] = next_size(sizes[0], tab.a, tab.b, tab.c);
 #pragma unroll
     for (int i = 0; i < Tl::kFm; i++) {
         const int m = m0 + s.row() + i * 16;
@@ -290,12 +344,12 @@ __global__ void __launch_bounds__(Tl::kBlock, Tl::kWavesEach) k_muon_product(Tab
                 if (there && live > 0) load_parts((const f16*)(held + o.a) + m * row, n, g);
 #pragma unroll
                 for (int e = 0; e < 8; e++)
-                    v[e] = fmaf(tab.c, v[e], tab.b * g[e]) * (kScaleP / kScale) + (n + e == m ? tab.a * kScaleP : 0.0f);
+                    v[e] = fmaf(pc, v[e], pb * g[e]) * (kScaleP / kScale) + (n + e == m ? pa * kScaleP : 0.0f);
             }
             if (kKind == kStep && tab.last) {
                 if (!there || live <= 0) continue;
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[e] *= 1.0f / kScale;
+                for (int e = 0; e < 8; e++) v[e] = ldexpf(v[e] * (1.0f / kScale), -last_e);
                 // a turned matrix: column n of the result is row n of X's
                 if (tall) store_result<true>(x, tab, matrix * x.out_step + (int64_t)n * x.cols + m, x.cols, live, v);
                 else store_result<false>(x, tab, matrix * x.out_step + (int64_t)m * x.cols + n, 1, live, v);
@@ -407,14 +461,15 @@ __global__ void __launch_bounds__(1024) k_muon_small(Table tab) {
     __syncthreads();
     sum = 0.0;
     for (int i = 0; i < 16; i++) sum += waves[i];
-    const float scale = (float)((double)kScale / (sqrt(sum) + (double)tab.eps));
+    Size size = first_size(sqrt(sum), tab.eps);
+    const Factor scaled = factor_of(sqrt(sum), tab.eps, size);
 #pragma unroll
     for (int k = 0; k < kEach; k++) {
         const int i = k * 1024 + tid;
         if (i >= n) continue;
         const int of = row_of(i), in = i - of * cols, r = tall ? in : of, c = tall ? of : in;
         f16 part[2];
-        split<f16, 2>(u[k] * scale, part);
+        split<f16, 2>(scaled(u[k]), part);
         *(f16*)(lx + r * kRowX + byte(r, c, 0)) = part[0];
         *(f16*)(lx + r * kRowX + byte(r, c, 1)) = part[1];
     }
@@ -467,12 +522,16 @@ __global__ void __launch_bounds__(1024) k_muon_small(Table tab) {
         for (int j = 0; j < kPieces; j++)
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const float o = next[j][e] * (1.0f / kScaleP / kScale);
+                const float o = ldexpf(next[j][e] * (1.0f / kScaleP / kScale), -size.e);
                 if (at[j][e] >= 0) out[at[j][e]] = from_f32<P>(tab.update ? fmaf(-x.rate, o, old[j][e] * tab.keep) : o);
             }
     };
     for (int step = 0; step < tab.steps; step++) {
         const float* abc = tab.triples + 3 * min(step, tab.count - 1);
+        const Size next_s = next_size(size, abc[0], abc[1], abc[2]);
+        const int less = size.e - next_s.e;
+        const float pa = ldexpf(abc[0], -less), pb = ldexpf(abc[1], -2 * size.e - less), pc = ldexpf(abc[2], -4 * size.e - less);
+        size = next_s;
         f4 sum_a = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < kL / 32; k++) {
@@ -494,8 +553,8 @@ __global__ void __launch_bounds__(1024) k_muon_small(Table tab) {
         }
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            v[e] = fmaf(abc[2], sum_p[e] * (1.0f / kScale), abc[1] * v[e]) * (kScaleP / kScale) +
-                   (pn * 16 + g * 4 + e == r ? abc[0] * kScaleP : 0.0f);
+            v[e] = fmaf(pc, sum_p[e] * (1.0f / kScale), pb * v[e]) * (kScaleP / kScale) +
+                   (pn * 16 + g * 4 + e == r ? pa * kScaleP : 0.0f);
         keep(lp, kRowA, r, pn * 16 + g * 4, v);
         __syncthreads();
         h8 p[kSmall / 32][2];
@@ -647,6 +706,7 @@ int iterate(Table& all, int steps, const float* coefficients, int64_t triples, h
         tab.a = c[0];
         tab.b = c[1];
         tab.c = c[2];
+        tab.step = i;
         tab.last = i == steps - 1;
         e = product<kGram>(tab, st);
         if (!e) e = product<kPoly>(tab, st);
@@ -657,7 +717,7 @@ int iterate(Table& all, int steps, const float* coefficients, int64_t triples, h
 }
 
 bool bad_settings(int steps, const float* coefficients, int triples, float eps) {
-    return steps < 1 || steps > 100 || !coefficients || triples < 1 || !(eps >= 0.0f);
+    return steps < 1 || steps > kMostSteps || !coefficients || triples < 1 || !(eps >= 0.0f);
 }
 // a launch has under 2^32 threads, 256 for a piece of 64 x 64
 bool bad_shape(int64_t count, int64_t rows, int64_t cols) {

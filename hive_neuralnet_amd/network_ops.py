@@ -189,8 +189,8 @@ def orthogonalize(self, u: torch.Tensor, steps: int = 5, coefficients=COEFFICIEN
 
     u float32 / float16 / bfloat16, its rows contiguous, rows and matrices
     evenly spaced; the result has its shape and type and is contiguous.  Matrices
-    are held in 22 bits a value between the products, which are summed in
-    float32; a, b and c may be such that X's entries stay below 7.9 in size and
+    are held in 22 bits a value between the products (or to within 2^-37 of their
+    norm, where that is more), which are summed in float32; a, b and c may be such that X's entries stay below 7.9 in size and
     those of a I + b A + c A A below 63."""
     dev = _float_tensor(u, "u")
     if u.dim() < 2 or u.shape[-1] == 0 or u.shape[-2] == 0:

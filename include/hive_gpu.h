@@ -629,9 +629,10 @@ int hg_gated_backward(const void* dh, int64_t dh_stride, const void* x, int type
  *   times X <- a X + (b A + c A A) X, A = X X^T (X turned where it is taller than
  *   wide), (a, b, c) = coefficients[i] for step i, the last of the `triples` for
  *   the steps past them (host memory, read before the call returns)
- * out[count][rows][cols] has u's type.  Values are held in 22 bits: entries of X and
- * A up to 7.9 in size, of a I + b A + c A A up to 63; past that the result is inf or
- * NaN.  rows, cols <= 2^17, count * (rows / 64 + 1)
+ * out[count][rows][cols] has u's type.  Values are held in 22 bits, or to within 2^-37 of
+ * |X| where that is more (so from 2^-15 of |X| down; |X| is held to its own size, however far |U| is
+ * below eps): entries of X and A up to 7.9 in size, of a I + b A + c A A up to 63; past
+ * that the result is inf or NaN.  rows, cols <= 2^17, count * (rows / 64 + 1)
  * (cols / 64 + 1) <= 2049^2, count <= 2^16, steps 1 to 100.
  * workspace: as many bytes, 256-byte aligned. */
 int64_t hg_orthogonalize_workspace(int64_t count, int64_t rows, int64_t cols);

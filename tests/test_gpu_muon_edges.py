@@ -1,0 +1,81 @@
+"""Orthogonalised updates of matrices far smaller than eps, and of float32's
+smallest.  Definition and tolerances: test_gpu_network_ops.py."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_network_ops import ABC, F32, U, _check_orthogonal, _iteration, _muon_reference, _randn, ext  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def _relative(rows, cols, steps):
+    """Where |X| stays far below 1, a step is X <- a X but for what rounds: X, A and P held in 22 bits (2^-22 each of the
+    value, 2^-38 of 1 a value, |X| being held at 1/8 and more), the sum of P's and X's products ((3 K / 16 + 80) u, K the
+    shorter side), and X and the result in float32 at both ends."""
+    short, long = min(rows, cols), max(rows, cols)
+    return steps * ((3 * short / 16 + 80) * U + 3 * 2.0 ** -22 + 2.0 ** -35 * math.sqrt(short * long) + 2.0 ** -35 * short) + 8 * U
+
+
+@pytest.mark.parametrize("size", [1e-9, 1e-11, 1e-12, 1e-14, 1e-16, 1e-22])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (40, 33), (64, 200), (300, 129), (500, 700)])
+def test_far_below_eps(ext, rows, cols, size):  # noqa: F811
+    """X = U / (|U| + eps) is held as exactly where |U| is far below eps as where it is not."""
+    u = _randn((rows, cols), rows, size / math.sqrt(rows * cols))
+    want, _ = _iteration(u)
+    got = ext.orthogonalize(u)
+    # X grows 3.4445 times a step: to 485 |U| / eps in five
+    assert 300 * size / 1e-7 < float(want.norm()) < 700 * size / 1e-7 or size > 1e-10 or rows * cols == 1
+    assert float((got.double() - want).norm()) <= _relative(rows, cols, 5) * float(want.norm())
+
+
+@pytest.mark.parametrize("rows,cols", [(40, 33), (300, 129)])
+def test_between_eps_and_one(ext, rows, cols):  # noqa: F811
+    """Sizes at which the iteration leaves its straight part after one, two, ... steps; more steps; other coefficients."""
+    for i in range(12):
+        u = _randn((rows, cols), i, 10.0 ** (-10 + 0.5 * i) / math.sqrt(rows * cols))
+        _check_orthogonal(ext.orthogonalize(u), u)
+    u = _randn((rows, cols), 20, 1e-13 / math.sqrt(rows * cols))
+    for steps in (1, 2, 9, 14):
+        _check_orthogonal(ext.orthogonalize(u, steps=steps), u, steps)
+    want, _ = _iteration(u, 3, (0.25, 0.5, 0.1))  # shrinks
+    got = ext.orthogonalize(u, steps=3, coefficients=(0.25, 0.5, 0.1))
+    assert float((got.double() - want).norm()) <= _relative(rows, cols, 3) * float(want.norm())
+
+
+def test_a_batch_of_all_sizes(ext):  # noqa: F811
+    """Each matrix by its own size."""
+    for shape in ((9, 30, 50), (9, 130, 300)):
+        sizes = torch.logspace(-18, 0, 9, device="cuda")
+        u = _randn(shape, 4, 1.0 / math.sqrt(shape[1] * shape[2])) * sizes.view(-1, 1, 1)
+        got = ext.orthogonalize(u)
+        for one, g, size in zip(u, got, sizes.tolist()):
+            if size < 1e-10:
+                want, _ = _iteration(one)
+                assert float((g.double() - want).norm()) <= _relative(*shape[1:], 5) * float(want.norm())
+            else:
+                _check_orthogonal(g, one)
+
+
+@pytest.mark.parametrize("rows,cols", [(20, 30), (200, 300)])
+def test_the_smallest_floats(ext, rows, cols):  # noqa: F811
+    """Matrices whose size is under 2^13 / float's largest, and of subnormal values, with an eps of 0."""
+    for size in (1e-36, 1e-38, 1e-42):
+        u = _randn((rows, cols), 3, size)
+        assert bool(u.any())
+        _check_orthogonal(ext.orthogonalize(u, eps=0.0), u, eps=0.0)
+    u = _randn((rows, cols), 3, 1e37)
+    _check_orthogonal(ext.orthogonalize(u, eps=0.0), u, eps=0.0)
+
+
+def test_a_step_with_gradients_far_below_eps(ext):  # noqa: F811
+    params = [_randn(s, i, 1e-6) for i, s in enumerate([(64, 122), (200, 300)])]
+    before = [p.clone() for p in params]
+    grads = [_randn(p.shape, 9 + i, 1e-15 / math.sqrt(p.numel())) for i, p in enumerate(params)]
+    ext.prepare_muon(params).step(grads, lr=1.0, momentum=0.0)
+    for p, b, g in zip(params, before, grads):
+        want, _, _ = _muon_reference(b, g, torch.zeros_like(b), 1.0, 0.0, True, 0.0, "spectral")
+        moved = float((want - b.double()).norm())
+        off = float((p.double() - want).norm())
+        assert off <= 1.01 * _relative(*p.shape, 5) * moved + U * float(want.norm()) + 2 * U * float(b.norm()), (off, moved)
