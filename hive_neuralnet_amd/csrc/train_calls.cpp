@@ -321,6 +321,7 @@ PyObject* sample_actions(PyObject*, PyObject* const* a, Py_ssize_t count) {
         logits->size(1) > 1 << 20 || (logits->stride(1) != 1 && logits->size(1) > 1) || logits->numel() == 0)
         return not_here();
     const int64_t rows = logits->size(0), width = logits->size(1);
+    if (rows > (width <= 1024 ? 1 << 25 : 1 << 21)) return not_here();
     constexpr double any = std::numeric_limits<double>::infinity();
     Setting t, p, min_p, k;
     if (!is_vector(uniforms, at, rows, at::kFloat) || (a[2] != Py_None && !is_vector(counts, at, rows, at::kLong)) ||

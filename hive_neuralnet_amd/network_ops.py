@@ -29,8 +29,11 @@ _c_double = ctypes.c_double
 
 ACTIVATIONS = {"sigmoid": 0, "silu": 1, "gelu": 2}  # HG_SIGMOID, HG_SILU, HG_GELU
 MAX_ROWS, MAX_COLS = 1 << 20, 1 << 19
+MAX_AREA = 1 << 35  # of each two of a gated block's rows, columns and hidden units
 MAX_WIDTH = 1 << 20  # slots of a row that a slot is drawn from
+MAX_DRAWS, HELD, MAX_LONG_DRAWS = 1 << 25, 1024, 1 << 21  # rows, and rows of more slots than a wave holds
 MAX_SIDE = 1 << 17  # of a matrix that is orthogonalised
+MAX_MATRICES, MAX_PIECES = 1 << 16, 2049 ** 2  # of a batch: matrices, pieces of 64 x 64 of them
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # singular values of 0.001 and more end between 0.7 and 1.2 in five steps
 
 SIGS = {
@@ -90,6 +93,8 @@ def _gated_sizes(x, w_gate, w_up):
         _matrix(w, name, (hidden, cols), x)
     if rows > MAX_ROWS or cols > MAX_COLS or hidden > MAX_COLS:
         raise ValueError(f"at most {MAX_ROWS} rows, {MAX_COLS} columns and hidden units, got {rows}, {cols}, {hidden}")
+    if max(rows * cols, rows * hidden, hidden * cols) > MAX_AREA:
+        raise ValueError(f"rows, columns and hidden units at most {MAX_AREA} each two of them, got {rows}, {cols}, {hidden}")
     if stride < 0:
         raise ValueError("x's rows must be in order")
     return dev, rows, cols, stride, hidden
@@ -198,6 +203,10 @@ def orthogonalize(self, u: torch.Tensor, steps: int = 5, coefficients=COEFFICIEN
     rows, cols = u.shape[-2:]
     if rows > MAX_SIDE or cols > MAX_SIDE:
         raise ValueError(f"at most {MAX_SIDE} rows and columns, got {rows} and {cols}")
+    count = u.numel() // (rows * cols)
+    if count > MAX_MATRICES or count * (rows // 64 + 1) * (cols // 64 + 1) > MAX_PIECES:
+        raise ValueError(f"at most {MAX_MATRICES} matrices and {MAX_PIECES} pieces of 64 x 64 of them a call, got {count} "
+                         f"of {rows} x {cols}")
     c, triples = _iteration(steps, coefficients, eps)
     out = torch.empty_like(u, memory_format=torch.contiguous_format)
     if u.numel() == 0:
@@ -208,7 +217,6 @@ def orthogonalize(self, u: torch.Tensor, steps: int = 5, coefficients=COEFFICIEN
         batch = u.view(-1, rows, cols) if u.dim() != 3 else u
     except RuntimeError:
         raise ValueError("u's matrices must be evenly spaced") from None
-    count = batch.shape[0]
     ws = u.new_empty((self._lib.hg_orthogonalize_workspace(count, rows, cols),), dtype=torch.uint8)
     _check(self._lib.hg_orthogonalize(u.data_ptr(), TYPES[u.dtype], count, rows, cols, batch.stride(1), batch.stride(0),
                                       steps, c, triples, eps, out.data_ptr(), ws.data_ptr(), _raw_stream(dev)),
@@ -360,6 +368,8 @@ def sample_actions(self, logits: torch.Tensor, uniforms: torch.Tensor, num_actio
     B, width, stride = _rows(logits, "logits")
     if width > MAX_WIDTH:
         raise ValueError(f"rows of at most {MAX_WIDTH} slots, got {width}")
+    if B > (MAX_DRAWS if width <= HELD else MAX_LONG_DRAWS):
+        raise ValueError(f"at most {MAX_DRAWS} rows, {MAX_LONG_DRAWS} of more than {HELD} slots, got {B} of {width}")
     u = _vector(uniforms, "uniforms", B, torch.float32, dev)
     n = None if num_actions is None else _vector(num_actions, "num_actions", B, torch.int64, dev)
     t, t_all = _setting(temperature, "temperature", B, torch.float32, dev)
