@@ -306,6 +306,7 @@ struct Setting {
             each = t->const_data_ptr();
             return true;
         }
+        if (!PyFloat_Check(o) && !PyLong_Check(o)) return false;  // other kinds of numbers, and what is none: network_ops.py
         all = PyFloat_AsDouble(o);
         return !bad_number() && all >= 0.0 && all <= most;
     }

@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import bisect
 import ctypes
+import numbers
 
 import torch
 
@@ -62,6 +63,16 @@ def bind(lib) -> None:
     """Gives train_calls.cpp the library's function (training_ops.bind comes first)."""
     if _calls is not None:
         _calls.bind_network(ctypes.cast(lib.hg_sample_actions, _c_void_p).value)
+
+
+def _number(value, name: str, whole: bool = False):
+    """A float, or an int where it has to be whole; any kind of real number is taken (numpy's, too)."""
+    if not isinstance(value, numbers.Integral if whole else numbers.Real):
+        raise ValueError(f"{name} must be a {'whole ' if whole else ''}number, got {value!r}")
+    try:
+        return int(value) if whole else float(value)
+    except OverflowError:
+        raise ValueError(f"{name} is past a float's range") from None
 
 
 def _activation(activation) -> int:
@@ -171,17 +182,22 @@ def gated_linear_backward(self, dh: torch.Tensor, x: torch.Tensor, w_gate: torch
 
 
 def _iteration(steps, coefficients, eps):
-    """The coefficients as an array of float triples, one for all steps or one each."""
+    """(steps, eps, coefficients as an array of float triples, how many): one triple for all steps, or one each."""
+    steps, eps = _number(steps, "steps", whole=True), _number(eps, "eps")
     if not 1 <= steps <= 100:
         raise ValueError(f"steps must be 1 to 100, got {steps}")
     if not eps >= 0.0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    triples = list(coefficients)
-    if triples and isinstance(triples[0], (int, float)):
-        triples = [triples]
+    try:
+        triples = list(coefficients)
+        if triples and isinstance(triples[0], numbers.Real):
+            triples = [triples]
+        triples = [[_number(v, "a coefficient") for v in t] for t in triples]
+    except TypeError:
+        triples = []
     if not triples or any(len(t) != 3 for t in triples):
         raise ValueError(f"coefficients must be (a, b, c) or a list of such, got {coefficients}")
-    return (ctypes.c_float * (3 * len(triples)))(*[v for t in triples for v in t]), len(triples)
+    return steps, eps, (ctypes.c_float * (3 * len(triples)))(*[v for t in triples for v in t]), len(triples)
 
 
 def orthogonalize(self, u: torch.Tensor, steps: int = 5, coefficients=COEFFICIENTS, eps: float = 1e-7) -> torch.Tensor:
@@ -207,7 +223,7 @@ def orthogonalize(self, u: torch.Tensor, steps: int = 5, coefficients=COEFFICIEN
     if count > MAX_MATRICES or count * (rows // 64 + 1) * (cols // 64 + 1) > MAX_PIECES:
         raise ValueError(f"at most {MAX_MATRICES} matrices and {MAX_PIECES} pieces of 64 x 64 of them a call, got {count} "
                          f"of {rows} x {cols}")
-    c, triples = _iteration(steps, coefficients, eps)
+    steps, eps, c, triples = _iteration(steps, coefficients, eps)
     out = torch.empty_like(u, memory_format=torch.contiguous_format)
     if u.numel() == 0:
         return out
@@ -295,7 +311,9 @@ class MuonPlan:
         parameters' versions rise."""
         if len(grads) != len(self.params):
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
-        c, triples = _iteration(steps, coefficients, eps)
+        steps, eps, c, triples = _iteration(steps, coefficients, eps)
+        lr, momentum, weight_decay = (_number(v, name) for v, name in (
+            (lr, "lr"), (momentum, "momentum"), (weight_decay, "weight_decay")))
         kind = next((g.dtype for g in grads if g is not None), torch.float32)
         if kind not in TYPES:
             raise ValueError(f"gradients must be float32, float16 or bfloat16, got {kind}")
@@ -335,9 +353,7 @@ def _setting(value, name: str, B: int, dtype: torch.dtype, dev: int):
     """(address or None, number) of a setting: a tensor of one value a row, or a number for all."""
     if isinstance(value, torch.Tensor):
         return _vector(value, name, B, dtype, dev), 0
-    if dtype is torch.int64 and not isinstance(value, int) or not isinstance(value, (int, float)):
-        raise ValueError(f"{name} must be a number or a tensor of one a row, got {value!r}")
-    return None, value
+    return None, _number(value, f"{name}, where it is no tensor of one a row,", whole=dtype is torch.int64)
 
 
 def sample_actions(self, logits: torch.Tensor, uniforms: torch.Tensor, num_actions=None, temperature=1.0, top_k=0,
