@@ -25,6 +25,7 @@ import torch
 from . import hive_gpu
 from .fnn import HiveFNN
 from .replay import FNNTrainingBatch, build_forward_batch
+from .training_ops import TYPES
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -73,7 +74,13 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
                  activation: str = "silu") -> torch.Tensor:
     """act(x w_gate^T + b_gate) * (x w_up^T + b_up) of
     HiveGpuExtension.gated_linear, differentiable once in all of its tensors.
-    Where no gradient is asked for, nothing is kept for one."""
+    Where no gradient is asked for, nothing is kept for one.  Under autocast all of
+    them are cast to its type, as torch's own products are."""
+    if torch.is_autocast_enabled("cuda"):
+        to = torch.get_autocast_dtype("cuda")
+        x, w_gate, w_up, b_gate, b_up = (
+            t.to(to) if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in TYPES else t
+            for t in (x, w_gate, w_up, b_gate, b_up))
     tensors = [t for t in (x, w_gate, w_up, b_gate, b_up) if isinstance(t, torch.Tensor)]
     if not torch.is_grad_enabled() or not any(t.requires_grad for t in tensors):
         return hive_gpu.load_extension().gated_linear(x, w_gate, w_up, b_gate, b_up, activation)

@@ -1,12 +1,12 @@
 """The gated block at the ends of its numbers: infinities of float32 tensors,
-float16 gradients past its range.  References and tolerances:
+float16 gradients past its range; under autocast.  References and tolerances:
 test_gpu_network_ops.py."""
 import math
 
 import pytest
 import torch
 
-from test_gpu_network_ops import BF16, F16, F32, U, _act, _gated, _randn, ext  # noqa: F401
+from test_gpu_network_ops import BF16, F16, F32, U, _act, _gated, ext  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -108,3 +108,27 @@ def test_float16_gradients_between_past_its_range(ext, rows, act, large):  # noq
         assert float(want.abs().max()) < 6e4 and float(want.abs().max()) > 1e-6, float(want.abs().max())
         over = (got.double() - want).abs() - off - 2.0 ** -11 * want.abs() * 1.01 - 2.0 ** -25
         assert got.isfinite().all() and float(over.max()) <= 0, float(over.max())
+
+
+@pytest.mark.parametrize("to", [BF16, F16], ids=str)
+def test_autocast(ext, to):  # noqa: F811
+    """What a layer under autocast hands over: float32 weights beside a float32 or 16-bit x.  The result and the gradients are
+    those of tensors cast by hand; the weights' come back in their own type."""
+    from hive_neuralnet_amd.training import gated_linear
+    x, wg, wu, bg, bu, dh = _gated(50, 40, 24, F32, 3)
+    leaves = [t.clone().requires_grad_() for t in (x, wg, wu, bg, bu)]
+    by_hand = [t.clone().requires_grad_() for t in (x, wg, wu, bg, bu)]
+    with torch.autocast("cuda", dtype=to):
+        h = gated_linear(*leaves)
+        with torch.no_grad():
+            assert torch.equal(gated_linear(x.to(to), *leaves[1:]), h)
+        with pytest.raises(ValueError):
+            gated_linear(leaves[0], *[t.double() for t in leaves[1:]])
+    want = gated_linear(*[t.to(to) for t in by_hand])
+    assert h.dtype == to and torch.equal(h, want)
+    h.backward(dh.to(to))
+    want.backward(dh.to(to))
+    for a, b in zip(leaves, by_hand):
+        assert a.grad.dtype == F32 and torch.equal(a.grad, b.grad) and bool(a.grad.any())
+    with torch.autocast("cuda", dtype=to, enabled=False):
+        assert gated_linear(*leaves).dtype == F32
