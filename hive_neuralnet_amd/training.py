@@ -336,6 +336,8 @@ class Muon(torch.optim.Optimizer):
             raise ValueError(f"the saved scale is {state_dict['scale']!r}, this one {self.scale!r}")
         if len(state_dict["param_groups"]) != len(self.param_groups):
             raise ValueError(f"{len(state_dict['param_groups'])} saved groups, {len(self.param_groups)} here")
+        for group, saved in zip(self.param_groups, state_dict["param_groups"]):
+            self._check_settings({**group, **saved})
         self._make_plans(state_dict["momentum"])
         for group, saved in zip(self.param_groups, state_dict["param_groups"]):
             group.update(saved)

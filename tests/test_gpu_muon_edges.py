@@ -79,3 +79,22 @@ def test_a_step_with_gradients_far_below_eps(ext):  # noqa: F811
         moved = float((want - b.double()).norm())
         off = float((p.double() - want).norm())
         assert off <= 1.01 * _relative(*p.shape, 5) * moved + U * float(want.norm()) + 2 * U * float(b.norm()), (off, moved)
+
+
+def test_a_saved_state_with_settings_out_of_range(ext):  # noqa: F811
+    """load_state_dict refuses what the constructor does, and leaves the optimizer as it was."""
+    from hive_neuralnet_amd.training import Muon
+    p = _randn((20, 12), 1).requires_grad_()
+    opt = Muon([p], lr=0.1)
+    p.grad = _randn((20, 12), 2)
+    opt.step()
+    saved = opt.state_dict()
+    held = [m.clone() for m in saved["momentum"][0]]
+    for bad in (dict(momentum=1.0), dict(lr=-1.0), dict(steps=0), dict(steps=101), dict(eps=float("nan")), dict(weight_decay=-1)):
+        state = {**saved, "momentum": [[torch.zeros_like(m) for m in held]],
+                 "param_groups": [{**saved["param_groups"][0], "lr": 0.5, **bad}]}
+        with pytest.raises(ValueError):
+            opt.load_state_dict(state)
+        assert opt.param_groups[0]["lr"] == 0.1 and all(torch.equal(a, b) for a, b in zip(opt.state_dict()["momentum"][0], held))
+    opt.load_state_dict({**saved, "param_groups": [{**saved["param_groups"][0], "lr": 0.5}]})
+    assert opt.param_groups[0]["lr"] == 0.5
