@@ -24,6 +24,7 @@ import torch
 
 from . import hive_gpu
 from .fnn import HiveFNN
+from .network_ops import COEFFICIENTS, _iteration
 from .replay import FNNTrainingBatch, build_forward_batch
 from .training_ops import TYPES
 
@@ -244,12 +245,14 @@ class Muon(torch.optim.Optimizer):
     rows / cols)); "rms": 0.2 sqrt(max(rows, cols)), a step as large as AdamW's.
     Parameters are contiguous matrices; vectors, embeddings and heads of one row go
     to another optimizer (`matrices` finds the ones of a network).  A parameter
-    without a gradient is left as it is."""
+    without a gradient is left as it is.  coefficients: orthogonalize's, one
+    triple for all of the iteration's steps or a list of them, one a step."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True,
-                 weight_decay: float = 0.0, steps: int = 5, eps: float = 1e-7, scale: str = "spectral"):
+                 weight_decay: float = 0.0, steps: int = 5, eps: float = 1e-7, scale: str = "spectral",
+                 coefficients=COEFFICIENTS):
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
-                                      steps=steps, eps=eps))
+                                      steps=steps, eps=eps, coefficients=coefficients))
         self._ext = hive_gpu.load_extension()
         self.scale = scale
         self._plans: list = []  # (group, plan)
@@ -287,8 +290,7 @@ class Muon(torch.optim.Optimizer):
                 raise ValueError(f"{key} must not be negative, got {group[key]}")
         if not 0.0 <= group["momentum"] < 1.0:
             raise ValueError(f"momentum must be in [0, 1), got {group['momentum']}")
-        if not 1 <= group["steps"] <= 100:
-            raise ValueError(f"steps must be 1 to 100, got {group['steps']}")
+        _iteration(group["steps"], group["coefficients"], group["eps"])
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -301,7 +303,8 @@ class Muon(torch.optim.Optimizer):
             grads = [None if p.grad is None else p.grad.contiguous() for p in plan.params]
             if any(g is not None for g in grads):
                 plan.step(grads, lr=group["lr"], momentum=group["momentum"], nesterov=group["nesterov"],
-                          weight_decay=group["weight_decay"], steps=group["steps"], eps=group["eps"])
+                          weight_decay=group["weight_decay"], steps=group["steps"], eps=group["eps"],
+                          coefficients=group["coefficients"])
         return loss
 
     def __getstate__(self):

@@ -98,3 +98,28 @@ def test_a_saved_state_with_settings_out_of_range(ext):  # noqa: F811
         assert opt.param_groups[0]["lr"] == 0.1 and all(torch.equal(a, b) for a, b in zip(opt.state_dict()["momentum"][0], held))
     opt.load_state_dict({**saved, "param_groups": [{**saved["param_groups"][0], "lr": 0.5}]})
     assert opt.param_groups[0]["lr"] == 0.5
+
+
+def test_an_optimizer_with_coefficients_of_its_own(ext):  # noqa: F811
+    """A group's coefficients are those of MuonPlan.step, and go through a saved state; a state saved without them leaves them."""
+    from hive_neuralnet_amd.training import Muon
+    schedule = [(3.0, -3.2, 1.2), (1.875, -1.25, 0.375)]
+    p, q = (_randn((20, 12), 1).requires_grad_() for _ in range(2))
+    opt = Muon([{"params": [p], "coefficients": schedule}], lr=0.1)
+    plan = ext.prepare_muon([q.detach()])
+    p.grad = _randn((20, 12), 2)
+    for _ in range(2):
+        opt.step()
+        plan.step([p.grad], lr=0.1, coefficients=schedule)
+    assert torch.equal(p.detach(), q.detach())
+    saved = opt.state_dict()
+    other = Muon([_randn((20, 12), 1).requires_grad_()])
+    other.load_state_dict(saved)
+    assert other.param_groups[0]["coefficients"] == schedule
+    older = {**saved, "param_groups": [{k: v for k, v in g.items() if k != "coefficients"} for g in saved["param_groups"]]}
+    other = Muon([_randn((20, 12), 1).requires_grad_()])
+    other.load_state_dict(older)
+    assert other.param_groups[0]["coefficients"] == ABC
+    for bad in ((1.0, 2.0), [], "abc", [(1.0, 2.0, 3.0), (1.0,)]):
+        with pytest.raises(ValueError):
+            Muon([_randn((20, 12), 1).requires_grad_()], coefficients=bad)
