@@ -696,7 +696,7 @@ template <typename T> int pack(const Packing& f, hipStream_t st) {
 // one), and the time around its slices, in nanoseconds, as measured at 8,192 x 8,192 x 8,192 and the like.
 template <typename Tl> struct Cost {
     static constexpr int size = Tl::kM * Tl::kN;
-    static constexpr double slice = Tl::kParts == 3 ? (size == 128 * 128 ? 1900 : size == 64 * 128 ? 1500 : 1100)
+    static constexpr double slice = Tl::kParts == 3 ? (size == 64 * 128 ? 1500 : 1100)
                                                     : (size == 256 * 256 ? 1650 : size == 128 * 128 ? 1000 : 700);
     static constexpr double around = size == 256 * 256 ? 6000 : size == 128 * 128 ? 4000 : 2500;
 };
@@ -727,21 +727,25 @@ template <typename Tl> Plan plan_of(int64_t m, int64_t n, int64_t slices, int64_
 template <typename T, typename F> int with_tile(int64_t m, int64_t n, int64_t k, int64_t most, F f) {
     using P = std::conditional_t<sizeof(T) == 4, bf16, T>;
     constexpr bool parts = sizeof(T) == 4;
-    using Middle = std::conditional_t<parts, Tile<P, 3, 1, 128, 128, 2, 2, 3, 1>, Tile<P, 1, 2, 128, 128, 2, 2, 2, 2>>;
     using Small = std::conditional_t<parts, Tile<P, 3, 1, 64, 64, 2, 2, 3, 2>, Tile<P, 1, 2, 64, 64, 2, 2, 3, 3>>;
     const int64_t slices = std::max<int64_t>(1, (k + 32 * Small::kSteps - 1) / (32 * Small::kSteps));
-    const Plan middle = plan_of<Middle>(m, n, slices, most), small = plan_of<Small>(m, n, slices, most);
-    // floats: 64 x 128 tiles, of which a compute unit holds two; 16-bit tensors: 256 x 256, which read the least
-    using Third = std::conditional_t<parts, Tile<P, 3, 1, 64, 128, 2, 2, 2, 2>, Tile<P, 1, 2, 256, 256, 2, 4, 2, 1>>;
-    const Plan third = plan_of<Third>(m, n, slices, most);
-    if (third.time <= middle.time && third.time <= small.time) return f(Third{}, third.splits);
-    if constexpr (!parts) {
+    const Plan small = plan_of<Small>(m, n, slices, most);
+    if constexpr (parts) {
+        // a compute unit holds two of 64 x 128 (one of 128 x 128 took 1,900 ns a slice, which two of these do in 1,500)
+        using Wide = Tile<P, 3, 1, 64, 128, 2, 2, 2, 2>;
+        const Plan wide = plan_of<Wide>(m, n, slices, most);
+        return wide.time <= small.time ? f(Wide{}, wide.splits) : f(Small{}, small.splits);
+    } else {
+        using Middle = Tile<P, 1, 2, 128, 128, 2, 2, 2, 2>;
+        using Large = Tile<P, 1, 2, 256, 256, 2, 4, 2, 1>;  // which read the least
+        const Plan middle = plan_of<Middle>(m, n, slices, most), large = plan_of<Large>(m, n, slices, most);
+        if (large.time <= middle.time && large.time <= small.time) return f(Large{}, large.splits);
         // a block a compute unit at most: twice the slices in flight (2,999 rows of 1,237 float16 to 515 units forward 29.1 us
         // -> 25.6; two teams 27.7)
         using Alone = Tile<P, 1, 2, 128, 128, 2, 2, 4, 1>;
         if (middle.time <= small.time && blocks_of<Middle>(m, n) * middle.splits <= 256) return f(Alone{}, middle.splits);
+        return middle.time <= small.time ? f(Middle{}, middle.splits) : f(Small{}, small.splits);
     }
-    return middle.time <= small.time ? f(Middle{}, middle.splits) : f(Small{}, small.splits);
 }
 
 // Where the kernels of whole rows take over (floats, us forward / both gradients, they and the tiles): 8,192 x 122 -> 64 13 / 32
