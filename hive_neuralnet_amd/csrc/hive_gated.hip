@@ -30,6 +30,8 @@ template <typename T> constexpr bool is_scaled = std::is_same_v<T, f16>;
 
 constexpr int64_t kMaxRows = 1 << 20, kMaxCols = 1 << 19;
 constexpr int64_t kMaxArea = (int64_t)1 << 35;  // a launch has under 2^32 threads, 256 for a piece of 64 x 64
+constexpr int64_t kWhole = 64;        // dgate and dup each begin at a whole slice of dx's sum
+constexpr int64_t kMostSplits = 256;  // of a sum over k
 
 // sigmoid(g) by the card's own exp2 and reciprocal, (|g| + 4) 2^-24 of itself off: the rounding of gate's sum is of that
 // size.  (With expf and a division, 118,271 rows of 122 floats to 64 units took 48 us instead of 44 forward, 107 instead of
@@ -815,7 +817,7 @@ int forward(const void* x, int64_t rows, int64_t cols, int64_t x_stride, const v
 template <typename T, bool kTurnedA>
 int product(const Operand& a, const Operand& b, const Operand& b_second, int64_t m, int64_t k, int64_t cut_k, int64_t rows,
             int64_t cut, void* first, void* second, int64_t n, const float* back, Arena& ws, hipStream_t st) {
-    return with_tile<T>(m, n, k, 256, [&](auto tile, int64_t splits) {
+    return with_tile<T>(m, n, k, kMostSplits, [&](auto tile, int64_t splits) {
         using Tl = decltype(tile);
         constexpr int deep = 32 * Tl::kSteps;
         Product f{};
@@ -872,7 +874,7 @@ int backward(const void* dh, int64_t dh_stride, const void* x, int64_t rows, int
     }
     using P = std::conditional_t<sizeof(T) == 4, bf16, T>;
     constexpr int parts = sizeof(T) == 4 ? 3 : 1;
-    const int64_t cut = up_to(hidden, 64), d_bytes = packed_bytes(2 * cut, parts);  // 64: whole slices of each half
+    const int64_t cut = up_to(hidden, kWhole), d_bytes = packed_bytes(2 * cut, parts);
     const int across = slope_across(cut), each = slope_each(rows, cut), deep = 256 / across * each;
     const int64_t blocks = (rows + deep - 1) / deep;
     const bool biases = dbg || dbu;
@@ -961,6 +963,19 @@ int64_t hg_gated_backward_workspace(int type, int64_t rows, int64_t cols, int64_
                                      some, some, some, ws, nullptr);
     });
     return ws.used;
+}
+
+int hg_gated_tiles(int type, int64_t rows, int64_t cols, int64_t hidden, int tiles[3]) {
+    if (bad_sizes(type, rows, cols, hidden, HG_SIGMOID) || rows == 0 || !tiles) return (int)hipErrorInvalidValue;
+    return with_type(type, [&](auto t) {
+        using T = decltype(t);
+        const bool narrow = is_narrow<T>(rows, cols, hidden);
+        auto name = [](auto tile, int64_t) { return name_of<decltype(tile)>(); };
+        tiles[0] = narrow ? 0 : with_tile<T>(rows, 2 * hidden, cols, 1, name);
+        tiles[1] = narrow ? 0 : with_tile<T>(rows, cols, 2 * up_to(hidden, kWhole), kMostSplits, name);
+        tiles[2] = narrow ? 0 : with_tile<T>(2 * up_to(hidden, kWhole), cols, rows, kMostSplits, name);
+        return 0;
+    });
 }
 
 int hg_gated_backward(const void* dh, int64_t dh_stride, const void* x, int type, int64_t rows, int64_t cols,

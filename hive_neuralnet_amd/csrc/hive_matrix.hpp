@@ -127,6 +127,11 @@ struct Tile {
     }
 };
 
+// a tile as a number: (rows * 1000 + columns) * 100 + stages * 10 + blocks of a compute unit, 10^8 more for each further team
+template <typename Tl> constexpr int name_of() {
+    return ((Tl::kTeams - 1) * 1000000 + Tl::kM * 1000 + Tl::kN) * 100 + Tl::kStages * 10 + Tl::kBlocks;
+}
+
 // The sums of one tile.  acc[i][j][e]: lane l holds C at row 16 i + l % 16 of the wave's part, which begins at row() of the
 // tile, and, with kHalves equal shares of the kFn j, column 4 (j % share) + e of those that begin at col() of half j / share.
 template <typename Tl, int kHalves, bool kTurnedB = false> struct Sums {

@@ -623,6 +623,11 @@ int hg_gated_backward(const void* dh, int64_t dh_stride, const void* x, int type
                       const float* up, int act, void* dx, void* dw_gate, void* dw_up, void* db_gate, void* db_up,
                       void* workspace, void* stream);
 
+/* Which tiles these sizes take (tests and profiles ask): of h, dx, and the weights'
+ * gradients, as (rows * 1000 + columns) * 100 + stages * 10 + blocks of a compute
+ * unit; 0 for the kernels of narrow float32 blocks. */
+int hg_gated_tiles(int type, int64_t rows, int64_t cols, int64_t hidden, int tiles[3]);
+
 /* The Newton-Schulz iteration of `count` matrices u[rows][cols] (matrix i at
  * u + i * u_step, its row r at r * u_row elements from there):
  *   X = U / (|U| + eps), |U| the root of the sum of its squares; then `steps`
