@@ -632,27 +632,41 @@ template <typename Tl> int64_t step_tiles(const Matrix& x, bool symmetric) {
     return symmetric ? (int64_t)m * (m + 1) / 2 : (int64_t)m * n;
 }
 
-// One product of every matrix of the table, in the largest tiles of which there are enough for the card (P X of 24 matrices
-// of 1,024 x 1,024 and 4,096 in 256 x 256 298 us, in 128 x 128 344).
+// f called with the tile that a product of the table's matrices takes, their blocks laid out by it: the largest tiles of which
+// there are enough for the card (P X of 24 matrices of 1,024 x 1,024 and 4,096 in 256 x 256 298 us, in 128 x 128 344).
+template <int kKind, typename F> int with_tile(Table& tab, F f) {
+    auto blocks = [&](auto tile) {
+        return lay_blocks(tab, [](const Matrix& x) { return step_tiles<decltype(tile)>(x, kKind != kStep); });
+    };
+    if constexpr (kKind == kStep) {
+        const Tile<f16, 2, 1, 256, 256, 2, 4, 2, 1, false> large;
+        if (blocks(large) >= 192) return f(large);
+    }
+    const Tile<f16, 2, 1, 128, 128, 2, 2, 2, 2> middle;
+    if (blocks(middle) >= 192) return f(middle);
+    // a block a compute unit at most: of two teams, so that a SIMD has two waves all the same (a matrix of 1,024 x 1,024:
+    // A 13.7 -> 12.8 us, P 14.4 -> 13.3, P X 16.0 -> 15.0)
+    const Tile<f16, 2, 1, 64, 64, 2, 2, 4, 1, true, 2> teams;
+    if (blocks(teams) <= 256) return f(teams);
+    const Tile<f16, 2, 1, 64, 64, 2, 2, 4, 2> small;  // the same tiles
+    return f(small);
+}
+
+// one product of every matrix of the table
 template <int kKind> int product(Table& tab, hipStream_t st) {
-    auto launch = [&](auto tile, int64_t least, int64_t most = 1ll << 40) {
+    return with_tile<kKind>(tab, [&](auto tile) {
         using Tl = decltype(tile);
-        const int64_t blocks = lay_blocks(tab, [](const Matrix& x) { return step_tiles<Tl>(x, kKind != kStep); });
-        if (blocks < least || blocks > most) return -1;
         const int64_t grid = lay_ranges(
             tab, [](const Matrix& x) { return step_tiles<Tl>(x, kKind != kStep); },
             [](const Matrix& x) { return (int64_t)(kKind == kGram ? std::max(x.rows, x.cols) : std::min(x.rows, x.cols)); });
         k_muon_product<kKind, Tl><<<(unsigned)grid, Tl::kBlock, 0, st>>>(tab);
         return launched();
-    };
-    int e = -1;
-    if constexpr (kKind == kStep) e = launch(Tile<f16, 2, 1, 256, 256, 2, 4, 2, 1, false>{}, 192);
-    if (e < 0) e = launch(Tile<f16, 2, 1, 128, 128, 2, 2, 2, 2>{}, 192);
-    // a block a compute unit at most: of two teams, so that a SIMD has two waves all the same (a matrix of 1,024 x 1,024:
-    // A 13.7 -> 12.8 us, P 14.4 -> 13.3, P X 16.0 -> 15.0)
-    if (e < 0) e = launch(Tile<f16, 2, 1, 64, 64, 2, 2, 4, 1, true, 2>{}, 0, 256);
-    if (e < 0) e = launch(Tile<f16, 2, 1, 64, 64, 2, 2, 4, 2>{}, 0);
-    return e;
+    });
+}
+
+// whether a block holds a matrix whose longer side is at most `side`
+bool fits_block(const Matrix& x, int side) {
+    return std::min(x.rows, x.cols) <= kSmall && std::max(x.rows, x.cols) <= side;
 }
 
 // the matrices of the table that `small` says, their whole iteration in one launch
@@ -673,9 +687,7 @@ template <int kL, typename F> int iterate_small(const Table& all, F small, hipSt
 int iterate(Table& all, int steps, const float* coefficients, int64_t triples, hipStream_t st) {
     all.steps = steps;
     all.count = (int)std::min<int64_t>(triples, steps);
-    auto fits = [&](const Matrix& x, int side) {
-        return std::min(x.rows, x.cols) <= kSmall && std::max(x.rows, x.cols) <= side && all.count <= kTriples;
-    };
+    auto fits = [&](const Matrix& x, int side) { return fits_block(x, side) && all.count <= kTriples; };
     for (int i = 0; i < 3 * all.count && i < 3 * kTriples; i++) all.triples[i] = coefficients[i];
     int e = iterate_small<128>(all, [&](const Matrix& x) { return fits(x, 128); }, st);
     if (!e) e = iterate_small<256>(all, [&](const Matrix& x) { return fits(x, 256) && !fits(x, 128); }, st);
@@ -747,6 +759,20 @@ int hg_orthogonalize(const void* u, int type, int64_t count, int64_t rows, int64
     tab.g_type = tab.out_type = type;
     tab.eps = eps;
     return iterate(tab, steps, coefficients, triples, (hipStream_t)stream);
+}
+
+int hg_orthogonalize_tiles(int64_t count, int64_t rows, int64_t cols, int tiles[2]) {
+    if (count < 1 || bad_shape(count, rows, cols) || !tiles) return (int)hipErrorInvalidValue;
+    Table tab{};
+    tab.n = 1;
+    tab.t[0].rows = (int)rows;
+    tab.t[0].cols = (int)cols;
+    tab.t[0].count = (int)count;
+    auto name = [](auto tile) { return name_of<decltype(tile)>(); };
+    const bool small = fits_block(tab.t[0], 256);
+    tiles[0] = small ? 0 : with_tile<kGram>(tab, name);
+    tiles[1] = small ? 0 : with_tile<kStep>(tab, name);
+    return 0;
 }
 
 int64_t hg_muon_step_workspace(const hg_muon_matrix* matrices, int64_t count) {

@@ -46,6 +46,7 @@ SIGS = {
     "hg_gated_tiles": [_c_int, _c_i64, _c_i64, _c_i64, _c_void_p],
     "hg_orthogonalize": [_c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_void_p, _c_int, _c_float,
                          _c_void_p, _c_void_p, _c_void_p],
+    "hg_orthogonalize_tiles": [_c_i64, _c_i64, _c_i64, _c_void_p],
     "hg_muon_step": [_c_void_p, _c_i64, _c_int, _c_int, _c_double, _c_double, _c_int, _c_double, _c_int, _c_void_p,
                      _c_int, _c_float, _c_void_p, _c_void_p],
     "hg_sample_actions": [_c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_void_p, _c_void_p, _c_void_p, _c_double,

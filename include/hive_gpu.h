@@ -644,6 +644,9 @@ int64_t hg_orthogonalize_workspace(int64_t count, int64_t rows, int64_t cols);
 int hg_orthogonalize(const void* u, int type, int64_t count, int64_t rows, int64_t cols, int64_t u_row, int64_t u_step,
                      int steps, const float* coefficients, int triples, float eps, void* out, void* workspace,
                      void* stream);
+/* hg_gated_tiles' numbers of A's and P's tiles, and of P X's, of up to 16 triples, 10^8
+ * more where two teams of a block share a tile; 0 for matrices that a block holds. */
+int hg_orthogonalize_tiles(int64_t count, int64_t rows, int64_t cols, int tiles[2]);
 
 /* One step of `count` matrices with it, in place:
  *   m = momentum m + g;  u = g + momentum m (nesterov) or m
