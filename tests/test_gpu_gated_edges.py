@@ -132,3 +132,61 @@ def test_autocast(ext, to):  # noqa: F811
         assert a.grad.dtype == F32 and torch.equal(a.grad, b.grad) and bool(a.grad.any())
     with torch.autocast("cuda", dtype=to, enabled=False):
         assert gated_linear(*leaves).dtype == F32
+
+
+def test_float16_gradients_in_graphs_and_streams(ext):  # noqa: F811
+    """The pass that finds the largest: a call repeats its bits beside another whose values are of another size, and in a graph
+    replayed on values of other sizes."""
+    x, wg, wu, bg, bu, dh = _gated(700, 72, 56, F16, 3)
+    _, gate, up = ext.gated_linear_forward(x, wg, wu, bg, bu)
+    sizes = (1.0, 2.0 ** -12, 2.0 ** 15)
+
+    def call(v):
+        return ext.gated_linear_backward(v, x, wg, wu, gate, up, need_bias=False)[:3]
+
+    grads = [(s * dh.float()).clamp(-6e4, 6e4).half() for s in sizes]
+    want = [call(v) for v in grads]
+    outs, streams = [], [torch.cuda.Stream() for _ in sizes]
+    for s, v in zip(streams, grads):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs.append(call(v))
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert all(torch.equal(a, b) for a, b in zip(o, w))
+    held = grads[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call(held)
+    for i in (1, 2, 0, 2):
+        held.copy_(grads[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[i])), i
+        call(grads[0])
+    zero = call(dh * 0)
+    assert not any(t.any() for t in zero)
+    # a power of two more of dh is as much more of its gradients, but for what float16 rounds them to
+    for a, b in zip(call((dh.float() * 4).half()), want[0]):
+        big = b.abs() > 2.0 ** -12
+        assert torch.equal(a[big].float(), 4 * b[big].float())
+
+
+def test_float16_gradients_that_are_not_finite(ext):  # noqa: F811
+    """An infinity or NaN in dh stays in its row of dx and its unit's weights, and does not scale the rest."""
+    x, wg, wu, bg, bu, dh = _gated(90, 72, 56, F16, 3)
+    _, gate, up = ext.gated_linear_forward(x, wg, wu, bg, bu)
+    clean = ext.gated_linear_backward(dh, x, wg, wu, gate, up)
+    bad = dh.clone()
+    bad[7, 9], bad[30, 11] = math.inf, math.nan
+    got = ext.gated_linear_backward(bad, x, wg, wu, gate, up)
+    rows = torch.ones((90,), dtype=torch.bool, device="cuda")
+    rows[[7, 30]] = False
+    units = torch.ones((56,), dtype=torch.bool, device="cuda")
+    units[[9, 11]] = False
+    # the largest that scales them may have stood in the two rows: equal to half a unit of the last place
+    for a, b, which in zip(got, clean, (rows, units, units, units, units)):
+        off = (a[which].double() - b[which].double()).abs()
+        assert float((off - 2.0 ** -10 * b[which].double().abs()).max()) <= 2.0 ** -10 * float(b.abs().max())
+    assert not got[0][7].isfinite().all() and got[0][30].isnan().all()
+    assert not any(t[9].isfinite().all() for t in got[1:]) and all(t[11].isnan().all() for t in got[1:])

@@ -1,5 +1,6 @@
 """Orthogonalised updates of matrices far smaller than eps, and of float32's
-smallest.  Definition and tolerances: test_gpu_network_ops.py."""
+smallest, coefficients that shrink, the optimizer's settings.  Definition and
+tolerances: test_gpu_network_ops.py."""
 import math
 
 import pytest
@@ -123,3 +124,21 @@ def test_an_optimizer_with_coefficients_of_its_own(ext):  # noqa: F811
     for bad in ((1.0, 2.0), [], "abc", [(1.0, 2.0, 3.0), (1.0,)]):
         with pytest.raises(ValueError):
             Muon([_randn((20, 12), 1).requires_grad_()], coefficients=bad)
+
+
+@pytest.mark.parametrize("rows,cols", [(40, 33), (300, 129)])
+@pytest.mark.parametrize("size", [1.0, 1e-12])
+def test_coefficients_that_shrink(ext, rows, cols, size):  # noqa: F811
+    """Steps that take X down tenfold each: it is held to its own size on the way, and given at it."""
+    u = _randn((rows, cols), 5, size / math.sqrt(rows * cols))
+    for triple in ((0.1, 0.05, 0.01), (0.1, 0.0, 0.0), (1e-5, 0.0, 0.0)):
+        want, _ = _iteration(u, 6, triple)
+        got = ext.orthogonalize(u, steps=6, coefficients=triple)
+        assert float(want.norm()) < 1e-5
+        # X's rounding is passed on by each step; b A + c A A is a tenth of P at most: half more than where it is next to none
+        assert float((got.double() - want).norm()) <= 1.5 * _relative(rows, cols, 6) * float(want.norm())
+    assert not ext.orthogonalize(u, steps=3, coefficients=(0.0, 0.0, 0.0)).any()
+    many = [(0.1, 0.05, 0.01)] * 20  # more of them than the kernel of small matrices takes
+    want, _ = _iteration(u, 20, many)
+    got = ext.orthogonalize(u, steps=20, coefficients=many)
+    assert float((got.double() - want).norm()) <= 1.5 * _relative(rows, cols, 20) * float(want.norm())
