@@ -15,8 +15,10 @@
 // TFLOP/s; a plain product of that size by the library 125 to 130), slopes 125 (540 MB, 4.3 TB/s), dx 166, dW 160 (830 and
 // 860 TFLOP/s: operands that are turned as they are read from LDS come at half the rate; with weights turned by a kernel
 // before it dx took 148, and that kernel 11).
-// One row of 2,048 to 8,192 units 12 us, 5.6 TB/s of weights.  2,999 rows of 1,237 float16 to 515 units 22.5 forward, 10
-// slopes, 19 dx, 27 dW, 13.5 to lay out what 16-byte loads cannot take.
+// One row of 2,048 to 8,192 units 12 us, 5.6 TB/s of weights.  2,999 rows of 1,237 float16 to 515 units 22.5 forward, 7 for
+// the largest slope, 11.5 slopes, 19 dx, 27 dW, 13.5 to lay out what 16-byte loads cannot take.  8,192 rows of 512 floats to
+// 2,048 units 695 both ways: forward 203, dx and dW 206 each (1,000 TFLOP/s of instructions, a sixth of it of
+// floats), slopes 80, packing.
 #include <algorithm>
 
 #include "hive_pack.hpp"

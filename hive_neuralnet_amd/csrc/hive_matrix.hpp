@@ -336,59 +336,59 @@ __device__ __forceinline__ void multiply(const Operand& a, int m0, const Operand
         }
     } else {
 #pragma unroll
-    for (int n = 0; n < Tl::kStages; n++) {
-        const From f = from(begin + n);
+        for (int n = 0; n < Tl::kStages; n++) {
+            const From f = from(begin + n);
 #pragma unroll
-        for (int i = 0; i < Tl::kLoads; i++) fetch(i, f, n);
-    }
-    wait_loads<(Tl::kStages - 1) * Tl::kLoads < 64 ? (Tl::kStages - 1) * Tl::kLoads : 63>();
-#pragma unroll
-    for (int r = 0; r < Tl::kReads; r++) read(r, 0, 0, 0);
-    int stage = 0;
-    // multiplies step `step` of slice k, whose operands are in half `half` of the registers, and reads the next step's.  At a
-    // slice's last step, the next slice has to be there; its own stage, which all waves have read, is free for the slice
-    // kStages further on.
-    auto multiply_step = [&](int k, auto step_, auto half_) {
-        constexpr int step = decltype(step_)::value, half = decltype(half_)::value;
-        constexpr bool last = step == Tl::kSteps - 1;
-        const int next = !last ? stage : stage + 1 == Tl::kStages ? 0 : stage + 1;
-        if (last) wait_loads<(Tl::kStages - 2) * Tl::kLoads>();
-        const From f = from(k + Tl::kStages);
-        int n = 0;
-#pragma unroll
-        for (int sum = Tl::kParts - 1; sum >= 0; sum--)  // the smallest products first
-#pragma unroll
-            for (int p = 0; p <= sum; p++)
-#pragma unroll
-                for (int i = 0; i < Tl::kFm; i++, n++) {
-#pragma unroll
-                    for (int j = 0; j < Tl::kFn; j++)
-                        s.acc[i][j] = mfma(vb[half][sum - p][j], va[half][p][i], s.acc[i][j]);
-                    // the reads in the first half of the step's time, the loads all through it
-#pragma unroll
-                    for (int r = 0; r < Tl::kReads; r++)
-                        if (r * Tl::kGroups / (2 * Tl::kReads) == n) read(r, half ^ 1, next, last ? 0 : step + 1);
-                    if (last)
-#pragma unroll
-                        for (int i = 0; i < Tl::kLoads; i++)
-                            if (i * Tl::kGroups / Tl::kLoads == n) fetch(i, f, stage);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-        stage = next;
-    };
-    using zero = std::integral_constant<int, 0>;
-    using one = std::integral_constant<int, 1>;
-    if constexpr (Tl::kSteps == 2) {
-        for (int k = begin; k < stop; k++) {
-            multiply_step(k, zero{}, zero{});
-            multiply_step(k, one{}, one{});
+            for (int i = 0; i < Tl::kLoads; i++) fetch(i, f, n);
         }
-    } else {
-        for (int k = begin; k < stop; k += 2) {
-            multiply_step(k, zero{}, zero{});
-            if (k + 1 < stop) multiply_step(k + 1, zero{}, one{});
+        wait_loads<(Tl::kStages - 1) * Tl::kLoads < 64 ? (Tl::kStages - 1) * Tl::kLoads : 63>();
+#pragma unroll
+        for (int r = 0; r < Tl::kReads; r++) read(r, 0, 0, 0);
+        int stage = 0;
+        // multiplies step `step` of slice k, whose operands are in half `half` of the registers, and reads the next step's.  At a
+        // slice's last step, the next slice has to be there; its own stage, which all waves have read, is free for the slice
+        // kStages further on.
+        auto multiply_step = [&](int k, auto step_, auto half_) {
+            constexpr int step = decltype(step_)::value, half = decltype(half_)::value;
+            constexpr bool last = step == Tl::kSteps - 1;
+            const int next = !last ? stage : stage + 1 == Tl::kStages ? 0 : stage + 1;
+            if (last) wait_loads<(Tl::kStages - 2) * Tl::kLoads>();
+            const From f = from(k + Tl::kStages);
+            int n = 0;
+#pragma unroll
+            for (int sum = Tl::kParts - 1; sum >= 0; sum--)  // the smallest products first
+#pragma unroll
+                for (int p = 0; p <= sum; p++)
+#pragma unroll
+                    for (int i = 0; i < Tl::kFm; i++, n++) {
+#pragma unroll
+                        for (int j = 0; j < Tl::kFn; j++)
+                            s.acc[i][j] = mfma(vb[half][sum - p][j], va[half][p][i], s.acc[i][j]);
+                        // the reads in the first half of the step's time, the loads all through it
+#pragma unroll
+                        for (int r = 0; r < Tl::kReads; r++)
+                            if (r * Tl::kGroups / (2 * Tl::kReads) == n) read(r, half ^ 1, next, last ? 0 : step + 1);
+                        if (last)
+#pragma unroll
+                            for (int i = 0; i < Tl::kLoads; i++)
+                                if (i * Tl::kGroups / Tl::kLoads == n) fetch(i, f, stage);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+            stage = next;
+        };
+        using zero = std::integral_constant<int, 0>;
+        using one = std::integral_constant<int, 1>;
+        if constexpr (Tl::kSteps == 2) {
+            for (int k = begin; k < stop; k++) {
+                multiply_step(k, zero{}, zero{});
+                multiply_step(k, one{}, one{});
+            }
+        } else {
+            for (int k = begin; k < stop; k += 2) {
+                multiply_step(k, zero{}, zero{});
+                if (k + 1 < stop) multiply_step(k + 1, zero{}, one{});
+            }
         }
-    }
     }
     wait_loads<0>();  // the LDS is free again
     if constexpr (Tl::kTeams > 1) {
@@ -467,8 +467,8 @@ template <typename T, int n> __device__ __forceinline__ void store_row(T* p, int
                     if (e < left) to[e] = x[e];
             }
         }
-        }
     }
+}
 
 // block t of `all` in an order that keeps blocks that run beside each other near each other: chiplet x has the blocks x, x + 8,
 // ..., and takes a range of its own of the work

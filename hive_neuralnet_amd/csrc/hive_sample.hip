@@ -23,9 +23,9 @@
 //
 // Measured (MI355X): 65,521 lists of up to 256 slots with top_p 53 us (a wave each; the sums and pivots of a cut bound
 // it, not the 35 MB), 192 rows of 85,834 bfloat16 with top_k and top_p 37 us, one row of as many float32 with
-// min_p 22 where at most 1,024 slots pass it, 162 with a top_p of 0.9, whose thousands of slots take four passes of weights
-// (their 64-bit series, 40 us a pass of what one compute unit adds up, bounds these; 233 where each cut began at its first
-// digit); one short list 3 us, 5.5 with the call.
+// min_p 22 where at most 1,024 slots pass it, 155 with a top_p of 0.9, whose thousands of slots take four passes of weights:
+// 279,000 vector instructions, 52 a key and pass of 64, which one compute unit issues for 116 us of these (the LDS atomics'
+// conflicts hold it for 4; 233 where each cut began at its first digit).  One short list 3 us, 5.5 with the call.
 #include <cmath>
 
 #include "hive_train.hpp"

@@ -35,7 +35,7 @@ MAX_WIDTH = 1 << 20  # slots of a row that a slot is drawn from
 MAX_DRAWS, HELD, MAX_LONG_DRAWS = 1 << 25, 1024, 1 << 21  # rows, and rows of more slots than a wave holds
 MAX_SIDE = 1 << 17  # of a matrix that is orthogonalised
 MAX_MATRICES, MAX_PIECES = 1 << 16, 2049 ** 2  # of a batch: matrices, pieces of 64 x 64 of them
-COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # singular values of 0.001 and more end between 0.7 and 1.2 in five steps
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # five steps: singular values from 0.0015 up end in 0.67 .. 1.21
 
 SIGS = {
     "hg_gated_forward": [_c_void_p, _c_int, _c_i64, _c_i64, _c_i64, _c_void_p, _c_void_p, _c_i64, _c_void_p, _c_void_p,
@@ -212,7 +212,7 @@ def orthogonalize(self, u: torch.Tensor, steps: int = 5, coefficients=COEFFICIEN
 
     u float32 / float16 / bfloat16, its rows contiguous, rows and matrices
     evenly spaced; the result has its shape and type and is contiguous.  Matrices
-    are held in 22 bits a value between the products (or to within 2^-37 of their
+    are held in 22 bits a value between the products (or to within 2^-36 of their
     norm, where that is more), which are summed in float32; a, b and c may be such that X's entries stay below 7.9 in size and
     those of a I + b A + c A A below 63."""
     dev = _float_tensor(u, "u")

@@ -634,7 +634,7 @@ int hg_gated_tiles(int type, int64_t rows, int64_t cols, int64_t hidden, int til
  *   times X <- a X + (b A + c A A) X, A = X X^T (X turned where it is taller than
  *   wide), (a, b, c) = coefficients[i] for step i, the last of the `triples` for
  *   the steps past them (host memory, read before the call returns)
- * out[count][rows][cols] has u's type.  Values are held in 22 bits, or to within 2^-37 of
+ * out[count][rows][cols] has u's type.  Values are held in 22 bits, or to within 2^-36 of
  * |X| where that is more (so from 2^-15 of |X| down; |X| is held to its own size, however far |U| is
  * below eps): entries of X and A up to 7.9 in size, of a I + b A + c A A up to 63; past
  * that the result is inf or NaN.  rows, cols <= 2^17, count * (rows / 64 + 1)
