@@ -315,6 +315,8 @@ class Muon(torch.optim.Optimizer):
     def __setstate__(self, state) -> None:
         own = state["muon"]
         super().__setstate__({k: v for k, v in state.items() if k != "muon"})
+        for group in self.param_groups:  # of a copy made when there was one triple for all
+            group.setdefault("coefficients", COEFFICIENTS)
         self._ext = hive_gpu.load_extension()
         self.scale = own["scale"]
         self._make_plans(own["momentum"])

@@ -142,3 +142,19 @@ def test_coefficients_that_shrink(ext, rows, cols, size):  # noqa: F811
     want, _ = _iteration(u, 20, many)
     got = ext.orthogonalize(u, steps=20, coefficients=many)
     assert float((got.double() - want).norm()) <= 1.5 * _relative(rows, cols, 20) * float(want.norm())
+
+
+def test_a_pickle_without_coefficients(ext):  # noqa: F811
+    """One made before they were a setting steps as it did."""
+    from hive_neuralnet_amd.training import Muon
+    p = _randn((20, 12), 1).requires_grad_()
+    opt = Muon([p], lr=0.1)
+    state = opt.__getstate__()
+    state["param_groups"] = [{k: v for k, v in g.items() if k != "coefficients"} for g in state["param_groups"]]
+    other = Muon.__new__(Muon)
+    other.__setstate__(state)
+    p.grad = _randn((20, 12), 2)
+    before = p.detach().clone()
+    other.step()
+    want, _, error = _muon_reference(before, p.grad, torch.zeros_like(before), 0.1, 0.95, True, 0.0, "spectral")
+    assert float((p.detach().double() - want).norm()) <= error + 4 * U * float(want.norm() + 8)
