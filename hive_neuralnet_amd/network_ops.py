@@ -311,8 +311,12 @@ class MuonPlan:
         cols)) of an "rms" one.  grads: one type, contiguous, the parameters'
         shapes; None leaves its matrix and momentum as they are.  The stepped
         parameters' versions rise."""
+        grads = list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
+        for i, g in enumerate(grads):
+            if g is not None and (not isinstance(g, torch.Tensor) or g.layout is not torch.strided):
+                raise ValueError(f"the gradient of params[{i}] must be a dense tensor or None, got {type(g).__name__}")
         steps, eps, c, triples = _iteration(steps, coefficients, eps)
         lr, momentum, weight_decay = (_number(v, name) for v, name in (
             (lr, "lr"), (momentum, "momentum"), (weight_decay, "weight_decay")))

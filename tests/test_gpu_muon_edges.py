@@ -158,3 +158,19 @@ def test_a_pickle_without_coefficients(ext):  # noqa: F811
     other.step()
     want, _, error = _muon_reference(before, p.grad, torch.zeros_like(before), 0.1, 0.95, True, 0.0, "spectral")
     assert float((p.detach().double() - want).norm()) <= error + 4 * U * float(want.norm() + 8)
+
+
+def test_gradients_of_other_kinds(ext):  # noqa: F811
+    """Any sequence of them is taken; what is no dense tensor is refused before anything is written."""
+    params = [_randn((20, 12), i) for i in range(2)]
+    plan = ext.prepare_muon(params)
+    before = [p.clone() for p in params]
+    g = _randn((20, 12), 5)
+    for bad in (1.0, "g", g.tolist(), g.cpu().numpy(), g.to_sparse()):
+        with pytest.raises(ValueError):
+            plan.step([g, bad])
+        with pytest.raises(ValueError):
+            plan.step([bad, None])
+    assert all(torch.equal(a, b) for a, b in zip(params, before)) and not any(m.any() for m in plan.momentum)
+    plan.step(x for x in (g, None))
+    assert not torch.equal(params[0], before[0]) and torch.equal(params[1], before[1])
